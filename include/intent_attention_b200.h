@@ -541,6 +541,135 @@ typedef struct iak_prefill_args {
 } iak_prefill_args;
 int iak_prefill(const iak_page_pools* pools, const iak_prefill_args* args, void* stream);
 
+/* ------------------------------------------------------------------------
+ * FP4 page pool: K/V rows in 4-bit floating point, one scale per row and 32
+ * channels (no counterpart in the reference, whose 4-bit pages are scaled per
+ * page).  A row is quantised when it is written and never again, so appending
+ * needs no staged copy of the open page.
+ *
+ * Block of 32 channels of a row: e = the smallest integer with 6 * 2^e >=
+ * max|x|, held in [-14, 13] and stored as the byte e + 127; element code = the
+ * E2M1 value nearest to x * 2^-e (ties to the even code), magnitudes above 6
+ * as 6, NaN as 0.  With e in [-14, 13] every value a pool can hold is zero or
+ * a normal half (2^-15 .. 49152), so the kernels' half operands are exact.
+ *
+ * head_dim D is 64, 128 or 256; page_size a multiple of 16.  With NB = D / 32
+ * a page holds
+ *   k_codes  page_size * D / 2 bytes: row r, word w * NB + b = the codes of
+ *            channels 32 b + 8 w .. + 7 (channel + i in bits 4i .. 4i + 3)
+ *   v_codes  page_size * D / 2 bytes: rows 2i and 2i + 1 share D bytes, byte c =
+ *            channel c of row 2i (low half) and of row 2i + 1 (high half)
+ *   k_scales page_size * NB bytes: per 16 rows [g 8][hi 2][NB], row g + 8 hi
+ *   v_scales page_size * NB bytes: per 16 rows [NB][t 4][j 4], row
+ *            2 t + (j & 1) + 8 (j >> 1)
+ * Scale bytes are those an append wrote, or 0 (rows never written).  The four
+ * planes are 16-byte aligned.
+ * ------------------------------------------------------------------------ */
+#define IAK_FP4_MAX_QUERIES 16
+typedef struct iak_fp4_pool {
+  void* k_codes; void* k_scales; void* v_codes; void* v_scales;
+  int64_t num_pages;
+  int32_t page_size, head_dim;
+} iak_fp4_pool;
+
+/* Rows in or out: row i < counts[b] (NULL = num_rows) of (sequence b, table
+ * head h) is token positions[b] + i (NULL = 0), that is row token % page_size
+ * of page page_table[b, h, token / page_size].  A row whose slot lies outside
+ * the table or whose page lies outside the pool is not written (iak_fp4_append;
+ * counted in *dropped when given) or read as zeros (iak_fp4_read, which also
+ * writes zeros to the rows from counts[b] on).  A call's (b, h) must not share
+ * the pages that it writes. */
+typedef struct iak_fp4_rows_args {
+  void* k; void* v; int32_t dtype;                 /* dense rows, IAK_DT_*, unit stride along D     */
+  int64_t k_stride_b, k_stride_h, k_stride_n, v_stride_b, v_stride_h, v_stride_n;
+  int32_t batch, num_table_heads, num_rows;
+  const int32_t* page_table; int64_t pt_stride_b, pt_stride_h; int32_t table_width;
+  const int32_t* positions; const int32_t* counts;   /* [batch] or NULL                             */
+  int32_t* dropped;                                  /* device counter or NULL                      */
+} iak_fp4_rows_args;
+int iak_fp4_append(const iak_fp4_pool* pool, const iak_fp4_rows_args* args, void* stream);
+int iak_fp4_read(const iak_fp4_pool* pool, const iak_fp4_rows_args* args, void* stream);
+
+/* Attention of the last num_queries (1 .. IAK_FP4_MAX_QUERIES) tokens of each
+ * sequence over its lengths[b] cached tokens: token t of (b, h) is row
+ * t % page_size of page page_table[b, h, t / page_size]; query m sees the
+ * tokens t < lengths[b] - (num_queries - 1 - m).  Lengths are held to
+ * [0, table_width * page_size]; tokens of pages outside the pool are not seen;
+ * a query that sees nothing gives 0.  G = Hq / Ht query heads share a table
+ * row.  q and out [B, Hq, M, D].
+ *   differential == 0: out = softmax(sm_scale q K') V
+ *   differential != 0: q and K rows are two halves of D / 2 channels,
+ *     x = softmax(sm_scale q1 K1') V - lam[head] softmax(sm_scale q2 K2') V,
+ *     out = out_scale * x, and with norm_weight (float [D])
+ *     out = out_scale * norm_weight * x / sqrt(mean(x^2) + eps).
+ * Scores, softmax statistics and sums are fp32; half / bf16 queries multiply
+ * as halves (exact after a power of two per row), fp32 ones as two halves.
+ * The workspace holds partial sums; its content need not survive the call. */
+typedef struct iak_fp4_decode_args {
+  const void* q; int32_t q_dtype; int64_t q_stride_b, q_stride_h, q_stride_m;
+  void* out; int32_t out_dtype; int64_t out_stride_b, out_stride_h, out_stride_m;
+  int32_t batch, num_q_heads, num_table_heads, num_queries;
+  const int32_t* page_table; int64_t pt_stride_b, pt_stride_h; int32_t table_width;
+  const int32_t* lengths;                            /* [batch]                                     */
+  float sm_scale;
+  int32_t differential;
+  const float* lam;                                  /* [Hq], differential only                     */
+  const float* norm_weight; float eps, out_scale;    /* differential only                           */
+} iak_fp4_decode_args;
+int iak_fp4_decode_workspace_size(const iak_fp4_pool* pool, const iak_fp4_decode_args* args, size_t* bytes);
+int iak_fp4_decode(const iak_fp4_pool* pool, const iak_fp4_decode_args* args, void* workspace,
+                   size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Page operations: which sequences hold which pages of a pool.
+ *
+ * Slot s of num_slots holds lengths[s] tokens in pages page_table[s, h, w],
+ * w < ceil(lengths[s] / page_size), of every table head h; refs[p] counts the
+ * table entries that hold page p, 0 = free.  Entries outside the pool are
+ * left alone.  All operations are integer-exact and independent of the order
+ * in which blocks run; *rejected (when given) counts what they refuse.  Lists
+ * are device arrays; nothing is read back.
+ * ------------------------------------------------------------------------ */
+#define IAK_MAX_PLANES 16
+typedef struct iak_seq_pages {
+  int32_t* refs; int64_t num_pages;
+  int32_t* page_table; int64_t pt_stride_s, pt_stride_h; int32_t table_width;
+  int32_t* lengths;
+  int32_t num_slots, num_table_heads, page_size;
+} iak_seq_pages;
+/* the bytes a page copy moves: page p of plane i at base[i] + p * bytes[i]; with page_tags, plane i is copied
+ * only for pages whose format (tag through tag_map, IAK_FMT_*) has its bit in formats[i], and the tag with it */
+typedef struct iak_page_planes {
+  void* base[IAK_MAX_PLANES]; int64_t bytes[IAK_MAX_PLANES]; uint32_t formats[IAK_MAX_PLANES];
+  int32_t num_planes;
+  void* page_tags; int32_t tag_bytes; uint8_t tag_map[16]; uint8_t tag_default;
+} iak_page_planes;
+
+int iak_pages_workspace_size(const iak_seq_pages* pages, size_t* bytes);
+/* new_tokens[s] more tokens for every slot: fresh pages are the free pages in
+ * ascending order, given out in order of (slot, head, table entry).  A slot
+ * that gets tokens and whose last page is part full and shared (refs > 1
+ * before the call) first gets a copy of its own of that page.  Refused, and
+ * counted once each: a slot with new_tokens < 0, one whose tokens would pass
+ * table_width pages, one whose open page lies outside the pool, and, when the
+ * free pages run out, the first slot that does not fit and every later one
+ * that gets tokens. */
+int iak_pages_grow(const iak_seq_pages* pages, const iak_page_planes* planes, const int32_t* new_tokens,
+                   int32_t* rejected, void* workspace, size_t workspace_bytes, void* stream);
+/* dst[i] becomes a sequence that shares all of src[i]'s pages.  Refused: a
+ * slot out of range, a dst that holds tokens, a dst listed before, a src that
+ * is also a dst of the call. */
+int iak_pages_fork(const iak_seq_pages* pages, const int32_t* src, const int32_t* dst, int32_t count,
+                   int32_t* rejected, void* stream);
+/* the listed slots let go of their pages (entries become -1, lengths 0); a slot listed again is skipped, one
+ * out of range refused */
+int iak_pages_free(const iak_seq_pages* pages, const int32_t* slots, int32_t count, int32_t* rejected, void* stream);
+/* moves the pages in use that lie at or above their number n to the free pages
+ * below n, both in ascending order, and renames them in the tables of all
+ * slots; *num_live = n */
+int iak_pages_compact(const iak_seq_pages* pages, const iak_page_planes* planes, int32_t* num_live,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,54 @@
+// FP4 page pool: layout arithmetic and conversions shared by the FP4 kernels.
+#pragma once
+
+#include "iak_internal.cuh"
+
+namespace iak {
+
+constexpr int kFp4ScaleMin = 127 - 14, kFp4ScaleMax = 127 + 13;   // scale bytes an append writes
+
+struct Fp4Pool {
+  uint8_t* kc; uint8_t* ks; uint8_t* vc; uint8_t* vs;
+  int64_t num_pages;
+  int PS, D;
+};
+
+// Scale byte of a block with largest magnitude amax: the smallest e with 6 * 2^e >= amax.  amax = m * 2^k,
+// 1 <= m < 2, and 6 = 1.5 * 4, so e = k - 2 for m <= 1.5 and k - 1 above; subnormals end at the lower bound.
+__device__ __forceinline__ int fp4_scale_byte(float amax) {
+  const unsigned u = __float_as_uint(amax);
+  const int k = static_cast<int>(u >> 23);              // biased; inf gives the upper bound
+  const int b = k - 2 + ((u & 0x7fffffu) > 0x400000u ? 1 : 0);
+  return min(max(b, kFp4ScaleMin), kFp4ScaleMax);
+}
+
+__device__ __forceinline__ float fp4_inv_scale(int byte) { return __uint_as_float((254 - byte) << 23); }
+__device__ __forceinline__ float fp4_scale(int byte) { return __uint_as_float(byte << 23); }
+
+// two E2M1 codes in a byte, `lo` in bits 0..3: nearest, ties to the even code, saturating at 6
+__device__ __forceinline__ unsigned fp4_pack2(float lo, float hi) {
+  unsigned short r;
+  asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\nmov.b16 %0, {b, 0};\n}" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// the four bytes of w as half pairs (bits 0..3 of a byte in the low half)
+__device__ __forceinline__ void fp4_unpack4(unsigned w, unsigned (&h)[4]) {
+  asm("{\n.reg .b8 b0, b1, b2, b3;\nmov.b32 {b0, b1, b2, b3}, %4;\n"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\ncvt.rn.f16x2.e2m1x2 %1, b1;\n"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\ncvt.rn.f16x2.e2m1x2 %3, b3;\n}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+
+// byte offsets inside the scale planes (64-bit: a long cache passes 2^31 rows * blocks)
+__device__ __forceinline__ int64_t fp4_k_scale_at(int64_t page, int row, int b, int PS, int NB) {
+  return ((page * (PS / 16) + (row >> 4)) * 8 + (row & 7)) * 2 * NB + ((row >> 3) & 1) * NB + b;
+}
+__device__ __forceinline__ int64_t fp4_v_scale_at(int64_t page, int row, int b, int PS, int NB) {
+  const int r = row & 15;
+  return (((page * (PS / 16) + (row >> 4)) * NB + b) * 4 + ((r & 7) >> 1)) * 4 + (r & 1) + 2 * (r >> 3);
+}
+
+int check_fp4_pool(const iak_fp4_pool* pool, const char* what);
+
+}  // namespace iak

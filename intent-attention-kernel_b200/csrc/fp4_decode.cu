@@ -1,0 +1,867 @@
+// Attention of a sequence's last tokens over an FP4 page pool (iak_fp4_decode), plain and differential.
+//
+// Mathematics.  A table head's queries form NC = G * M * (1 or 2) softmax columns (differential: two per query, the
+// first with q2 = 0 and the second with q1 = 0, so that both halves run as one product).  Per tile of 32 keys
+//   S' = K Q',  P = exp2(S - m),  O' += V' P'
+// with running maximum m and sum l per column, fp32.  Keys are the rows of the first product and the contraction of
+// the second, columns the narrow side (n = 8 per mma.m16n8k16), so that few queries waste little.
+//   K: a lane's 32-bit word holds 8 channels of one row; the byte pairs become half pairs in one conversion each, and
+//      a row's block scale 2^e multiplies the fp32 product of its 32 channels (4 lanes x 8), not its elements.
+//   V: a byte holds one channel of two neighbouring keys, so that its half pair lies along the contraction; it is
+//      multiplied by the two keys' scales (exact: the pool's values are halves).
+//   P: from the accumulator's layout to the operand's by movmatrix.
+// What bounds it: the cache's bytes, 4.25 bits an element.  Work is cut into equal runs of 32-key tiles over all
+// (sequence, table head, column group) units, one run per resident block, so that ragged batches and single long
+// sequences fill the GPU alike; a unit cut over several blocks leaves partial (m, l, O) that a second kernel joins in
+// order of the blocks (no atomics: results do not depend on timing).  Each warp streams its own tiles through a
+// two-stage ring of 16-byte asynchronous copies; a lane copies exactly what it will read, so the ring needs no
+// barrier.
+#include <algorithm>
+#include <cfloat>
+#include <mutex>
+
+#include "fp4.cuh"
+
+namespace iak {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
+constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
+constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
+constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small P stay normal halves
+
+struct DecP {
+  Fp4Pool pool;
+  int gpp;                           // groups of 16 rows per page
+  const void* q; int q_dtype; int64_t q_sb, q_sh, q_sm;
+  void* out; int out_dtype; int64_t o_sb, o_sh, o_sm;
+  int B, Hq, Ht, G, M;
+  const int32_t* pt; int64_t pt_sb, pt_sh; int W;
+  const int32_t* lengths;
+  float scale;                       // |sm_scale| * log2(e)
+  float sign;                        // of sm_scale
+  int diff; const float* lam; const float* norm_w; float eps, out_scale;
+  int NC;                            // softmax columns of a table head
+  int CG;                            // column groups of 8 * NT
+  int HC;                            // units of a sequence: Ht * CG
+  int grid;                          // blocks of the main kernel
+  int direct;                        // one block per unit, nothing to join
+  int min_tiles;                     // tiles a block takes at least
+  float* ws;
+};
+
+// ------------------------------------------------------------------ schedule
+__device__ __forceinline__ int seq_len(const DecP& p, int b) {
+  return min(max(p.lengths[b], 0), p.W * p.pool.PS);
+}
+// tiles of one unit; an empty sequence has one, which writes its zeros
+__device__ __forceinline__ int seq_tiles(const DecP& p, int b) {
+  return max(1, static_cast<int>((static_cast<int64_t>(seq_len(p, b)) + kTileKeys - 1) / kTileKeys));
+}
+
+// all tiles of the call (every lane of every warp has it)
+__device__ __forceinline__ int64_t total_tiles(const DecP& p) {
+  const int lane = threadIdx.x & 31;
+  int64_t sum = 0;
+  for (int b = lane; b < p.B; b += 32) sum += seq_tiles(p, b);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  return sum * p.HC;
+}
+
+// sequence that holds tile t, and t's offset among that sequence's tiles
+__device__ __forceinline__ void find_sequence(const DecP& p, int64_t t, int& b, int64_t& off) {
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int base = 0; base < p.B; base += 32) {
+    const int i = base + lane;
+    int64_t n = i < p.B ? static_cast<int64_t>(seq_tiles(p, i)) * p.HC : 0;
+    int64_t inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(~0u, inc, o);
+      if (lane >= o) inc += v;
+    }
+    const unsigned hit = __ballot_sync(~0u, i < p.B && before + inc > t);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      b = base + l;
+      off = t - (before + __shfl_sync(~0u, inc - n, l));
+      return;
+    }
+    before += __shfl_sync(~0u, inc, 31);
+  }
+  b = p.B;
+  off = 0;
+}
+
+__device__ __forceinline__ int64_t blocks_used(const DecP& p, int64_t total) {
+  const int64_t most = (total + p.min_tiles - 1) / p.min_tiles;
+  return most < p.grid ? most : p.grid;
+}
+
+// ---------------------------------------------------------------------- PTX
+__device__ __forceinline__ void mma16816(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
+                                         unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ unsigned transpose8x8(unsigned x) {
+  unsigned r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ unsigned pack_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const unsigned*>(&h);
+}
+__device__ __forceinline__ unsigned mul_half2(unsigned a, unsigned b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const unsigned*>(&r);
+}
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(unsigned dst, const void* src, bool ok) {
+  const int n = ok ? BYTES : 0;      // 0 source bytes: the destination is zero-filled
+  if (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ unsigned lds32(unsigned a) {
+  unsigned r;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
+  return r;
+}
+template <int NW>
+__device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
+  if constexpr (NW == 1) {
+    w[0] = lds32(a);
+  } else if constexpr (NW == 2) {
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+  } else {
+    static_assert(NW == 4, "words per access");
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a));
+  }
+}
+
+// ------------------------------------------------------------- shared layout
+template <int NB>
+struct Lay {
+  static constexpr int D = NB * 32;
+  static constexpr int kPiece = NB >= 4 ? 16 : 8;          // bytes of one access
+  static constexpr int kPieces = NB * 4 / kPiece;          // accesses of a lane's NB words
+  static constexpr int kPlane = 32 * NB * 4;               // a lane-ordered set of NB words
+  static constexpr int kScaleK = 2 * NB;                   // a lane's K scale bytes: rows g and g + 8
+  static constexpr int kKs = 4 * kPlane;                   // offsets inside a group
+  static constexpr int kVs = kKs + 32 * kScaleK;
+  static constexpr int kGroup = kVs + 32 * 4;
+  static constexpr int kStage = 2 * kGroup;
+  static constexpr int kRing = kWarps * 2 * kStage;
+  static constexpr int kOutStride = D + 4;                 // floats of one column in the join buffer
+};
+
+template <int NB, int NT, bool SPLIT>
+constexpr int smem_bytes() {
+  return Lay<NB>::kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + 8 * NT * 8 + kWarps * 8 * NT * 8;
+}
+
+// x: one row's D values, lane i holding channels i, i + 32, ..
+template <int NB>
+__device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m, float (&x)[NB]) {
+  const int lane = threadIdx.x & 31;
+  if (p.diff) {
+    float mul = p.out_scale;
+    if (p.norm_w) {
+      float sq = 0.f;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) sq = fmaf(x[i], x[i], sq);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
+      mul *= rsqrtf(sq * (1.f / (NB * 32)) + p.eps);
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) x[i] *= p.norm_w ? mul * p.norm_w[i * 32 + lane] : mul;
+  }
+  const int64_t at = b * p.o_sb + head * p.o_sh + m * p.o_sm;
+#pragma unroll
+  for (int i = 0; i < NB; ++i) store_from_float(p.out, p.out_dtype, at + i * 32 + lane, x[i]);
+}
+
+__device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
+
+// ---------------------------------------------------------------- main kernel
+template <int NB, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
+  using L = Lay<NB>;
+  constexpr int D = L::D;
+  constexpr int MT = D / 16;
+  constexpr int COLS = 8 * NT;
+  extern __shared__ __align__(16) char smem[];
+  char* q_frag = smem + L::kRing;                                   // [hi, lo][NT][NB][lane] 16 bytes
+  float* col_scale = reinterpret_cast<float*>(q_frag + NT * NB * 512 * (SPLIT ? 2 : 1));
+  int* col_limit = reinterpret_cast<int*>(col_scale + COLS);
+  float* warp_m = reinterpret_cast<float*>(col_limit + COLS);      // [warp][COLS]
+  float* warp_l = warp_m + kWarps * COLS;
+  float* join = reinterpret_cast<float*>(smem);                    // [warp][8][kOutStride], over the ring
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
+  const unsigned ring = smem_base + warp * 2 * L::kStage;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  int b;
+  int64_t left, off;
+  bool begins_run = true;
+  if (p.direct) {
+    b = blockIdx.x / p.HC;
+    const int n = seq_tiles(p, b);
+    off = static_cast<int64_t>(blockIdx.x - b * p.HC) * n;
+    left = n;
+  } else {
+    const int64_t total = total_tiles(p);
+    const int64_t used = blocks_used(p, total);
+    if (blockIdx.x >= used) return;
+    const int64_t t0 = total * blockIdx.x / used;
+    left = total * (blockIdx.x + 1) / used - t0;
+    find_sequence(p, t0, b, off);
+  }
+
+  while (left > 0 && b < p.B) {
+    // ------------------------------------------------------------ one segment
+    const int len = seq_len(p, b);
+    const int n_tiles = seq_tiles(p, b);
+    const int unit = static_cast<int>(off / n_tiles);             // of the sequence: table head, column group
+    const int c_begin = static_cast<int>(off - static_cast<int64_t>(unit) * n_tiles);
+    const int c_end = static_cast<int>(min(static_cast<int64_t>(n_tiles), c_begin + left));
+    const int h = unit / p.CG, cg = unit - h * p.CG;
+    const int32_t* table = p.pt + b * p.pt_sb + h * p.pt_sh;
+
+    // queries: 8 channels per thread, halves after a power of two that puts the row's largest in [1, 2)
+    constexpr int CH = D / 8;
+    for (int i = threadIdx.x; i < COLS * CH; i += kThreads) {
+      const int col = i / CH, ch = i - col * CH;
+      const int j = cg * COLS + col;
+      const int row = p.diff ? j >> 1 : j;
+      float x[8] = {};
+      const bool mine = j < p.NC && (!p.diff || (ch * 2 >= CH) == (j & 1));
+      if (mine) {
+        const int gi = row / p.M, m = row - gi * p.M;
+        const int64_t at = b * p.q_sb + (h * p.G + gi) * p.q_sh + m * p.q_sm + ch * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = load_as_float(p.q, p.q_dtype, at + e) * p.sign;
+      }
+      float amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+#pragma unroll
+      for (int o = 1; o < CH; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+      // exponent of amax, held to normal numbers on both sides
+      const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
+      const float down = __uint_as_float((254 - ex) << 23);
+      unsigned hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float y0 = x[2 * e] * down, y1 = x[2 * e + 1] * down;
+        hi[e] = pack_half2(y0, y1);
+        if (SPLIT) {
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+          lo[e] = pack_half2(y0 - back.x, y1 - back.y);
+        }
+      }
+      uint4* dst = reinterpret_cast<uint4*>(q_frag) + ((col >> 3) * NB + (ch >> 2)) * 32 + (col & 7) * 4 + (ch & 3);
+      *dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if (SPLIT) dst[NT * NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (ch == 0) {
+        col_scale[col] = fmaxf(p.scale * __uint_as_float(ex << 23), 1e-37f);
+        col_limit[col] = j < p.NC ? len - (p.M - 1 - row % p.M) : len;
+      }
+    }
+    __syncthreads();
+    float sc[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      sc[nt][0] = col_scale[nt * 8 + 2 * t];
+      sc[nt][1] = col_scale[nt * 8 + 2 * t + 1];
+    }
+
+    // ----------------------------------------------------- the copies' cursor
+    int c_fetch = c_begin + warp;                 // tile whose page ids are read next
+    int slot = (c_fetch * 2) / p.gpp, sub = c_fetch * 2 - slot * p.gpp;
+    const int step_slot = (2 * kWarps) / p.gpp, step_sub = 2 * kWarps - step_slot * p.gpp;
+    int id[2], in_page[2];                        // of the tile fetched last
+    auto fetch = [&]() {
+      int s1 = slot, u1 = sub + 1;
+      if (u1 == p.gpp) { u1 = 0; ++s1; }
+      in_page[0] = sub;
+      in_page[1] = u1;
+      id[0] = id[1] = -1;
+      if (c_fetch < c_end) {
+        if (c_fetch * kTileKeys < len) id[0] = __ldg(table + slot);
+        if (c_fetch * kTileKeys + 16 < len) id[1] = __ldg(table + s1);
+      }
+      c_fetch += kWarps;
+      slot += step_slot;
+      sub += step_sub;
+      if (sub >= p.gpp) { sub -= p.gpp; ++slot; }
+    };
+    unsigned ok_bits = 0;                         // [stage][group]: the group's page exists
+    auto issue = [&](int stage) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool ok = id[u] >= 0 && id[u] < p.pool.num_pages;
+        const int64_t page = ok ? id[u] : 0;
+        const int bit = stage * 2 + u;
+        ok_bits = (ok_bits & ~(1u << bit)) | (static_cast<unsigned>(ok) << bit);
+        const int64_t row = page * p.pool.PS + in_page[u] * 16;
+        const int64_t group = page * p.gpp + in_page[u];
+        const uint8_t* k = p.pool.kc + (row + g) * (16 * NB) + t * (4 * NB);
+        const uint8_t* v = p.pool.vc + (row / 2 + t) * (32 * NB) + g * (4 * NB);
+        const unsigned dst = ring + stage * L::kStage + u * L::kGroup;
+#pragma unroll
+        for (int i = 0; i < L::kPieces; ++i) {
+          const unsigned to = dst + (i * 32 + lane) * L::kPiece;
+          copy_async<L::kPiece>(to, k + i * L::kPiece, ok);
+          copy_async<L::kPiece>(to + L::kPlane, k + 8 * (16 * NB) + i * L::kPiece, ok);
+          copy_async<L::kPiece>(to + 2 * L::kPlane, v + i * L::kPiece, ok);
+          copy_async<L::kPiece>(to + 3 * L::kPlane, v + 4 * (32 * NB) + i * L::kPiece, ok);
+        }
+        copy_async<L::kScaleK>(dst + L::kKs + lane * L::kScaleK, p.pool.ks + (group * 8 + g) * (2 * NB), ok);
+        copy_async<4>(dst + L::kVs + lane * 4, p.pool.vs + (group * NB + g * NB / 8) * 16 + t * 4, ok);
+      }
+      copy_commit();
+    };
+    auto read_words = [&](unsigned at, unsigned (&w)[NB]) {
+      constexpr int PW = L::kPiece / 4;
+#pragma unroll
+      for (int i = 0; i < L::kPieces; ++i) {
+        unsigned part[PW];
+        lds_words<PW>(at + (i * 32 + lane) * L::kPiece, part);
+#pragma unroll
+        for (int j = 0; j < PW; ++j) w[i * PW + j] = part[j];
+      }
+    };
+
+    float o[NT][MT][4];
+    float m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m_run[nt][0] = m_run[nt][1] = -FLT_MAX;
+      l_run[nt][0] = l_run[nt][1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+    }
+
+    fetch();
+    issue(0);
+    fetch();
+    issue(1);
+    fetch();
+    int stage = 0;
+    for (int c = c_begin + warp; c < c_end; c += kWarps, stage ^= 1) {
+      copy_wait<1>();
+      const unsigned at = ring + stage * L::kStage;
+      const int key0 = c * kTileKeys;
+      const bool full = ((ok_bits >> (2 * stage)) & 3) == 3 && key0 + kTileKeys <= len - (p.M - 1);
+
+      // ---------------------------------------------------------- S' = K Q'
+      float s[2][NT][4];
+      {
+        unsigned kw[2][2][NB];
+        unsigned ksw[2][(2 * NB + 3) / 4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          read_words(at + u * L::kGroup, kw[u][0]);
+          read_words(at + u * L::kGroup + L::kPlane, kw[u][1]);
+          lds_words<L::kScaleK / 4>(at + u * L::kGroup + L::kKs + lane * L::kScaleK, ksw[u]);
+        }
+#pragma unroll
+        for (int bk = 0; bk < NB; ++bk) {
+          uint4 q_hi[NT], q_lo[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            q_hi[nt] = reinterpret_cast<const uint4*>(q_frag)[(nt * NB + bk) * 32 + lane];
+            if (SPLIT) q_lo[nt] = reinterpret_cast<const uint4*>(q_frag)[(NT * NB + nt * NB + bk) * 32 + lane];
+          }
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            unsigned r0[4], r1[4];
+            fp4_unpack4(kw[u][0][bk], r0);
+            fp4_unpack4(kw[u][1][bk], r1);
+            const int i0 = bk, i1 = NB + bk;          // scale bytes of rows g and g + 8
+            const float s0 = fp4_scale((ksw[u][i0 / 4] >> (8 * (i0 % 4))) & 255);
+            const float s1 = fp4_scale((ksw[u][i1 / 4] >> (8 * (i1 % 4))) & 255);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float acc[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816(acc, r0[0], r1[0], r0[1], r1[1], q_hi[nt].x, q_hi[nt].y);
+              mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_hi[nt].z, q_hi[nt].w);
+              if (SPLIT) {
+                mma16816(acc, r0[0], r1[0], r0[1], r1[1], q_lo[nt].x, q_lo[nt].y);
+                mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_lo[nt].z, q_lo[nt].w);
+              }
+              if (bk == 0) {
+                s[u][nt][0] = acc[0] * s0; s[u][nt][1] = acc[1] * s0;
+                s[u][nt][2] = acc[2] * s1; s[u][nt][3] = acc[3] * s1;
+              } else {
+                s[u][nt][0] = fmaf(acc[0], s0, s[u][nt][0]); s[u][nt][1] = fmaf(acc[1], s0, s[u][nt][1]);
+                s[u][nt][2] = fmaf(acc[2], s1, s[u][nt][2]); s[u][nt][3] = fmaf(acc[3], s1, s[u][nt][3]);
+              }
+            }
+          }
+        }
+      }
+      if (!full) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const bool ok = (ok_bits >> (2 * stage + u)) & 1;
+          const int key = key0 + u * 16 + g;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool seen = ok && key + (i >> 1) * 8 < col_limit[nt * 8 + 2 * t + (i & 1)];
+              if (!seen) s[u][nt][i] = -INFINITY;
+            }
+          }
+        }
+      }
+
+      // ---------------------------------------------------------- softmax
+      float mx[NT][2];
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+          raise = raise || fmaf(mx[nt][e], sc[nt][e], -m_run[nt][e]) > kLazy;
+        }
+      }
+      if (__any_sync(~0u, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v = mx[nt][e];
+            v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
+            const float m_new = fmaxf(m_run[nt][e], fmaf(v, sc[nt][e], -kHead));
+            f[e] = fast_exp2(m_run[nt][e] - m_new);
+            m_run[nt][e] = m_new;
+            l_run[nt][e] *= f[e];
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            o[nt][i][0] *= f[0]; o[nt][i][1] *= f[1];
+            o[nt][i][2] *= f[0]; o[nt][i][3] *= f[1];
+          }
+        }
+      }
+      unsigned pf[2][NT][2], pl[2][NT][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = fast_exp2(fmaf(s[u][nt][i], sc[nt][i & 1], -m_run[nt][i & 1]));
+            l_run[nt][i & 1] += x[i];
+          }
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const unsigned hi = pack_half2(x[2 * r], x[2 * r + 1]);
+            pf[u][nt][r] = transpose8x8(hi);
+            if (SPLIT) {
+              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+              pl[u][nt][r] = transpose8x8(pack_half2(x[2 * r] - back.x, x[2 * r + 1] - back.y));
+            }
+          }
+        }
+      }
+
+      // ---------------------------------------------------------- O' += V' P'
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        unsigned vw[2][NB];
+        read_words(at + u * L::kGroup + 2 * L::kPlane, vw[0]);
+        read_words(at + u * L::kGroup + 3 * L::kPlane, vw[1]);
+        unsigned vs = lds32(at + u * L::kGroup + L::kVs + lane * 4);   // keys 2t, 2t + 1, 2t + 8, 2t + 9
+        if (!full) {          // rows behind the sequence hold anything: scale 0 keeps NaN out of the sums
+          const int key = key0 + u * 16 + 2 * t;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (key + (i & 1) + 8 * (i >> 1) >= len) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
+          }
+        }
+        // byte e + 127 -> half 2^e: (byte - 112) << 10 in both halves at once
+        const unsigned v01 = __byte_perm(vs, 0, 0x4140) * 1024u - 112u * 1024u * 65537u;
+        const unsigned v23 = __byte_perm(vs, 0, 0x4342) * 1024u - 112u * 1024u * 65537u;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          unsigned r0[4], r1[4];
+          fp4_unpack4(vw[0][j], r0);
+          fp4_unpack4(vw[1][j], r1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            r0[i] = mul_half2(r0[i], v01);
+            r1[i] = mul_half2(r1[i], v23);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pf[u][nt][0], pf[u][nt][1]);
+            mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pf[u][nt][0], pf[u][nt][1]);
+            if (SPLIT) {
+              mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pl[u][nt][0], pl[u][nt][1]);
+              mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pl[u][nt][0], pl[u][nt][1]);
+            }
+          }
+        }
+      }
+      issue(stage);
+      fetch();
+    }
+    copy_wait<0>();
+
+    // ------------------------------------------------------ join the 8 warps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = l_run[nt][e];
+        v += __shfl_xor_sync(~0u, v, 4);
+        v += __shfl_xor_sync(~0u, v, 8);
+        v += __shfl_xor_sync(~0u, v, 16);
+        if (g == 0) {
+          warp_m[warp * COLS + nt * 8 + 2 * t + e] = m_run[nt][e];
+          warp_l[warp * COLS + nt * 8 + 2 * t + e] = v;
+        }
+      }
+    }
+    __syncthreads();                              // every warp has read its ring to the end
+    const bool whole = c_begin == 0 && c_end == n_tiles;
+    const int which = begins_run ? 0 : 1;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = -FLT_MAX;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + nt * 8 + 2 * t + e]);
+        f[e] = fast_exp2(m_run[nt][e] - top);
+      }
+      float* dst = join + (warp * 8 + 2 * t) * L::kOutStride + g * (4 * NB);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[nt][i][0] * f[0], o[nt][i][2] * f[0]);
+        *reinterpret_cast<float2*>(dst + L::kOutStride + 2 * i) = make_float2(o[nt][i][1] * f[1], o[nt][i][3] * f[1]);
+      }
+      __syncthreads();
+      // a warp takes the columns of one output row
+      const int per = p.diff ? 2 : 1;
+      if (warp * per < 8) {
+        float x[NB];
+        bool write = true;
+        int row = 0;
+        for (int half = 0; half < per; ++half) {
+          const int lc = warp * per + half, col = nt * 8 + lc, j = cg * COLS + col;
+          if (j >= p.NC) { write = false; break; }
+          float top = -FLT_MAX, l = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + col]);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) l += warp_l[w * COLS + col] * fast_exp2(warp_m[w * COLS + col] - top);
+          float acc[NB];
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            acc[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) acc[i] += join[(w * 8 + lc) * L::kOutStride + i * 32 + lane];
+          }
+          if (!whole) {
+            float* part = p.ws + ((static_cast<int64_t>(blockIdx.x) * 2 + which) * COLS + col) * (D + 2);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) part[i * 32 + lane] = acc[i];
+            if (lane == 0) { part[D] = top; part[D + 1] = l; }
+            write = false;
+            continue;
+          }
+          const float inv = safe_inverse(l);
+          row = p.diff ? j >> 1 : j;
+          const float weight = half ? -p.lam[h * p.G + row / p.M] * inv : inv;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], weight, x[i]) : acc[i] * weight;
+        }
+        if (write) finish_row<NB>(p, b, h * p.G + row / p.M, row % p.M, x);
+      }
+      __syncthreads();
+    }
+
+    left -= c_end - c_begin;
+    off += c_end - c_begin;
+    begins_run = false;
+    if (off == static_cast<int64_t>(n_tiles) * p.HC) {
+      off = 0;
+      ++b;
+    }
+  }
+}
+
+// ---------------------------------------------------------------- join kernel
+// One block per (unit, output row): the units cut over several blocks, their partials in order of the blocks.
+constexpr int kJoinWarps = 4;
+
+template <int NB, int NT>
+__global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p) {
+  constexpr int D = NB * 32, COLS = 8 * NT;
+  const int per = p.diff ? 2 : 1;
+  const int rows = COLS / per;
+  const int64_t u_all = blockIdx.x / rows;
+  const int r = static_cast<int>(blockIdx.x - u_all * rows);
+  const int b = static_cast<int>(u_all / p.HC), unit = static_cast<int>(u_all - static_cast<int64_t>(b) * p.HC);
+  const int h = unit / p.CG, cg = unit - h * p.CG;
+  const int j0 = cg * COLS + r * per;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // tiles before this unit
+  int64_t before = 0, total = 0;
+  for (int i = lane; i < p.B; i += 32) {
+    const int n = seq_tiles(p, i);
+    total += n;
+    if (i < b) before += n;
+  }
+#pragma unroll
+  for (int s = 16; s; s >>= 1) {
+    total += __shfl_xor_sync(~0u, total, s);
+    before += __shfl_xor_sync(~0u, before, s);
+  }
+  total *= p.HC;
+  const int n = seq_tiles(p, b);
+  const int64_t t_begin = before * p.HC + static_cast<int64_t>(unit) * n, t_last = t_begin + n - 1;
+  const int64_t used = blocks_used(p, total);
+  // block of tile t: the largest i with floor(total * i / used) <= t
+  const int first = static_cast<int>(((t_begin + 1) * used - 1) / total);
+  const int last = static_cast<int>(((t_last + 1) * used - 1) / total);
+  const int first_which = total * first / used == t_begin ? 0 : 1;
+  // every block waits, so that this kernel never ends before the main one
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (first == last || j0 >= p.NC) return;      // written whole, or no such row
+
+  __shared__ float part_sum[kJoinWarps][D];
+  __shared__ float part_m[kJoinWarps], part_l[kJoinWarps];
+  float x[NB];
+  for (int half = 0; half < per; ++half) {
+    const int col = r * per + half;
+    float top = -FLT_MAX, l = 0.f, acc[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) acc[i] = 0.f;
+    for (int c = first + warp; c <= last; c += kJoinWarps) {
+      const float* part = p.ws + ((static_cast<int64_t>(c) * 2 + (c == first ? first_which : 0)) * COLS + col) * (D + 2);
+      const float m = part[D], m_new = fmaxf(top, m);
+      const float f_old = fast_exp2(top - m_new), f_new = fast_exp2(m - m_new);
+      l = l * f_old + part[D + 1] * f_new;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) acc[i] = acc[i] * f_old + part[i * 32 + lane] * f_new;
+      top = m_new;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) part_sum[warp][i * 32 + lane] = acc[i];
+    if (lane == 0) { part_m[warp] = top; part_l[warp] = l; }
+    __syncthreads();
+    if (warp == 0) {
+      float all = -FLT_MAX, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) all = fmaxf(all, part_m[w]);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = fast_exp2(part_m[w] - all);
+        sum += part_l[w] * f;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] = fmaf(part_sum[w][i * 32 + lane], f, acc[i]);
+      }
+      const int row = p.diff ? (j0 >> 1) : j0;
+      const float inv = safe_inverse(sum);
+      const float weight = half ? -p.lam[h * p.G + row / p.M] * inv : inv;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], weight, x[i]) : acc[i] * weight;
+      if (half == per - 1) finish_row<NB>(p, b, h * p.G + row / p.M, row % p.M, x);
+    }
+    __syncthreads();
+  }
+}
+
+// -------------------------------------------------------------------- launch
+struct Plan { int grid; bool direct; size_t ws; };
+
+template <int NB, int NT, bool SPLIT>
+int resident_blocks(int* blocks) {
+  static std::mutex mu;
+  static int cache[64] = {0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return check_cuda(e, "cudaGetDevice");
+  std::lock_guard<std::mutex> lock(mu);
+  if (dev < 0 || dev >= 64 || cache[dev] == 0) {
+    auto kern = fp4_decode_kernel<NB, NT, SPLIT>;
+    const int smem = smem_bytes<NB, NT, SPLIT>();
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return check_cuda(e, "fp4_decode shared memory");
+    int per_sm = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kThreads, smem);
+    if (e != cudaSuccess) return check_cuda(e, "fp4_decode occupancy");
+    if (per_sm < 1) return fail(IAK_ERR_UNSUPPORTED, "fp4_decode does not fit on an SM");
+    if (dev < 0 || dev >= 64) { *blocks = per_sm * device_sm_count(); return IAK_OK; }
+    cache[dev] = per_sm * device_sm_count();
+  }
+  *blocks = cache[dev];
+  return IAK_OK;
+}
+
+template <int NB, int NT, bool SPLIT>
+int make_plan(DecP& p, Plan* plan) {
+  p.CG = (p.NC + 8 * NT - 1) / (8 * NT);
+  const int64_t hc = static_cast<int64_t>(p.Ht) * p.CG, units = hc * p.B;
+  if (units * 8 * NT > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: too many rows for one launch");
+  p.HC = static_cast<int>(hc);
+  p.min_tiles = kWarps;
+  const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + kTileKeys - 1) / kTileKeys;
+  // a unit that one tile per warp covers is one block's work: no joining
+  plan->direct = most <= kWarps;
+  int blocks = 0;
+  if (int st = resident_blocks<NB, NT, SPLIT>(&blocks)) return st;
+  if (plan->direct) {
+    plan->grid = static_cast<int>(units);
+    plan->ws = 0;
+  } else {
+    const int64_t useful = (most * units + kWarps - 1) / kWarps;
+    plan->grid = static_cast<int>(std::min<int64_t>(blocks, useful));
+    plan->ws = static_cast<size_t>(plan->grid) * 2 * 8 * NT * (NB * 32 + 2) * sizeof(float);
+  }
+  p.grid = plan->grid;
+  p.direct = plan->direct ? 1 : 0;
+  return IAK_OK;
+}
+
+template <int NB, int NT, bool SPLIT>
+int run_shape(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cudaStream_t s) {
+  Plan plan;
+  if (int st = make_plan<NB, NT, SPLIT>(p, &plan)) return st;
+  if (need) *need = plan.ws;
+  if (!launch) return IAK_OK;
+  if (plan.ws > ws_bytes || (plan.ws && !ws))
+    return fail(IAK_ERR_WORKSPACE, "iak_fp4_decode needs %zu workspace bytes, got %zu", plan.ws, ws_bytes);
+  p.ws = static_cast<float*>(ws);
+  fp4_decode_kernel<NB, NT, SPLIT><<<plan.grid, kThreads, smem_bytes<NB, NT, SPLIT>(), s>>>(p);
+  if (int st = check_cuda(cudaGetLastError(), "fp4_decode launch")) return st;
+  if (plan.direct) return IAK_OK;
+  cudaLaunchConfig_t cfg = {};
+  const int rows = 8 * NT / (p.diff ? 2 : 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.B) * p.HC * rows));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  // starts while the main kernel's last blocks run; it waits for them before it reads a partial
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const DecP cp = p;
+  return check_cuda(cudaLaunchKernelEx(&cfg, fp4_join_kernel<NB, NT>, cp), "fp4_join launch");
+}
+
+// columns per block: as many n = 8 tiles as the columns need, up to what the accumulators leave registers for;
+// more columns read the cache again
+template <int NB, bool SPLIT>
+int run_cols(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cudaStream_t s) {
+  if (p.NC <= 8) return run_shape<NB, 1, SPLIT>(p, launch, ws, ws_bytes, need, s);
+  if (p.NC <= 16 || NB == 8 || SPLIT) return run_shape<NB, 2, SPLIT>(p, launch, ws, ws_bytes, need, s);
+  if constexpr (NB < 8 && !SPLIT) return run_shape<NB, 4, SPLIT>(p, launch, ws, ws_bytes, need, s);
+  return IAK_ERR_UNSUPPORTED;
+}
+
+template <int NB>
+int run_types(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cudaStream_t s) {
+  // fp32 queries: q and P as the sum of two halves
+  if (p.q_dtype == IAK_DT_F32) return run_cols<NB, true>(p, launch, ws, ws_bytes, need, s);
+  return run_cols<NB, false>(p, launch, ws, ws_bytes, need, s);
+}
+
+int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool launch, void* ws, size_t ws_bytes,
+                size_t* need, void* stream) {
+  const char* what = "iak_fp4_decode";
+  if (need) *need = 0;
+  if (!pool || !a) return fail(IAK_ERR_INVALID_ARG, "%s: null arguments", what);
+  if (int st = check_fp4_pool(pool, what)) return st;
+  if (a->batch < 0 || a->num_q_heads < 0 || a->num_table_heads < 0 || a->num_queries < 0 || a->table_width < 0)
+    return fail(IAK_ERR_INVALID_ARG, "%s: negative size", what);
+  if (a->q_dtype < IAK_DT_F32 || a->q_dtype > IAK_DT_BF16 || a->out_dtype < IAK_DT_F32 || a->out_dtype > IAK_DT_BF16)
+    return fail(IAK_ERR_INVALID_ARG, "%s: bad dtype", what);
+  if (a->num_queries > IAK_FP4_MAX_QUERIES)
+    return fail(IAK_ERR_UNSUPPORTED, "%s: %d queries, at most %d", what, a->num_queries, IAK_FP4_MAX_QUERIES);
+  if (a->batch == 0 || a->num_q_heads == 0 || a->num_queries == 0) return IAK_OK;
+  if (a->num_table_heads == 0 || a->num_q_heads % a->num_table_heads)
+    return fail(IAK_ERR_INVALID_ARG, "%s: query heads (%d) must be a multiple of table heads (%d)", what,
+                a->num_q_heads, a->num_table_heads);
+  if (!(a->sm_scale - a->sm_scale == 0.f)) return fail(IAK_ERR_INVALID_ARG, "%s: sm_scale is not finite", what);
+  if (launch) {
+    if (!a->q || !a->out || !a->lengths || (a->table_width > 0 && !a->page_table))
+      return fail(IAK_ERR_INVALID_ARG, "%s: null q, out, lengths or page_table", what);
+    if (a->differential && !a->lam) return fail(IAK_ERR_INVALID_ARG, "%s: differential attention needs lam", what);
+  }
+  DecP p = {};
+  p.pool = {static_cast<uint8_t*>(pool->k_codes), static_cast<uint8_t*>(pool->k_scales),
+            static_cast<uint8_t*>(pool->v_codes), static_cast<uint8_t*>(pool->v_scales), pool->num_pages,
+            pool->page_size, pool->head_dim};
+  p.gpp = pool->page_size / 16;
+  p.q = a->q; p.q_dtype = a->q_dtype; p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h; p.q_sm = a->q_stride_m;
+  p.out = a->out; p.out_dtype = a->out_dtype;
+  p.o_sb = a->out_stride_b; p.o_sh = a->out_stride_h; p.o_sm = a->out_stride_m;
+  p.B = a->batch; p.Hq = a->num_q_heads; p.Ht = a->num_table_heads; p.G = p.Hq / p.Ht; p.M = a->num_queries;
+  p.pt = a->page_table; p.pt_sb = a->pt_stride_b; p.pt_sh = a->pt_stride_h;
+  p.W = pool->num_pages > 0 ? a->table_width : 0;      // an empty pool holds no token
+  p.lengths = a->lengths;
+  p.scale = (a->sm_scale < 0.f ? -a->sm_scale : a->sm_scale) * 1.44269504088896340736f;
+  p.sign = a->sm_scale < 0.f ? -1.f : 1.f;
+  p.diff = a->differential ? 1 : 0;
+  p.lam = a->lam; p.norm_w = a->norm_weight; p.eps = a->eps; p.out_scale = a->out_scale;
+  const int64_t nc = static_cast<int64_t>(p.G) * p.M * (1 + p.diff);
+  if (nc > (1 << 20)) return fail(IAK_ERR_UNSUPPORTED, "%s: too many query heads", what);
+  p.NC = static_cast<int>(nc);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (static_cast<int64_t>(p.W) * p.pool.PS > kMaxTokens)
+    return fail(IAK_ERR_UNSUPPORTED, "%s: tables of more than %d tokens", what, kMaxTokens);
+  if (pool->head_dim == 64) return run_types<2>(p, launch, ws, ws_bytes, need, s);
+  if (pool->head_dim == 128) return run_types<4>(p, launch, ws, ws_bytes, need, s);
+  return run_types<8>(p, launch, ws, ws_bytes, need, s);
+}
+
+}  // namespace
+}  // namespace iak
+
+extern "C" int iak_fp4_decode_workspace_size(const iak_fp4_pool* pool, const iak_fp4_decode_args* args, size_t* bytes) {
+  if (!bytes) return iak::fail(IAK_ERR_INVALID_ARG, "iak_fp4_decode: null arguments");
+  return iak::decode_call(pool, args, false, nullptr, 0, bytes, nullptr);
+}
+
+extern "C" int iak_fp4_decode(const iak_fp4_pool* pool, const iak_fp4_decode_args* args, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  return iak::decode_call(pool, args, true, workspace, workspace_bytes, nullptr, stream);
+}

@@ -1,0 +1,530 @@
+// Page operations of a paged cache: grow (allocate, copy-on-write), fork, free, compact.
+//
+// A page is free when no table entry holds it (refs 0), so freeing only counts down and needs no order, and the pages
+// to hand out are the lowest free ones: the k-th free page goes to the k-th page wanted, whatever order blocks run in.
+// Finding them reads refs once, 4 bytes a page; one cluster of 8 blocks does it, each with an eighth of the pages,
+// the eighths' counts exchanged through distributed shared memory.  What follows (page copies, table entries) is a
+// second kernel over all SMs; copies move 2 * page bytes at 16 bytes a lane, which bounds a compaction.  Small calls
+// are bound by their launches.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "iak_internal.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace iak {
+namespace {
+
+constexpr int kCluster = 8;
+constexpr int kPlanThreads = 1024;
+constexpr int kActThreads = 256;
+constexpr int kListThreads = 512;
+
+struct Seq {
+  int32_t* refs; int num_pages;
+  int32_t* table; int64_t sb, sh; int W;
+  int32_t* lengths;
+  int S, Ht, PS;
+};
+struct Planes {
+  char* base[IAK_MAX_PLANES]; int64_t bytes[IAK_MAX_PLANES]; uint32_t formats[IAK_MAX_PLANES];
+  int num;
+  void* tags; int tag_bytes; uint8_t tag_map[16]; uint8_t tag_default;
+};
+
+__device__ __forceinline__ int pages_of(int tokens, int PS) {
+  return tokens <= 0 ? 0 : (tokens - 1) / PS + 1;      // no sum that could pass 2^31
+}
+// pages a slot holds: never more than its table has entries
+__device__ __forceinline__ int held_pages(const Seq& q, int s) { return min(pages_of(q.lengths[s], q.PS), q.W); }
+__device__ __forceinline__ bool in_pool(const Seq& q, int id) { return id >= 0 && id < q.num_pages; }
+
+// sum over the block's threads before this one; *all = the block's sum
+__device__ __forceinline__ int block_before(int v, int* all) {
+  __shared__ int warp_sum[kPlanThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(~0u, inc, o);
+    if (lane >= o) inc += x;
+  }
+  __syncthreads();                                     // an earlier call's readers are done
+  if (lane == 31) warp_sum[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    int x = lane < warps ? warp_sum[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(~0u, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane < warps) warp_sum[lane] = x;
+  }
+  __syncthreads();
+  *all = warp_sum[warps - 1];
+  return inc - v + (warp ? warp_sum[warp - 1] : 0);
+}
+
+// copy page `from` to page `to` by one warp: the planes of the page's format, and its tag
+__device__ __forceinline__ void copy_page(const Planes& pl, int64_t from, int64_t to) {
+  const int lane = threadIdx.x & 31;
+  uint32_t mask = ~0u;
+  if (pl.tags) {
+    const int tag = pl.tag_bytes == 1 ? static_cast<int>(static_cast<const uint8_t*>(pl.tags)[from])
+                                      : static_cast<const int32_t*>(pl.tags)[from];
+    mask = 1u << ((tag >= 0 && tag < 16) ? pl.tag_map[tag] : pl.tag_default);
+    __syncwarp();
+    if (lane == 0) {
+      if (pl.tag_bytes == 1) static_cast<uint8_t*>(pl.tags)[to] = static_cast<uint8_t>(tag);
+      else static_cast<int32_t*>(pl.tags)[to] = tag;
+    }
+  }
+  for (int i = 0; i < pl.num; ++i) {
+    if (pl.tags && !(pl.formats[i] & mask)) continue;
+    const int64_t n = pl.bytes[i];
+    const char* src = pl.base[i] + from * n;
+    char* dst = pl.base[i] + to * n;
+    const uintptr_t low = reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(n);
+    if ((low & 15) == 0) {
+      const uint4* s = reinterpret_cast<const uint4*>(src);
+      uint4* d = reinterpret_cast<uint4*>(dst);
+      const int64_t m = n / 16;
+      int64_t at = lane;
+      for (; at + 7 * 32 < m; at += 8 * 32) {
+        uint4 r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = __ldcs(s + at + j * 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) __stcs(d + at + j * 32, r[j]);
+      }
+      for (; at < m; at += 32) d[at] = s[at];
+    } else if ((low & 3) == 0) {
+      for (int64_t at = lane; at < n / 4; at += 32)
+        reinterpret_cast<uint32_t*>(dst)[at] = reinterpret_cast<const uint32_t*>(src)[at];
+    } else {
+      for (int64_t at = lane; at < n; at += 32) dst[at] = src[at];
+    }
+  }
+}
+
+// the slice of the pages that block `rank` of the cluster scans, whole runs of a block's threads
+__device__ __forceinline__ void slice_of(int pages, int rank, int* begin, int* end) {
+  const int64_t per = ((static_cast<int64_t>(pages) + kCluster - 1) / kCluster + kPlanThreads - 1) / kPlanThreads * kPlanThreads;
+  *begin = static_cast<int>(min(static_cast<int64_t>(pages), per * rank));
+  *end = static_cast<int>(min(static_cast<int64_t>(pages), per * (rank + 1)));
+}
+
+// pages in use in [begin, end)
+__device__ __forceinline__ int count_live(const int32_t* refs, int begin, int end) {
+  int live = 0;
+  for (int p = begin + threadIdx.x; p < end; p += kPlanThreads) live += refs[p] > 0;
+  int all;
+  block_before(live, &all);
+  return all;
+}
+
+// ------------------------------------------------------------------------ grow
+// Scratch: first[S * Ht] = rank of the (slot, head)'s first new page, < 0 = gets none; shared[S * Ht] (copy the open
+// page); old_pages[S], fresh[S]; new_ids[rank].
+struct GrowScratch { int32_t* first; int32_t* shared; int32_t* old_pages; int32_t* fresh; int32_t* new_ids; };
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPlanThreads)
+grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const GrowScratch w) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank());
+  __shared__ int live_here, wanted;
+  int begin, end;
+  slice_of(q.num_pages, rank, &begin, &end);
+  const int live = count_live(q.refs, begin, end);
+  if (threadIdx.x == 0) live_here = live;
+  cluster.sync();
+  int free_before = 0, free_all = 0;                   // free pages below this slice, in all
+  for (int r = 0; r < kCluster; ++r) {
+    int bb, be;
+    slice_of(q.num_pages, r, &bb, &be);
+    const int f = be - bb - *cluster.map_shared_rank(&live_here, r);
+    if (r < rank) free_before += f;
+    free_all += f;
+  }
+  if (rank == 0) {
+    // ranks of the pages wanted, in order of (slot, head); one thread per (slot, head)
+    __shared__ int cut;                                // first slot that the free pages do not reach
+    if (threadIdx.x == 0) cut = q.S;
+    int64_t base = 0;
+    const int64_t n = static_cast<int64_t>(q.S) * q.Ht;
+    int refused = 0;
+    for (int64_t i0 = 0; i0 < n; i0 += kPlanThreads) {
+      const int64_t i = i0 + threadIdx.x;
+      int need = 0;
+      if (i < n) {
+        const int s = static_cast<int>(i / q.Ht), h = static_cast<int>(i - static_cast<int64_t>(s) * q.Ht);
+        const int len = max(q.lengths[s], 0), add = more[s];
+        const int64_t total = static_cast<int64_t>(len) + add;
+        bool ok = add > 0 && total <= static_cast<int64_t>(q.W) * q.PS && total <= 0x7fffffff;
+        const int old = ok ? pages_of(len, q.PS) : 0;
+        const bool open = ok && len % q.PS != 0;
+        bool copy = false;
+        if (open) {
+          // an open page outside the pool refuses the slot, for all of its heads
+          for (int k = 0; k < q.Ht; ++k) ok = ok && in_pool(q, q.table[s * q.sb + k * q.sh + old - 1]);
+          copy = ok && q.refs[q.table[s * q.sb + h * q.sh + old - 1]] > 1;
+        }
+        const int fresh = ok ? pages_of(static_cast<int>(total), q.PS) - old : 0;
+        need = fresh + (copy ? 1 : 0);
+        w.shared[i] = copy;
+        if (h == 0) {
+          w.old_pages[s] = old;
+          w.fresh[s] = fresh;
+          if (add != 0 && !ok) ++refused;
+        }
+        w.first[i] = ok ? 0 : -1;
+      }
+      int all;
+      const int before = block_before(need, &all);
+      if (i < n) {
+        const int64_t at = base + before;
+        const int s = static_cast<int>(i / q.Ht);
+        if (w.first[i] == 0) {
+          if (at + need > free_all) atomicMin(&cut, s);
+          w.first[i] = static_cast<int32_t>(min(at, static_cast<int64_t>(0x7fffffff)));
+        }
+      }
+      base += all;
+    }
+    __syncthreads();
+    // a slot that does not fit, and every later one that gets tokens, stays as it is
+    const int last = cut;
+    int64_t take = 0;
+    for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
+      const int s = static_cast<int>(i / q.Ht), h = static_cast<int>(i - static_cast<int64_t>(s) * q.Ht);
+      if (w.first[i] < 0) continue;
+      if (s >= last) {
+        w.first[i] = -1;
+        if (h == 0) ++refused;
+      } else {
+        take = max(take, static_cast<int64_t>(w.first[i]) + w.fresh[s] + w.shared[i]);
+        if (h == 0) q.lengths[s] = max(q.lengths[s], 0) + more[s];
+      }
+    }
+    if (threadIdx.x == 0) wanted = 0;
+    __syncthreads();
+    atomicMax(&wanted, static_cast<int>(take));
+    if (rejected && refused) atomicAdd(rejected, refused);
+  }
+  cluster.sync();
+  const int want = *cluster.map_shared_rank(&wanted, 0);
+  // the free pages of this slice, in ascending order
+  int at = free_before;
+  for (int p0 = begin; p0 < end && at < want; p0 += kPlanThreads) {
+    const int p = p0 + threadIdx.x;
+    const int is_free = p < end && q.refs[p] <= 0;
+    int all;
+    const int before = block_before(is_free, &all);
+    if (is_free && at + before < want) w.new_ids[at + before] = p;
+    at += all;
+  }
+  cluster.sync();                                      // no block leaves while another may read its counts
+}
+
+__global__ void __launch_bounds__(kActThreads) grow_act_kernel(const Seq q, const Planes pl, const GrowScratch w) {
+  const int warps = kActThreads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t n = static_cast<int64_t>(q.S) * q.Ht;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * warps + warp; i < n; i += static_cast<int64_t>(gridDim.x) * warps) {
+    const int first = w.first[i];
+    if (first < 0) continue;
+    const int s = static_cast<int>(i / q.Ht), h = static_cast<int>(i - static_cast<int64_t>(s) * q.Ht);
+    int32_t* row = q.table + s * q.sb + h * q.sh;
+    const int old = w.old_pages[s], fresh = w.fresh[s], copy = w.shared[i];
+    if (copy) {
+      const int from = row[old - 1], to = w.new_ids[first];
+      copy_page(pl, from, to);
+      __syncwarp();
+      if (lane == 0) {
+        row[old - 1] = to;
+        q.refs[to] = 1;
+        atomicSub(&q.refs[from], 1);
+      }
+    }
+    for (int k = lane; k < fresh; k += 32) {
+      const int id = w.new_ids[first + copy + k];
+      row[old + k] = id;
+      q.refs[id] = 1;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ fork, free
+// A cluster per listed item: all its blocks read the slot's length before one of them writes it.
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kListThreads)
+fork_kernel(const Seq q, const int32_t* src, const int32_t* dst, int n, int32_t* rejected) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int i = blockIdx.x / kCluster, rank = static_cast<int>(cluster.block_rank());
+  const int from = src[i], to = dst[i];
+  bool bad = from < 0 || from >= q.S || to < 0 || to >= q.S;
+  if (!bad) bad = q.lengths[to] > 0;
+  for (int j = threadIdx.x; j < n; j += kListThreads) bad = bad || dst[j] == from || (j < i && dst[j] == to);
+  bad = __syncthreads_or(bad);
+  const int held = bad ? 0 : held_pages(q, from);
+  const int len = bad ? 0 : q.lengths[from];
+  cluster.sync();
+  if (bad) {
+    if (rejected && rank == 0 && threadIdx.x == 0) atomicAdd(rejected, 1);
+    return;
+  }
+  const int64_t entries = static_cast<int64_t>(q.Ht) * held;
+  for (int64_t e = rank * kListThreads + threadIdx.x; e < entries; e += kCluster * kListThreads) {
+    const int h = static_cast<int>(e / held), w = static_cast<int>(e - static_cast<int64_t>(h) * held);
+    const int id = q.table[from * q.sb + h * q.sh + w];
+    q.table[to * q.sb + h * q.sh + w] = id;
+    if (in_pool(q, id)) atomicAdd(&q.refs[id], 1);
+  }
+  if (rank == 0 && threadIdx.x == 0) q.lengths[to] = len;
+}
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kListThreads)
+free_kernel(const Seq q, const int32_t* slots, int n, int32_t* rejected) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int i = blockIdx.x / kCluster, rank = static_cast<int>(cluster.block_rank());
+  const int s = slots[i];
+  const bool bad = s < 0 || s >= q.S;
+  bool again = false;
+  for (int j = threadIdx.x; j < i; j += kListThreads) again = again || slots[j] == s;
+  again = __syncthreads_or(again);
+  const int held = bad || again ? 0 : held_pages(q, s);
+  cluster.sync();
+  if (bad) {
+    if (rejected && rank == 0 && threadIdx.x == 0) atomicAdd(rejected, 1);
+    return;
+  }
+  if (again) return;
+  const int64_t entries = static_cast<int64_t>(q.Ht) * held;
+  for (int64_t e = rank * kListThreads + threadIdx.x; e < entries; e += kCluster * kListThreads) {
+    const int h = static_cast<int>(e / held), w = static_cast<int>(e - static_cast<int64_t>(h) * held);
+    int32_t* at = q.table + s * q.sb + h * q.sh + w;
+    const int id = *at;
+    *at = -1;
+    if (in_pool(q, id)) atomicSub(&q.refs[id], 1);
+  }
+  if (rank == 0 && threadIdx.x == 0) q.lengths[s] = 0;
+}
+
+// --------------------------------------------------------------------- compact
+// Scratch: head[0] = pages in use n, head[1] = pages to move; from[k] and to[k] of move k; rank_of[page] of the pages
+// that move.
+struct CompactScratch { int32_t* head; int32_t* from; int32_t* to; int32_t* rank_of; };
+
+__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPlanThreads)
+compact_plan_kernel(const Seq q, int32_t* num_live, const CompactScratch w) {
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank());
+  __shared__ int live_here, live_below_n;              // live pages of the slice; of the slice and below n
+  int begin, end;
+  slice_of(q.num_pages, rank, &begin, &end);
+  const int live = count_live(q.refs, begin, end);
+  if (threadIdx.x == 0) live_here = live;
+  cluster.sync();
+  int live_before = 0, n = 0;
+  for (int r = 0; r < kCluster; ++r) {
+    const int x = *cluster.map_shared_rank(&live_here, r);
+    if (r < rank) live_before += x;
+    n += x;
+  }
+  const int below = count_live(q.refs, begin, min(end, max(n, begin)));
+  if (threadIdx.x == 0) live_below_n = below;
+  cluster.sync();
+  int stay = 0;                                        // live pages below n: they keep their place
+  for (int r = 0; r < kCluster; ++r) stay += *cluster.map_shared_rank(&live_below_n, r);
+  if (rank == 0 && threadIdx.x == 0) {
+    w.head[0] = n;
+    w.head[1] = n - stay;
+    if (num_live) *num_live = n;
+  }
+  int at = live_before;                                // live pages before p
+  for (int p0 = begin; p0 < end; p0 += kPlanThreads) {
+    const int p = p0 + threadIdx.x;
+    const int is_live = p < end && q.refs[p] > 0;
+    int all;
+    const int before = at + block_before(is_live, &all);
+    if (p < end) {
+      if (p < n && !is_live) w.to[p - before] = p;
+      if (p >= n && is_live) {
+        w.from[before - stay] = p;
+        w.rank_of[p] = before - stay;
+      }
+    }
+    at += all;
+  }
+  cluster.sync();
+}
+
+__global__ void __launch_bounds__(kActThreads) compact_act_kernel(const Seq q, const Planes pl, const CompactScratch w) {
+  const int n = w.head[0], moves = w.head[1];
+  if (moves == 0) return;
+  const int warps = kActThreads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int k = blockIdx.x * warps + warp; k < moves; k += gridDim.x * warps) {
+    const int from = w.from[k], to = w.to[k];
+    copy_page(pl, from, to);
+    if (lane == 0) {
+      q.refs[to] = q.refs[from];
+      q.refs[from] = 0;
+    }
+  }
+  // table entries of moved pages; rank_of holds anything for other pages, so the move has to agree
+  const int64_t rows = static_cast<int64_t>(q.S) * q.Ht;
+  for (int64_t r = static_cast<int64_t>(blockIdx.x) * warps + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * warps) {
+    const int s = static_cast<int>(r / q.Ht), h = static_cast<int>(r - static_cast<int64_t>(s) * q.Ht);
+    int32_t* row = q.table + s * q.sb + h * q.sh;
+    const int held = held_pages(q, s);
+    for (int e = lane; e < held; e += 32) {
+      const int id = row[e];
+      if (!in_pool(q, id) || id < n) continue;
+      const int k = w.rank_of[id];
+      if (k >= 0 && k < moves && w.from[k] == id) row[e] = w.to[k];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------ host
+int check_seq(const iak_seq_pages* a, const char* what, Seq* q) {
+  if (!a) return fail(IAK_ERR_INVALID_ARG, "%s: null arguments", what);
+  if (a->num_pages < 0 || a->num_pages > 0x7fffffffLL || a->num_slots < 0 || a->num_table_heads < 0 || a->table_width < 0)
+    return fail(IAK_ERR_INVALID_ARG, "%s: bad size", what);
+  if (a->page_size <= 0) return fail(IAK_ERR_INVALID_ARG, "%s: page_size must be positive", what);
+  const bool entries = a->num_slots > 0 && a->num_table_heads > 0 && a->table_width > 0;
+  if ((a->num_slots > 0 && !a->lengths) || (a->num_pages > 0 && !a->refs) || (entries && !a->page_table))
+    return fail(IAK_ERR_INVALID_ARG, "%s: null refs, page_table or lengths", what);
+  *q = {a->refs, static_cast<int>(a->num_pages), a->page_table, a->pt_stride_s, a->pt_stride_h, a->table_width,
+        a->lengths, a->num_slots, a->num_table_heads, a->page_size};
+  return IAK_OK;
+}
+
+int check_planes(const iak_page_planes* a, const char* what, Planes* p) {
+  *p = {};
+  if (!a) return fail(IAK_ERR_INVALID_ARG, "%s: null planes", what);
+  if (a->num_planes < 0 || a->num_planes > IAK_MAX_PLANES) return fail(IAK_ERR_INVALID_ARG, "%s: bad num_planes", what);
+  for (int i = 0; i < a->num_planes; ++i) {
+    if (!a->base[i] || a->bytes[i] <= 0) return fail(IAK_ERR_INVALID_ARG, "%s: empty plane %d", what, i);
+    p->base[i] = static_cast<char*>(a->base[i]);
+    p->bytes[i] = a->bytes[i];
+    p->formats[i] = a->formats[i];
+  }
+  p->num = a->num_planes;
+  p->tags = a->page_tags;
+  if (a->page_tags && a->tag_bytes != 1 && a->tag_bytes != 4)
+    return fail(IAK_ERR_INVALID_ARG, "%s: tag_bytes must be 1 or 4", what);
+  p->tag_bytes = a->tag_bytes;
+  for (int i = 0; i < 16; ++i) {
+    if (a->page_tags && a->tag_map[i] >= 32) return fail(IAK_ERR_INVALID_ARG, "%s: bad tag_map", what);
+    p->tag_map[i] = a->tag_map[i];
+  }
+  if (a->page_tags && a->tag_default >= 32) return fail(IAK_ERR_INVALID_ARG, "%s: bad tag_default", what);
+  p->tag_default = a->tag_default;
+  return IAK_OK;
+}
+
+// int32 words of scratch: the larger of what grow and compact use
+size_t scratch_words(const iak_seq_pages* a) {
+  const size_t rows = static_cast<size_t>(a->num_slots) * a->num_table_heads;
+  const size_t grow = 2 * rows + 2 * static_cast<size_t>(a->num_slots) + static_cast<size_t>(a->num_pages);
+  const size_t compact = 2 + 3 * static_cast<size_t>(a->num_pages);
+  return std::max(grow, compact);
+}
+
+int check_ws(const iak_seq_pages* a, void* ws, size_t bytes, const char* what) {
+  const size_t need = scratch_words(a) * 4;
+  if (bytes < need || !ws) return fail(IAK_ERR_WORKSPACE, "%s needs %zu workspace bytes, got %zu", what, need, bytes);
+  if (reinterpret_cast<uintptr_t>(ws) % 4) return fail(IAK_ERR_INVALID_ARG, "%s: workspace not aligned", what);
+  return IAK_OK;
+}
+
+int launch_list_ok(int32_t count, const char* what) {
+  if (count < 0) return fail(IAK_ERR_INVALID_ARG, "%s: negative count", what);
+  if (count > 0x7fffffff / kCluster) return fail(IAK_ERR_UNSUPPORTED, "%s: too many slots", what);
+  return IAK_OK;
+}
+
+}  // namespace
+}  // namespace iak
+
+using namespace iak;
+
+extern "C" int iak_pages_workspace_size(const iak_seq_pages* pages, size_t* bytes) {
+  Seq q;
+  if (!bytes) return fail(IAK_ERR_INVALID_ARG, "iak_pages_workspace_size: null arguments");
+  *bytes = 0;
+  if (int st = check_seq(pages, "iak_pages_workspace_size", &q)) return st;
+  *bytes = scratch_words(pages) * 4;
+  return IAK_OK;
+}
+
+extern "C" int iak_pages_grow(const iak_seq_pages* pages, const iak_page_planes* planes, const int32_t* new_tokens,
+                              int32_t* rejected, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "iak_pages_grow";
+  Seq q;
+  Planes pl;
+  if (int st = check_seq(pages, what, &q)) return st;
+  if (int st = check_planes(planes, what, &pl)) return st;
+  if (q.S == 0 || q.Ht == 0) return IAK_OK;
+  if (!new_tokens) return fail(IAK_ERR_INVALID_ARG, "%s: null new_tokens", what);
+  if (int st = check_ws(pages, workspace, workspace_bytes, what)) return st;
+  const int64_t rows = static_cast<int64_t>(q.S) * q.Ht;
+  GrowScratch w;
+  w.first = static_cast<int32_t*>(workspace);
+  w.shared = w.first + rows;
+  w.old_pages = w.shared + rows;
+  w.fresh = w.old_pages + q.S;
+  w.new_ids = w.fresh + q.S;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  grow_plan_kernel<<<kCluster, kPlanThreads, 0, s>>>(q, new_tokens, rejected, w);
+  if (int st = check_cuda(cudaGetLastError(), "grow plan launch")) return st;
+  const int64_t blocks = std::min<int64_t>((rows + kActThreads / 32 - 1) / (kActThreads / 32), 8 * device_sm_count());
+  grow_act_kernel<<<static_cast<unsigned>(blocks), kActThreads, 0, s>>>(q, pl, w);
+  return check_cuda(cudaGetLastError(), "grow launch");
+}
+
+extern "C" int iak_pages_fork(const iak_seq_pages* pages, const int32_t* src, const int32_t* dst, int32_t count,
+                              int32_t* rejected, void* stream) {
+  const char* what = "iak_pages_fork";
+  Seq q;
+  if (int st = check_seq(pages, what, &q)) return st;
+  if (int st = launch_list_ok(count, what)) return st;
+  if (count == 0) return IAK_OK;
+  if (!src || !dst) return fail(IAK_ERR_INVALID_ARG, "%s: null src or dst", what);
+  fork_kernel<<<count * kCluster, kListThreads, 0, static_cast<cudaStream_t>(stream)>>>(q, src, dst, count, rejected);
+  return check_cuda(cudaGetLastError(), "fork launch");
+}
+
+extern "C" int iak_pages_free(const iak_seq_pages* pages, const int32_t* slots, int32_t count, int32_t* rejected,
+                              void* stream) {
+  const char* what = "iak_pages_free";
+  Seq q;
+  if (int st = check_seq(pages, what, &q)) return st;
+  if (int st = launch_list_ok(count, what)) return st;
+  if (count == 0) return IAK_OK;
+  if (!slots) return fail(IAK_ERR_INVALID_ARG, "%s: null slots", what);
+  free_kernel<<<count * kCluster, kListThreads, 0, static_cast<cudaStream_t>(stream)>>>(q, slots, count, rejected);
+  return check_cuda(cudaGetLastError(), "free launch");
+}
+
+extern "C" int iak_pages_compact(const iak_seq_pages* pages, const iak_page_planes* planes, int32_t* num_live,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "iak_pages_compact";
+  Seq q;
+  Planes pl;
+  if (int st = check_seq(pages, what, &q)) return st;
+  if (int st = check_planes(planes, what, &pl)) return st;
+  if (int st = check_ws(pages, workspace, workspace_bytes, what)) return st;
+  CompactScratch w;
+  w.head = static_cast<int32_t*>(workspace);
+  w.from = w.head + 2;
+  w.to = w.from + q.num_pages;
+  w.rank_of = w.to + q.num_pages;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  compact_plan_kernel<<<kCluster, kPlanThreads, 0, s>>>(q, num_live, w);
+  if (int st = check_cuda(cudaGetLastError(), "compact plan launch")) return st;
+  compact_act_kernel<<<8 * device_sm_count(), kActThreads, 0, s>>>(q, pl, w);
+  return check_cuda(cudaGetLastError(), "compact launch");
+}

@@ -5,7 +5,8 @@ Exports the reference's hot-path surface (layout types, precision policy,
 router + kernel metadata, the fused / six-tag / adaptive decode entry points
 and their helpers) backed by libiak_b200.so, plus the B200 extensions
 (``PagePool`` quantise-on-write pools, device metadata packing, split-KV
-partial export / merge).  As in the reference package, the name
+partial export / merge, the ``Fp4Pool`` cache with its plain and differential
+attention, and the page operations of ``SequencePages``).  As in the reference package, the name
 ``fused_selected_quant_decode`` refers to the function (the submodule is
 still importable with ``from intent_attention.fused_selected_quant_decode import ...``).
 """
@@ -43,6 +44,8 @@ from .triton_adaptive_format_attention import (
     make_adaptive_page_tables,
 )
 from .paged import KVStage, PagePool, append_tokens, convert_pages, merge_partials, pack_metadata, paged_decode
+from .fp4_cache import Fp4Pool, append_fp4, differential_decode_fp4, paged_decode_fp4, read_fp4
+from .sequence_pages import SequencePages, compact_pages, fork_sequences, free_sequences, grow_sequences
 from .device_router import LayoutBatch, RoutedPages, encode_layouts, route_layouts, route_pages
 from .split_kv import (
     SequenceShardedDecoder,
@@ -64,6 +67,8 @@ __all__ = [
     "AdaptiveFormatKernelConfig", "AdaptivePageFormat", "adaptive_format_decode_attention_triton",
     "make_adaptive_page_tables",
     "PagePool", "merge_partials", "pack_metadata", "paged_decode", "KVStage", "append_tokens", "convert_pages",
+    "Fp4Pool", "append_fp4", "read_fp4", "paged_decode_fp4", "differential_decode_fp4",
+    "SequencePages", "grow_sequences", "fork_sequences", "free_sequences", "compact_pages",
     "LayoutBatch", "RoutedPages", "encode_layouts", "route_layouts", "route_pages",
     "SequenceShardedDecoder", "decode_partial_block", "merge_partial_blocks", "shard_bounds", "shard_page_lists",
 ]

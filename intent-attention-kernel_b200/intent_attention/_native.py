@@ -164,6 +164,57 @@ class PeerExchange(ctypes.Structure):
                 ("head_dim", c_i32)]
 
 
+FP4_MAX_QUERIES = 16
+
+
+class Fp4PoolStruct(ctypes.Structure):
+    _fields_ = [("k_codes", c_void_p), ("k_scales", c_void_p), ("v_codes", c_void_p), ("v_scales", c_void_p),
+                ("num_pages", c_i64), ("page_size", c_i32), ("head_dim", c_i32)]
+
+
+class Fp4RowsArgs(ctypes.Structure):
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("dtype", c_i32),
+        ("k_stride_b", c_i64), ("k_stride_h", c_i64), ("k_stride_n", c_i64),
+        ("v_stride_b", c_i64), ("v_stride_h", c_i64), ("v_stride_n", c_i64),
+        ("batch", c_i32), ("num_table_heads", c_i32), ("num_rows", c_i32),
+        ("page_table", c_void_p), ("pt_stride_b", c_i64), ("pt_stride_h", c_i64), ("table_width", c_i32),
+        ("positions", c_void_p), ("counts", c_void_p), ("dropped", c_void_p),
+    ]
+
+
+class Fp4DecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_dtype", c_i32), ("q_stride_b", c_i64), ("q_stride_h", c_i64), ("q_stride_m", c_i64),
+        ("out", c_void_p), ("out_dtype", c_i32), ("out_stride_b", c_i64), ("out_stride_h", c_i64),
+        ("out_stride_m", c_i64),
+        ("batch", c_i32), ("num_q_heads", c_i32), ("num_table_heads", c_i32), ("num_queries", c_i32),
+        ("page_table", c_void_p), ("pt_stride_b", c_i64), ("pt_stride_h", c_i64), ("table_width", c_i32),
+        ("lengths", c_void_p), ("sm_scale", ctypes.c_float),
+        ("differential", c_i32), ("lam", c_void_p), ("norm_weight", c_void_p),
+        ("eps", ctypes.c_float), ("out_scale", ctypes.c_float),
+    ]
+
+
+MAX_PLANES = 16
+
+
+class SeqPages(ctypes.Structure):
+    _fields_ = [
+        ("refs", c_void_p), ("num_pages", c_i64),
+        ("page_table", c_void_p), ("pt_stride_s", c_i64), ("pt_stride_h", c_i64), ("table_width", c_i32),
+        ("lengths", c_void_p), ("num_slots", c_i32), ("num_table_heads", c_i32), ("page_size", c_i32),
+    ]
+
+
+class PagePlanes(ctypes.Structure):
+    _fields_ = [
+        ("base", c_void_p * MAX_PLANES), ("bytes", c_i64 * MAX_PLANES), ("formats", ctypes.c_uint32 * MAX_PLANES),
+        ("num_planes", c_i32),
+        ("page_tags", c_void_p), ("tag_bytes", c_i32), ("tag_map", ctypes.c_uint8 * 16), ("tag_default", ctypes.c_uint8),
+    ]
+
+
 # name -> (restype, argtypes); mirrors every declaration of the public header
 SIGNATURES = {
     "iak_version": (ctypes.c_int, []),
@@ -181,6 +232,19 @@ SIGNATURES = {
     "iak_append_tokens": (ctypes.c_int, [ctypes.POINTER(PagePools), ctypes.POINTER(AppendArgs), c_void_p]),
     "iak_convert_pages": (ctypes.c_int, [ctypes.POINTER(PagePools), ctypes.POINTER(ConvertArgs), c_void_p]),
     "iak_prefill": (ctypes.c_int, [ctypes.POINTER(PagePools), ctypes.POINTER(PrefillArgs), c_void_p]),
+    "iak_fp4_append": (ctypes.c_int, [ctypes.POINTER(Fp4PoolStruct), ctypes.POINTER(Fp4RowsArgs), c_void_p]),
+    "iak_fp4_read": (ctypes.c_int, [ctypes.POINTER(Fp4PoolStruct), ctypes.POINTER(Fp4RowsArgs), c_void_p]),
+    "iak_fp4_decode_workspace_size": (ctypes.c_int, [ctypes.POINTER(Fp4PoolStruct), ctypes.POINTER(Fp4DecodeArgs),
+                                                     ctypes.POINTER(ctypes.c_size_t)]),
+    "iak_fp4_decode": (ctypes.c_int, [ctypes.POINTER(Fp4PoolStruct), ctypes.POINTER(Fp4DecodeArgs), c_void_p,
+                                      ctypes.c_size_t, c_void_p]),
+    "iak_pages_workspace_size": (ctypes.c_int, [ctypes.POINTER(SeqPages), ctypes.POINTER(ctypes.c_size_t)]),
+    "iak_pages_grow": (ctypes.c_int, [ctypes.POINTER(SeqPages), ctypes.POINTER(PagePlanes), c_void_p, c_void_p,
+                                      c_void_p, ctypes.c_size_t, c_void_p]),
+    "iak_pages_fork": (ctypes.c_int, [ctypes.POINTER(SeqPages), c_void_p, c_void_p, c_i32, c_void_p, c_void_p]),
+    "iak_pages_free": (ctypes.c_int, [ctypes.POINTER(SeqPages), c_void_p, c_i32, c_void_p, c_void_p]),
+    "iak_pages_compact": (ctypes.c_int, [ctypes.POINTER(SeqPages), ctypes.POINTER(PagePlanes), c_void_p, c_void_p,
+                                         ctypes.c_size_t, c_void_p]),
     "iak_quantize_pages": (ctypes.c_int, [ctypes.POINTER(QuantArgs), c_void_p]),
     "iak_decode_noalloc": (ctypes.c_int, [ctypes.POINTER(PagePools), ctypes.POINTER(DecodeArgs), c_void_p]),
     "iak_decode_exchange": (ctypes.c_int, [ctypes.POINTER(PagePools), ctypes.POINTER(DecodeArgs),

@@ -1,0 +1,288 @@
+"""GPU page operations (grow, fork, free, compact) against the sequential oracle, exact; and a serving run of them
+with append and attention."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import fp4 as of
+
+pytestmark = pytest.mark.gpu
+
+
+def _ia():
+    import intent_attention
+    return intent_attention
+
+
+def _i32(x):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+
+
+def _state(seed, P, PS, S, Ht, W, lengths, share=0.2, D=64):
+    """A pool of fp16 pages and slots that hold random pages, some of them shared."""
+    ia = _ia()
+    g = np.random.default_rng(seed)
+    refs = np.zeros(P, np.int32)
+    table = np.full((S, Ht, W), -1, np.int32)
+    order = list(g.permutation(P))
+    given = []
+    for s in range(S):
+        for h in range(Ht):
+            for w in range(-(-lengths[s] // PS)):
+                if given and g.random() < share:
+                    p = given[g.integers(len(given))]
+                else:
+                    p = order.pop()
+                    given.append(p)
+                table[s, h, w] = p
+                refs[p] += 1
+    k, v = (g.standard_normal((P, PS, D)).astype(np.float16) for _ in range(2))
+    pool = ia.PagePool(P, PS, D, k_f16=torch.from_numpy(k).cuda(), v_f16=torch.from_numpy(v).cuda())
+    pages = ia.SequencePages(_i32(refs), _i32(table), _i32(lengths), PS)
+    return pool, pages, of.Pages(refs, table, np.asarray(lengths, np.int32), PS, (k, v))
+
+
+def _same(pool, pages, want, data=True):
+    np.testing.assert_array_equal(pages.lengths.cpu().numpy(), want.lengths)
+    np.testing.assert_array_equal(pages.table.cpu().numpy(), want.table)
+    np.testing.assert_array_equal(pages.refs.cpu().numpy(), want.refs)
+    if data:
+        np.testing.assert_array_equal(pool.k_f16.cpu().numpy(), want.planes[0])
+        np.testing.assert_array_equal(pool.v_f16.cpu().numpy(), want.planes[1])
+
+
+def _counter():
+    return torch.zeros(1, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("P,PS,S,Ht,W", [(64, 16, 4, 1, 6), (5000, 16, 33, 4, 9), (20000, 8, 64, 8, 12),
+                                         (9001, 3, 700, 2, 5), (1, 16, 1, 1, 1)])
+def test_grow(P, PS, S, Ht, W):
+    g = np.random.default_rng(P)
+    lengths = g.integers(0, W * PS // 2 + 1, S).tolist() if P > 1 else [0]
+    pool, pages, want = _state(P, P, PS, S, Ht, W, lengths)
+    more = g.integers(0, W * PS // 2 + 1, S)
+    more[g.random(S) < 0.3] = 0
+    more[-1] = 1
+    if S > 3:
+        more[1], more[2] = -4, W * PS + 1
+    r = _counter()
+    _ia().grow_sequences(pool, pages, _i32(more), rejected=r)
+    want.grow(more)
+    _same(pool, pages, want)
+    assert int(r) == want.rejected
+
+
+def test_grow_runs_out():
+    """Everything up to the first slot that does not fit; later ones stay, those without tokens too."""
+    pool, pages, want = _state(3, 40, 16, 6, 2, 8, [17, 5, 0, 40, 16, 3], share=0.5)
+    more = [16, 30, 60, 16, 1, 0]
+    r = _counter()
+    _ia().grow_sequences(pool, pages, _i32(more), rejected=r)
+    want.grow(more)
+    _same(pool, pages, want)
+    assert int(r) == want.rejected
+    more = [100, 1, 90, 1, 100, 13]
+    _ia().grow_sequences(pool, pages, _i32(more), rejected=r)
+    want.grow(more)
+    _same(pool, pages, want)
+    assert int(r) == want.rejected > 0
+
+
+def test_grow_refuses_a_missing_open_page():
+    pool, pages, want = _state(5, 64, 16, 3, 2, 4, [20, 16, 5], share=0.0)
+    for t in (pages.table, ):
+        t[0, 1, 1] = -1
+    want.table[0, 1, 1] = -1
+    r = _counter()
+    _ia().grow_sequences(pool, pages, _i32([1, 1, 1]), rejected=r)
+    want.grow([1, 1, 1])
+    _same(pool, pages, want)
+    assert int(r) == want.rejected == 1
+
+
+@pytest.mark.parametrize("S,Ht,W", [(8, 1, 3), (24, 8, 40), (64, 3, 300)])
+def test_fork_and_free(S, Ht, W):
+    g = np.random.default_rng(S)
+    PS = 16
+    lengths = [int(g.integers(0, W * PS + 1)) if s < S // 2 else 0 for s in range(S)]
+    pool, pages, want = _state(S, S * Ht * W + 5, PS, S, Ht, W, lengths)
+    src = g.integers(0, S // 2, S // 2 + 3)
+    dst = np.concatenate([g.permutation(np.arange(S // 2, S))[:S // 2 - 1], [0, S, S // 2, -1]])
+    r = _counter()
+    _ia().fork_sequences(pages, _i32(src), _i32(dst), rejected=r)
+    want.fork(list(src), list(dst))
+    _same(pool, pages, want)
+    assert int(r) == want.rejected > 0
+    slots = list(g.permutation(S)[:S // 2 + 1]) + [S + 1, -1]
+    slots += slots[:2]
+    _ia().free_sequences(pages, _i32(slots), rejected=r)
+    want.free(slots)
+    _same(pool, pages, want)
+    assert int(r) == want.rejected
+    _ia().free_sequences(pages, _i32(list(range(S))))
+    assert int(pages.refs.abs().max()) == 0 and int((pages.table >= 0).sum()) == 0
+
+
+def test_fork_of_a_destination_is_refused():
+    pool, pages, want = _state(7, 64, 16, 4, 1, 4, [40, 0, 0, 0])
+    r = _counter()
+    _ia().fork_sequences(pages, _i32([0, 1, 2, 3]), _i32([1, 2, 2, 3]), rejected=r)
+    want.fork([0, 1, 2, 3], [1, 2, 2, 3])
+    _same(pool, pages, want)
+    assert int(r) == want.rejected == 3
+    assert pages.lengths.tolist() == [40, 40, 0, 0]
+
+
+@pytest.mark.parametrize("P,S,Ht,W", [(64, 3, 1, 4), (8192, 16, 4, 20), (70001, 32, 8, 100), (1, 1, 1, 1)])
+def test_compact(P, S, Ht, W):
+    g = np.random.default_rng(P)
+    lengths = g.integers(0, W * 16 + 1, S).tolist()
+    pool, pages, want = _state(P + 1, P, 16, S, Ht, W, lengths, share=0.3)
+    n = _ia().compact_pages(pool, pages)
+    assert int(n) == want.compact()
+    _same(pool, pages, want)
+    assert bool((pages.refs[:int(n)] > 0).all()) and not bool(pages.refs[int(n):].any())
+    assert int(_ia().compact_pages(pool, pages)) == want.compact()      # nothing left to move
+    _same(pool, pages, want)
+
+
+def test_tagged_pages_copy_their_format():
+    """Only the planes of a page's format move, with its tag; odd plane sizes included."""
+    ia = _ia()
+    P, PS, D = 40, 16, 64
+    pool = ia.PagePool.allocate(P, PS, D, scale_mode="page", zero=True)
+    g = np.random.default_rng(0)
+    fmts = g.integers(1, 6, P).astype(np.uint8)
+    pool.quantize_(torch.randn(P, PS, D, device="cuda"), torch.randn(P, PS, D, device="cuda"),
+                   torch.from_numpy(fmts).cuda())
+    from intent_attention.paged import make_tag_map
+    tag_map = make_tag_map({c: c for c in range(6)})
+    for dtype in (torch.uint8, torch.int32):
+        before = {n: getattr(pool, n).clone() for n in vars(pool) if torch.is_tensor(getattr(pool, n))}
+        tags = torch.from_numpy(fmts).cuda().to(dtype)
+        ids = g.permutation(P)[:9]
+        refs = np.zeros(P, np.int32)
+        refs[ids] = 1
+        pages = ia.SequencePages(_i32(refs), _i32(ids.reshape(1, 1, 9)), _i32([9 * PS]), PS)
+        ia.compact_pages(pool, pages, page_tags=tags, tag_map=tag_map)
+        new = pages.table.cpu().numpy().ravel()
+        for a, b in zip(ids, new):
+            assert int(tags[b]) == fmts[a]
+            names = {1: ["f16"], 2: ["fp8", "scale"], 3: ["i8", "scale"], 4: ["i4", "scale"],
+                     5: ["i4", "i4r", "scale", "res_scale"]}[int(fmts[a])]
+            for n in names:
+                for side in "kv":
+                    assert torch.equal(getattr(pool, f"{side}_{n}")[b], before[f"{side}_{n}"][a])
+        for n, t in before.items():
+            getattr(pool, n).copy_(t)
+
+
+def test_page_ops_captured():
+    ia = _ia()
+    pool, pages, want = _state(9, 4000, 16, 12, 4, 10, [100, 33, 64, 0, 0, 0, 0, 0, 0, 0, 0, 0], share=0.0)
+    saved = [t.clone() for t in (pages.refs, pages.table, pages.lengths)]
+    src, dst = _i32([0, 0, 1, 2]), _i32([5, 6, 7, 8])
+    more, gone = _i32([1] * 12), _i32([0, 3])
+
+    def step():
+        ia.fork_sequences(pages, src, dst)
+        ia.grow_sequences(pool, pages, more)
+        ia.free_sequences(pages, gone)
+        return ia.compact_pages(pool, pages)
+
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        n = step()
+    for t, s in zip((pages.refs, pages.table, pages.lengths), saved):
+        t.copy_(s)
+    for _ in range(2):                        # the second replay forks onto slots that hold tokens: refused
+        gr.replay()
+        want.fork([0, 0, 1, 2], [5, 6, 7, 8])
+        want.grow([1] * 12)
+        want.free([0, 3])
+        assert int(n) == want.compact()
+        _same(pool, pages, want)
+
+
+def test_serving_run():
+    """Prompt, decode, fork, copy-on-write, free and compact on one FP4 pool: every sequence keeps giving what
+    attention over its own tokens gives."""
+    ia = _ia()
+    g = np.random.default_rng(4)
+    P, PS, D, S, Ht, W, Hq = 600, 16, 128, 6, 2, 12, 8
+    pool = ia.Fp4Pool.allocate(P, PS, D)
+    pages = ia.SequencePages.allocate(P, PS, S, Ht, W)
+    held = {s: (np.zeros((Ht, 0, D)), np.zeros((Ht, 0, D))) for s in range(S)}
+
+    def write(counts):
+        """New tokens of every slot: room, then rows."""
+        n = max(counts)
+        start = pages.lengths.clone()
+        k = torch.randn(S, Ht, n, D, device="cuda", generator=gen).bfloat16()
+        v = torch.randn(S, Ht, n, D, device="cuda", generator=gen).bfloat16()
+        ia.grow_sequences(pool, pages, _i32(counts))
+        ia.append_fp4(pool, k, v, pages.table, start, _i32(counts))
+        for s in range(S):
+            held[s] = tuple(np.concatenate([a, of.values(x[s, :, :counts[s]].double().cpu().numpy())], 1)
+                            for a, x in zip(held[s], (k, v)))
+
+    def check():
+        q = torch.randn(S, Hq, D, device="cuda", generator=gen).half()
+        got = ia.paged_decode_fp4(q, pool, pages.table, pages.lengths)
+        for s in range(S):
+            assert int(pages.lengths[s]) == held[s][0].shape[1]
+            for h in range(Hq):
+                k, v = (x[h // (Hq // Ht)] for x in held[s])
+                want, A, reach = of.attention(q[s, h][None].double().cpu().numpy(), k, v,
+                                              np.ones((1, k.shape[0]), bool), D ** -0.5)
+                tol = A * (2.0 ** -11 + 2 * (D + 2) * 2.0 ** -24 * reach[:, None] + 2.0 ** -17) + 2.0 ** -11 * np.abs(want) + 2.0 ** -24
+                assert (np.abs(got[s, h].double().cpu().numpy() - want) <= tol).all()
+
+    gen = torch.Generator("cuda").manual_seed(1)
+    write([37, 64, 100, 0, 0, 0])
+    check()
+    for _ in range(3):
+        write([1, 1, 1, 0, 0, 0])
+    check()
+    ia.fork_sequences(pages, _i32([0, 0, 1]), _i32([3, 4, 5]))
+    held[3], held[4], held[5] = held[0], held[0], held[1]
+    check()
+    write([1, 2, 0, 1, 3, 1])
+    check()
+    ia.free_sequences(pages, _i32([0, 2]))
+    held[0] = held[2] = (np.zeros((Ht, 0, D)), np.zeros((Ht, 0, D)))
+    n = ia.compact_pages(pool, pages)
+    assert int(pages.table.max()) < int(n)
+    check()
+    write([50, 1, 0, 1, 1, 1])
+    check()
+
+
+def test_page_refusals():
+    ia = _ia()
+    pool, pages, _ = _state(1, 32, 16, 2, 1, 4, [10, 0])
+    ok = _i32([1, 1])
+    other = ia.SequencePages.allocate(31, 16, 2, 1, 4)
+    bad = [
+        lambda: ia.grow_sequences(pool, pages, _i32([1])),
+        lambda: ia.grow_sequences(pool, pages, ok.long()),
+        lambda: ia.grow_sequences(pool, other, ok),
+        lambda: ia.compact_pages(pool, ia.SequencePages.allocate(32, 8, 2, 1, 4)),
+        lambda: ia.compact_pages(pool, pages, page_tags=torch.zeros(32, dtype=torch.uint8, device="cuda")),
+        lambda: ia.compact_pages(pool, pages, page_tags=torch.zeros(3, dtype=torch.uint8, device="cuda"),
+                                 tag_map=[0] * 16),
+        lambda: ia.fork_sequences(pages, _i32([0, 1]), _i32([1])),
+        lambda: ia.fork_sequences(pages, _i32([0]).long(), _i32([1])),
+        lambda: ia.free_sequences(ia.SequencePages(pages.refs, pages.table[0], pages.lengths, 16), ok),
+        lambda: ia.free_sequences(ia.SequencePages(pages.refs, pages.table, pages.lengths[:1], 16), ok),
+        lambda: ia.free_sequences(pages, ok, rejected=torch.zeros(2, dtype=torch.int32, device="cuda")),
+    ]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()
+    with pytest.raises(RuntimeError):
+        ia.fork_sequences(pages, torch.zeros(1, dtype=torch.int32), _i32([1]))
+    ia.fork_sequences(pages, _i32([]), _i32([]))
+    ia.free_sequences(pages, _i32([]))
