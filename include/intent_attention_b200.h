@@ -553,21 +553,25 @@ int iak_prefill(const iak_page_pools* pools, const iak_prefill_args* args, void*
  * as 6, NaN as 0.  With e in [-14, 13] every value a pool can hold is zero or
  * a normal half (2^-15 .. 49152), so the kernels' half operands are exact.
  *
- * head_dim D is 64, 128 or 256; page_size a multiple of 16.  With NB = D / 32
- * a page holds
- *   k_codes  page_size * D / 2 bytes: row r, word w * NB + b = the codes of
- *            channels 32 b + 8 w .. + 7 (channel + i in bits 4i .. 4i + 3)
- *   v_codes  page_size * D / 2 bytes: rows 2i and 2i + 1 share D bytes, byte c =
- *            channel c of row 2i (low half) and of row 2i + 1 (high half)
- *   k_scales page_size * NB bytes: per 16 rows [g 8][hi 2][NB], row g + 8 hi
- *   v_scales page_size * NB bytes: per 16 rows [NB][t 4][j 4], row
- *            2 t + (j & 1) + 8 (j >> 1)
- * Scale bytes are those an append wrote, or 0 (rows never written).  The four
- * planes are 16-byte aligned.
+ * head_dim D is 64, 128 or 256; page_size a multiple of 16.  With NB = D / 32,
+ * 16 rows of K and V lie together in 544 * NB bytes (page p: the page_size / 16
+ * such groups from byte p * page_size / 16 * 544 * NB on), ordered as the
+ * attention kernel's lanes read them.  Lane 4 g + t (g 0..7, t 0..3) has NB
+ * words of 4 bytes per set, stored in pieces of PW = min(NB, 4) words, word w of
+ * lane l at word ((w / PW) * 32 + l) * PW + w % PW of the set:
+ *   bytes 0 ..         K rows 0..7, then K rows 8..15 (a set each): lane 4 g + t's
+ *                      word b = the codes of row g (g + 8), channels 32 b + 8 t .. + 7
+ *                      (channel + i in bits 4i .. 4i + 3)
+ *   bytes 256 NB ..    V rows 0..7, then V rows 8..15: lane 4 g + t's bytes k =
+ *                      channel 4 NB g + k of row 2 t (low half) and 2 t + 1 (high half)
+ *   bytes 512 NB ..    K scales [g 8][hi 2][NB], of row g + 8 hi
+ *   bytes 528 NB ..    V scales [NB][t 4][j 4], of row 2 t + (j & 1) + 8 (j >> 1)
+ * Rows never written may hold anything: no call reads them.  The data is
+ * 16-byte aligned.
  * ------------------------------------------------------------------------ */
 #define IAK_FP4_MAX_QUERIES 16
 typedef struct iak_fp4_pool {
-  void* k_codes; void* k_scales; void* v_codes; void* v_scales;
+  void* data;
   int64_t num_pages;
   int32_t page_size, head_dim;
 } iak_fp4_pool;

@@ -8,7 +8,7 @@ namespace iak {
 constexpr int kFp4ScaleMin = 127 - 14, kFp4ScaleMax = 127 + 13;   // scale bytes an append writes
 
 struct Fp4Pool {
-  uint8_t* kc; uint8_t* ks; uint8_t* vc; uint8_t* vs;
+  uint8_t* data;
   int64_t num_pages;
   int PS, D;
 };
@@ -40,14 +40,27 @@ __device__ __forceinline__ void fp4_unpack4(unsigned w, unsigned (&h)[4]) {
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 }
 
-// byte offsets inside the scale planes (64-bit: a long cache passes 2^31 rows * blocks)
-__device__ __forceinline__ int64_t fp4_k_scale_at(int64_t page, int row, int b, int PS, int NB) {
-  return ((page * (PS / 16) + (row >> 4)) * 8 + (row & 7)) * 2 * NB + ((row >> 3) & 1) * NB + b;
-}
-__device__ __forceinline__ int64_t fp4_v_scale_at(int64_t page, int row, int b, int PS, int NB) {
-  const int r = row & 15;
-  return (((page * (PS / 16) + (row >> 4)) * NB + b) * 4 + ((r & 7) >> 1)) * 4 + (r & 1) + 2 * (r >> 3);
-}
+// A group of 16 rows: byte offsets (the public header has the layout in words).
+template <int NB>
+struct Fp4Group {
+  static constexpr int kPW = NB < 4 ? NB : 4;          // words of a lane's piece
+  static constexpr int kSet = 128 * NB;                // 8 rows of K, or of V
+  static constexpr int kV = 2 * kSet, kKs = 4 * kSet, kVs = kKs + 16 * NB;
+  static constexpr int kBytes = 544 * NB;
+  static __host__ __device__ constexpr int word(int lane, int w) { return ((w / kPW) * 32 + lane) * kPW + w % kPW; }
+  // K word of row r's channels 32 b + 8 t ..
+  static __device__ __forceinline__ int k_word(int r, int b, int t) {
+    return (r >> 3) * kSet + 4 * word((r & 7) * 4 + t, b);
+  }
+  // the byte of channel c (a multiple of 8, with the next 7) of rows r and r + 1, r even
+  static __device__ __forceinline__ int v_bytes(int r, int c) {
+    return kV + (r >> 3) * kSet + 4 * word(c / (4 * NB) * 4 + ((r & 7) >> 1), (c % (4 * NB)) >> 2);
+  }
+  static __device__ __forceinline__ int k_scale(int r, int b) { return kKs + ((r & 7) * 2 + (r >> 3)) * NB + b; }
+  static __device__ __forceinline__ int v_scale(int r, int b) {
+    return kVs + (b * 4 + ((r & 7) >> 1)) * 4 + (r & 1) + 2 * (r >> 3);
+  }
+};
 
 int check_fp4_pool(const iak_fp4_pool* pool, const char* what);
 

@@ -14,13 +14,15 @@
 // (sequence, table head, column group) units, one run per resident block, so that ragged batches and single long
 // sequences fill the GPU alike; a unit cut over several blocks leaves partial (m, l, O) that a second kernel joins in
 // order of the blocks (no atomics: results do not depend on timing).  Each warp streams its own tiles through a
-// two-stage ring of 16-byte asynchronous copies; a lane copies exactly what it will read, so the ring needs no
-// barrier.
+// ring of bulk copies, one per 16 rows (32 where a page holds both): a group's codes and scales lie together in the
+// order in which lanes read them, so a copy needs no address arithmetic beyond its start and reads are free of bank
+// conflicts.
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
 
 #include "fp4.cuh"
+#include "tc_ptx.cuh"
 
 namespace iak {
 namespace {
@@ -35,6 +37,7 @@ constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small 
 struct DecP {
   Fp4Pool pool;
   int gpp;                           // groups of 16 rows per page
+  int step_slot, step_sub;           // what kWarps tiles move a group's (table entry, group of the page) by
   const void* q; int q_dtype; int64_t q_sb, q_sh, q_sm;
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sm;
   int B, Hq, Ht, G, M;
@@ -110,6 +113,14 @@ __device__ __forceinline__ void mma16816(float (&d)[4], unsigned a0, unsigned a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same product on its own: d = A B
+__device__ __forceinline__ void mma16816_new(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3,
+                                             unsigned b0, unsigned b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ unsigned transpose8x8(unsigned x) {
   unsigned r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -123,23 +134,6 @@ __device__ __forceinline__ unsigned mul_half2(unsigned a, unsigned b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const unsigned*>(&r);
 }
-__device__ __forceinline__ float fast_exp2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-template <int BYTES>
-__device__ __forceinline__ void copy_async(unsigned dst, const void* src, bool ok) {
-  const int n = ok ? BYTES : 0;      // 0 source bytes: the destination is zero-filled
-  if (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(BYTES), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 __device__ __forceinline__ unsigned lds32(unsigned a) {
   unsigned r;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
@@ -161,23 +155,22 @@ __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
 // ------------------------------------------------------------- shared layout
 template <int NB>
 struct Lay {
+  using Gr = Fp4Group<NB>;
   static constexpr int D = NB * 32;
-  static constexpr int kPiece = NB >= 4 ? 16 : 8;          // bytes of one access
-  static constexpr int kPieces = NB * 4 / kPiece;          // accesses of a lane's NB words
-  static constexpr int kPlane = 32 * NB * 4;               // a lane-ordered set of NB words
-  static constexpr int kScaleK = 2 * NB;                   // a lane's K scale bytes: rows g and g + 8
-  static constexpr int kKs = 4 * kPlane;                   // offsets inside a group
-  static constexpr int kVs = kKs + 32 * kScaleK;
-  static constexpr int kGroup = kVs + 32 * 4;
-  static constexpr int kStage = 2 * kGroup;
-  static constexpr int kRing = kWarps * 2 * kStage;
+  static constexpr int kStages = 3;
+  static constexpr int kStage = 2 * Gr::kBytes;
+  static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kOutStride = D + 4;                 // floats of one column in the join buffer
+  static_assert(kWarps * 8 * kOutStride * 4 <= kRing, "the join buffer lies over the ring");
 };
 
 template <int NB, int NT, bool SPLIT>
 constexpr int smem_bytes() {
-  return Lay<NB>::kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + 8 * NT * 8 + kWarps * 8 * NT * 8;
+  return Lay<NB>::kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + 8 * NT * 8 + kWarps * 8 * NT * 8 +
+         kWarps * Lay<NB>::kStages * 8;
 }
+
+__device__ unsigned int g_fp4_timeouts = 0;
 
 // x: one row's D values, lane i holding channels i, i + 32, ..
 template <int NB>
@@ -207,6 +200,7 @@ __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f :
 template <int NB, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
   using L = Lay<NB>;
+  using Gr = Fp4Group<NB>;
   constexpr int D = L::D;
   constexpr int MT = D / 16;
   constexpr int COLS = 8 * NT;
@@ -216,16 +210,25 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
   int* col_limit = reinterpret_cast<int*>(col_scale + COLS);
   float* warp_m = reinterpret_cast<float*>(col_limit + COLS);      // [warp][COLS]
   float* warp_l = warp_m + kWarps * COLS;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(warp_l + kWarps * COLS);   // [warp][stage]: the stage's bytes are there
   float* join = reinterpret_cast<float*>(smem);                    // [warp][8][kOutStride], over the ring
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
-  const unsigned ring = smem_base + warp * 2 * L::kStage;
+  const unsigned ring = smem_base + warp * L::kStages * L::kStage;
+  const unsigned bar = static_cast<unsigned>(__cvta_generic_to_shared(bars)) + warp * L::kStages * 8;
+  if (lane < L::kStages) tc::mbar_init(bar + lane * 8, 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  tc::fence_proxy_async();
+  __syncwarp();
+  unsigned phases = 0;                            // bit i: parity of stage i's next completion
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int b;
   int64_t left, off;
   bool begins_run = true;
+  int stage = 0;
+  bool gave_up = false;
   if (p.direct) {
     b = blockIdx.x / p.HC;
     const int n = seq_tiles(p, b);
@@ -301,55 +304,46 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
     // ----------------------------------------------------- the copies' cursor
     int c_fetch = c_begin + warp;                 // tile whose page ids are read next
     int slot = (c_fetch * 2) / p.gpp, sub = c_fetch * 2 - slot * p.gpp;
-    const int step_slot = (2 * kWarps) / p.gpp, step_sub = 2 * kWarps - step_slot * p.gpp;
-    int id[2], in_page[2];                        // of the tile fetched last
+    int id[2], at_sub;                            // of the tile fetched last
     auto fetch = [&]() {
-      int s1 = slot, u1 = sub + 1;
-      if (u1 == p.gpp) { u1 = 0; ++s1; }
-      in_page[0] = sub;
-      in_page[1] = u1;
+      at_sub = sub;
       id[0] = id[1] = -1;
       if (c_fetch < c_end) {
+        const int s1 = sub + 1 == p.gpp ? slot + 1 : slot;
         if (c_fetch * kTileKeys < len) id[0] = __ldg(table + slot);
         if (c_fetch * kTileKeys + 16 < len) id[1] = __ldg(table + s1);
       }
       c_fetch += kWarps;
-      slot += step_slot;
-      sub += step_sub;
+      slot += p.step_slot;
+      sub += p.step_sub;
       if (sub >= p.gpp) { sub -= p.gpp; ++slot; }
     };
     unsigned ok_bits = 0;                         // [stage][group]: the group's page exists
     auto issue = [&](int stage) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const bool ok = id[u] >= 0 && id[u] < p.pool.num_pages;
-        const int64_t page = ok ? id[u] : 0;
-        const int bit = stage * 2 + u;
-        ok_bits = (ok_bits & ~(1u << bit)) | (static_cast<unsigned>(ok) << bit);
-        const int64_t row = page * p.pool.PS + in_page[u] * 16;
-        const int64_t group = page * p.gpp + in_page[u];
-        const uint8_t* k = p.pool.kc + (row + g) * (16 * NB) + t * (4 * NB);
-        const uint8_t* v = p.pool.vc + (row / 2 + t) * (32 * NB) + g * (4 * NB);
-        const unsigned dst = ring + stage * L::kStage + u * L::kGroup;
-#pragma unroll
-        for (int i = 0; i < L::kPieces; ++i) {
-          const unsigned to = dst + (i * 32 + lane) * L::kPiece;
-          copy_async<L::kPiece>(to, k + i * L::kPiece, ok);
-          copy_async<L::kPiece>(to + L::kPlane, k + 8 * (16 * NB) + i * L::kPiece, ok);
-          copy_async<L::kPiece>(to + 2 * L::kPlane, v + i * L::kPiece, ok);
-          copy_async<L::kPiece>(to + 3 * L::kPlane, v + 4 * (32 * NB) + i * L::kPiece, ok);
+      const bool ok0 = id[0] >= 0 && id[0] < p.pool.num_pages, ok1 = id[1] >= 0 && id[1] < p.pool.num_pages;
+      ok_bits = (ok_bits & ~(3u << (2 * stage))) | ((ok0 ? 1u : 0u) | (ok1 ? 2u : 0u)) << (2 * stage);
+      if (lane == 0) {
+        const unsigned to = ring + stage * L::kStage, full = bar + stage * 8;
+        const bool wraps = at_sub + 1 == p.gpp;
+        const uint8_t* g0 = p.pool.data + (static_cast<int64_t>(id[0]) * p.gpp + at_sub) * Gr::kBytes;
+        tc::mbar_arrive_expect_tx(full, (ok0 ? Gr::kBytes : 0) + (ok1 ? Gr::kBytes : 0));
+        if (ok0 && ok1 && !wraps) {
+          tc::bulk_load(to, g0, 2 * Gr::kBytes, full);
+        } else {
+          if (ok0) tc::bulk_load(to, g0, Gr::kBytes, full);
+          const int sub1 = wraps ? 0 : at_sub + 1;
+          if (ok1)
+            tc::bulk_load(to + Gr::kBytes, p.pool.data + (static_cast<int64_t>(id[1]) * p.gpp + sub1) * Gr::kBytes,
+                          Gr::kBytes, full);
         }
-        copy_async<L::kScaleK>(dst + L::kKs + lane * L::kScaleK, p.pool.ks + (group * 8 + g) * (2 * NB), ok);
-        copy_async<4>(dst + L::kVs + lane * 4, p.pool.vs + (group * NB + g * NB / 8) * 16 + t * 4, ok);
       }
-      copy_commit();
     };
     auto read_words = [&](unsigned at, unsigned (&w)[NB]) {
-      constexpr int PW = L::kPiece / 4;
+      constexpr int PW = Gr::kPW;
 #pragma unroll
-      for (int i = 0; i < L::kPieces; ++i) {
+      for (int i = 0; i < NB / PW; ++i) {
         unsigned part[PW];
-        lds_words<PW>(at + (i * 32 + lane) * L::kPiece, part);
+        lds_words<PW>(at + (i * 32 + lane) * (PW * 4), part);
 #pragma unroll
         for (int j = 0; j < PW; ++j) w[i * PW + j] = part[j];
       }
@@ -365,28 +359,42 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
     }
 
+    int ahead = c_begin + warp;                   // next tile to issue
+#pragma unroll
+    for (int i = 0; i < L::kStages - 1; ++i) {
+      fetch();
+      // stages are used in turn over all segments
+      if (ahead < c_end && !gave_up) issue(stage + i < L::kStages ? stage + i : stage + i - L::kStages);
+      ahead += kWarps;
+    }
     fetch();
-    issue(0);
-    fetch();
-    issue(1);
-    fetch();
-    int stage = 0;
-    for (int c = c_begin + warp; c < c_end; c += kWarps, stage ^= 1) {
-      copy_wait<1>();
+    for (int c = c_begin + warp; c < c_end && !gave_up; c += kWarps) {
+      // the stage read in the last round is free: every lane is past its reads
+      __syncwarp();
+      if (ahead < c_end) issue(stage == 0 ? L::kStages - 1 : stage - 1);
+      ahead += kWarps;
+      fetch();
+      if (!__all_sync(~0u, tc::mbar_wait(bar + stage * 8, (phases >> stage) & 1))) {
+        gave_up = true;                           // the call's output is undefined from here on
+        break;
+      }
+      phases ^= 1u << stage;
       const unsigned at = ring + stage * L::kStage;
       const int key0 = c * kTileKeys;
-      const bool full = ((ok_bits >> (2 * stage)) & 3) == 3 && key0 + kTileKeys <= len - (p.M - 1);
+      const unsigned ok_here = (ok_bits >> (2 * stage)) & 3;
+      const bool full = ok_here == 3 && key0 + kTileKeys <= len - (p.M - 1);
+      stage = stage + 1 == L::kStages ? 0 : stage + 1;
 
       // ---------------------------------------------------------- S' = K Q'
       float s[2][NT][4];
       {
         unsigned kw[2][2][NB];
-        unsigned ksw[2][(2 * NB + 3) / 4];
+        unsigned ksw[2][NB / 2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          read_words(at + u * L::kGroup, kw[u][0]);
-          read_words(at + u * L::kGroup + L::kPlane, kw[u][1]);
-          lds_words<L::kScaleK / 4>(at + u * L::kGroup + L::kKs + lane * L::kScaleK, ksw[u]);
+          read_words(at + u * Gr::kBytes, kw[u][0]);
+          read_words(at + u * Gr::kBytes + Gr::kSet, kw[u][1]);
+          lds_words<NB / 2>(at + u * Gr::kBytes + Gr::kKs + g * 2 * NB, ksw[u]);
         }
 #pragma unroll
         for (int bk = 0; bk < NB; ++bk) {
@@ -402,12 +410,12 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
             fp4_unpack4(kw[u][0][bk], r0);
             fp4_unpack4(kw[u][1][bk], r1);
             const int i0 = bk, i1 = NB + bk;          // scale bytes of rows g and g + 8
-            const float s0 = fp4_scale((ksw[u][i0 / 4] >> (8 * (i0 % 4))) & 255);
-            const float s1 = fp4_scale((ksw[u][i1 / 4] >> (8 * (i1 % 4))) & 255);
+            const float s0 = fp4_scale(__byte_perm(ksw[u][i0 / 4], 0, 0x4440 + i0 % 4));
+            const float s1 = fp4_scale(__byte_perm(ksw[u][i1 / 4], 0, 0x4440 + i1 % 4));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              float acc[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816(acc, r0[0], r1[0], r0[1], r1[1], q_hi[nt].x, q_hi[nt].y);
+              float acc[4];
+              mma16816_new(acc, r0[0], r1[0], r0[1], r1[1], q_hi[nt].x, q_hi[nt].y);
               mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_hi[nt].z, q_hi[nt].w);
               if (SPLIT) {
                 mma16816(acc, r0[0], r1[0], r0[1], r1[1], q_lo[nt].x, q_lo[nt].y);
@@ -427,7 +435,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
       if (!full) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const bool ok = (ok_bits >> (2 * stage + u)) & 1;
+          const bool ok = (ok_here >> u) & 1;
           const int key = key0 + u * 16 + g;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -462,7 +470,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
             v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
             v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
             const float m_new = fmaxf(m_run[nt][e], fmaf(v, sc[nt][e], -kHead));
-            f[e] = fast_exp2(m_run[nt][e] - m_new);
+            f[e] = tc::ex2(m_run[nt][e] - m_new);
             m_run[nt][e] = m_new;
             l_run[nt][e] *= f[e];
           }
@@ -481,7 +489,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
           float x[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[i] = fast_exp2(fmaf(s[u][nt][i], sc[nt][i & 1], -m_run[nt][i & 1]));
+            x[i] = tc::ex2(fmaf(s[u][nt][i], sc[nt][i & 1], -m_run[nt][i & 1]));
             l_run[nt][i & 1] += x[i];
           }
 #pragma unroll
@@ -500,14 +508,15 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         unsigned vw[2][NB];
-        read_words(at + u * L::kGroup + 2 * L::kPlane, vw[0]);
-        read_words(at + u * L::kGroup + 3 * L::kPlane, vw[1]);
-        unsigned vs = lds32(at + u * L::kGroup + L::kVs + lane * 4);   // keys 2t, 2t + 1, 2t + 8, 2t + 9
-        if (!full) {          // rows behind the sequence hold anything: scale 0 keeps NaN out of the sums
+        read_words(at + u * Gr::kBytes + Gr::kV, vw[0]);
+        read_words(at + u * Gr::kBytes + Gr::kV + Gr::kSet, vw[1]);
+        // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the lane's channels' block
+        unsigned vs = lds32(at + u * Gr::kBytes + Gr::kVs + (g * NB / 8) * 16 + t * 4);
+        if (!full) {          // rows behind the sequence or without a page hold anything: scale 0 keeps NaN away
           const int key = key0 + u * 16 + 2 * t;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            if (key + (i & 1) + 8 * (i >> 1) >= len) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
+            if (!((ok_here >> u) & 1) || key + (i & 1) + 8 * (i >> 1) >= len) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
           }
         }
         // byte e + 127 -> half 2^e: (byte - 112) << 10 in both halves at once
@@ -534,10 +543,13 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
           }
         }
       }
-      issue(stage);
-      fetch();
     }
-    copy_wait<0>();
+
+    if (gave_up && phases != ~0u) {               // once: count it, and let the copies in flight land before the block ends
+      if (lane == 0) atomicAdd(&g_fp4_timeouts, 1u);
+      for (int i = 0; i < L::kStages; ++i) tc::mbar_wait(bar + i * 8, (phases >> i) & 1);
+      phases = ~0u;
+    }
 
     // ------------------------------------------------------ join the 8 warps
 #pragma unroll
@@ -565,7 +577,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
         float top = -FLT_MAX;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + nt * 8 + 2 * t + e]);
-        f[e] = fast_exp2(m_run[nt][e] - top);
+        f[e] = tc::ex2(m_run[nt][e] - top);
       }
       float* dst = join + (warp * 8 + 2 * t) * L::kOutStride + g * (4 * NB);
 #pragma unroll
@@ -587,7 +599,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
 #pragma unroll
           for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + col]);
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) l += warp_l[w * COLS + col] * fast_exp2(warp_m[w * COLS + col] - top);
+          for (int w = 0; w < kWarps; ++w) l += warp_l[w * COLS + col] * tc::ex2(warp_m[w * COLS + col] - top);
           float acc[NB];
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
@@ -611,6 +623,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
         }
         if (write) finish_row<NB>(p, b, h * p.G + row / p.M, row % p.M, x);
       }
+      tc::fence_proxy_async();                    // the next segment's copies write where these lines read
       __syncthreads();
     }
 
@@ -674,7 +687,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p)
     for (int c = first + warp; c <= last; c += kJoinWarps) {
       const float* part = p.ws + ((static_cast<int64_t>(c) * 2 + (c == first ? first_which : 0)) * COLS + col) * (D + 2);
       const float m = part[D], m_new = fmaxf(top, m);
-      const float f_old = fast_exp2(top - m_new), f_new = fast_exp2(m - m_new);
+      const float f_old = tc::ex2(top - m_new), f_new = tc::ex2(m - m_new);
       l = l * f_old + part[D + 1] * f_new;
 #pragma unroll
       for (int i = 0; i < NB; ++i) acc[i] = acc[i] * f_old + part[i * 32 + lane] * f_new;
@@ -692,7 +705,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p)
       for (int i = 0; i < NB; ++i) acc[i] = 0.f;
 #pragma unroll
       for (int w = 0; w < kJoinWarps; ++w) {
-        const float f = fast_exp2(part_m[w] - all);
+        const float f = tc::ex2(part_m[w] - all);
         sum += part_l[w] * f;
 #pragma unroll
         for (int i = 0; i < NB; ++i) acc[i] = fmaf(part_sum[w][i * 32 + lane], f, acc[i]);
@@ -827,10 +840,10 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
     if (a->differential && !a->lam) return fail(IAK_ERR_INVALID_ARG, "%s: differential attention needs lam", what);
   }
   DecP p = {};
-  p.pool = {static_cast<uint8_t*>(pool->k_codes), static_cast<uint8_t*>(pool->k_scales),
-            static_cast<uint8_t*>(pool->v_codes), static_cast<uint8_t*>(pool->v_scales), pool->num_pages,
-            pool->page_size, pool->head_dim};
+  p.pool = {static_cast<uint8_t*>(pool->data), pool->num_pages, pool->page_size, pool->head_dim};
   p.gpp = pool->page_size / 16;
+  p.step_slot = 2 * kWarps / p.gpp;
+  p.step_sub = 2 * kWarps % p.gpp;
   p.q = a->q; p.q_dtype = a->q_dtype; p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h; p.q_sm = a->q_stride_m;
   p.out = a->out; p.out_dtype = a->out_dtype;
   p.o_sb = a->out_stride_b; p.o_sh = a->out_stride_h; p.o_sm = a->out_stride_m;
@@ -854,6 +867,20 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
 }
 
 }  // namespace
+
+int read_fp4_timeouts(unsigned int* value, bool reset) {
+  unsigned int v = 0;
+  int st = check_cuda(cudaMemcpyFromSymbol(&v, g_fp4_timeouts, sizeof(v)), "read fp4 timeouts");
+  if (st) return st;
+  if (reset && v) {
+    const unsigned int zero = 0;
+    st = check_cuda(cudaMemcpyToSymbol(g_fp4_timeouts, &zero, sizeof(zero)), "reset fp4 timeouts");
+    if (st) return st;
+  }
+  *value = v;
+  return IAK_OK;
+}
+
 }  // namespace iak
 
 extern "C" int iak_fp4_decode_workspace_size(const iak_fp4_pool* pool, const iak_fp4_decode_args* args, size_t* bytes) {

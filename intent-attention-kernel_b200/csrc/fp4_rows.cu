@@ -2,9 +2,10 @@
 //
 // Both are copies: per row and channel they move 2 * (element size + 17/32) bytes, which bounds them for long
 // prompts; a decode step's few rows are bound by the launch.  One thread owns 8 channels of the two rows 2i and
-// 2i + 1, which share their bytes of the V plane: it reads (writes) 16 bytes of each of the four dense rows, so that
-// its loads are independent of one another and neighbouring threads cover whole lines.  A block's largest magnitude
-// spans 4 neighbouring lanes.  A V byte whose other row is not part of the call keeps that row's half.
+// 2i + 1, which share their bytes of V: it moves 16 bytes of each of the four dense rows, independent of one another.
+// A warp has 4 such row pairs by 64 channels, so that it covers 128-byte runs of the dense rows (16-bit types) and
+// 64-byte runs of the group.  A block's largest magnitude spans 4 neighbouring lanes.  A V byte whose other row is not
+// part of the call keeps that row's half.
 #include "fp4.cuh"
 
 namespace iak {
@@ -17,7 +18,7 @@ struct RowsParams {
   int B, Ht, N;
   const int32_t* pt; int64_t pt_sb, pt_sh; int W;
   const int32_t* positions; const int32_t* counts; int32_t* dropped;
-  int64_t pairs;      // row pairs a (b, h) can touch: N / 2 + 1
+  int64_t octets;     // runs of 8 aligned rows that a (b, h) can touch
 };
 
 constexpr int kRowThreads = 256;
@@ -78,41 +79,41 @@ __device__ __forceinline__ void store8(void* base, int dtype, int64_t at, const 
 // where a thread works: its (b, h), row pair and 8 channels; tokens are 64-bit
 struct Place {
   int b, h, l;            // l: which 8 channels
-  int64_t tok0;           // token of the pair's first row
-  int64_t i0;             // its index among the call's rows (-1 when the pair starts before them)
+  int64_t i0;             // the pair's first row among the call's (negative when it starts before them)
   bool in0, in1;          // rows that the call covers (index in [0, N))
   bool real0, real1;      // rows below counts[b]
-  int64_t page; int row;  // page < 0: no such page
+  uint8_t* group;         // the 16 rows' bytes, or null: no such page
+  int row;                // of the group, even
 };
 
 template <int NB>
 __device__ __forceinline__ bool find_place(const RowsParams& p, Place& w) {
-  constexpr int LP = NB * 4;                 // lanes of a row pair
+  constexpr int LP = NB * 16;                // threads of 8 rows: 4 row pairs, D / 8 channel runs
   const int64_t at = static_cast<int64_t>(blockIdx.x) * (kRowThreads / LP) + threadIdx.x / LP;
-  const int64_t bh = at / p.pairs;
-  if (bh >= static_cast<int64_t>(p.B) * p.Ht) return false;   // whole groups of LP lanes leave together
-  w.l = threadIdx.x % LP;
+  const int64_t bh = at / p.octets;
+  if (bh >= static_cast<int64_t>(p.B) * p.Ht) return false;   // whole groups of LP threads leave together
+  w.l = (threadIdx.x % LP / 32) * 8 + (threadIdx.x & 7);
   w.b = static_cast<int>(bh / p.Ht);
   w.h = static_cast<int>(bh - static_cast<int64_t>(w.b) * p.Ht);
   const int64_t pos = p.positions ? p.positions[w.b] : 0;
   const int n = p.counts ? min(max(p.counts[w.b], 0), p.N) : p.N;
-  w.tok0 = (pos & ~int64_t(1)) + 2 * (at - bh * p.pairs);
-  w.i0 = w.tok0 - pos;
+  const int64_t tok0 = (pos & ~int64_t(7)) + 8 * (at - bh * p.octets) + 2 * ((threadIdx.x >> 3) & 3);
+  w.i0 = tok0 - pos;
   w.in0 = w.i0 >= 0 && w.i0 < p.N;
   w.in1 = w.i0 + 1 >= 0 && w.i0 + 1 < p.N;
   w.real0 = w.in0 && w.i0 < n;
   w.real1 = w.in1 && w.i0 + 1 < n;
-  w.page = -1;
-  w.row = 0;
-  if (w.tok0 >= 0) {                         // page sizes are even: both rows lie in one page
-    const int64_t slot = w.tok0 / p.pool.PS;
-    w.row = static_cast<int>(w.tok0 - slot * p.pool.PS);
-    if (slot < p.W && (w.real0 || w.real1)) {
+  w.group = nullptr;
+  w.row = static_cast<int>(tok0 & 15);       // page sizes are multiples of 16: so are pages' first tokens
+  if (tok0 >= 0 && (w.real0 || w.real1)) {
+    const int64_t slot = tok0 / p.pool.PS;
+    if (slot < p.W) {
       const int id = p.pt[w.b * p.pt_sb + w.h * p.pt_sh + slot];
-      if (id >= 0 && id < p.pool.num_pages) w.page = id;
+      if (id >= 0 && id < p.pool.num_pages)
+        w.group = p.pool.data + ((static_cast<int64_t>(id) * p.pool.PS + (tok0 - slot * p.pool.PS)) >> 4) * Fp4Group<NB>::kBytes;
     }
   }
-  return w.in0 || w.in1;
+  return w.in0 || w.in1;                     // the 4 lanes of a block agree
 }
 
 // 8 values of a block of 4 lanes -> their codes (value i in bits 4i) and the block's scale byte
@@ -146,14 +147,13 @@ template <int NB, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) fp4_append_kernel(const RowsParams p) {
   Place w;
   if (!find_place<NB>(p, w)) return;
-  if (w.page < 0) {
+  if (!w.group) {
     if (p.dropped && w.l == 0) {
       const int n = (w.real0 ? 1 : 0) + (w.real1 ? 1 : 0);
       if (n) atomicAdd(p.dropped, n);
     }
     return;
   }
-  constexpr int D = NB * 32;
   const int blk = w.l >> 2, t = w.l & 3;      // the thread's block and its word of the block
   float k0[8] = {}, k1[8] = {}, v0[8] = {}, v1[8] = {};
   const int64_t kat = w.b * p.k_sb + w.h * p.k_sh + w.i0 * p.k_sn + w.l * 8;
@@ -169,11 +169,10 @@ __global__ void __launch_bounds__(kRowThreads) fp4_append_kernel(const RowsParam
   int kb0, kb1, vb0, vb1;
   const unsigned kw0 = quantize8(k0, kb0), kw1 = quantize8(k1, kb1);
   const unsigned vw0 = quantize8(v0, vb0), vw1 = quantize8(v1, vb1);
-  const Fp4Pool& P = p.pool;
-  uint32_t* krow = reinterpret_cast<uint32_t*>(P.kc + (w.page * P.PS + w.row) * (D / 2));
-  if (w.real0) krow[t * NB + blk] = kw0;
-  if (w.real1) krow[D / 8 + t * NB + blk] = kw1;
-  uint2* vrow = reinterpret_cast<uint2*>(P.vc + (w.page * P.PS + w.row) * (D / 2) + w.l * 8);
+  using Gr = Fp4Group<NB>;
+  if (w.real0) *reinterpret_cast<uint32_t*>(w.group + Gr::k_word(w.row, blk, t)) = kw0;
+  if (w.real1) *reinterpret_cast<uint32_t*>(w.group + Gr::k_word(w.row + 1, blk, t)) = kw1;
+  uint2* vrow = reinterpret_cast<uint2*>(w.group + Gr::v_bytes(w.row, w.l * 8));
   uint2 vz = make_uint2(zip_codes(vw0, vw1), zip_codes(vw0 >> 16, vw1 >> 16));
   if (!(w.real0 && w.real1)) {                // the other row's half stays as it is
     const uint2 old = *vrow;
@@ -184,12 +183,12 @@ __global__ void __launch_bounds__(kRowThreads) fp4_append_kernel(const RowsParam
   *vrow = vz;
   if (t == 0) {
     if (w.real0) {
-      P.ks[fp4_k_scale_at(w.page, w.row, blk, P.PS, NB)] = static_cast<uint8_t>(kb0);
-      P.vs[fp4_v_scale_at(w.page, w.row, blk, P.PS, NB)] = static_cast<uint8_t>(vb0);
+      w.group[Gr::k_scale(w.row, blk)] = static_cast<uint8_t>(kb0);
+      w.group[Gr::v_scale(w.row, blk)] = static_cast<uint8_t>(vb0);
     }
     if (w.real1) {
-      P.ks[fp4_k_scale_at(w.page, w.row + 1, blk, P.PS, NB)] = static_cast<uint8_t>(kb1);
-      P.vs[fp4_v_scale_at(w.page, w.row + 1, blk, P.PS, NB)] = static_cast<uint8_t>(vb1);
+      w.group[Gr::k_scale(w.row + 1, blk)] = static_cast<uint8_t>(kb1);
+      w.group[Gr::v_scale(w.row + 1, blk)] = static_cast<uint8_t>(vb1);
     }
   }
 }
@@ -223,18 +222,16 @@ template <int NB, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams p) {
   Place w;
   if (!find_place<NB>(p, w)) return;
-  constexpr int D = NB * 32;
   float k0[8] = {}, k1[8] = {}, v0[8] = {}, v1[8] = {};
-  if (w.page >= 0) {
+  if (w.group) {
+    using Gr = Fp4Group<NB>;
     const int blk = w.l >> 2, t = w.l & 3;
-    const Fp4Pool& P = p.pool;
-    const uint32_t* krow = reinterpret_cast<const uint32_t*>(P.kc + (w.page * P.PS + w.row) * (D / 2));
-    const unsigned kw0 = krow[t * NB + blk], kw1 = krow[D / 8 + t * NB + blk];
-    const uint2 vz = *reinterpret_cast<const uint2*>(P.vc + (w.page * P.PS + w.row) * (D / 2) + w.l * 8);
-    const int64_t ks = fp4_k_scale_at(w.page, w.row, blk, P.PS, NB);   // row + 1: the next g
-    const uint16_t vs = *reinterpret_cast<const uint16_t*>(P.vs + fp4_v_scale_at(w.page, w.row, blk, P.PS, NB));
-    dequant_k(kw0, fp4_scale(P.ks[ks]), k0);
-    dequant_k(kw1, fp4_scale(P.ks[ks + 2 * NB]), k1);
+    const unsigned kw0 = *reinterpret_cast<const uint32_t*>(w.group + Gr::k_word(w.row, blk, t));
+    const unsigned kw1 = *reinterpret_cast<const uint32_t*>(w.group + Gr::k_word(w.row + 1, blk, t));
+    const uint2 vz = *reinterpret_cast<const uint2*>(w.group + Gr::v_bytes(w.row, w.l * 8));
+    const uint16_t vs = *reinterpret_cast<const uint16_t*>(w.group + Gr::v_scale(w.row, blk));
+    dequant_k(kw0, fp4_scale(w.group[Gr::k_scale(w.row, blk)]), k0);
+    dequant_k(kw1, fp4_scale(w.group[Gr::k_scale(w.row + 1, blk)]), k1);
     dequant_v(vz, fp4_scale(vs & 255), fp4_scale(vs >> 8), v0, v1);
     // rows from counts[b] on are zeros, whatever the page holds behind the sequence
     if (!w.real0) {
@@ -260,8 +257,8 @@ __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams 
 
 template <int NB>
 int launch_rows(const RowsParams& p, bool append, bool vec, cudaStream_t s) {
-  const int64_t per = kRowThreads / (NB * 4);
-  const int64_t blocks = (static_cast<int64_t>(p.B) * p.Ht * p.pairs + per - 1) / per;
+  const int64_t per = kRowThreads / (NB * 16);
+  const int64_t blocks = (static_cast<int64_t>(p.B) * p.Ht * p.octets + per - 1) / per;
   if (blocks > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4 rows: too many rows for one launch");
   const unsigned g = static_cast<unsigned>(blocks);
   if (append) {
@@ -285,16 +282,14 @@ int rows_call(const iak_fp4_pool* pool, const iak_fp4_rows_args* a, bool append,
   if (!a->k || !a->v || (a->table_width > 0 && !a->page_table))
     return fail(IAK_ERR_INVALID_ARG, "%s: null k, v or page_table", what);
   RowsParams p;
-  p.pool = {static_cast<uint8_t*>(pool->k_codes), static_cast<uint8_t*>(pool->k_scales),
-            static_cast<uint8_t*>(pool->v_codes), static_cast<uint8_t*>(pool->v_scales), pool->num_pages,
-            pool->page_size, pool->head_dim};
+  p.pool = {static_cast<uint8_t*>(pool->data), pool->num_pages, pool->page_size, pool->head_dim};
   p.k = a->k; p.v = a->v; p.dtype = a->dtype;
   p.k_sb = a->k_stride_b; p.k_sh = a->k_stride_h; p.k_sn = a->k_stride_n;
   p.v_sb = a->v_stride_b; p.v_sh = a->v_stride_h; p.v_sn = a->v_stride_n;
   p.B = a->batch; p.Ht = a->num_table_heads; p.N = a->num_rows;
   p.pt = a->page_table; p.pt_sb = a->pt_stride_b; p.pt_sh = a->pt_stride_h; p.W = a->table_width;
   p.positions = a->positions; p.counts = a->counts; p.dropped = a->dropped;
-  p.pairs = a->num_rows / 2 + 1;
+  p.octets = (static_cast<int64_t>(a->num_rows) + 14) / 8;
   // 16-byte accesses need every row start on 16 bytes
   const int64_t per16 = a->dtype == IAK_DT_F32 ? 4 : 8;
   bool vec = reinterpret_cast<uintptr_t>(a->k) % 16 == 0 && reinterpret_cast<uintptr_t>(a->v) % 16 == 0;
@@ -314,11 +309,9 @@ int check_fp4_pool(const iak_fp4_pool* pool, const char* what) {
     return fail(IAK_ERR_UNSUPPORTED, "%s: page_size %d is not a multiple of 16", what, pool->page_size);
   if (pool->num_pages < 0 || pool->num_pages > 0x7fffffffLL)
     return fail(IAK_ERR_INVALID_ARG, "%s: num_pages out of range", what);
-  for (const void* ptr : {pool->k_codes, pool->k_scales, pool->v_codes, pool->v_scales}) {
-    if (!ptr && pool->num_pages > 0) return fail(IAK_ERR_INVALID_ARG, "%s: null pool plane", what);
-    if (reinterpret_cast<uintptr_t>(ptr) % 16)
-      return fail(IAK_ERR_INVALID_ARG, "%s: pool planes must be 16-byte aligned", what);
-  }
+  if (!pool->data && pool->num_pages > 0) return fail(IAK_ERR_INVALID_ARG, "%s: null pool data", what);
+  if (reinterpret_cast<uintptr_t>(pool->data) % 16)
+    return fail(IAK_ERR_INVALID_ARG, "%s: pool data must be 16-byte aligned", what);
   return IAK_OK;
 }
 

@@ -168,7 +168,7 @@ FP4_MAX_QUERIES = 16
 
 
 class Fp4PoolStruct(ctypes.Structure):
-    _fields_ = [("k_codes", c_void_p), ("k_scales", c_void_p), ("v_codes", c_void_p), ("v_scales", c_void_p),
+    _fields_ = [("data", c_void_p),
                 ("num_pages", c_i64), ("page_size", c_i32), ("head_dim", c_i32)]
 
 

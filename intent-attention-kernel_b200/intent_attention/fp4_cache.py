@@ -27,120 +27,118 @@ from typing import Optional, Tuple
 import torch
 
 from . import _native as N
-from .paged import _DT, _ptr, _require_cuda, _stream
+from .paged import _DT, _require_cuda
 
 HEAD_DIMS = (64, 128, 256)
+
+# Per-call host work is most of a small call's time, so the helpers below test the few properties that the kernels rely
+# on and build their messages only when one fails.
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_NO_SWITCH = contextlib.nullcontext()
 
 
 def _on(device: torch.device):
     """The library launches on the current device; switch only when it is another one."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index is None or device.index == _current_device():
+        return _NO_SWITCH
     return torch.cuda.device(device)
 
 
+def _raw_stream(device: torch.device) -> int:
+    if device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _index_tensor(t: Optional[torch.Tensor], name: str, device: torch.device, numel: Optional[int] = None):
-    """An int32 vector on ``device`` with unit stride; None passes."""
+    """Address of a contiguous int32 tensor on ``device``; None passes."""
     if t is None:
         return None
-    _require_cuda(t, name)
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _require_cuda(t, name)
     if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the pool on {device}")
-    if t.dtype != torch.int32 or not t.is_contiguous():
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype is not torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor")
     if numel is not None and t.numel() != numel:
         raise ValueError(f"{name} must have {numel} entries, got {t.numel()}")
-    return t
+    return t.data_ptr()
 
 
-def _page_table(page_table: torch.Tensor, device: torch.device, batch: Optional[int] = None,
-                heads: Optional[int] = None) -> torch.Tensor:
-    _require_cuda(page_table, "page_table")
-    if page_table.device != device:
-        raise ValueError(f"page_table is on {page_table.device}, the pool on {device}")
-    if page_table.dim() != 3 or page_table.dtype != torch.int32:
+def _page_table(t: torch.Tensor, device: torch.device, batch: Optional[int] = None, heads: Optional[int] = None):
+    """(address, stride of b, stride of h, Ht, W) of an int32 [B, Ht, W] table."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _require_cuda(t, "page_table")
+    if t.device != device:
+        raise ValueError(f"page_table is on {t.device}, expected {device}")
+    if t.dim() != 3 or t.dtype is not torch.int32:
         raise ValueError("page_table must be int32 [B, Ht, W]")
-    if page_table.stride(2) != 1 and page_table.shape[2] > 1:
+    B, Ht, W = t.shape
+    sb, sh, sw = t.stride()
+    if sw != 1 and W > 1:
         raise ValueError("page_table rows must be contiguous")
-    if (batch is not None and page_table.shape[0] != batch) or (heads is not None and page_table.shape[1] != heads):
-        raise ValueError(f"page_table must be [{batch}, {heads if heads is not None else 'Ht'}, W], "
-                         f"got {tuple(page_table.shape)}")
-    return page_table
+    if (batch is not None and B != batch) or (heads is not None and Ht != heads):
+        raise ValueError(f"page_table must be [{batch}, {heads if heads is not None else 'Ht'}, W], got {(B, Ht, W)}")
+    return t.data_ptr(), sb, sh, Ht, W
 
 
 @dataclass
 class Fp4Pool:
     """K/V pages of one layer on one device in 4-bit floating point.
 
-    The byte order inside a page is the kernels' own (``include/intent_attention_b200.h``);
-    ``append_fp4`` writes it and ``read_fp4`` reads it back.
+    ``data`` uint8 [num_pages, page_size / 16, 17 * head_dim] holds 16 rows of K and V, codes and scales, in each
+    last dimension.  The byte order there is the kernels' own (``include/intent_attention_b200.h``); ``append_fp4``
+    writes it and ``read_fp4`` reads it back.
     """
 
     num_pages: int
     page_size: int
     head_dim: int
-    k_codes: torch.Tensor
-    k_scales: torch.Tensor
-    v_codes: torch.Tensor
-    v_scales: torch.Tensor
+    data: torch.Tensor
 
     @classmethod
     def allocate(cls, num_pages: int, page_size: int, head_dim: int, device="cuda", zero: bool = False) -> "Fp4Pool":
-        """A pool of ``num_pages`` pages; ``zero`` clears the codes too (the scales always start at 0)."""
+        """A pool of ``num_pages`` pages (``zero``: all rows 0; otherwise rows hold nothing until written)."""
         if head_dim not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
         if page_size <= 0 or page_size % 16:
             raise ValueError(f"page_size must be a positive multiple of 16, got {page_size}")
         if num_pages < 0:
             raise ValueError("num_pages must not be negative")
-        dev = torch.device(device)
-        codes, scales = (num_pages, page_size, head_dim // 2), (num_pages, page_size, head_dim // 32)
         mk = torch.zeros if zero else torch.empty
         return cls(num_pages, page_size, head_dim,
-                   mk(codes, dtype=torch.uint8, device=dev), torch.zeros(scales, dtype=torch.uint8, device=dev),
-                   mk(codes, dtype=torch.uint8, device=dev), torch.zeros(scales, dtype=torch.uint8, device=dev))
+                   mk((num_pages, page_size // 16, 17 * head_dim), dtype=torch.uint8, device=torch.device(device)))
 
     @property
     def device(self) -> torch.device:
-        return self.k_codes.device
+        return self.data.device
 
     def tensors(self):
-        return [self.k_codes, self.k_scales, self.v_codes, self.v_scales]
+        return [self.data]
 
     def nbytes(self) -> int:
-        return sum(t.numel() for t in self.tensors())
+        return self.data.numel()
 
     def struct(self) -> N.Fp4PoolStruct:
-        s = N.Fp4PoolStruct()
-        rows = self.num_pages * self.page_size
-        for name, t, per in (("k_codes", self.k_codes, 2), ("k_scales", self.k_scales, 32),
-                             ("v_codes", self.v_codes, 2), ("v_scales", self.v_scales, 32)):
-            _require_cuda(t, name)
-            if t.device != self.device:
-                raise ValueError("the pool's planes lie on different devices")
-            if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() != rows * (self.head_dim // per):
-                raise ValueError(f"{name} must be contiguous uint8 of {rows * (self.head_dim // per)} bytes")
-            setattr(s, name, t.data_ptr())
-        s.num_pages, s.page_size, s.head_dim = self.num_pages, self.page_size, self.head_dim
-        return s
+        t = self.data
+        if not t.is_cuda:
+            _require_cuda(t, "pool data")
+        if t.dtype is not torch.uint8 or not t.is_contiguous() \
+                or t.numel() != self.num_pages * (self.page_size // 16) * 17 * self.head_dim:
+            raise ValueError("pool data must be contiguous uint8 [num_pages, page_size / 16, 17 * head_dim]")
+        return N.Fp4PoolStruct(t.data_ptr(), self.num_pages, self.page_size, self.head_dim)
 
 
 # ---------------------------------------------------------------------- #
 #  Rows in and out
 # ---------------------------------------------------------------------- #
 
-def _rows_args(pool: Fp4Pool, k, v, page_table, positions, counts) -> N.Fp4RowsArgs:
+def _rows_args(dev, k, v, page_table, positions, counts, dropped=None) -> N.Fp4RowsArgs:
     B, Ht, n, _ = k.shape
-    a = N.Fp4RowsArgs()
-    a.k, a.v, a.dtype = k.data_ptr(), v.data_ptr(), _DT[k.dtype]
-    a.k_stride_b, a.k_stride_h, a.k_stride_n = k.stride(0), k.stride(1), k.stride(2)
-    a.v_stride_b, a.v_stride_h, a.v_stride_n = v.stride(0), v.stride(1), v.stride(2)
-    a.batch, a.num_table_heads, a.num_rows = B, Ht, n
-    pt = _page_table(page_table, pool.device, B, Ht)
-    a.page_table, a.pt_stride_b, a.pt_stride_h, a.table_width = pt.data_ptr(), pt.stride(0), pt.stride(1), pt.shape[2]
-    a.positions = _ptr(_index_tensor(positions, "positions", pool.device, B))
-    a.counts = _ptr(_index_tensor(counts, "counts", pool.device, B))
-    return a
+    pt, pt_sb, pt_sh, _, W = _page_table(page_table, dev, B, Ht)
+    return N.Fp4RowsArgs(k.data_ptr(), v.data_ptr(), _DT[k.dtype], *k.stride()[:3], *v.stride()[:3], B, Ht, n,
+                         pt, pt_sb, pt_sh, W, _index_tensor(positions, "positions", dev, B),
+                         _index_tensor(counts, "counts", dev, B), _index_tensor(dropped, "dropped", dev, 1))
 
 
 def append_fp4(pool: Fp4Pool, k_new: torch.Tensor, v_new: torch.Tensor, page_table: torch.Tensor,
@@ -156,10 +154,11 @@ def append_fp4(pool: Fp4Pool, k_new: torch.Tensor, v_new: torch.Tensor, page_tab
     belong to one (b, h) each, and a sequence is written by one call at a time:
     two rows of V share their bytes.
     """
+    dev = pool.device
     for name, x in (("k_new", k_new), ("v_new", v_new)):
         _require_cuda(x, name)
-        if x.device != pool.device:
-            raise ValueError(f"{name} is on {x.device}, the pool on {pool.device}")
+        if x.device != dev:
+            raise ValueError(f"{name} is on {x.device}, the pool on {dev}")
     if k_new.dim() != 4 or k_new.shape != v_new.shape or k_new.shape[3] != pool.head_dim:
         raise ValueError(f"k_new / v_new must both be [B, Ht, n, {pool.head_dim}]")
     if k_new.dtype != v_new.dtype or k_new.dtype not in _DT:
@@ -168,11 +167,10 @@ def append_fp4(pool: Fp4Pool, k_new: torch.Tensor, v_new: torch.Tensor, page_tab
         k_new = k_new.contiguous()
     if v_new.stride(3) != 1:
         v_new = v_new.contiguous()
-    a = _rows_args(pool, k_new, v_new, page_table, positions, counts)
-    a.dropped = _ptr(_index_tensor(dropped, "dropped", pool.device, 1))
+    a = _rows_args(dev, k_new, v_new, page_table, positions, counts, dropped)
     s = pool.struct()
-    with _on(pool.device):
-        N.check(N.lib().iak_fp4_append(ctypes.byref(s), ctypes.byref(a), _stream(pool.device)), "iak_fp4_append")
+    with _on(dev):
+        N.check(N.lib().iak_fp4_append(ctypes.byref(s), ctypes.byref(a), _raw_stream(dev)), "iak_fp4_append")
 
 
 def read_fp4(pool: Fp4Pool, page_table: torch.Tensor, positions: Optional[torch.Tensor], num_rows: int,
@@ -182,26 +180,27 @@ def read_fp4(pool: Fp4Pool, page_table: torch.Tensor, positions: Optional[torch.
     [B, Ht, num_rows, D].  Every value a pool holds is exact in all three float
     types.  Rows from ``counts[b]`` on, and rows of slots or pages that do not
     exist, are 0.  ``out``: a (k, v) pair to write into."""
-    _page_table(page_table, pool.device)
+    dev = pool.device
+    _page_table(page_table, dev)
     if num_rows < 0:
         raise ValueError("num_rows must not be negative")
     shape = (page_table.shape[0], page_table.shape[1], num_rows, pool.head_dim)
     if out is None:
         if dtype not in _DT:
             raise ValueError("dtype must be float32 / float16 / bfloat16")
-        k, v = (torch.empty(shape, dtype=dtype, device=pool.device) for _ in range(2))
+        k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
     else:
         k, v = out
         for name, x in (("out[0]", k), ("out[1]", v)):
             _require_cuda(x, name)
-            if tuple(x.shape) != shape or x.device != pool.device or x.dtype not in _DT or x.dtype != k.dtype:
-                raise ValueError(f"{name} must be a {shape} float tensor on {pool.device}, both of one dtype")
+            if tuple(x.shape) != shape or x.device != dev or x.dtype not in _DT or x.dtype != k.dtype:
+                raise ValueError(f"{name} must be a {shape} float tensor on {dev}, both of one dtype")
             if x.stride(3) != 1:
                 raise ValueError(f"{name} needs a unit stride along head_dim")
-    a = _rows_args(pool, k, v, page_table, positions, counts)
+    a = _rows_args(dev, k, v, page_table, positions, counts)
     s = pool.struct()
-    with _on(pool.device):
-        N.check(N.lib().iak_fp4_read(ctypes.byref(s), ctypes.byref(a), _stream(pool.device)), "iak_fp4_read")
+    with _on(dev):
+        N.check(N.lib().iak_fp4_read(ctypes.byref(s), ctypes.byref(a), _raw_stream(dev)), "iak_fp4_read")
     return k, v
 
 
@@ -225,40 +224,36 @@ def _decode(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Tensor, lengths: t
     M = q.shape[2] if q.dim() == 4 else 1
     if M > N.FP4_MAX_QUERIES:
         raise ValueError(f"at most {N.FP4_MAX_QUERIES} queries per sequence, got {M}: read_fp4 the context for a prompt")
-    pt = _page_table(page_table, dev, B)
-    Ht = pt.shape[1]
+    pt, pt_sb, pt_sh, Ht, W = _page_table(page_table, dev, B)
     if Hq and (Ht == 0 or Hq % Ht):
         raise ValueError(f"query heads ({Hq}) must be a multiple of page-table heads ({Ht})")
     if lengths is None:
         raise ValueError("lengths [B] is required")
-    _index_tensor(lengths, "lengths", dev, B)
+    ln = _index_tensor(lengths, "lengths", dev, B)
     if out is None:
         out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
-    _require_cuda(out, "out")
-    if out.shape != q.shape or out.device != dev or out.dtype not in _DT or out.stride(-1) != 1:
-        raise ValueError(f"out must be a {tuple(q.shape)} float tensor on {dev} with a contiguous last dim")
-    a = N.Fp4DecodeArgs()
-    a.q, a.q_dtype, a.q_stride_b, a.q_stride_h = q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1)
-    a.out, a.out_dtype, a.out_stride_b, a.out_stride_h = out.data_ptr(), _DT[out.dtype], out.stride(0), out.stride(1)
-    if q.dim() == 4:
-        a.q_stride_m, a.out_stride_m = q.stride(2), out.stride(2)
-    a.batch, a.num_q_heads, a.num_table_heads, a.num_queries = B, Hq, Ht, M
-    a.page_table, a.pt_stride_b, a.pt_stride_h, a.table_width = pt.data_ptr(), pt.stride(0), pt.stride(1), pt.shape[2]
-    a.lengths, a.sm_scale = lengths.data_ptr(), sm_scale
+        if out.dtype not in _DT:
+            raise ValueError(f"out dtype {out.dtype} unsupported")
+    else:
+        _require_cuda(out, "out")
+        if out.shape != q.shape or out.device != dev or out.dtype not in _DT or out.stride(-1) != 1:
+            raise ValueError(f"out must be a {tuple(q.shape)} float tensor on {dev} with a contiguous last dim")
+    qs, os_ = q.stride(), out.stride()
+    a = N.Fp4DecodeArgs(q.data_ptr(), _DT[q.dtype], qs[0], qs[1], qs[2] if q.dim() == 4 else 0,
+                        out.data_ptr(), _DT[out.dtype], os_[0], os_[1], os_[2] if q.dim() == 4 else 0,
+                        B, Hq, Ht, M, pt, pt_sb, pt_sh, W, ln, sm_scale)
     if differential is not None:
-        lam, norm_weight, eps, out_scale = differential
-        a.differential, a.lam, a.norm_weight = 1, lam.data_ptr(), _ptr(norm_weight)
-        a.eps, a.out_scale = eps, out_scale
+        a.differential, a.lam, a.norm_weight, a.eps, a.out_scale = (1, *differential)
     s = pool.struct()
     L = N.lib()
     nbytes = ctypes.c_size_t(0)
+    ps, pa = ctypes.byref(s), ctypes.byref(a)
     with _on(dev):
-        N.check(L.iak_fp4_decode_workspace_size(ctypes.byref(s), ctypes.byref(a), ctypes.byref(nbytes)),
-                "iak_fp4_decode_workspace_size")
+        N.check(L.iak_fp4_decode_workspace_size(ps, pa, ctypes.byref(nbytes)), "iak_fp4_decode_workspace_size")
+        n = nbytes.value
         # of this call alone: calls on other streams, or captured into other graphs, never share it
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev) if nbytes.value else None
-        N.check(L.iak_fp4_decode(ctypes.byref(s), ctypes.byref(a), _ptr(ws), nbytes.value, _stream(dev)),
-                "iak_fp4_decode")
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        N.check(L.iak_fp4_decode(ps, pa, ws.data_ptr() if n else None, n, _raw_stream(dev)), "iak_fp4_decode")
     return out
 
 
@@ -294,16 +289,15 @@ def differential_decode_fp4(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Te
     """
     def weight(t, name, n):
         _require_cuda(t, name)
-        if t.device != pool.device or t.dtype != torch.float32 or t.numel() != n or not t.is_contiguous():
+        if t.device != pool.device or t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
             raise ValueError(f"{name} must be {n} contiguous float32 values on {pool.device}")
-        return t
+        return t.data_ptr()
 
     if not isinstance(q, torch.Tensor) or q.dim() < 2:
         raise ValueError("q must be [B, Hq, D] or [B, Hq, M, D]")
-    weight(lam, "lam", q.shape[1])
-    if norm_weight is not None:
-        weight(norm_weight, "norm_weight", pool.head_dim)
+    lam_ptr = weight(lam, "lam", q.shape[1])
+    norm_ptr = None if norm_weight is None else weight(norm_weight, "norm_weight", pool.head_dim)
     if not (eps >= 0.0 and math.isfinite(eps) and math.isfinite(out_scale)):
         raise ValueError("eps must be finite and not negative, out_scale finite")
     scale = 1.0 / math.sqrt(pool.head_dim // 2) if sm_scale is None else float(sm_scale)
-    return _decode(q, pool, page_table, lengths, scale, out, out_dtype, (lam, norm_weight, float(eps), float(out_scale)))
+    return _decode(q, pool, page_table, lengths, scale, out, out_dtype, (lam_ptr, norm_ptr, float(eps), float(out_scale)))

@@ -22,8 +22,8 @@ from typing import Optional, Sequence, Union
 import torch
 
 from . import _native as N
-from .fp4_cache import Fp4Pool, _index_tensor, _on
-from .paged import PagePool, _ptr, _require_cuda, _stream, _tags_args
+from .fp4_cache import Fp4Pool, _index_tensor, _on, _page_table, _raw_stream
+from .paged import PagePool, _require_cuda, _tags_args
 
 _BIT = {f: 1 << getattr(N, f"FMT_{f}") for f in ("F16", "FP8", "INT8", "INT4", "INT4R")}
 _SCALED = _BIT["FP8"] | _BIT["INT8"] | _BIT["INT4"] | _BIT["INT4R"]
@@ -50,64 +50,60 @@ class SequencePages:
                    torch.zeros(num_slots, dtype=torch.int32, device=dev), page_size)
 
     def struct(self) -> N.SeqPages:
+        if not self.refs.is_cuda:
+            _require_cuda(self.refs, "refs")
         dev = self.refs.device
-        _index_tensor(self.refs, "refs", dev)
-        _index_tensor(self.lengths, "lengths", dev)
-        _require_cuda(self.table, "table")
-        t = self.table
-        if t.device != dev or t.dtype != torch.int32 or t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
-            raise ValueError(f"table must be int32 [slots, Ht, W] with contiguous rows on {dev}")
-        if self.lengths.numel() != t.shape[0]:
-            raise ValueError(f"lengths must have {t.shape[0]} entries, got {self.lengths.numel()}")
         if self.page_size <= 0:
             raise ValueError("page_size must be positive")
-        s = N.SeqPages()
-        s.refs, s.num_pages = self.refs.data_ptr(), self.refs.numel()
-        s.page_table, s.pt_stride_s, s.pt_stride_h, s.table_width = t.data_ptr(), t.stride(0), t.stride(1), t.shape[2]
-        s.lengths, s.num_slots, s.num_table_heads = self.lengths.data_ptr(), t.shape[0], t.shape[1]
-        s.page_size = self.page_size
-        return s
+        pt, ss, sh, Ht, W = _page_table(self.table, dev)
+        slots = self.table.shape[0]
+        return N.SeqPages(_index_tensor(self.refs, "refs", dev), self.refs.numel(), pt, ss, sh, W,
+                          _index_tensor(self.lengths, "lengths", dev, slots), slots, Ht, self.page_size)
 
 
 def _planes(pool: Union[PagePool, Fp4Pool], pages: SequencePages, page_tags, tag_map, tag_default) -> N.PagePlanes:
     if pool.num_pages != pages.refs.numel() or pool.page_size != pages.page_size:
         raise ValueError(f"pages count {pages.refs.numel()} pages of {pages.page_size} rows, the pool has "
                          f"{pool.num_pages} of {pool.page_size}")
+    dev = pages.refs.device
     if isinstance(pool, Fp4Pool):
-        pool.struct()                         # checks the planes
         named = [(t, 0) for t in pool.tensors()]
     else:
         named = [(getattr(pool, f"{side}_{n}"), f) for n, f in _PLANE_FORMATS.items() for side in ("k", "v")]
         named = [(t, f) for t, f in named if t is not None]
     s = N.PagePlanes()
-    for i, (t, formats) in enumerate(named):
-        _require_cuda(t, "page pool")
-        if t.device != pages.refs.device:
-            raise ValueError(f"the pool is on {t.device}, its pages on {pages.refs.device}")
+    n = 0
+    for t, formats in named:
+        if not t.is_cuda:
+            _require_cuda(t, "page pool")
+        if t.device != dev:
+            raise ValueError(f"the pool is on {t.device}, its pages on {dev}")
         if not t.is_contiguous() or t.shape[0] != pool.num_pages:
             raise ValueError("page pools must be contiguous [num_pages, ...] tensors")
-        if t.numel():
-            s.base[i], s.bytes[i], s.formats[i] = t.data_ptr(), t.numel() // pool.num_pages * t.element_size(), formats
-            s.num_planes = i + 1
+        size = t.numel() * t.element_size()
+        if size:
+            s.base[n], s.bytes[n], s.formats[n] = t.data_ptr(), size // pool.num_pages, formats
+            n += 1
+    s.num_planes = n
     if page_tags is not None:
         if isinstance(pool, Fp4Pool):
             raise ValueError("an Fp4Pool has one format: no page_tags")
         if tag_map is None:
             raise ValueError("page_tags needs a tag_map")
         s.page_tags, s.tag_bytes = _tags_args(page_tags)
-        if page_tags.numel() < pool.num_pages or page_tags.device != pages.refs.device:
-            raise ValueError(f"page_tags must hold {pool.num_pages} tags on {pages.refs.device}")
+        if page_tags.numel() < pool.num_pages or page_tags.device != dev:
+            raise ValueError(f"page_tags must hold {pool.num_pages} tags on {dev}")
         for i, f in enumerate(tag_map):
             s.tag_map[i] = f
         s.tag_default = tag_default
     return s
 
 
-def _workspace(pages: SequencePages, s: N.SeqPages) -> torch.Tensor:
+def _workspace(dev: torch.device, s: N.SeqPages) -> torch.Tensor:
     n = ctypes.c_size_t(0)
     N.check(N.lib().iak_pages_workspace_size(ctypes.byref(s), ctypes.byref(n)), "iak_pages_workspace_size")
     # of this call alone, as calls captured into different graphs must not share it
-    return torch.empty(n.value, dtype=torch.uint8, device=pages.refs.device)
+    return torch.empty(n.value, dtype=torch.uint8, device=dev)
 
 
 def grow_sequences(pool: Union[PagePool, Fp4Pool], pages: SequencePages, new_tokens: torch.Tensor,
@@ -125,13 +121,14 @@ def grow_sequences(pool: Union[PagePool, Fp4Pool], pages: SequencePages, new_tok
     every later one that gets tokens.
     """
     s = pages.struct()
-    _index_tensor(new_tokens, "new_tokens", pages.refs.device, pages.table.shape[0])
-    _index_tensor(rejected, "rejected", pages.refs.device, 1)
+    dev = pages.refs.device
+    more = _index_tensor(new_tokens, "new_tokens", dev, s.num_slots)
+    count = _index_tensor(rejected, "rejected", dev, 1)
     pl = _planes(pool, pages, page_tags, tag_map, tag_default)
-    with _on(pages.refs.device):
-        ws = _workspace(pages, s)
-        N.check(N.lib().iak_pages_grow(ctypes.byref(s), ctypes.byref(pl), new_tokens.data_ptr(), _ptr(rejected),
-                                       ws.data_ptr(), ws.numel(), _stream(pages.refs.device)), "iak_pages_grow")
+    with _on(dev):
+        ws = _workspace(dev, s)
+        N.check(N.lib().iak_pages_grow(ctypes.byref(s), ctypes.byref(pl), more, count, ws.data_ptr(), ws.numel(),
+                                       _raw_stream(dev)), "iak_pages_grow")
 
 
 def fork_sequences(pages: SequencePages, src: torch.Tensor, dst: torch.Tensor,
@@ -142,23 +139,23 @@ def fork_sequences(pages: SequencePages, src: torch.Tensor, dst: torch.Tensor,
     a src that is also a dst of the call.
     """
     s = pages.struct()
-    _index_tensor(src, "src", pages.refs.device)
-    _index_tensor(dst, "dst", pages.refs.device, src.numel())
-    _index_tensor(rejected, "rejected", pages.refs.device, 1)
-    with _on(pages.refs.device):
-        N.check(N.lib().iak_pages_fork(ctypes.byref(s), src.data_ptr(), dst.data_ptr(), src.numel(), _ptr(rejected),
-                                       _stream(pages.refs.device)), "iak_pages_fork")
+    dev = pages.refs.device
+    a, n = _index_tensor(src, "src", dev), src.numel()
+    b = _index_tensor(dst, "dst", dev, n)
+    count = _index_tensor(rejected, "rejected", dev, 1)
+    with _on(dev):
+        N.check(N.lib().iak_pages_fork(ctypes.byref(s), a, b, n, count, _raw_stream(dev)), "iak_pages_fork")
 
 
 def free_sequences(pages: SequencePages, slots: torch.Tensor, rejected: Optional[torch.Tensor] = None) -> None:
     """The listed slots (int32 on the device) let go of their pages: table entries -1, length 0.  A slot listed
     twice is freed once; one out of range is refused."""
     s = pages.struct()
-    _index_tensor(slots, "slots", pages.refs.device)
-    _index_tensor(rejected, "rejected", pages.refs.device, 1)
-    with _on(pages.refs.device):
-        N.check(N.lib().iak_pages_free(ctypes.byref(s), slots.data_ptr(), slots.numel(), _ptr(rejected),
-                                       _stream(pages.refs.device)), "iak_pages_free")
+    dev = pages.refs.device
+    a = _index_tensor(slots, "slots", dev)
+    count = _index_tensor(rejected, "rejected", dev, 1)
+    with _on(dev):
+        N.check(N.lib().iak_pages_free(ctypes.byref(s), a, slots.numel(), count, _raw_stream(dev)), "iak_pages_free")
 
 
 def compact_pages(pool: Union[PagePool, Fp4Pool], pages: SequencePages, page_tags: Optional[torch.Tensor] = None,
@@ -170,10 +167,11 @@ def compact_pages(pool: Union[PagePool, Fp4Pool], pages: SequencePages, page_tag
     planes of each page's format move, and its tag.
     """
     s = pages.struct()
+    dev = pages.refs.device
     pl = _planes(pool, pages, page_tags, tag_map, tag_default)
-    live = torch.empty((), dtype=torch.int32, device=pages.refs.device)
-    with _on(pages.refs.device):
-        ws = _workspace(pages, s)
+    live = torch.empty((), dtype=torch.int32, device=dev)
+    with _on(dev):
+        ws = _workspace(dev, s)
         N.check(N.lib().iak_pages_compact(ctypes.byref(s), ctypes.byref(pl), live.data_ptr(), ws.data_ptr(),
-                                          ws.numel(), _stream(pages.refs.device)), "iak_pages_compact")
+                                          ws.numel(), _raw_stream(dev)), "iak_pages_compact")
     return live

@@ -52,7 +52,7 @@ def test_oracle_values():
 
 def _pool():
     p = N.Fp4PoolStruct()
-    p.k_codes = p.k_scales = p.v_codes = p.v_scales = 256
+    p.data = 256
     p.num_pages, p.page_size, p.head_dim = 4, 16, 128
     return p
 
@@ -69,8 +69,8 @@ def test_fp4_args_rejected_on_the_host():
         assert fn(r(p), r(a), None) == N.IAK_ERR_INVALID_ARG
         a.dtype = 0
         for field, value, want in (("head_dim", 96, N.IAK_ERR_UNSUPPORTED), ("page_size", 24, N.IAK_ERR_UNSUPPORTED),
-                                   ("page_size", 0, N.IAK_ERR_UNSUPPORTED), ("k_codes", 8, N.IAK_ERR_INVALID_ARG),
-                                   ("v_scales", None, N.IAK_ERR_INVALID_ARG), ("num_pages", -1, N.IAK_ERR_INVALID_ARG)):
+                                   ("page_size", 0, N.IAK_ERR_UNSUPPORTED), ("data", 8, N.IAK_ERR_INVALID_ARG),
+                                   ("data", None, N.IAK_ERR_INVALID_ARG), ("num_pages", -1, N.IAK_ERR_INVALID_ARG)):
             p = _pool()
             setattr(p, field, value)
             assert fn(r(p), r(a), None) == want, field
