@@ -14,7 +14,7 @@
 // (sequence, table head, column group) units, one run per resident block, so that ragged batches and single long
 // sequences fill the GPU alike; a unit cut over several blocks leaves partial (m, l, O) that a second kernel joins in
 // order of the blocks (no atomics: results do not depend on timing).  Each warp streams its own tiles through a
-// ring of bulk copies, one per 16 rows (32 where a page holds both): a group's codes and scales lie together in the
+// ring of bulk copies, one per 16 rows: a group's codes and scales lie together in the
 // order in which lanes read them, so a copy needs no address arithmetic beyond its start and reads are free of bank
 // conflicts.
 #include <algorithm>
@@ -37,7 +37,6 @@ constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small 
 struct DecP {
   Fp4Pool pool;
   int gpp;                           // groups of 16 rows per page
-  int step_slot, step_sub;           // what kWarps tiles move a group's (table entry, group of the page) by
   const void* q; int q_dtype; int64_t q_sb, q_sh, q_sm;
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sm;
   int B, Hq, Ht, G, M;
@@ -217,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
   const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
   const unsigned ring = smem_base + warp * L::kStages * L::kStage;
   const unsigned bar = static_cast<unsigned>(__cvta_generic_to_shared(bars)) + warp * L::kStages * 8;
-  if (lane < L::kStages) tc::mbar_init(bar + lane * 8, 1);
+  if (lane < L::kStages) tc::mbar_init(bar + lane * 8, 2);   // a stage's two groups arrive apart
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   tc::fence_proxy_async();
   __syncwarp();
@@ -252,6 +251,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
     const int c_end = static_cast<int>(min(static_cast<int64_t>(n_tiles), c_begin + left));
     const int h = unit / p.CG, cg = unit - h * p.CG;
     const int32_t* table = p.pt + b * p.pt_sb + h * p.pt_sh;
+    const int full_end = len - (p.M - 1);         // every query sees the tokens before it
 
     // queries: 8 channels per thread, halves after a power of two that puts the row's largest in [1, 2)
     constexpr int CH = D / 8;
@@ -301,42 +301,45 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
       sc[nt][1] = col_scale[nt * 8 + 2 * t + 1];
     }
 
-    // ----------------------------------------------------- the copies' cursor
-    int c_fetch = c_begin + warp;                 // tile whose page ids are read next
-    int slot = (c_fetch * 2) / p.gpp, sub = c_fetch * 2 - slot * p.gpp;
-    int id[2], at_sub;                            // of the tile fetched last
-    auto fetch = [&]() {
-      at_sub = sub;
-      id[0] = id[1] = -1;
-      if (c_fetch < c_end) {
-        const int s1 = sub + 1 == p.gpp ? slot + 1 : slot;
-        if (c_fetch * kTileKeys < len) id[0] = __ldg(table + slot);
-        if (c_fetch * kTileKeys + 16 < len) id[1] = __ldg(table + s1);
-      }
-      c_fetch += kWarps;
-      slot += p.step_slot;
-      sub += p.step_sub;
-      if (sub >= p.gpp) { sub -= p.gpp; ++slot; }
+    // ---------------------------------------------------------- copies
+    // The warp's tiles are c_begin + warp + kWarps k.  Of every 16 of them lane 2 i + u owns group u of tile i: it
+    // reads the page id (a batch ahead), holds the source address and issues the copy.
+    const int first = c_begin + warp;
+    const int n_mine = c_end > first ? (c_end - first + kWarps - 1) / kWarps : 0;
+    auto group_of = [&](int k) { return (first + kWarps * (k + (lane >> 1))) * 2 + (lane & 1); };
+    auto load_id = [&](int k) {
+      const int gr = group_of(k);
+      return k + (lane >> 1) < n_mine && gr * 16 < len ? __ldg(table + static_cast<unsigned>(gr) / p.gpp) : -1;
     };
-    unsigned ok_bits = 0;                         // [stage][group]: the group's page exists
-    auto issue = [&](int stage) {
-      const bool ok0 = id[0] >= 0 && id[0] < p.pool.num_pages, ok1 = id[1] >= 0 && id[1] < p.pool.num_pages;
-      ok_bits = (ok_bits & ~(3u << (2 * stage))) | ((ok0 ? 1u : 0u) | (ok1 ? 2u : 0u)) << (2 * stage);
-      if (lane == 0) {
-        const unsigned to = ring + stage * L::kStage, full = bar + stage * 8;
-        const bool wraps = at_sub + 1 == p.gpp;
-        const uint8_t* g0 = p.pool.data + (static_cast<int64_t>(id[0]) * p.gpp + at_sub) * Gr::kBytes;
-        tc::mbar_arrive_expect_tx(full, (ok0 ? Gr::kBytes : 0) + (ok1 ? Gr::kBytes : 0));
-        if (ok0 && ok1 && !wraps) {
-          tc::bulk_load(to, g0, 2 * Gr::kBytes, full);
-        } else {
-          if (ok0) tc::bulk_load(to, g0, Gr::kBytes, full);
-          const int sub1 = wraps ? 0 : at_sub + 1;
-          if (ok1)
-            tc::bulk_load(to + Gr::kBytes, p.pool.data + (static_cast<int64_t>(id[1]) * p.gpp + sub1) * Gr::kBytes,
-                          Gr::kBytes, full);
+    const uint8_t* src = nullptr;
+    bool src_ok = false;
+    unsigned batch_ok = 0;
+    auto take_batch = [&](int k, int id) {
+      const unsigned sub = static_cast<unsigned>(group_of(k)) % p.gpp;
+      src_ok = id >= 0 && id < p.pool.num_pages;
+      src = p.pool.data + (static_cast<int64_t>(id) * p.gpp + sub) * Gr::kBytes;
+      batch_ok = __ballot_sync(~0u, src_ok);
+    };
+    int next_id = load_id(0);
+    int k_issue = 0;
+    unsigned history = 0;                         // two bits per tile issued, the last in bits 0, 1: its pages exist
+    unsigned to_stage = stage;
+    auto issue = [&]() {
+      if (k_issue < n_mine) {
+        const int i = k_issue & 15;
+        if (i == 0) {
+          take_batch(k_issue, next_id);
+          next_id = load_id(k_issue + 16);
         }
+        if ((lane >> 1) == i) {
+          const unsigned full = bar + to_stage * 8;
+          tc::mbar_arrive_expect_tx(full, src_ok ? Gr::kBytes : 0);
+          if (src_ok) tc::bulk_load(ring + to_stage * L::kStage + (lane & 1) * Gr::kBytes, src, Gr::kBytes, full);
+        }
+        history |= (batch_ok >> (2 * i)) & 3;
       }
+      ++k_issue;
+      to_stage = to_stage + 1 == L::kStages ? 0 : to_stage + 1;
     };
     auto read_words = [&](unsigned at, unsigned (&w)[NB]) {
       constexpr int PW = Gr::kPW;
@@ -359,31 +362,27 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
     }
 
-    int ahead = c_begin + warp;                   // next tile to issue
 #pragma unroll
     for (int i = 0; i < L::kStages - 1; ++i) {
-      fetch();
-      // stages are used in turn over all segments
-      if (ahead < c_end && !gave_up) issue(stage + i < L::kStages ? stage + i : stage + i - L::kStages);
-      ahead += kWarps;
+      history <<= 2;
+      if (!gave_up) issue();
     }
-    fetch();
-    for (int c = c_begin + warp; c < c_end && !gave_up; c += kWarps) {
+    int key0 = first * kTileKeys;
+    for (int k = 0; k < n_mine && !gave_up; ++k, key0 += kWarps * kTileKeys) {
       // the stage read in the last round is free: every lane is past its reads
       __syncwarp();
-      if (ahead < c_end) issue(stage == 0 ? L::kStages - 1 : stage - 1);
-      ahead += kWarps;
-      fetch();
-      if (!__all_sync(~0u, tc::mbar_wait(bar + stage * 8, (phases >> stage) & 1))) {
+      history <<= 2;
+      issue();
+      const unsigned done = bar + stage * 8, parity = (phases >> stage) & 1;
+      if (!__all_sync(~0u, tc::mbar_try_wait(done, parity)) && !__all_sync(~0u, tc::mbar_wait(done, parity))) {
         gave_up = true;                           // the call's output is undefined from here on
         break;
       }
       phases ^= 1u << stage;
       const unsigned at = ring + stage * L::kStage;
-      const int key0 = c * kTileKeys;
-      const unsigned ok_here = (ok_bits >> (2 * stage)) & 3;
-      const bool full = ok_here == 3 && key0 + kTileKeys <= len - (p.M - 1);
       stage = stage + 1 == L::kStages ? 0 : stage + 1;
+      const unsigned ok_here = (history >> (2 * (L::kStages - 1))) & 3;
+      const bool full = ok_here == 3 && key0 + kTileKeys <= full_end;
 
       // ---------------------------------------------------------- S' = K Q'
       float s[2][NT][4];
@@ -842,8 +841,6 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
   DecP p = {};
   p.pool = {static_cast<uint8_t*>(pool->data), pool->num_pages, pool->page_size, pool->head_dim};
   p.gpp = pool->page_size / 16;
-  p.step_slot = 2 * kWarps / p.gpp;
-  p.step_sub = 2 * kWarps % p.gpp;
   p.q = a->q; p.q_dtype = a->q_dtype; p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h; p.q_sm = a->q_stride_m;
   p.out = a->out; p.out_dtype = a->out_dtype;
   p.o_sb = a->out_stride_b; p.o_sh = a->out_stride_h; p.o_sm = a->out_stride_m;
