@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
+constexpr int kMaxGrid = 1024;      // blocks of the main kernel when units are cut
 constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
 constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
@@ -104,6 +105,27 @@ __device__ __forceinline__ int64_t blocks_used(const DecP& p, int64_t total) {
   return most < p.grid ? most : p.grid;
 }
 
+// What the join kernel reads of the border at the start of a block's run: the unit cut there, if this is its first cut.
+struct Border { int b, h, j0, last; };        // last: last block with a part of the unit; -1 = nothing to join here
+__device__ __forceinline__ Border* borders(const DecP& p, int cols) {
+  return reinterpret_cast<Border*>(p.ws + static_cast<size_t>(p.grid) * 2 * cols * (p.pool.D + 2));
+}
+__device__ __forceinline__ void write_border(const DecP& p, int64_t total, int64_t used, int64_t t0, int b, int64_t off,
+                                             int cols) {
+  const int n = seq_tiles(p, b);
+  const int unit = static_cast<int>(off / n), c = static_cast<int>(off - static_cast<int64_t>(unit) * n);
+  const int64_t begin = t0 - c;               // the unit's first tile
+  const int64_t before = blockIdx.x ? total * (blockIdx.x - 1) / used : 0;
+  Border d = {b, unit / p.CG, (unit % p.CG) * cols, -1};
+  if (c != 0 && before <= begin) {
+    // block of the unit's last tile t: the largest i with floor(total * i / used) <= t; bit 30 of j0 says that
+    // the block before began its run with this unit
+    d.last = static_cast<int>(((begin + n) * used - 1) / total);
+    if (before == begin) d.j0 |= 1 << 30;
+  }
+  borders(p, cols)[blockIdx.x] = d;
+}
+
 // ---------------------------------------------------------------------- PTX
 __device__ __forceinline__ void mma16816(float (&d)[4], unsigned a0, unsigned a1, unsigned a2, unsigned a3, unsigned b0,
                                          unsigned b1) {
@@ -152,6 +174,9 @@ __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
 }
 
 // ------------------------------------------------------------- shared layout
+struct Cursor { int64_t left, off; int b, pad; };          // tiles left to the block, next tile of sequence b
+struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, pad; };
+
 template <int NB>
 struct Lay {
   using Gr = Fp4Group<NB>;
@@ -160,13 +185,13 @@ struct Lay {
   static constexpr int kStage = 2 * Gr::kBytes;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kOutStride = D + 4;                 // floats of one column in the join buffer
-  static_assert(kWarps * 8 * kOutStride * 4 <= kRing, "the join buffer lies over the ring");
+  static_assert(8 * kOutStride * 4 <= kStage, "a warp's sums for the join lie in one stage of its ring");
 };
 
 template <int NB, int NT, bool SPLIT>
 constexpr int smem_bytes() {
   return Lay<NB>::kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + 8 * NT * 8 + kWarps * 8 * NT * 8 +
-         kWarps * Lay<NB>::kStages * 8;
+         kWarps * Lay<NB>::kStages * 8 + kWarps * (static_cast<int>(sizeof(Cursor)) + 2 * static_cast<int>(sizeof(Segment)) + 4);
 }
 
 __device__ unsigned int g_fp4_timeouts = 0;
@@ -196,8 +221,14 @@ __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m
 __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // ---------------------------------------------------------------- main kernel
+// blocks of an SM: two where shared memory holds two rings and the accumulators leave the registers
 template <int NB, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
+constexpr int blocks_per_sm() {
+  return NB <= 4 && NT * NB <= 8 && !(SPLIT && NT * NB > 4) ? 2 : 1;
+}
+
+template <int NB, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_decode_kernel(const DecP p) {
   using L = Lay<NB>;
   using Gr = Fp4Group<NB>;
   constexpr int D = L::D;
@@ -210,7 +241,11 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
   float* warp_m = reinterpret_cast<float*>(col_limit + COLS);      // [warp][COLS]
   float* warp_l = warp_m + kWarps * COLS;
   uint64_t* bars = reinterpret_cast<uint64_t*>(warp_l + kWarps * COLS);   // [warp][stage]: the stage's bytes are there
-  float* join = reinterpret_cast<float*>(smem);                    // [warp][8][kOutStride], over the ring
+  Cursor* cursor = reinterpret_cast<Cursor*>(bars + kWarps * L::kStages);         // [warp]
+  Segment* segment = reinterpret_cast<Segment*>(cursor + kWarps);                 // [warp][2]
+  unsigned* join_at = reinterpret_cast<unsigned*>(segment + 2 * kWarps);          // [warp]: its stage for the join
+  // groups of 16 keys that go through the products together: two where the accumulators leave registers for them
+  constexpr int U = NT == 1 && NB <= 4 ? 2 : 1;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
@@ -223,124 +258,152 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
   unsigned phases = 0;                            // bit i: parity of stage i's next completion
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  int b;
-  int64_t left, off;
-  bool begins_run = true;
-  int stage = 0;
+
+  // ------------------------------------------------------------- segments
+  // A segment is the block's run of one unit's tiles.  What only a segment's ends need lies in shared memory, a copy for
+  // each warp: [0] the segment whose copies run, [1] the one before it.
+  int n_mine = 0;                                 // the warp's tiles of the segment
   bool gave_up = false;
-  if (p.direct) {
-    b = blockIdx.x / p.HC;
-    const int n = seq_tiles(p, b);
-    off = static_cast<int64_t>(blockIdx.x - b * p.HC) * n;
-    left = n;
-  } else {
-    const int64_t total = total_tiles(p);
-    const int64_t used = blocks_used(p, total);
-    if (blockIdx.x >= used) return;
-    const int64_t t0 = total * blockIdx.x / used;
-    left = total * (blockIdx.x + 1) / used - t0;
-    find_sequence(p, t0, b, off);
+  int stage = 0;
+  {
+    Cursor cur;
+    cur.b = 0;
+    cur.left = cur.off = 0;
+    if (p.direct) {
+      cur.b = blockIdx.x / p.HC;
+      const int n = seq_tiles(p, cur.b);
+      cur.off = static_cast<int64_t>(blockIdx.x - cur.b * p.HC) * n;
+      cur.left = n;
+    } else {
+      const int64_t total = total_tiles(p);
+      const int64_t used = blocks_used(p, total);
+      if (blockIdx.x >= used) return;
+      const int64_t t0 = total * blockIdx.x / used;
+      cur.left = total * (blockIdx.x + 1) / used - t0;
+      find_sequence(p, t0, cur.b, cur.off);
+      if (warp == kWarps - 1 && lane == 0) write_border(p, total, used, t0, cur.b, cur.off, 8 * NT);
+    }
+    if (cur.left <= 0 || cur.b >= p.B) return;    // (every block of the grid has work: for safety)
+    if (lane == 0) cursor[warp] = cur;
+    __syncwarp();
   }
-
-  while (left > 0 && b < p.B) {
-    // ------------------------------------------------------------ one segment
-    const int len = seq_len(p, b);
-    const int n_tiles = seq_tiles(p, b);
-    const int unit = static_cast<int>(off / n_tiles);             // of the sequence: table head, column group
-    const int c_begin = static_cast<int>(off - static_cast<int64_t>(unit) * n_tiles);
-    const int c_end = static_cast<int>(min(static_cast<int64_t>(n_tiles), c_begin + left));
-    const int h = unit / p.CG, cg = unit - h * p.CG;
-    const int32_t* table = p.pt + b * p.pt_sb + h * p.pt_sh;
-    const int full_end = len - (p.M - 1);         // every query sees the tokens before it
-
-    // queries: 8 channels per thread, halves after a power of two that puts the row's largest in [1, 2)
-    constexpr int CH = D / 8;
-    for (int i = threadIdx.x; i < COLS * CH; i += kThreads) {
-      const int col = i / CH, ch = i - col * CH;
-      const int j = cg * COLS + col;
-      const int row = p.diff ? j >> 1 : j;
-      float x[8] = {};
-      const bool mine = j < p.NC && (!p.diff || (ch * 2 >= CH) == (j & 1));
-      if (mine) {
-        const int gi = row / p.M, m = row - gi * p.M;
-        const int64_t at = b * p.q_sb + (h * p.G + gi) * p.q_sh + m * p.q_sm + ch * 8;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = load_as_float(p.q, p.q_dtype, at + e) * p.sign;
-      }
-      float amax = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-#pragma unroll
-      for (int o = 1; o < CH; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-      // exponent of amax, held to normal numbers on both sides
-      const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
-      const float down = __uint_as_float((254 - ex) << 23);
-      unsigned hi[4], lo[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y0 = x[2 * e] * down, y1 = x[2 * e + 1] * down;
-        hi[e] = pack_half2(y0, y1);
-        if (SPLIT) {
-          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-          lo[e] = pack_half2(y0 - back.x, y1 - back.y);
-        }
-      }
-      uint4* dst = reinterpret_cast<uint4*>(q_frag) + ((col >> 3) * NB + (ch >> 2)) * 32 + (col & 7) * 4 + (ch & 3);
-      *dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if (SPLIT) dst[NT * NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      if (ch == 0) {
-        col_scale[col] = fmaxf(p.scale * __uint_as_float(ex << 23), 1e-37f);
-        col_limit[col] = j < p.NC ? len - (p.M - 1 - row % p.M) : len;
-      }
+  // false: no segment is left
+  auto open_segment = [&]() {
+    Cursor cur = cursor[warp];
+    if (cur.left <= 0 || cur.b >= p.B) return false;
+    Segment sg;
+    sg.b = cur.b;
+    sg.len = seq_len(p, cur.b);
+    sg.n_tiles = seq_tiles(p, cur.b);
+    const int unit = static_cast<int>(cur.off / sg.n_tiles);      // of the sequence: table head, column group
+    sg.c_begin = static_cast<int>(cur.off - static_cast<int64_t>(unit) * sg.n_tiles);
+    sg.c_end = static_cast<int>(min(static_cast<int64_t>(sg.n_tiles), sg.c_begin + cur.left));
+    sg.h = unit / p.CG;
+    sg.cg = unit - sg.h * p.CG;
+    const int n = sg.c_end - sg.c_begin;
+    cur.left -= n;
+    cur.off += n;
+    if (cur.off == static_cast<int64_t>(sg.n_tiles) * p.HC) {
+      cur.off = 0;
+      ++cur.b;
     }
-    __syncthreads();
-    float sc[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      sc[nt][0] = col_scale[nt * 8 + 2 * t];
-      sc[nt][1] = col_scale[nt * 8 + 2 * t + 1];
+    __syncwarp();
+    if (lane == 0) {
+      segment[2 * warp + 1] = segment[2 * warp];
+      segment[2 * warp] = sg;
+      cursor[warp] = cur;
     }
-
-    // ---------------------------------------------------------- copies
-    // The warp's tiles are c_begin + warp + kWarps k.  Of every 16 of them lane 2 i + u owns group u of tile i: it
-    // reads the page id (a batch ahead), holds the source address and issues the copy.
-    const int first = c_begin + warp;
-    const int n_mine = c_end > first ? (c_end - first + kWarps - 1) / kWarps : 0;
-    auto group_of = [&](int k) { return (first + kWarps * (k + (lane >> 1))) * 2 + (lane & 1); };
-    auto load_id = [&](int k) {
-      const int gr = group_of(k);
-      return k + (lane >> 1) < n_mine && gr * 16 < len ? __ldg(table + static_cast<unsigned>(gr) / p.gpp) : -1;
-    };
-    const uint8_t* src = nullptr;
-    bool src_ok = false;
-    unsigned batch_ok = 0;
-    auto take_batch = [&](int k, int id) {
-      const unsigned sub = static_cast<unsigned>(group_of(k)) % p.gpp;
-      src_ok = id >= 0 && id < p.pool.num_pages;
-      src = p.pool.data + (static_cast<int64_t>(id) * p.gpp + sub) * Gr::kBytes;
-      batch_ok = __ballot_sync(~0u, src_ok);
-    };
-    int next_id = load_id(0);
-    int k_issue = 0;
-    unsigned history = 0;                         // two bits per tile issued, the last in bits 0, 1: its pages exist
-    unsigned to_stage = stage;
-    auto issue = [&]() {
-      if (k_issue < n_mine) {
-        const int i = k_issue & 15;
-        if (i == 0) {
-          take_batch(k_issue, next_id);
-          next_id = load_id(k_issue + 16);
+    __syncwarp();
+    const int first = sg.c_begin + warp;
+    n_mine = sg.c_end > first && !gave_up ? (sg.c_end - first + kWarps - 1) / kWarps : 0;
+    return true;
+  };
+  auto stage_queries = [&]() {
+    const Segment& sg = segment[2 * warp];
+      // queries: 8 channels per thread, halves after a power of two that puts the row's largest in [1, 2)
+      constexpr int CH = D / 8;
+      for (int i = threadIdx.x; i < COLS * CH; i += kThreads) {
+        const int col = i / CH, ch = i - col * CH;
+        const int j = sg.cg * COLS + col;
+        const int row = p.diff ? j >> 1 : j;
+        float x[8] = {};
+        const bool mine = j < p.NC && (!p.diff || (ch * 2 >= CH) == (j & 1));
+        if (mine) {
+          const int gi = row / p.M, m = row - gi * p.M;
+          const int64_t at = sg.b * p.q_sb + (sg.h * p.G + gi) * p.q_sh + m * p.q_sm + ch * 8;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = load_as_float(p.q, p.q_dtype, at + e) * p.sign;
         }
-        if ((lane >> 1) == i) {
-          const unsigned full = bar + to_stage * 8;
-          tc::mbar_arrive_expect_tx(full, src_ok ? Gr::kBytes : 0);
-          if (src_ok) tc::bulk_load(ring + to_stage * L::kStage + (lane & 1) * Gr::kBytes, src, Gr::kBytes, full);
+        float amax = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+#pragma unroll
+        for (int o = 1; o < CH; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+        // exponent of amax, held to normal numbers on both sides
+        const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
+        const float down = __uint_as_float((254 - ex) << 23);
+        unsigned hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y0 = x[2 * e] * down, y1 = x[2 * e + 1] * down;
+          hi[e] = pack_half2(y0, y1);
+          if (SPLIT) {
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+            lo[e] = pack_half2(y0 - back.x, y1 - back.y);
+          }
         }
-        history |= (batch_ok >> (2 * i)) & 3;
+        uint4* dst = reinterpret_cast<uint4*>(q_frag) + ((col >> 3) * NB + (ch >> 2)) * 32 + (col & 7) * 4 + (ch & 3);
+        *dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (SPLIT) dst[NT * NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (ch == 0) {
+          col_scale[col] = fmaxf(p.scale * __uint_as_float(ex << 23), 1e-37f);
+          col_limit[col] = j < p.NC ? sg.len - (p.M - 1 - row % p.M) : sg.len;
+        }
       }
-      ++k_issue;
-      to_stage = to_stage + 1 == L::kStages ? 0 : to_stage + 1;
-    };
+  };
+
+  // ---------------------------------------------------------------- copies
+  // The warp's tiles are c_begin + warp + kWarps k.  Of every 16 of them lane 2 i + u owns group u of tile i: it reads
+  // the page id (a batch ahead), holds the source address and issues the copy.
+  int next_id = -1;
+  unsigned history = 0;                           // two bits per tile issued, the last in bits 0, 1: its pages exist
+  const uint8_t* src = nullptr;
+  bool src_ok = false;
+  unsigned batch_ok = 0;
+  auto group_of = [&](int k) { return (segment[2 * warp].c_begin + warp + kWarps * (k + (lane >> 1))) * 2 + (lane & 1); };
+  auto load_id = [&](int k) {
+    const Segment& sg = segment[2 * warp];
+    const int gr = group_of(k);
+    return k + (lane >> 1) < n_mine && gr * 16 < sg.len
+               ? __ldg(p.pt + sg.b * p.pt_sb + sg.h * p.pt_sh + static_cast<unsigned>(gr) / p.gpp) : -1;
+  };
+  auto issue = [&](int k, int to_stage) {
+    history <<= 2;
+    if (k < n_mine) {
+      const int i = k & 15;
+      if (i == 0) {
+        const unsigned sub = static_cast<unsigned>(group_of(k)) % p.gpp;
+        src_ok = next_id >= 0 && next_id < p.pool.num_pages;
+        src = p.pool.data + (static_cast<int64_t>(next_id) * p.gpp + sub) * Gr::kBytes;
+        batch_ok = __ballot_sync(~0u, src_ok);
+        next_id = load_id(k + 16);
+      }
+      if ((lane >> 1) == i) {
+        const unsigned full = bar + to_stage * 8;
+        tc::mbar_arrive_expect_tx(full, src_ok ? Gr::kBytes : 0);
+        if (src_ok) tc::bulk_load(ring + to_stage * L::kStage + (lane & 1) * Gr::kBytes, src, Gr::kBytes, full);
+      }
+      history |= (batch_ok >> (2 * i)) & 3;
+    }
+  };
+  auto start_copies = [&]() {
+    next_id = load_id(0);
+    int to = stage;
+    for (int i = 0; i < L::kStages - 1; ++i) {
+      issue(i, to);
+      to = to + 1 == L::kStages ? 0 : to + 1;
+    }
+  };
     auto read_words = [&](unsigned at, unsigned (&w)[NB]) {
       constexpr int PW = Gr::kPW;
 #pragma unroll
@@ -352,30 +415,37 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
       }
     };
 
+  open_segment();
+  start_copies();
+  stage_queries();
+  __syncthreads();
+
+  bool begins_run = true;
+  while (true) {
+    float sc[NT][2];
     float o[NT][MT][4];
     float m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      sc[nt][0] = col_scale[nt * 8 + 2 * t];
+      sc[nt][1] = col_scale[nt * 8 + 2 * t + 1];
       m_run[nt][0] = m_run[nt][1] = -FLT_MAX;
       l_run[nt][0] = l_run[nt][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
     }
-
-#pragma unroll
-    for (int i = 0; i < L::kStages - 1; ++i) {
-      history <<= 2;
-      if (!gave_up) issue();
-    }
-    int key0 = first * kTileKeys;
-    for (int k = 0; k < n_mine && !gave_up; ++k, key0 += kWarps * kTileKeys) {
+    const int full_end = segment[2 * warp].len - (p.M - 1);   // every query sees the tokens before it
+    int key0 = (segment[2 * warp].c_begin + warp) * kTileKeys;
+    for (int k = 0; k < n_mine; ++k, key0 += kWarps * kTileKeys) {
       // the stage read in the last round is free: every lane is past its reads
       __syncwarp();
-      history <<= 2;
-      issue();
+      issue(k + L::kStages - 1, stage == 0 ? L::kStages - 1 : stage - 1);
       const unsigned done = bar + stage * 8, parity = (phases >> stage) & 1;
       if (!__all_sync(~0u, tc::mbar_try_wait(done, parity)) && !__all_sync(~0u, tc::mbar_wait(done, parity))) {
-        gave_up = true;                           // the call's output is undefined from here on
+        // the call's output is undefined from here on; the copies in flight land before the block ends
+        gave_up = true;
+        if (lane == 0) atomicAdd(&g_fp4_timeouts, 1u);
+        for (int i = 0; i < L::kStages; ++i) tc::mbar_wait(bar + i * 8, (phases >> i) & 1);
         break;
       }
       phases ^= 1u << stage;
@@ -384,173 +454,179 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
       const unsigned ok_here = (history >> (2 * (L::kStages - 1))) & 3;
       const bool full = ok_here == 3 && key0 + kTileKeys <= full_end;
 
-      // ---------------------------------------------------------- S' = K Q'
-      float s[2][NT][4];
-      {
-        unsigned kw[2][2][NB];
-        unsigned ksw[2][NB / 2];
+#pragma unroll 1
+      for (int v = 0; v < 2; v += U) {
+        // ---------------------------------------------------------- S' = K Q'
+        float s[U][NT][4];
+        {
+          unsigned kw[U][2][NB];
+          unsigned ksw[U][NB / 2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          read_words(at + u * Gr::kBytes, kw[u][0]);
-          read_words(at + u * Gr::kBytes + Gr::kSet, kw[u][1]);
-          lds_words<NB / 2>(at + u * Gr::kBytes + Gr::kKs + g * 2 * NB, ksw[u]);
-        }
-#pragma unroll
-        for (int bk = 0; bk < NB; ++bk) {
-          uint4 q_hi[NT], q_lo[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            q_hi[nt] = reinterpret_cast<const uint4*>(q_frag)[(nt * NB + bk) * 32 + lane];
-            if (SPLIT) q_lo[nt] = reinterpret_cast<const uint4*>(q_frag)[(NT * NB + nt * NB + bk) * 32 + lane];
+          for (int u = 0; u < U; ++u) {
+            read_words(at + (v + u) * Gr::kBytes, kw[u][0]);
+            read_words(at + (v + u) * Gr::kBytes + Gr::kSet, kw[u][1]);
+            lds_words<NB / 2>(at + (v + u) * Gr::kBytes + Gr::kKs + g * 2 * NB, ksw[u]);
           }
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            unsigned r0[4], r1[4];
-            fp4_unpack4(kw[u][0][bk], r0);
-            fp4_unpack4(kw[u][1][bk], r1);
-            const int i0 = bk, i1 = NB + bk;          // scale bytes of rows g and g + 8
-            const float s0 = fp4_scale(__byte_perm(ksw[u][i0 / 4], 0, 0x4440 + i0 % 4));
-            const float s1 = fp4_scale(__byte_perm(ksw[u][i1 / 4], 0, 0x4440 + i1 % 4));
+          for (int bk = 0; bk < NB; ++bk) {
+            uint4 q_hi[NT], q_lo[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              float acc[4];
-              mma16816_new(acc, r0[0], r1[0], r0[1], r1[1], q_hi[nt].x, q_hi[nt].y);
-              mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_hi[nt].z, q_hi[nt].w);
-              if (SPLIT) {
-                mma16816(acc, r0[0], r1[0], r0[1], r1[1], q_lo[nt].x, q_lo[nt].y);
-                mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_lo[nt].z, q_lo[nt].w);
-              }
-              if (bk == 0) {
-                s[u][nt][0] = acc[0] * s0; s[u][nt][1] = acc[1] * s0;
-                s[u][nt][2] = acc[2] * s1; s[u][nt][3] = acc[3] * s1;
-              } else {
-                s[u][nt][0] = fmaf(acc[0], s0, s[u][nt][0]); s[u][nt][1] = fmaf(acc[1], s0, s[u][nt][1]);
-                s[u][nt][2] = fmaf(acc[2], s1, s[u][nt][2]); s[u][nt][3] = fmaf(acc[3], s1, s[u][nt][3]);
+              q_hi[nt] = reinterpret_cast<const uint4*>(q_frag)[(nt * NB + bk) * 32 + lane];
+              if (SPLIT) q_lo[nt] = reinterpret_cast<const uint4*>(q_frag)[(NT * NB + nt * NB + bk) * 32 + lane];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              unsigned r0[4], r1[4];
+              fp4_unpack4(kw[u][0][bk], r0);
+              fp4_unpack4(kw[u][1][bk], r1);
+              const int i0 = bk, i1 = NB + bk;          // scale bytes of rows g and g + 8
+              const float s0 = fp4_scale(__byte_perm(ksw[u][i0 / 4], 0, 0x4440 + i0 % 4));
+              const float s1 = fp4_scale(__byte_perm(ksw[u][i1 / 4], 0, 0x4440 + i1 % 4));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float acc[4];
+                mma16816_new(acc, r0[0], r1[0], r0[1], r1[1], q_hi[nt].x, q_hi[nt].y);
+                mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_hi[nt].z, q_hi[nt].w);
+                if (SPLIT) {
+                  mma16816(acc, r0[0], r1[0], r0[1], r1[1], q_lo[nt].x, q_lo[nt].y);
+                  mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_lo[nt].z, q_lo[nt].w);
+                }
+                if (bk == 0) {
+                  s[u][nt][0] = acc[0] * s0; s[u][nt][1] = acc[1] * s0;
+                  s[u][nt][2] = acc[2] * s1; s[u][nt][3] = acc[3] * s1;
+                } else {
+                  s[u][nt][0] = fmaf(acc[0], s0, s[u][nt][0]); s[u][nt][1] = fmaf(acc[1], s0, s[u][nt][1]);
+                  s[u][nt][2] = fmaf(acc[2], s1, s[u][nt][2]); s[u][nt][3] = fmaf(acc[3], s1, s[u][nt][3]);
+                }
               }
             }
           }
         }
-      }
-      if (!full) {
+        if (!full) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const bool ok = (ok_here >> u) & 1;
-          const int key = key0 + u * 16 + g;
+          for (int u = 0; u < U; ++u) {
+            const bool ok = (ok_here >> (v + u)) & 1;
+            const int key = key0 + (v + u) * 16 + g;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
+            for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool seen = ok && key + (i >> 1) * 8 < col_limit[nt * 8 + 2 * t + (i & 1)];
-              if (!seen) s[u][nt][i] = -INFINITY;
+              for (int i = 0; i < 4; ++i) {
+                const bool seen = ok && key + (i >> 1) * 8 < col_limit[nt * 8 + 2 * t + (i & 1)];
+                if (!seen) s[u][nt][i] = -INFINITY;
+              }
             }
           }
         }
-      }
 
-      // ---------------------------------------------------------- softmax
-      float mx[NT][2];
-      bool raise = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mx[nt][e] = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-          raise = raise || fmaf(mx[nt][e], sc[nt][e], -m_run[nt][e]) > kLazy;
-        }
-      }
-      if (__any_sync(~0u, raise)) {
+        // ---------------------------------------------------------- softmax
+        float mx[NT][2];
+        bool raise = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float v = mx[nt][e];
-            v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
-            v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
-            v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
-            const float m_new = fmaxf(m_run[nt][e], fmaf(v, sc[nt][e], -kHead));
-            f[e] = tc::ex2(m_run[nt][e] - m_new);
-            m_run[nt][e] = m_new;
-            l_run[nt][e] *= f[e];
-          }
-#pragma unroll
-          for (int i = 0; i < MT; ++i) {
-            o[nt][i][0] *= f[0]; o[nt][i][1] *= f[1];
-            o[nt][i][2] *= f[0]; o[nt][i][3] *= f[1];
+            mx[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+            if (U == 2) mx[nt][e] = fmaxf(mx[nt][e], fmaxf(s[U - 1][nt][e], s[U - 1][nt][e + 2]));
+            raise = raise || fmaf(mx[nt][e], sc[nt][e], -m_run[nt][e]) > kLazy;
           }
         }
-      }
-      unsigned pf[2][NT][2], pl[2][NT][2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float x[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[i] = tc::ex2(fmaf(s[u][nt][i], sc[nt][i & 1], -m_run[nt][i & 1]));
-            l_run[nt][i & 1] += x[i];
-          }
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const unsigned hi = pack_half2(x[2 * r], x[2 * r + 1]);
-            pf[u][nt][r] = transpose8x8(hi);
-            if (SPLIT) {
-              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-              pl[u][nt][r] = transpose8x8(pack_half2(x[2 * r] - back.x, x[2 * r + 1] - back.y));
-            }
-          }
-        }
-      }
-
-      // ---------------------------------------------------------- O' += V' P'
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        unsigned vw[2][NB];
-        read_words(at + u * Gr::kBytes + Gr::kV, vw[0]);
-        read_words(at + u * Gr::kBytes + Gr::kV + Gr::kSet, vw[1]);
-        // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the lane's channels' block
-        unsigned vs = lds32(at + u * Gr::kBytes + Gr::kVs + (g * NB / 8) * 16 + t * 4);
-        if (!full) {          // rows behind the sequence or without a page hold anything: scale 0 keeps NaN away
-          const int key = key0 + u * 16 + 2 * t;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if (!((ok_here >> u) & 1) || key + (i & 1) + 8 * (i >> 1) >= len) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
-          }
-        }
-        // byte e + 127 -> half 2^e: (byte - 112) << 10 in both halves at once
-        const unsigned v01 = __byte_perm(vs, 0, 0x4140) * 1024u - 112u * 1024u * 65537u;
-        const unsigned v23 = __byte_perm(vs, 0, 0x4342) * 1024u - 112u * 1024u * 65537u;
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          unsigned r0[4], r1[4];
-          fp4_unpack4(vw[0][j], r0);
-          fp4_unpack4(vw[1][j], r1);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            r0[i] = mul_half2(r0[i], v01);
-            r1[i] = mul_half2(r1[i], v23);
-          }
+        if (__any_sync(~0u, raise)) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pf[u][nt][0], pf[u][nt][1]);
-            mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pf[u][nt][0], pf[u][nt][1]);
-            if (SPLIT) {
-              mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pl[u][nt][0], pl[u][nt][1]);
-              mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pl[u][nt][0], pl[u][nt][1]);
+            float f[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = mx[nt][e];
+              v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
+              v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
+              v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
+              const float m_new = fmaxf(m_run[nt][e], fmaf(v, sc[nt][e], -kHead));
+              f[e] = tc::ex2(m_run[nt][e] - m_new);
+              m_run[nt][e] = m_new;
+              l_run[nt][e] *= f[e];
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              o[nt][i][0] *= f[0]; o[nt][i][1] *= f[1];
+              o[nt][i][2] *= f[0]; o[nt][i][3] *= f[1];
+            }
+          }
+        }
+        unsigned pf[U][NT][2], pl[U][NT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              x[i] = tc::ex2(fmaf(s[u][nt][i], sc[nt][i & 1], -m_run[nt][i & 1]));
+              l_run[nt][i & 1] += x[i];
+            }
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const unsigned hi = pack_half2(x[2 * r], x[2 * r + 1]);
+              pf[u][nt][r] = transpose8x8(hi);
+              if (SPLIT) {
+                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                pl[u][nt][r] = transpose8x8(pack_half2(x[2 * r] - back.x, x[2 * r + 1] - back.y));
+              }
+            }
+          }
+        }
+
+        // ---------------------------------------------------------- O' += V' P'
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          unsigned vw[2][NB];
+          read_words(at + (v + u) * Gr::kBytes + Gr::kV, vw[0]);
+          read_words(at + (v + u) * Gr::kBytes + Gr::kV + Gr::kSet, vw[1]);
+          // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the lane's channels' block
+          unsigned vs = lds32(at + (v + u) * Gr::kBytes + Gr::kVs + (g * NB / 8) * 16 + t * 4);
+          if (!full) {          // rows behind the sequence or without a page hold anything: scale 0 keeps NaN away
+            const int key = key0 + (v + u) * 16 + 2 * t;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (!((ok_here >> (v + u)) & 1) || key + (i & 1) + 8 * (i >> 1) >= full_end + p.M - 1) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
+            }
+          }
+          // byte e + 127 -> half 2^e: (byte - 112) << 10 in both halves at once
+          const unsigned v01 = __byte_perm(vs, 0, 0x4140) * 1024u - 112u * 1024u * 65537u;
+          const unsigned v23 = __byte_perm(vs, 0, 0x4342) * 1024u - 112u * 1024u * 65537u;
+#pragma unroll
+          for (int j = 0; j < NB; ++j) {
+            unsigned r0[4], r1[4];
+            fp4_unpack4(vw[0][j], r0);
+            fp4_unpack4(vw[1][j], r1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              r0[i] = mul_half2(r0[i], v01);
+              r1[i] = mul_half2(r1[i], v23);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pf[u][nt][0], pf[u][nt][1]);
+              mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pf[u][nt][0], pf[u][nt][1]);
+              if (SPLIT) {
+                mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pl[u][nt][0], pl[u][nt][1]);
+                mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pl[u][nt][0], pl[u][nt][1]);
+              }
             }
           }
         }
       }
     }
 
-    if (gave_up && phases != ~0u) {               // once: count it, and let the copies in flight land before the block ends
-      if (lane == 0) atomicAdd(&g_fp4_timeouts, 1u);
-      for (int i = 0; i < L::kStages; ++i) tc::mbar_wait(bar + i * 8, (phases >> i) & 1);
-      phases = ~0u;
-    }
+    // the next segment's first copies are on their way while this one's warps join; the stage that they leave free
+    // takes the warp's sums
+    const unsigned my_join = warp * L::kStages * L::kStage + (stage == 0 ? L::kStages - 1 : stage - 1) * L::kStage;
+    __syncwarp();
+    const bool more = open_segment();
+    if (more) start_copies();
 
     // ------------------------------------------------------ join the 8 warps
+    if (lane == 0) join_at[warp] = my_join;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -565,8 +641,11 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
         }
       }
     }
-    __syncthreads();                              // every warp has read its ring to the end
-    const bool whole = c_begin == 0 && c_end == n_tiles;
+    __syncthreads();                              // every warp is past its last read of the queries
+    if (more) stage_queries();
+    const Segment& done_sg = segment[2 * warp + (more ? 1 : 0)];
+    const int h = done_sg.h, cg = done_sg.cg;
+    const bool whole = done_sg.c_begin == 0 && done_sg.c_end == done_sg.n_tiles;
     const int which = begins_run ? 0 : 1;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -578,7 +657,7 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
         for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + nt * 8 + 2 * t + e]);
         f[e] = tc::ex2(m_run[nt][e] - top);
       }
-      float* dst = join + (warp * 8 + 2 * t) * L::kOutStride + g * (4 * NB);
+      float* dst = reinterpret_cast<float*>(smem + my_join) + 2 * t * L::kOutStride + g * (4 * NB);
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[nt][i][0] * f[0], o[nt][i][2] * f[0]);
@@ -604,7 +683,8 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
           for (int i = 0; i < NB; ++i) {
             acc[i] = 0.f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) acc[i] += join[(w * 8 + lc) * L::kOutStride + i * 32 + lane];
+            for (int w = 0; w < kWarps; ++w)
+              acc[i] += reinterpret_cast<const float*>(smem + join_at[w])[lc * L::kOutStride + i * 32 + lane];
           }
           if (!whole) {
             float* part = p.ws + ((static_cast<int64_t>(blockIdx.x) * 2 + which) * COLS + col) * (D + 2);
@@ -620,101 +700,100 @@ __global__ void __launch_bounds__(kThreads) fp4_decode_kernel(const DecP p) {
 #pragma unroll
           for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], weight, x[i]) : acc[i] * weight;
         }
-        if (write) finish_row<NB>(p, b, h * p.G + row / p.M, row % p.M, x);
+        if (write) finish_row<NB>(p, done_sg.b, h * p.G + row / p.M, row % p.M, x);
       }
       tc::fence_proxy_async();                    // the next segment's copies write where these lines read
       __syncthreads();
     }
 
-    left -= c_end - c_begin;
-    off += c_end - c_begin;
     begins_run = false;
-    if (off == static_cast<int64_t>(n_tiles) * p.HC) {
-      off = 0;
-      ++b;
-    }
+    if (!more) break;
   }
 }
 
 // ---------------------------------------------------------------- join kernel
-// One block per (unit, output row): the units cut over several blocks, their partials in order of the blocks.
-constexpr int kJoinWarps = 4;
+// One block per (border between two blocks' runs, output row): where a unit is first cut, its partials are added in
+// order of the blocks that left them.
+constexpr int kJoinWarps = 8;
+
+__host__ __device__ inline int join_rows(int NC, int cols, int diff) {
+  return (NC < cols ? NC : cols) / (diff ? 2 : 1);
+}
 
 template <int NB, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p) {
   constexpr int D = NB * 32, COLS = 8 * NT;
+  __shared__ float weight[kMaxGrid];               // of each part
+  __shared__ float part_sum[kJoinWarps][D];
+  __shared__ float warp_x[kJoinWarps];
   const int per = p.diff ? 2 : 1;
-  const int rows = COLS / per;
-  const int64_t u_all = blockIdx.x / rows;
-  const int r = static_cast<int>(blockIdx.x - u_all * rows);
-  const int b = static_cast<int>(u_all / p.HC), unit = static_cast<int>(u_all - static_cast<int64_t>(b) * p.HC);
-  const int h = unit / p.CG, cg = unit - h * p.CG;
-  const int j0 = cg * COLS + r * per;
+  const int rows = join_rows(p.NC, COLS, p.diff);
+  const int border = 1 + blockIdx.x / rows, r = blockIdx.x % rows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // tiles before this unit
-  int64_t before = 0, total = 0;
-  for (int i = lane; i < p.B; i += 32) {
-    const int n = seq_tiles(p, i);
-    total += n;
-    if (i < b) before += n;
-  }
-#pragma unroll
-  for (int s = 16; s; s >>= 1) {
-    total += __shfl_xor_sync(~0u, total, s);
-    before += __shfl_xor_sync(~0u, before, s);
-  }
-  total *= p.HC;
-  const int n = seq_tiles(p, b);
-  const int64_t t_begin = before * p.HC + static_cast<int64_t>(unit) * n, t_last = t_begin + n - 1;
-  const int64_t used = blocks_used(p, total);
-  // block of tile t: the largest i with floor(total * i / used) <= t
-  const int first = static_cast<int>(((t_begin + 1) * used - 1) / total);
-  const int last = static_cast<int>(((t_last + 1) * used - 1) / total);
-  const int first_which = total * first / used == t_begin ? 0 : 1;
+  const int64_t used = blocks_used(p, total_tiles(p));
   // every block waits, so that this kernel never ends before the main one
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (first == last || j0 >= p.NC) return;      // written whole, or no such row
-
-  __shared__ float part_sum[kJoinWarps][D];
-  __shared__ float part_m[kJoinWarps], part_l[kJoinWarps];
+  if (border >= used) return;
+  Border d = borders(p, COLS)[border];
+  if (d.last < 0) return;
+  const int first = border - 1, first_which = d.j0 >> 30 ? 0 : 1, n = d.last - first + 1;
+  const int j0 = (d.j0 & ~(1 << 30)) + r * per;
+  if (j0 >= p.NC) return;
+  auto part_of = [&](int i, int col) {
+    return p.ws + ((static_cast<int64_t>(first + i) * 2 + (i == 0 ? first_which : 0)) * COLS + col) * (D + 2);
+  };
   float x[NB];
   for (int half = 0; half < per; ++half) {
     const int col = r * per + half;
-    float top = -FLT_MAX, l = 0.f, acc[NB];
+    // the largest maximum, then every part's weight and the sum of l
+    float top = -FLT_MAX;
+    for (int i = threadIdx.x; i < n; i += kJoinWarps * 32) top = fmaxf(top, part_of(i, col)[D]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    if (lane == 0) warp_x[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, warp_x[w]);
+    __syncthreads();
+    float l = 0.f;
+    for (int i = threadIdx.x; i < n; i += kJoinWarps * 32) {
+      const float* part = part_of(i, col);
+      const float f = tc::ex2(part[D] - top);
+      weight[i] = f;
+      l = fmaf(part[D + 1], f, l);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
+    if (lane == 0) warp_x[warp] = l;
+    __syncthreads();
+    float acc[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) acc[i] = 0.f;
-    for (int c = first + warp; c <= last; c += kJoinWarps) {
-      const float* part = p.ws + ((static_cast<int64_t>(c) * 2 + (c == first ? first_which : 0)) * COLS + col) * (D + 2);
-      const float m = part[D], m_new = fmaxf(top, m);
-      const float f_old = tc::ex2(top - m_new), f_new = tc::ex2(m - m_new);
-      l = l * f_old + part[D + 1] * f_new;
+#pragma unroll 4
+    for (int c = warp; c < n; c += kJoinWarps) {
+      const float* part = part_of(c, col);
+      const float f = weight[c];
 #pragma unroll
-      for (int i = 0; i < NB; ++i) acc[i] = acc[i] * f_old + part[i * 32 + lane] * f_new;
-      top = m_new;
+      for (int i = 0; i < NB; ++i) acc[i] = fmaf(part[i * 32 + lane], f, acc[i]);
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) part_sum[warp][i * 32 + lane] = acc[i];
-    if (lane == 0) { part_m[warp] = top; part_l[warp] = l; }
     __syncthreads();
     if (warp == 0) {
-      float all = -FLT_MAX, sum = 0.f;
+      float sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) all = fmaxf(all, part_m[w]);
-#pragma unroll
-      for (int i = 0; i < NB; ++i) acc[i] = 0.f;
-#pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) {
-        const float f = tc::ex2(part_m[w] - all);
-        sum += part_l[w] * f;
-#pragma unroll
-        for (int i = 0; i < NB; ++i) acc[i] = fmaf(part_sum[w][i * 32 + lane], f, acc[i]);
-      }
+      for (int w = 0; w < kJoinWarps; ++w) sum += warp_x[w];
       const int row = p.diff ? (j0 >> 1) : j0;
       const float inv = safe_inverse(sum);
-      const float weight = half ? -p.lam[h * p.G + row / p.M] * inv : inv;
+      const float scale = half ? -p.lam[d.h * p.G + row / p.M] * inv : inv;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], weight, x[i]) : acc[i] * weight;
-      if (half == per - 1) finish_row<NB>(p, b, h * p.G + row / p.M, row % p.M, x);
+      for (int i = 0; i < NB; ++i) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) v += part_sum[w][i * 32 + lane];
+        x[i] = half ? fmaf(v, scale, x[i]) : v * scale;
+      }
+      if (half == per - 1) finish_row<NB>(p, d.b, d.h * p.G + row / p.M, row % p.M, x);
     }
     __syncthreads();
   }
@@ -764,8 +843,8 @@ int make_plan(DecP& p, Plan* plan) {
     plan->ws = 0;
   } else {
     const int64_t useful = (most * units + kWarps - 1) / kWarps;
-    plan->grid = static_cast<int>(std::min<int64_t>(blocks, useful));
-    plan->ws = static_cast<size_t>(plan->grid) * 2 * 8 * NT * (NB * 32 + 2) * sizeof(float);
+    plan->grid = static_cast<int>(std::min<int64_t>(std::min(blocks, kMaxGrid), useful));
+    plan->ws = static_cast<size_t>(plan->grid) * (2 * 8 * NT * (NB * 32 + 2) * sizeof(float) + sizeof(Border));
   }
   p.grid = plan->grid;
   p.direct = plan->direct ? 1 : 0;
@@ -783,10 +862,9 @@ int run_shape(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cud
   p.ws = static_cast<float*>(ws);
   fp4_decode_kernel<NB, NT, SPLIT><<<plan.grid, kThreads, smem_bytes<NB, NT, SPLIT>(), s>>>(p);
   if (int st = check_cuda(cudaGetLastError(), "fp4_decode launch")) return st;
-  if (plan.direct) return IAK_OK;
+  if (plan.grid == 1 || plan.direct) return IAK_OK;
   cudaLaunchConfig_t cfg = {};
-  const int rows = 8 * NT / (p.diff ? 2 : 1);
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.B) * p.HC * rows));
+  cfg.gridDim = dim3(static_cast<unsigned>((plan.grid - 1) * join_rows(p.NC, 8 * NT, p.diff)));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = s;
   // starts while the main kernel's last blocks run; it waits for them before it reads a partial
