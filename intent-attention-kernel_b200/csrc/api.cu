@@ -267,9 +267,6 @@ int iak_device_status(uint32_t* decode_timeouts, uint32_t* mla_timeouts, uint32_
                       int32_t reset) {
   unsigned int v[3] = {0, 0, 0};
   int st = read_decode_timeouts(&v[0], reset != 0);
-  unsigned int fp4 = 0;
-  if (!st) st = read_fp4_timeouts(&fp4, reset != 0);
-  v[0] += fp4;
   if (!st) st = read_mla_timeouts(&v[1], reset != 0);
   if (!st) st = read_prefill_timeouts(&v[2], reset != 0);
   if (st) return st;

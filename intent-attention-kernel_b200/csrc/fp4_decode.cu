@@ -14,9 +14,10 @@
 // (sequence, table head, column group) units, one run per resident block, so that ragged batches and single long
 // sequences fill the GPU alike; a unit cut over several blocks leaves partial (m, l, O) that a second kernel joins in
 // order of the blocks (no atomics: results do not depend on timing).  Each warp streams its own tiles through a
-// ring of bulk copies, one per 16 rows: a group's codes and scales lie together in the
-// order in which lanes read them, so a copy needs no address arithmetic beyond its start and reads are free of bank
-// conflicts.
+// ring of 16-byte asynchronous copies: a group's codes and scales lie together in the order in which lanes read them,
+// so that copies and reads are linear in the lane, free of bank conflicts, and five copies per 16 rows need one address.
+// (Bulk copies, one per 16 rows, were measured and are slower here: each wants its operands in uniform registers, and
+// setting them up cost more issue slots than five plain copies, of which this kernel has none to spare.)
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
@@ -155,11 +156,30 @@ __device__ __forceinline__ unsigned mul_half2(unsigned a, unsigned b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const unsigned*>(&r);
 }
+// four scale bytes e + 127 -> 2^e: two conversions to bf16 pairs, whose bits are the upper halves of the floats
+__device__ __forceinline__ void scales4(unsigned w, float* s) {
+  unsigned lo, hi;
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.bf16x2.ue8m0x2 %0, a;\ncvt.rn.bf16x2.ue8m0x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi) : "r"(w));
+  s[0] = __uint_as_float(lo << 16);
+  s[1] = __uint_as_float(lo & 0xffff0000u);
+  s[2] = __uint_as_float(hi << 16);
+  s[3] = __uint_as_float(hi & 0xffff0000u);
+}
 __device__ __forceinline__ unsigned lds32(unsigned a) {
   unsigned r;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
   return r;
 }
+__device__ __forceinline__ void copy16(unsigned dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// a volatile statement, as the reads of the copied bytes are: they keep their order
+__device__ __forceinline__ void warp_sync() { asm volatile("bar.warp.sync 0xffffffff;" ::: "memory"); }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 template <int NW>
 __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
   if constexpr (NW == 1) {
@@ -191,10 +211,8 @@ struct Lay {
 template <int NB, int NT, bool SPLIT>
 constexpr int smem_bytes() {
   return Lay<NB>::kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + 8 * NT * 8 + kWarps * 8 * NT * 8 +
-         kWarps * Lay<NB>::kStages * 8 + kWarps * (static_cast<int>(sizeof(Cursor)) + 2 * static_cast<int>(sizeof(Segment)) + 4);
+         kWarps * (static_cast<int>(sizeof(Cursor)) + 2 * static_cast<int>(sizeof(Segment)) + 4);
 }
-
-__device__ unsigned int g_fp4_timeouts = 0;
 
 // x: one row's D values, lane i holding channels i, i + 32, ..
 template <int NB>
@@ -240,8 +258,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   int* col_limit = reinterpret_cast<int*>(col_scale + COLS);
   float* warp_m = reinterpret_cast<float*>(col_limit + COLS);      // [warp][COLS]
   float* warp_l = warp_m + kWarps * COLS;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(warp_l + kWarps * COLS);   // [warp][stage]: the stage's bytes are there
-  Cursor* cursor = reinterpret_cast<Cursor*>(bars + kWarps * L::kStages);         // [warp]
+  Cursor* cursor = reinterpret_cast<Cursor*>(warp_l + kWarps * COLS);              // [warp]
   Segment* segment = reinterpret_cast<Segment*>(cursor + kWarps);                 // [warp][2]
   unsigned* join_at = reinterpret_cast<unsigned*>(segment + 2 * kWarps);          // [warp]: its stage for the join
   // groups of 16 keys that go through the products together: two where the accumulators leave registers for them
@@ -250,20 +267,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
   const unsigned ring = smem_base + warp * L::kStages * L::kStage;
-  const unsigned bar = static_cast<unsigned>(__cvta_generic_to_shared(bars)) + warp * L::kStages * 8;
-  if (lane < L::kStages) tc::mbar_init(bar + lane * 8, 2);   // a stage's two groups arrive apart
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  tc::fence_proxy_async();
-  __syncwarp();
-  unsigned phases = 0;                            // bit i: parity of stage i's next completion
-
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ------------------------------------------------------------- segments
   // A segment is the block's run of one unit's tiles.  What only a segment's ends need lies in shared memory, a copy for
   // each warp: [0] the segment whose copies run, [1] the one before it.
   int n_mine = 0;                                 // the warp's tiles of the segment
-  bool gave_up = false;
   int stage = 0;
   {
     Cursor cur;
@@ -315,7 +324,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     }
     __syncwarp();
     const int first = sg.c_begin + warp;
-    n_mine = sg.c_end > first && !gave_up ? (sg.c_end - first + kWarps - 1) / kWarps : 0;
+    // (an empty pool has no group that could stand in for the missing ones: its tiles are left out)
+    n_mine = sg.c_end > first && p.pool.num_pages > 0 ? (sg.c_end - first + kWarps - 1) / kWarps : 0;
     return true;
   };
   auto stage_queries = [&]() {
@@ -363,13 +373,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   };
 
   // ---------------------------------------------------------------- copies
-  // The warp's tiles are c_begin + warp + kWarps k.  Of every 16 of them lane 2 i + u owns group u of tile i: it reads
-  // the page id (a batch ahead), holds the source address and issues the copy.
-  int next_id = -1;
+  // The warp's tiles are c_begin + warp + kWarps k.  Of every 16 of them lane 2 i + u looks up group u of tile i: it
+  // reads the page id a batch ahead and holds the group's number in the pool (0 for a page that does not exist: its
+  // rows are masked).
+  int next_id = -1, src_group = 0;
   unsigned history = 0;                           // two bits per tile issued, the last in bits 0, 1: its pages exist
-  const uint8_t* src = nullptr;
-  bool src_ok = false;
   unsigned batch_ok = 0;
+  const uint8_t* const lane_data = p.pool.data + lane * 16;
   auto group_of = [&](int k) { return (segment[2 * warp].c_begin + warp + kWarps * (k + (lane >> 1))) * 2 + (lane & 1); };
   auto load_id = [&](int k) {
     const Segment& sg = segment[2 * warp];
@@ -382,19 +392,23 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     if (k < n_mine) {
       const int i = k & 15;
       if (i == 0) {
-        const unsigned sub = static_cast<unsigned>(group_of(k)) % p.gpp;
-        src_ok = next_id >= 0 && next_id < p.pool.num_pages;
-        src = p.pool.data + (static_cast<int64_t>(next_id) * p.gpp + sub) * Gr::kBytes;
-        batch_ok = __ballot_sync(~0u, src_ok);
+        const bool ok = next_id >= 0 && next_id < p.pool.num_pages;
+        src_group = ok ? next_id * p.gpp + static_cast<int>(static_cast<unsigned>(group_of(k)) % p.gpp) : 0;
+        batch_ok = __ballot_sync(~0u, ok);
         next_id = load_id(k + 16);
       }
-      if ((lane >> 1) == i) {
-        const unsigned full = bar + to_stage * 8;
-        tc::mbar_arrive_expect_tx(full, src_ok ? Gr::kBytes : 0);
-        if (src_ok) tc::bulk_load(ring + to_stage * L::kStage + (lane & 1) * Gr::kBytes, src, Gr::kBytes, full);
-      }
       history |= (batch_ok >> (2 * i)) & 3;
+      const unsigned to = ring + to_stage * L::kStage + lane * 16;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* from = lane_data + static_cast<int64_t>(__shfl_sync(~0u, src_group, 2 * i + u)) * Gr::kBytes;
+#pragma unroll
+        for (int c = 0; c < Gr::kBytes / 512; ++c) copy16(to + u * Gr::kBytes + c * 512, from + c * 512);
+        constexpr int rest = Gr::kBytes % 512 / 16;               // lanes of the last copy
+        if (lane < rest) copy16(to + u * Gr::kBytes + Gr::kBytes / 512 * 512, from + Gr::kBytes / 512 * 512);
+      }
     }
+    copy_commit();
   };
   auto start_copies = [&]() {
     next_id = load_id(0);
@@ -438,17 +452,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     int key0 = (segment[2 * warp].c_begin + warp) * kTileKeys;
     for (int k = 0; k < n_mine; ++k, key0 += kWarps * kTileKeys) {
       // the stage read in the last round is free: every lane is past its reads
-      __syncwarp();
+      warp_sync();
       issue(k + L::kStages - 1, stage == 0 ? L::kStages - 1 : stage - 1);
-      const unsigned done = bar + stage * 8, parity = (phases >> stage) & 1;
-      if (!__all_sync(~0u, tc::mbar_try_wait(done, parity)) && !__all_sync(~0u, tc::mbar_wait(done, parity))) {
-        // the call's output is undefined from here on; the copies in flight land before the block ends
-        gave_up = true;
-        if (lane == 0) atomicAdd(&g_fp4_timeouts, 1u);
-        for (int i = 0; i < L::kStages; ++i) tc::mbar_wait(bar + i * 8, (phases >> i) & 1);
-        break;
-      }
-      phases ^= 1u << stage;
+      copy_wait<L::kStages - 1>();
+      warp_sync();
       const unsigned at = ring + stage * L::kStage;
       stage = stage + 1 == L::kStages ? 0 : stage + 1;
       const unsigned ok_here = (history >> (2 * (L::kStages - 1))) & 3;
@@ -460,12 +467,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
         float s[U][NT][4];
         {
           unsigned kw[U][2][NB];
-          unsigned ksw[U][NB / 2];
+          float ks[U][2 * NB];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             read_words(at + (v + u) * Gr::kBytes, kw[u][0]);
             read_words(at + (v + u) * Gr::kBytes + Gr::kSet, kw[u][1]);
-            lds_words<NB / 2>(at + (v + u) * Gr::kBytes + Gr::kKs + g * 2 * NB, ksw[u]);
+            unsigned ksw[NB / 2];
+            lds_words<NB / 2>(at + (v + u) * Gr::kBytes + Gr::kKs + g * 2 * NB, ksw);
+#pragma unroll
+            for (int i = 0; i < NB / 2; ++i) scales4(ksw[i], &ks[u][4 * i]);
           }
 #pragma unroll
           for (int bk = 0; bk < NB; ++bk) {
@@ -480,9 +490,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
               unsigned r0[4], r1[4];
               fp4_unpack4(kw[u][0][bk], r0);
               fp4_unpack4(kw[u][1][bk], r1);
-              const int i0 = bk, i1 = NB + bk;          // scale bytes of rows g and g + 8
-              const float s0 = fp4_scale(__byte_perm(ksw[u][i0 / 4], 0, 0x4440 + i0 % 4));
-              const float s1 = fp4_scale(__byte_perm(ksw[u][i1 / 4], 0, 0x4440 + i1 % 4));
+              const float s0 = ks[u][bk], s1 = ks[u][NB + bk];   // of rows g and g + 8
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 float acc[4];
@@ -702,7 +710,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
         }
         if (write) finish_row<NB>(p, done_sg.b, h * p.G + row / p.M, row % p.M, x);
       }
-      tc::fence_proxy_async();                    // the next segment's copies write where these lines read
       __syncthreads();
     }
 
@@ -919,6 +926,7 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
   DecP p = {};
   p.pool = {static_cast<uint8_t*>(pool->data), pool->num_pages, pool->page_size, pool->head_dim};
   p.gpp = pool->page_size / 16;
+  if (pool->num_pages * p.gpp > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "%s: more than 2^31 groups of rows", what);
   p.q = a->q; p.q_dtype = a->q_dtype; p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h; p.q_sm = a->q_stride_m;
   p.out = a->out; p.out_dtype = a->out_dtype;
   p.o_sb = a->out_stride_b; p.o_sh = a->out_stride_h; p.o_sm = a->out_stride_m;
@@ -942,19 +950,6 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
 }
 
 }  // namespace
-
-int read_fp4_timeouts(unsigned int* value, bool reset) {
-  unsigned int v = 0;
-  int st = check_cuda(cudaMemcpyFromSymbol(&v, g_fp4_timeouts, sizeof(v)), "read fp4 timeouts");
-  if (st) return st;
-  if (reset && v) {
-    const unsigned int zero = 0;
-    st = check_cuda(cudaMemcpyToSymbol(g_fp4_timeouts, &zero, sizeof(zero)), "reset fp4 timeouts");
-    if (st) return st;
-  }
-  *value = v;
-  return IAK_OK;
-}
 
 }  // namespace iak
 

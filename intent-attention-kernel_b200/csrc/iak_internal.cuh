@@ -23,7 +23,6 @@ int device_sm_count();
 int device_clock_khz();
 // timeout counters of each kernel family (defined beside the kernels)
 int read_decode_timeouts(unsigned int* value, bool reset);
-int read_fp4_timeouts(unsigned int* value, bool reset);   // counted with the decode family
 int read_mla_timeouts(unsigned int* value, bool reset);
 int read_prefill_timeouts(unsigned int* value, bool reset);
 // default budget of a bounded device-side wait: about 2 s at the boost clock
