@@ -30,7 +30,6 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxGrid = 1024;      // blocks of the main kernel when units are cut
 constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
 constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
@@ -52,6 +51,7 @@ struct DecP {
   int HC;                            // units of a sequence: Ht * CG
   int grid;                          // blocks of the main kernel
   int direct;                        // one block per unit, nothing to join
+  int by_unit;                       // cuts are recorded per unit, not per border
   int min_tiles;                     // tiles a block takes at least
   float* ws;
 };
@@ -106,25 +106,21 @@ __device__ __forceinline__ int64_t blocks_used(const DecP& p, int64_t total) {
   return most < p.grid ? most : p.grid;
 }
 
-// What the join kernel reads of the border at the start of a block's run: the unit cut there, if this is its first cut.
-struct Border { int b, h, j0, last; };        // last: last block with a part of the unit; -1 = nothing to join here
-__device__ __forceinline__ Border* borders(const DecP& p, int cols) {
-  return reinterpret_cast<Border*>(p.ws + static_cast<size_t>(p.grid) * 2 * cols * (p.pool.D + 2));
+// What the join kernel reads of a unit cut over several blocks.  Where there are fewer units than blocks a record per
+// unit, written by the block that has its first tile; else one per border between two blocks, written by the block
+// that the border begins and empty unless it is a unit's first cut.
+struct Cut { int b, h, j0, first, which, last; };   // first, last: blocks with a part; which: first's; last < 0: none
+__device__ __forceinline__ Cut* cuts(const DecP& p, int cols) {
+  return reinterpret_cast<Cut*>(p.ws + static_cast<size_t>(p.grid) * 2 * cols * (p.pool.D + 2));
 }
-__device__ __forceinline__ void write_border(const DecP& p, int64_t total, int64_t used, int64_t t0, int b, int64_t off,
-                                             int cols) {
-  const int n = seq_tiles(p, b);
-  const int unit = static_cast<int>(off / n), c = static_cast<int>(off - static_cast<int64_t>(unit) * n);
-  const int64_t begin = t0 - c;               // the unit's first tile
-  const int64_t before = blockIdx.x ? total * (blockIdx.x - 1) / used : 0;
-  Border d = {b, unit / p.CG, (unit % p.CG) * cols, -1};
-  if (c != 0 && before <= begin) {
-    // block of the unit's last tile t: the largest i with floor(total * i / used) <= t; bit 30 of j0 says that
-    // the block before began its run with this unit
-    d.last = static_cast<int>(((begin + n) * used - 1) / total);
-    if (before == begin) d.j0 |= 1 << 30;
-  }
-  borders(p, cols)[blockIdx.x] = d;
+// the unit of sequence b that begins with tile `begin`, of which block `first` has the first part
+__device__ __forceinline__ Cut make_cut(const DecP& p, int64_t total, int64_t used, int b, int unit, int64_t begin, int n,
+                                        int64_t first, int cols) {
+  Cut d = {b, unit / p.CG, (unit % p.CG) * cols, static_cast<int>(first), total * first / used == begin ? 0 : 1, -1};
+  // block of the unit's last tile t: the largest i with floor(total * i / used) <= t
+  const int last = static_cast<int>(((begin + n) * used - 1) / total);
+  if (last > d.first) d.last = last;
+  return d;
 }
 
 // ---------------------------------------------------------------------- PTX
@@ -194,7 +190,7 @@ __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
 }
 
 // ------------------------------------------------------------- shared layout
-struct Cursor { int64_t left, off; int b, pad; };          // tiles left to the block, next tile of sequence b
+struct Cursor { int64_t left, off, at; int b, pad; };   // tiles left to the block; the next one, of sequence b and of all
 struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, pad; };
 
 template <int NB>
@@ -242,7 +238,7 @@ __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f :
 // blocks of an SM: two where shared memory holds two rings and the accumulators leave the registers
 template <int NB, int NT, bool SPLIT>
 constexpr int blocks_per_sm() {
-  return NB <= 4 && NT * NB <= 8 && !(SPLIT && NT * NB > 4) ? 2 : 1;
+  return NB <= 4 && NT <= 2 && !(SPLIT && NT * NB > 4) ? 2 : 1;
 }
 
 template <int NB, int NT, bool SPLIT>
@@ -261,8 +257,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   Cursor* cursor = reinterpret_cast<Cursor*>(warp_l + kWarps * COLS);              // [warp]
   Segment* segment = reinterpret_cast<Segment*>(cursor + kWarps);                 // [warp][2]
   unsigned* join_at = reinterpret_cast<unsigned*>(segment + 2 * kWarps);          // [warp]: its stage for the join
-  // groups of 16 keys that go through the products together: two where the accumulators leave registers for them
-  constexpr int U = NT == 1 && NB <= 4 ? 2 : 1;
+  // Groups of 16 keys that go through the products together: two, for the independent work, except where the
+  // accumulators then leave too few registers.  (32 sequences of 32k, D 128, 16 columns: 328 us with one and two blocks
+  // an SM, 354 with two and one block; 32 columns: 152 with two, 168 with one, 8 sequences.)
+  constexpr int U = NT == 2 && NB >= 4 ? 1 : 2;
+
+  __shared__ int64_t run_total, run_used;         // kept by the last warp's first lane
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
@@ -275,9 +275,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   int n_mine = 0;                                 // the warp's tiles of the segment
   int stage = 0;
   {
-    Cursor cur;
-    cur.b = 0;
-    cur.left = cur.off = 0;
+    Cursor cur = {};
     if (p.direct) {
       cur.b = blockIdx.x / p.HC;
       const int n = seq_tiles(p, cur.b);
@@ -290,7 +288,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
       const int64_t t0 = total * blockIdx.x / used;
       cur.left = total * (blockIdx.x + 1) / used - t0;
       find_sequence(p, t0, cur.b, cur.off);
-      if (warp == kWarps - 1 && lane == 0) write_border(p, total, used, t0, cur.b, cur.off, 8 * NT);
+      cur.at = t0;
+      if (warp == kWarps - 1 && lane == 0) {
+        run_total = total;
+        run_used = used;
+        if (!p.by_unit) {
+          const int n = seq_tiles(p, cur.b), unit = static_cast<int>(cur.off / n);
+          const int64_t begin = t0 - cur.off + static_cast<int64_t>(unit) * n;
+          Cut d = {0, 0, 0, 0, 0, -1};
+          if (begin < t0 && total * (blockIdx.x - 1) / used <= begin)
+            d = make_cut(p, total, used, cur.b, unit, begin, n, blockIdx.x - 1, COLS);
+          cuts(p, COLS)[blockIdx.x] = d;
+        }
+      }
     }
     if (cur.left <= 0 || cur.b >= p.B) return;    // (every block of the grid has work: for safety)
     if (lane == 0) cursor[warp] = cur;
@@ -310,8 +320,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     sg.h = unit / p.CG;
     sg.cg = unit - sg.h * p.CG;
     const int n = sg.c_end - sg.c_begin;
+    if (!p.direct && p.by_unit && warp == kWarps - 1 && lane == 0 && sg.c_begin == 0)
+      cuts(p, COLS)[sg.b * p.HC + unit] =
+          make_cut(p, run_total, run_used, sg.b, unit, cur.at, sg.n_tiles, blockIdx.x, COLS);
     cur.left -= n;
     cur.off += n;
+    cur.at += n;
     if (cur.off == static_cast<int64_t>(sg.n_tiles) * p.HC) {
       cur.off = 0;
       ++cur.b;
@@ -719,8 +733,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
 }
 
 // ---------------------------------------------------------------- join kernel
-// One block per (border between two blocks' runs, output row): where a unit is first cut, its partials are added in
-// order of the blocks that left them.
+// One block per (record of a cut, output row): the unit's partials are added in order of the blocks that left them.
 constexpr int kJoinWarps = 8;
 
 __host__ __device__ inline int join_rows(int NC, int cols, int diff) {
@@ -730,76 +743,77 @@ __host__ __device__ inline int join_rows(int NC, int cols, int diff) {
 template <int NB, int NT>
 __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p) {
   constexpr int D = NB * 32, COLS = 8 * NT;
-  __shared__ float weight[kMaxGrid];               // of each part
-  __shared__ float part_sum[kJoinWarps][D];
-  __shared__ float warp_x[kJoinWarps];
+  __shared__ float part_sum[kJoinWarps][D + 2];
   const int per = p.diff ? 2 : 1;
   const int rows = join_rows(p.NC, COLS, p.diff);
-  const int border = 1 + blockIdx.x / rows, r = blockIdx.x % rows;
+  const int record = blockIdx.x / rows + (p.by_unit ? 0 : 1), r = blockIdx.x % rows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t used = blocks_used(p, total_tiles(p));
+  const int64_t used = p.by_unit ? 0 : blocks_used(p, total_tiles(p));
   // every block waits, so that this kernel never ends before the main one
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (border >= used) return;
-  Border d = borders(p, COLS)[border];
-  if (d.last < 0) return;
-  const int first = border - 1, first_which = d.j0 >> 30 ? 0 : 1, n = d.last - first + 1;
-  const int j0 = (d.j0 & ~(1 << 30)) + r * per;
-  if (j0 >= p.NC) return;
-  auto part_of = [&](int i, int col) {
-    return p.ws + ((static_cast<int64_t>(first + i) * 2 + (i == 0 ? first_which : 0)) * COLS + col) * (D + 2);
-  };
+  if (!p.by_unit && record >= used) return;
+  const Cut d = cuts(p, COLS)[record];
+  const int n = d.last - d.first + 1, j0 = d.j0 + r * per;
+  if (d.last < 0 || j0 >= p.NC) return;
   float x[NB];
   for (int half = 0; half < per; ++half) {
     const int col = r * per + half;
-    // the largest maximum, then every part's weight and the sum of l
-    float top = -FLT_MAX;
-    for (int i = threadIdx.x; i < n; i += kJoinWarps * 32) top = fmaxf(top, part_of(i, col)[D]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    if (lane == 0) warp_x[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, warp_x[w]);
-    __syncthreads();
-    float l = 0.f;
-    for (int i = threadIdx.x; i < n; i += kJoinWarps * 32) {
-      const float* part = part_of(i, col);
-      const float f = tc::ex2(part[D] - top);
-      weight[i] = f;
-      l = fmaf(part[D + 1], f, l);
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(~0u, l, o);
-    if (lane == 0) warp_x[warp] = l;
-    __syncthreads();
-    float acc[NB];
+    // warp w: parts w, w + 8, .., four at a time, so that their loads run together
+    float top = -FLT_MAX, l = 0.f, acc[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) acc[i] = 0.f;
-#pragma unroll 4
-    for (int c = warp; c < n; c += kJoinWarps) {
-      const float* part = part_of(c, col);
-      const float f = weight[c];
+    constexpr int kAt = NB <= 4 ? 4 : 2;
+    for (int c = warp; c < n; c += kAt * kJoinWarps) {
+      float m[kAt], pl[kAt], v[kAt][NB];
 #pragma unroll
-      for (int i = 0; i < NB; ++i) acc[i] = fmaf(part[i * 32 + lane], f, acc[i]);
+      for (int k = 0; k < kAt; ++k) {
+        const int part = min(c + k * kJoinWarps, n - 1);
+        const float* at = p.ws + ((static_cast<int64_t>(d.first + part) * 2 + (part == 0 ? d.which : 0)) * COLS + col) * (D + 2);
+        m[k] = at[D];
+        pl[k] = at[D + 1];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) v[k][i] = at[i * 32 + lane];
+      }
+      float next = top;
+#pragma unroll
+      for (int k = 0; k < kAt; ++k) next = fmaxf(next, m[k]);
+      const float old = tc::ex2(top - next);
+      l *= old;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) acc[i] *= old;
+#pragma unroll
+      for (int k = 0; k < kAt; ++k) {
+        const float f = tc::ex2(m[k] - next);
+        if (c + k * kJoinWarps < n) {              // (a part read in place of a missing one may hold NaN)
+          l = fmaf(pl[k], f, l);
+#pragma unroll
+          for (int i = 0; i < NB; ++i) acc[i] = fmaf(v[k][i], f, acc[i]);
+        }
+      }
+      top = next;
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) part_sum[warp][i * 32 + lane] = acc[i];
+    if (lane == 0) { part_sum[warp][D] = top; part_sum[warp][D + 1] = l; }
     __syncthreads();
     if (warp == 0) {
-      float sum = 0.f;
+      float all = -FLT_MAX, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) sum += warp_x[w];
+      for (int w = 0; w < kJoinWarps; ++w) all = fmaxf(all, part_sum[w][D]);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) acc[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWarps; ++w) {
+        const float f = tc::ex2(part_sum[w][D] - all);
+        sum = fmaf(part_sum[w][D + 1], f, sum);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) acc[i] = fmaf(part_sum[w][i * 32 + lane], f, acc[i]);
+      }
       const int row = p.diff ? (j0 >> 1) : j0;
       const float inv = safe_inverse(sum);
       const float scale = half ? -p.lam[d.h * p.G + row / p.M] * inv : inv;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) v += part_sum[w][i * 32 + lane];
-        x[i] = half ? fmaf(v, scale, x[i]) : v * scale;
-      }
+      for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], scale, x[i]) : acc[i] * scale;
       if (half == per - 1) finish_row<NB>(p, d.b, d.h * p.G + row / p.M, row % p.M, x);
     }
     __syncthreads();
@@ -850,11 +864,12 @@ int make_plan(DecP& p, Plan* plan) {
     plan->ws = 0;
   } else {
     const int64_t useful = (most * units + kWarps - 1) / kWarps;
-    plan->grid = static_cast<int>(std::min<int64_t>(std::min(blocks, kMaxGrid), useful));
-    plan->ws = static_cast<size_t>(plan->grid) * (2 * 8 * NT * (NB * 32 + 2) * sizeof(float) + sizeof(Border));
+    plan->grid = static_cast<int>(std::min<int64_t>(blocks, useful));
+    plan->ws = static_cast<size_t>(plan->grid) * (2 * 8 * NT * (NB * 32 + 2) * sizeof(float) + sizeof(Cut));
   }
   p.grid = plan->grid;
   p.direct = plan->direct ? 1 : 0;
+  p.by_unit = units <= plan->grid ? 1 : 0;
   return IAK_OK;
 }
 
@@ -871,7 +886,7 @@ int run_shape(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cud
   if (int st = check_cuda(cudaGetLastError(), "fp4_decode launch")) return st;
   if (plan.grid == 1 || plan.direct) return IAK_OK;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((plan.grid - 1) * join_rows(p.NC, 8 * NT, p.diff)));
+  cfg.gridDim = dim3(static_cast<unsigned>((p.by_unit ? p.B * p.HC : plan.grid - 1) * join_rows(p.NC, 8 * NT, p.diff)));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = s;
   // starts while the main kernel's last blocks run; it waits for them before it reads a partial
