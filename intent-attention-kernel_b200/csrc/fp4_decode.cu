@@ -1,7 +1,7 @@
 // Attention of a sequence's last tokens over an FP4 page pool (iak_fp4_decode), plain and differential.
 //
 // Mathematics.  A table head's queries form NC = G * M * (1 or 2) softmax columns (differential: two per query, the
-// first with q2 = 0 and the second with q1 = 0, so that both halves run as one product).  Per tile of 32 keys
+// first with q2 = 0 and the second with q1 = 0, so that both halves run as one product).  Per tile of 32 keys (16 for D 256)
 //   S' = K Q',  P = exp2(S - m),  O' += V' P'
 // with running maximum m and sum l per column, fp32.  Keys are the rows of the first product and the contraction of
 // the second, columns the narrow side (n = 8 per mma.m16n8k16), so that few queries waste little.
@@ -10,7 +10,7 @@
 //   V: a byte holds one channel of two neighbouring keys, so that its half pair lies along the contraction; it is
 //      multiplied by the two keys' scales (exact: the pool's values are halves).
 //   P: from the accumulator's layout to the operand's by movmatrix.
-// What bounds it: the cache's bytes, 4.25 bits an element.  Work is cut into equal runs of 32-key tiles over all
+// What bounds it: the cache's bytes, 4.25 bits an element.  Work is cut into equal runs of tiles over all
 // (sequence, table head, column group) units, one run per resident block, so that ragged batches and single long
 // sequences fill the GPU alike; a unit cut over several blocks leaves partial (m, l, O) that a second kernel joins in
 // order of the blocks (no atomics: results do not depend on timing).  Each warp streams its own tiles through a
@@ -30,7 +30,6 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
 constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
 constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small P stay normal halves
@@ -53,6 +52,7 @@ struct DecP {
   int direct;                        // one block per unit, nothing to join
   int by_unit;                       // cuts are recorded per unit, not per border
   int min_tiles;                     // tiles a block takes at least
+  int tile_shift;                    // log2 of a tile's keys
   float* ws;
 };
 
@@ -62,13 +62,13 @@ __device__ __forceinline__ int seq_len(const DecP& p, int b) {
 }
 // tiles of one unit; an empty sequence has one, which writes its zeros
 __device__ __forceinline__ int seq_tiles(const DecP& p, int b) {
-  return max(1, static_cast<int>((static_cast<int64_t>(seq_len(p, b)) + kTileKeys - 1) / kTileKeys));
+  return max(1, (seq_len(p, b) + (1 << p.tile_shift) - 1) >> p.tile_shift);
 }
 
-// all tiles of the call (every lane of every warp has it)
-__device__ __forceinline__ int64_t total_tiles(const DecP& p) {
+// all tiles of the call (every lane of every warp has it); the host keeps their number within 31 bits
+__device__ __forceinline__ int total_tiles(const DecP& p) {
   const int lane = threadIdx.x & 31;
-  int64_t sum = 0;
+  int sum = 0;
   for (int b = lane; b < p.B; b += 32) sum += seq_tiles(p, b);
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
@@ -76,51 +76,52 @@ __device__ __forceinline__ int64_t total_tiles(const DecP& p) {
 }
 
 // sequence that holds tile t, and t's offset among that sequence's tiles
-__device__ __forceinline__ void find_sequence(const DecP& p, int64_t t, int& b, int64_t& off) {
+__device__ __forceinline__ void find_sequence(const DecP& p, int t, int& b, int& off) {
   const int lane = threadIdx.x & 31;
-  int64_t before = 0;
+  int before = 0;
+  b = p.B;
+  off = 0;
   for (int base = 0; base < p.B; base += 32) {
     const int i = base + lane;
-    int64_t n = i < p.B ? static_cast<int64_t>(seq_tiles(p, i)) * p.HC : 0;
-    int64_t inc = n;
+    const int n = i < p.B ? seq_tiles(p, i) * p.HC : 0;
+    int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(~0u, inc, o);
+      const int v = __shfl_up_sync(~0u, inc, o);
       if (lane >= o) inc += v;
     }
-    const unsigned hit = __ballot_sync(~0u, i < p.B && before + inc > t);
+    const unsigned hit = __ballot_sync(~0u, before + inc > t);
     if (hit) {
       const int l = __ffs(hit) - 1;
       b = base + l;
       off = t - (before + __shfl_sync(~0u, inc - n, l));
-      return;
+      break;
     }
     before += __shfl_sync(~0u, inc, 31);
   }
-  b = p.B;
-  off = 0;
 }
 
-__device__ __forceinline__ int64_t blocks_used(const DecP& p, int64_t total) {
-  const int64_t most = (total + p.min_tiles - 1) / p.min_tiles;
-  return most < p.grid ? most : p.grid;
+// The tiles in equal runs: `used` blocks, the first `more` of them with each + 1 tiles.
+struct Runs { int used, each, more; };
+__device__ __forceinline__ Runs make_runs(const DecP& p, int total) {
+  Runs r;
+  r.used = static_cast<int>(min((static_cast<unsigned>(total) + p.min_tiles - 1) / p.min_tiles, static_cast<unsigned>(p.grid)));
+  r.each = total / r.used;
+  r.more = total - r.each * r.used;
+  return r;
+}
+__device__ __forceinline__ int run_begin(const Runs& r, int i) { return i * r.each + min(i, r.more); }
+__device__ __forceinline__ int block_of(const Runs& r, int t) {
+  const int large = r.more * (r.each + 1);
+  return t < large ? t / (r.each + 1) : r.more + (t - large) / r.each;
 }
 
-// What the join kernel reads of a unit cut over several blocks.  Where there are fewer units than blocks a record per
+// What the join kernel reads of a unit cut over several blocks.  Where there are no more units than blocks a record per
 // unit, written by the block that has its first tile; else one per border between two blocks, written by the block
 // that the border begins and empty unless it is a unit's first cut.
 struct Cut { int b, h, j0, first, which, last; };   // first, last: blocks with a part; which: first's; last < 0: none
 __device__ __forceinline__ Cut* cuts(const DecP& p, int cols) {
   return reinterpret_cast<Cut*>(p.ws + static_cast<size_t>(p.grid) * 2 * cols * (p.pool.D + 2));
-}
-// the unit of sequence b that begins with tile `begin`, of which block `first` has the first part
-__device__ __forceinline__ Cut make_cut(const DecP& p, int64_t total, int64_t used, int b, int unit, int64_t begin, int n,
-                                        int64_t first, int cols) {
-  Cut d = {b, unit / p.CG, (unit % p.CG) * cols, static_cast<int>(first), total * first / used == begin ? 0 : 1, -1};
-  // block of the unit's last tile t: the largest i with floor(total * i / used) <= t
-  const int last = static_cast<int>(((begin + n) * used - 1) / total);
-  if (last > d.first) d.last = last;
-  return d;
 }
 
 // ---------------------------------------------------------------------- PTX
@@ -190,30 +191,45 @@ __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
 }
 
 // ------------------------------------------------------------- shared layout
-struct Cursor { int64_t left, off, at; int b, pad; };   // tiles left to the block; the next one, of sequence b and of all
-struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, pad; };
+struct Cursor { int left, off, at, b; };   // tiles left to the block; the next one, of sequence b and of all
+struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, at; };   // at: its first tile, of all
 
 template <int NB>
 struct Lay {
   using Gr = Fp4Group<NB>;
   static constexpr int D = NB * 32;
+  // Groups of a warp's tile: two; one for D 256, whose ring then leaves room for a second block on the SM.
+  static constexpr int TG = NB == 8 ? 1 : 2;
+  static constexpr int kTile = 16 * TG;
   static constexpr int kStages = 3;
-  static constexpr int kStage = 2 * Gr::kBytes;
+  static constexpr int kStage = TG * Gr::kBytes;
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kOutStride = D + 4;                 // floats of one column in the join buffer
+  // A warp's sums for the join lie in one stage, D / JH channels at a time; in pass dh place i of a lane's NB / JH values
+  // is channel(dh, 32 i + lane).
+  static constexpr int JH = NB == 8 ? 2 : 1;
+  static constexpr int kRun = 4 * NB / JH;                 // a lane's channels that lie side by side
+  static constexpr int kOutStride = D / JH + 4;            // floats of one column in the join buffer
+  static __device__ __forceinline__ int channel(int dh, int pos) {
+    return JH == 1 ? pos : pos / kRun * (4 * NB) + dh * kRun + pos % kRun;
+  }
   static_assert(8 * kOutStride * 4 <= kStage, "a warp's sums for the join lie in one stage of its ring");
 };
 
 template <int NB, int NT, bool SPLIT>
 constexpr int smem_bytes() {
   return Lay<NB>::kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + 8 * NT * 8 + kWarps * 8 * NT * 8 +
-         kWarps * (static_cast<int>(sizeof(Cursor)) + 2 * static_cast<int>(sizeof(Segment)) + 4);
+         kWarps * (static_cast<int>(sizeof(Cursor)) + 2 * static_cast<int>(sizeof(Segment)) + 4) +
+         static_cast<int>(sizeof(Runs));
 }
 
-// x: one row's D values, lane i holding channels i, i + 32, ..
-template <int NB>
+// x: one row's D values; lane i's value of place k is channel i + 32 k, or in the main kernel's order (SPREAD)
+template <int NB, bool SPREAD>
 __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m, float (&x)[NB]) {
+  using L = Lay<NB>;
   const int lane = threadIdx.x & 31;
+  auto channel = [&](int k) {
+    return SPREAD ? L::channel(k / (NB / L::JH), k % (NB / L::JH) * 32 + lane) : k * 32 + lane;
+  };
   if (p.diff) {
     float mul = p.out_scale;
     if (p.norm_w) {
@@ -225,11 +241,11 @@ __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m
       mul *= rsqrtf(sq * (1.f / (NB * 32)) + p.eps);
     }
 #pragma unroll
-    for (int i = 0; i < NB; ++i) x[i] *= p.norm_w ? mul * p.norm_w[i * 32 + lane] : mul;
+    for (int i = 0; i < NB; ++i) x[i] *= p.norm_w ? mul * p.norm_w[channel(i)] : mul;
   }
   const int64_t at = b * p.o_sb + head * p.o_sh + m * p.o_sm;
 #pragma unroll
-  for (int i = 0; i < NB; ++i) store_from_float(p.out, p.out_dtype, at + i * 32 + lane, x[i]);
+  for (int i = 0; i < NB; ++i) store_from_float(p.out, p.out_dtype, at + channel(i), x[i]);
 }
 
 __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
@@ -238,7 +254,7 @@ __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f :
 // blocks of an SM: two where shared memory holds two rings and the accumulators leave the registers
 template <int NB, int NT, bool SPLIT>
 constexpr int blocks_per_sm() {
-  return NB <= 4 && NT <= 2 && !(SPLIT && NT * NB > 4) ? 2 : 1;
+  return NT <= 2 && NT * NB <= 8 && !(SPLIT && NT * NB > 4) ? 2 : 1;
 }
 
 template <int NB, int NT, bool SPLIT>
@@ -248,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   constexpr int D = L::D;
   constexpr int MT = D / 16;
   constexpr int COLS = 8 * NT;
-  extern __shared__ __align__(16) char smem[];
+  extern __shared__ __align__(128) char smem[];   // (no static shared memory: it would move the ring off its 128 bytes)
   char* q_frag = smem + L::kRing;                                   // [hi, lo][NT][NB][lane] 16 bytes
   float* col_scale = reinterpret_cast<float*>(q_frag + NT * NB * 512 * (SPLIT ? 2 : 1));
   int* col_limit = reinterpret_cast<int*>(col_scale + COLS);
@@ -257,12 +273,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   Cursor* cursor = reinterpret_cast<Cursor*>(warp_l + kWarps * COLS);              // [warp]
   Segment* segment = reinterpret_cast<Segment*>(cursor + kWarps);                 // [warp][2]
   unsigned* join_at = reinterpret_cast<unsigned*>(segment + 2 * kWarps);          // [warp]: its stage for the join
+  Runs& runs = *reinterpret_cast<Runs*>(join_at + kWarps);                        // kept by thread 0
   // Groups of 16 keys that go through the products together: two, for the independent work, except where the
   // accumulators then leave too few registers.  (32 sequences of 32k, D 128, 16 columns: 328 us with one and two blocks
   // an SM, 354 with two and one block; 32 columns: 152 with two, 168 with one, 8 sequences.)
-  constexpr int U = NT == 2 && NB >= 4 ? 1 : 2;
+  constexpr int TG = L::TG, U = TG == 1 || (NT == 2 && NB >= 4) ? 1 : 2;
 
-  __shared__ int64_t run_total, run_used;         // kept by the last warp's first lane
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
@@ -278,31 +294,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     Cursor cur = {};
     if (p.direct) {
       cur.b = blockIdx.x / p.HC;
-      const int n = seq_tiles(p, cur.b);
-      cur.off = static_cast<int64_t>(blockIdx.x - cur.b * p.HC) * n;
-      cur.left = n;
+      cur.left = seq_tiles(p, cur.b);
+      cur.off = (blockIdx.x - cur.b * p.HC) * cur.left;
     } else {
-      const int64_t total = total_tiles(p);
-      const int64_t used = blocks_used(p, total);
-      if (blockIdx.x >= used) return;
-      const int64_t t0 = total * blockIdx.x / used;
-      cur.left = total * (blockIdx.x + 1) / used - t0;
-      find_sequence(p, t0, cur.b, cur.off);
-      cur.at = t0;
-      if (warp == kWarps - 1 && lane == 0) {
-        run_total = total;
-        run_used = used;
-        if (!p.by_unit) {
-          const int n = seq_tiles(p, cur.b), unit = static_cast<int>(cur.off / n);
-          const int64_t begin = t0 - cur.off + static_cast<int64_t>(unit) * n;
-          Cut d = {0, 0, 0, 0, 0, -1};
-          if (begin < t0 && total * (blockIdx.x - 1) / used <= begin)
-            d = make_cut(p, total, used, cur.b, unit, begin, n, blockIdx.x - 1, COLS);
-          cuts(p, COLS)[blockIdx.x] = d;
-        }
-      }
+      const Runs r = make_runs(p, total_tiles(p));
+      if (blockIdx.x >= r.used) return;
+      cur.at = run_begin(r, blockIdx.x);
+      cur.left = run_begin(r, blockIdx.x + 1) - cur.at;
+      find_sequence(p, cur.at, cur.b, cur.off);
+      if (threadIdx.x == 0) runs = r;
     }
-    if (cur.left <= 0 || cur.b >= p.B) return;    // (every block of the grid has work: for safety)
     if (lane == 0) cursor[warp] = cur;
     __syncwarp();
   }
@@ -314,19 +315,17 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     sg.b = cur.b;
     sg.len = seq_len(p, cur.b);
     sg.n_tiles = seq_tiles(p, cur.b);
-    const int unit = static_cast<int>(cur.off / sg.n_tiles);      // of the sequence: table head, column group
-    sg.c_begin = static_cast<int>(cur.off - static_cast<int64_t>(unit) * sg.n_tiles);
-    sg.c_end = static_cast<int>(min(static_cast<int64_t>(sg.n_tiles), sg.c_begin + cur.left));
+    sg.at = cur.at;
+    const int unit = cur.off / sg.n_tiles;                        // of the sequence: table head, column group
+    sg.c_begin = cur.off - unit * sg.n_tiles;
+    sg.c_end = min(sg.n_tiles, sg.c_begin + cur.left);
     sg.h = unit / p.CG;
     sg.cg = unit - sg.h * p.CG;
     const int n = sg.c_end - sg.c_begin;
-    if (!p.direct && p.by_unit && warp == kWarps - 1 && lane == 0 && sg.c_begin == 0)
-      cuts(p, COLS)[sg.b * p.HC + unit] =
-          make_cut(p, run_total, run_used, sg.b, unit, cur.at, sg.n_tiles, blockIdx.x, COLS);
     cur.left -= n;
     cur.off += n;
     cur.at += n;
-    if (cur.off == static_cast<int64_t>(sg.n_tiles) * p.HC) {
+    if (cur.off == sg.n_tiles * p.HC) {
       cur.off = 0;
       ++cur.b;
     }
@@ -356,7 +355,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
           const int gi = row / p.M, m = row - gi * p.M;
           const int64_t at = sg.b * p.q_sb + (sg.h * p.G + gi) * p.q_sh + m * p.q_sm + ch * 8;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = load_as_float(p.q, p.q_dtype, at + e) * p.sign;
+          for (int e = 0; e < 8; ++e) {
+          if (SPLIT) {
+            x[e] = static_cast<const float*>(p.q)[at + e] * p.sign;
+          } else {
+            const uint16_t u = static_cast<const uint16_t*>(p.q)[at + e];
+            x[e] = (p.q_dtype == IAK_DT_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float(u << 16)) * p.sign;
+          }
+        }
         }
         float amax = 0.f;
 #pragma unroll
@@ -387,35 +393,36 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   };
 
   // ---------------------------------------------------------------- copies
-  // The warp's tiles are c_begin + warp + kWarps k.  Of every 16 of them lane 2 i + u looks up group u of tile i: it
-  // reads the page id a batch ahead and holds the group's number in the pool (0 for a page that does not exist: its
+  // The warp's tiles are c_begin + warp + kWarps k.  Of every 32 / TG of them lane TG i + u looks up group u of tile i:
+  // it reads the page id a batch ahead and holds the group's number in the pool (0 for a page that does not exist: its
   // rows are masked).
   int next_id = -1, src_group = 0;
-  unsigned history = 0;                           // two bits per tile issued, the last in bits 0, 1: its pages exist
+  unsigned history = 0;                           // TG bits per tile issued, the last lowest: its groups' pages exist
+  constexpr int kBatch = 32 / TG;
   unsigned batch_ok = 0;
   const uint8_t* const lane_data = p.pool.data + lane * 16;
-  auto group_of = [&](int k) { return (segment[2 * warp].c_begin + warp + kWarps * (k + (lane >> 1))) * 2 + (lane & 1); };
+  auto group_of = [&](int k) { return (segment[2 * warp].c_begin + warp + kWarps * (k + lane / TG)) * TG + lane % TG; };
   auto load_id = [&](int k) {
     const Segment& sg = segment[2 * warp];
     const int gr = group_of(k);
-    return k + (lane >> 1) < n_mine && gr * 16 < sg.len
+    return k + lane / TG < n_mine && gr * 16 < sg.len
                ? __ldg(p.pt + sg.b * p.pt_sb + sg.h * p.pt_sh + static_cast<unsigned>(gr) / p.gpp) : -1;
   };
   auto issue = [&](int k, int to_stage) {
-    history <<= 2;
+    history <<= TG;
     if (k < n_mine) {
-      const int i = k & 15;
+      const int i = k % kBatch;
       if (i == 0) {
         const bool ok = next_id >= 0 && next_id < p.pool.num_pages;
         src_group = ok ? next_id * p.gpp + static_cast<int>(static_cast<unsigned>(group_of(k)) % p.gpp) : 0;
         batch_ok = __ballot_sync(~0u, ok);
-        next_id = load_id(k + 16);
+        next_id = load_id(k + kBatch);
       }
-      history |= (batch_ok >> (2 * i)) & 3;
+      history |= (batch_ok >> (TG * i)) & ((1 << TG) - 1);
       const unsigned to = ring + to_stage * L::kStage + lane * 16;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint8_t* from = lane_data + static_cast<int64_t>(__shfl_sync(~0u, src_group, 2 * i + u)) * Gr::kBytes;
+      for (int u = 0; u < TG; ++u) {
+        const uint8_t* from = lane_data + static_cast<int64_t>(__shfl_sync(~0u, src_group, TG * i + u)) * Gr::kBytes;
 #pragma unroll
         for (int c = 0; c < Gr::kBytes / 512; ++c) copy16(to + u * Gr::kBytes + c * 512, from + c * 512);
         constexpr int rest = Gr::kBytes % 512 / 16;               // lanes of the last copy
@@ -427,6 +434,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   auto start_copies = [&]() {
     next_id = load_id(0);
     int to = stage;
+#pragma unroll 1
     for (int i = 0; i < L::kStages - 1; ++i) {
       issue(i, to);
       to = to + 1 == L::kStages ? 0 : to + 1;
@@ -443,16 +451,121 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
       }
     };
 
-  open_segment();
-  start_copies();
-  stage_queries();
-  __syncthreads();
-
-  bool begins_run = true;
+  // Each pass opens the next segment and starts its copies, joins the warps' sums of the last one, and runs the tiles.
+  // (One place in the code for each: a cold call fetches its instructions from memory.)
+  float o[NT][MT][4];
+  float m_run[NT][2], l_run[NT][2];
+  bool pending = false, begins_run = true;
   while (true) {
+    __syncwarp();
+    const bool more = open_segment();
+    if (more) start_copies();
+
+    if (pending) {
+      // ------------------------------------------------------ join the 8 warps
+      // in the stage of each warp's ring that the next segment's copies leave free
+      const unsigned my_join = warp * L::kStages * L::kStage + (stage == 0 ? L::kStages - 1 : stage - 1) * L::kStage;
+      if (lane == 0) join_at[warp] = my_join;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float v = l_run[nt][e];
+          v += __shfl_xor_sync(~0u, v, 4);
+          v += __shfl_xor_sync(~0u, v, 8);
+          v += __shfl_xor_sync(~0u, v, 16);
+          if (g == 0) {
+            warp_m[warp * COLS + nt * 8 + 2 * t + e] = m_run[nt][e];
+            warp_l[warp * COLS + nt * 8 + 2 * t + e] = v;
+          }
+        }
+      }
+      __syncthreads();                              // and every warp is past its last read of the queries
+      const Segment& done_sg = segment[2 * warp + (more ? 1 : 0)];
+      const int h = done_sg.h, cg = done_sg.cg;
+      const bool whole = done_sg.c_begin == 0 && done_sg.c_end == done_sg.n_tiles;
+      const int which = begins_run ? 0 : 1;
+      if (!p.direct && threadIdx.x == 0) {
+        const int begin = done_sg.at - done_sg.c_begin;             // the unit's first tile
+        Cut d = {done_sg.b, h, cg * COLS, static_cast<int>(blockIdx.x), which, -1};
+        if (p.by_unit) {
+          if (!whole) d.last = block_of(runs, begin + done_sg.n_tiles - 1);
+          if (done_sg.c_begin == 0) cuts(p, COLS)[done_sg.b * p.HC + h * p.CG + cg] = d;
+        } else if (begins_run) {
+          d.first = blockIdx.x - 1;
+          if (done_sg.c_begin > 0 && run_begin(runs, d.first) <= begin) {
+            d.which = run_begin(runs, d.first) == begin ? 0 : 1;
+            d.last = block_of(runs, begin + done_sg.n_tiles - 1);
+          }
+          cuts(p, COLS)[blockIdx.x] = d;
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float f[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float top = -FLT_MAX;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + nt * 8 + 2 * t + e]);
+          f[e] = tc::ex2(m_run[nt][e] - top);
+        }
+        const int per = p.diff ? 2 : 1;             // columns of an output row; a warp takes a row
+        const bool has_row = warp * per < 8 && cg * COLS + nt * 8 + warp * per < p.NC;
+        const int row = (cg * COLS + nt * 8) / per + warp;
+        float x[NB];
+#pragma unroll
+        for (int dh = 0; dh < L::JH; ++dh) {
+          float* dst = reinterpret_cast<float*>(smem + my_join) + 2 * t * L::kOutStride + g * L::kRun;
+#pragma unroll
+          for (int k = 0; k < MT / L::JH; ++k) {
+            const int i = dh * (MT / L::JH) + k;
+            *reinterpret_cast<float2*>(dst + 2 * k) = make_float2(o[nt][i][0] * f[0], o[nt][i][2] * f[0]);
+            *reinterpret_cast<float2*>(dst + L::kOutStride + 2 * k) = make_float2(o[nt][i][1] * f[1], o[nt][i][3] * f[1]);
+          }
+          __syncthreads();
+          if (has_row) {
+            for (int half = 0; half < per; ++half) {
+              const int lc = warp * per + half, col = nt * 8 + lc;
+              float top = -FLT_MAX, l = 0.f;
+#pragma unroll
+              for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + col]);
+#pragma unroll
+              for (int w = 0; w < kWarps; ++w) l += warp_l[w * COLS + col] * tc::ex2(warp_m[w * COLS + col] - top);
+              float acc[NB / L::JH];
+#pragma unroll
+              for (int i = 0; i < NB / L::JH; ++i) {
+                acc[i] = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w)
+                  acc[i] += reinterpret_cast<const float*>(smem + join_at[w])[lc * L::kOutStride + i * 32 + lane];
+              }
+              if (!whole) {
+                float* part = p.ws + ((static_cast<int64_t>(blockIdx.x) * 2 + which) * COLS + col) * (D + 2);
+#pragma unroll
+                for (int i = 0; i < NB / L::JH; ++i) part[L::channel(dh, i * 32 + lane)] = acc[i];
+                if (lane == 0 && dh == 0) { part[D] = top; part[D + 1] = l; }
+              } else {
+                const float inv = safe_inverse(l);
+                const float weight = half ? -p.lam[h * p.G + row / p.M] * inv : inv;
+#pragma unroll
+                for (int i = 0; i < NB / L::JH; ++i) {
+                  float& xi = x[dh * (NB / L::JH) + i];
+                  xi = half ? fmaf(acc[i], weight, xi) : acc[i] * weight;
+                }
+              }
+            }
+          }
+          __syncthreads();
+        }
+        if (has_row && whole) finish_row<NB, true>(p, done_sg.b, h * p.G + row / p.M, row % p.M, x);
+      }
+      begins_run = false;
+    }
+    if (!more) break;
+    stage_queries();
+    __syncthreads();
     float sc[NT][2];
-    float o[NT][MT][4];
-    float m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       sc[nt][0] = col_scale[nt * 8 + 2 * t];
@@ -463,8 +576,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
     }
     const int full_end = segment[2 * warp].len - (p.M - 1);   // every query sees the tokens before it
-    int key0 = (segment[2 * warp].c_begin + warp) * kTileKeys;
-    for (int k = 0; k < n_mine; ++k, key0 += kWarps * kTileKeys) {
+    int key0 = (segment[2 * warp].c_begin + warp) * L::kTile;
+    for (int k = 0; k < n_mine; ++k, key0 += kWarps * L::kTile) {
       // the stage read in the last round is free: every lane is past its reads
       warp_sync();
       issue(k + L::kStages - 1, stage == 0 ? L::kStages - 1 : stage - 1);
@@ -472,11 +585,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
       warp_sync();
       const unsigned at = ring + stage * L::kStage;
       stage = stage + 1 == L::kStages ? 0 : stage + 1;
-      const unsigned ok_here = (history >> (2 * (L::kStages - 1))) & 3;
-      const bool full = ok_here == 3 && key0 + kTileKeys <= full_end;
+      const unsigned ok_here = (history >> (TG * (L::kStages - 1))) & ((1 << TG) - 1);
+      const bool full = ok_here == (1 << TG) - 1 && key0 + L::kTile <= full_end;
 
 #pragma unroll 1
-      for (int v = 0; v < 2; v += U) {
+      for (int v = 0; v < TG; v += U) {
         // ---------------------------------------------------------- S' = K Q'
         float s[U][NT][4];
         {
@@ -640,95 +753,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
       }
     }
 
-    // the next segment's first copies are on their way while this one's warps join; the stage that they leave free
-    // takes the warp's sums
-    const unsigned my_join = warp * L::kStages * L::kStage + (stage == 0 ? L::kStages - 1 : stage - 1) * L::kStage;
-    __syncwarp();
-    const bool more = open_segment();
-    if (more) start_copies();
-
-    // ------------------------------------------------------ join the 8 warps
-    if (lane == 0) join_at[warp] = my_join;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float v = l_run[nt][e];
-        v += __shfl_xor_sync(~0u, v, 4);
-        v += __shfl_xor_sync(~0u, v, 8);
-        v += __shfl_xor_sync(~0u, v, 16);
-        if (g == 0) {
-          warp_m[warp * COLS + nt * 8 + 2 * t + e] = m_run[nt][e];
-          warp_l[warp * COLS + nt * 8 + 2 * t + e] = v;
-        }
-      }
-    }
-    __syncthreads();                              // every warp is past its last read of the queries
-    if (more) stage_queries();
-    const Segment& done_sg = segment[2 * warp + (more ? 1 : 0)];
-    const int h = done_sg.h, cg = done_sg.cg;
-    const bool whole = done_sg.c_begin == 0 && done_sg.c_end == done_sg.n_tiles;
-    const int which = begins_run ? 0 : 1;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float f[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float top = -FLT_MAX;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + nt * 8 + 2 * t + e]);
-        f[e] = tc::ex2(m_run[nt][e] - top);
-      }
-      float* dst = reinterpret_cast<float*>(smem + my_join) + 2 * t * L::kOutStride + g * (4 * NB);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[nt][i][0] * f[0], o[nt][i][2] * f[0]);
-        *reinterpret_cast<float2*>(dst + L::kOutStride + 2 * i) = make_float2(o[nt][i][1] * f[1], o[nt][i][3] * f[1]);
-      }
-      __syncthreads();
-      // a warp takes the columns of one output row
-      const int per = p.diff ? 2 : 1;
-      if (warp * per < 8) {
-        float x[NB];
-        bool write = true;
-        int row = 0;
-        for (int half = 0; half < per; ++half) {
-          const int lc = warp * per + half, col = nt * 8 + lc, j = cg * COLS + col;
-          if (j >= p.NC) { write = false; break; }
-          float top = -FLT_MAX, l = 0.f;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + col]);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) l += warp_l[w * COLS + col] * tc::ex2(warp_m[w * COLS + col] - top);
-          float acc[NB];
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            acc[i] = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w)
-              acc[i] += reinterpret_cast<const float*>(smem + join_at[w])[lc * L::kOutStride + i * 32 + lane];
-          }
-          if (!whole) {
-            float* part = p.ws + ((static_cast<int64_t>(blockIdx.x) * 2 + which) * COLS + col) * (D + 2);
-#pragma unroll
-            for (int i = 0; i < NB; ++i) part[i * 32 + lane] = acc[i];
-            if (lane == 0) { part[D] = top; part[D + 1] = l; }
-            write = false;
-            continue;
-          }
-          const float inv = safe_inverse(l);
-          row = p.diff ? j >> 1 : j;
-          const float weight = half ? -p.lam[h * p.G + row / p.M] * inv : inv;
-#pragma unroll
-          for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], weight, x[i]) : acc[i] * weight;
-        }
-        if (write) finish_row<NB>(p, done_sg.b, h * p.G + row / p.M, row % p.M, x);
-      }
-      __syncthreads();
-    }
-
-    begins_run = false;
-    if (!more) break;
+    pending = true;
   }
 }
 
@@ -748,7 +773,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p)
   const int rows = join_rows(p.NC, COLS, p.diff);
   const int record = blockIdx.x / rows + (p.by_unit ? 0 : 1), r = blockIdx.x % rows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t used = p.by_unit ? 0 : blocks_used(p, total_tiles(p));
+  const int used = p.by_unit ? 0 : make_runs(p, total_tiles(p)).used;
   // every block waits, so that this kernel never ends before the main one
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!p.by_unit && record >= used) return;
@@ -814,7 +839,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p)
       const float scale = half ? -p.lam[d.h * p.G + row / p.M] * inv : inv;
 #pragma unroll
       for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], scale, x[i]) : acc[i] * scale;
-      if (half == per - 1) finish_row<NB>(p, d.b, d.h * p.G + row / p.M, row % p.M, x);
+      if (half == per - 1) finish_row<NB, false>(p, d.b, d.h * p.G + row / p.M, row % p.M, x);
     }
     __syncthreads();
   }
@@ -854,9 +879,12 @@ int make_plan(DecP& p, Plan* plan) {
   if (units * 8 * NT > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: too many rows for one launch");
   p.HC = static_cast<int>(hc);
   p.min_tiles = kWarps;
-  const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + kTileKeys - 1) / kTileKeys;
+  p.tile_shift = Lay<NB>::kTile == 32 ? 5 : 4;
+  const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + Lay<NB>::kTile - 1) / Lay<NB>::kTile;
   // a unit that one tile per warp covers is one block's work: no joining
   plan->direct = most <= kWarps;
+  if (most * units > 0x7fffffffLL - 64)
+    return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: tables of more than 2^31 tiles of %d tokens", Lay<NB>::kTile);
   int blocks = 0;
   if (int st = resident_blocks<NB, NT, SPLIT>(&blocks)) return st;
   if (plan->direct) {
@@ -899,14 +927,15 @@ int run_shape(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cud
   return check_cuda(cudaLaunchKernelEx(&cfg, fp4_join_kernel<NB, NT>, cp), "fp4_join launch");
 }
 
-// columns per block: as many n = 8 tiles as the columns need, up to what the accumulators leave registers for;
-// more columns read the cache again
+// Columns per block: as many n = 8 tiles as the columns need, up to what the accumulators leave registers for; more
+// columns read the cache again.
 template <int NB, bool SPLIT>
 int run_cols(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cudaStream_t s) {
-  if (p.NC <= 8) return run_shape<NB, 1, SPLIT>(p, launch, ws, ws_bytes, need, s);
-  if (p.NC <= 16 || NB == 8 || SPLIT) return run_shape<NB, 2, SPLIT>(p, launch, ws, ws_bytes, need, s);
-  if constexpr (NB < 8 && !SPLIT) return run_shape<NB, 4, SPLIT>(p, launch, ws, ws_bytes, need, s);
-  return IAK_ERR_UNSUPPORTED;
+  if constexpr (NB < 8 && !SPLIT) {
+    if (p.NC > 16) return run_shape<NB, 4, SPLIT>(p, launch, ws, ws_bytes, need, s);
+  }
+  if (p.NC > 8) return run_shape<NB, 2, SPLIT>(p, launch, ws, ws_bytes, need, s);
+  return run_shape<NB, 1, SPLIT>(p, launch, ws, ws_bytes, need, s);
 }
 
 template <int NB>

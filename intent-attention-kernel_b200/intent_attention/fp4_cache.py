@@ -133,10 +133,12 @@ class Fp4Pool:
 #  Rows in and out
 # ---------------------------------------------------------------------- #
 
-def _rows_args(dev, k, v, page_table, positions, counts, dropped=None) -> N.Fp4RowsArgs:
+def _rows_args(dev, k, v, table, positions, counts, dropped=None) -> N.Fp4RowsArgs:
+    pt, pt_sb, pt_sh, _, W = table
     B, Ht, n, _ = k.shape
-    pt, pt_sb, pt_sh, _, W = _page_table(page_table, dev, B, Ht)
-    return N.Fp4RowsArgs(k.data_ptr(), v.data_ptr(), _DT[k.dtype], *k.stride()[:3], *v.stride()[:3], B, Ht, n,
+    ksb, ksh, ksn, _ = k.stride()
+    vsb, vsh, vsn, _ = v.stride()
+    return N.Fp4RowsArgs(k.data_ptr(), v.data_ptr(), _DT[k.dtype], ksb, ksh, ksn, vsb, vsh, vsn, B, Ht, n,
                          pt, pt_sb, pt_sh, W, _index_tensor(positions, "positions", dev, B),
                          _index_tensor(counts, "counts", dev, B), _index_tensor(dropped, "dropped", dev, 1))
 
@@ -155,11 +157,12 @@ def append_fp4(pool: Fp4Pool, k_new: torch.Tensor, v_new: torch.Tensor, page_tab
     two rows of V share their bytes.
     """
     dev = pool.device
-    for name, x in (("k_new", k_new), ("v_new", v_new)):
-        _require_cuda(x, name)
-        if x.device != dev:
-            raise ValueError(f"{name} is on {x.device}, the pool on {dev}")
-    if k_new.dim() != 4 or k_new.shape != v_new.shape or k_new.shape[3] != pool.head_dim:
+    _require_cuda(k_new, "k_new")
+    _require_cuda(v_new, "v_new")
+    if k_new.device != dev or v_new.device != dev:
+        raise ValueError(f"k_new is on {k_new.device}, v_new on {v_new.device}, the pool on {dev}")
+    shape = k_new.shape
+    if len(shape) != 4 or shape != v_new.shape or shape[3] != pool.head_dim:
         raise ValueError(f"k_new / v_new must both be [B, Ht, n, {pool.head_dim}]")
     if k_new.dtype != v_new.dtype or k_new.dtype not in _DT:
         raise ValueError("k_new / v_new must share a float32 / float16 / bfloat16 dtype")
@@ -167,7 +170,8 @@ def append_fp4(pool: Fp4Pool, k_new: torch.Tensor, v_new: torch.Tensor, page_tab
         k_new = k_new.contiguous()
     if v_new.stride(3) != 1:
         v_new = v_new.contiguous()
-    a = _rows_args(dev, k_new, v_new, page_table, positions, counts, dropped)
+    table = _page_table(page_table, dev, shape[0], shape[1])
+    a = _rows_args(dev, k_new, v_new, table, positions, counts, dropped)
     s = pool.struct()
     with _on(dev):
         N.check(N.lib().iak_fp4_append(ctypes.byref(s), ctypes.byref(a), _raw_stream(dev)), "iak_fp4_append")
@@ -181,14 +185,15 @@ def read_fp4(pool: Fp4Pool, page_table: torch.Tensor, positions: Optional[torch.
     types.  Rows from ``counts[b]`` on, and rows of slots or pages that do not
     exist, are 0.  ``out``: a (k, v) pair to write into."""
     dev = pool.device
-    _page_table(page_table, dev)
+    table = _page_table(page_table, dev)
     if num_rows < 0:
         raise ValueError("num_rows must not be negative")
     shape = (page_table.shape[0], page_table.shape[1], num_rows, pool.head_dim)
     if out is None:
         if dtype not in _DT:
             raise ValueError("dtype must be float32 / float16 / bfloat16")
-        k, v = torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev)
+        k = torch.empty(shape, dtype=dtype, device=dev)
+        v = torch.empty_like(k)
     else:
         k, v = out
         for name, x in (("out[0]", k), ("out[1]", v)):
@@ -197,7 +202,7 @@ def read_fp4(pool: Fp4Pool, page_table: torch.Tensor, positions: Optional[torch.
                 raise ValueError(f"{name} must be a {shape} float tensor on {dev}, both of one dtype")
             if x.stride(3) != 1:
                 raise ValueError(f"{name} needs a unit stride along head_dim")
-    a = _rows_args(dev, k, v, page_table, positions, counts)
+    a = _rows_args(dev, k, v, table, positions, counts)
     s = pool.struct()
     with _on(dev):
         N.check(N.lib().iak_fp4_read(ctypes.byref(s), ctypes.byref(a), _raw_stream(dev)), "iak_fp4_read")
@@ -214,14 +219,17 @@ def _decode(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Tensor, lengths: t
     dev = pool.device
     if q.device != dev:
         raise ValueError(f"q is on {q.device}, the pool on {dev}")
-    if q.dim() not in (3, 4) or q.shape[-1] != pool.head_dim:
-        raise ValueError(f"q must be [B, Hq, {pool.head_dim}] or [B, Hq, M, {pool.head_dim}], got {tuple(q.shape)}")
+    shape, strides = q.shape, q.stride()
+    dims = len(shape)
+    if dims not in (3, 4) or shape[-1] != pool.head_dim:
+        raise ValueError(f"q must be [B, Hq, {pool.head_dim}] or [B, Hq, M, {pool.head_dim}], got {tuple(shape)}")
     if q.dtype not in _DT:
         raise ValueError(f"q dtype {q.dtype} unsupported")
-    if q.stride(-1) != 1:
+    if strides[-1] != 1:
         q = q.contiguous()
-    B, Hq = q.shape[0], q.shape[1]
-    M = q.shape[2] if q.dim() == 4 else 1
+        strides = q.stride()
+    B, Hq = shape[0], shape[1]
+    M = shape[2] if dims == 4 else 1
     if M > N.FP4_MAX_QUERIES:
         raise ValueError(f"at most {N.FP4_MAX_QUERIES} queries per sequence, got {M}: read_fp4 the context for a prompt")
     pt, pt_sb, pt_sh, Ht, W = _page_table(page_table, dev, B)
@@ -230,17 +238,19 @@ def _decode(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Tensor, lengths: t
     if lengths is None:
         raise ValueError("lengths [B] is required")
     ln = _index_tensor(lengths, "lengths", dev, B)
-    if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=dev)
-        if out.dtype not in _DT:
-            raise ValueError(f"out dtype {out.dtype} unsupported")
-    else:
+    if out is not None:
         _require_cuda(out, "out")
-        if out.shape != q.shape or out.device != dev or out.dtype not in _DT or out.stride(-1) != 1:
-            raise ValueError(f"out must be a {tuple(q.shape)} float tensor on {dev} with a contiguous last dim")
-    qs, os_ = q.stride(), out.stride()
-    a = N.Fp4DecodeArgs(q.data_ptr(), _DT[q.dtype], qs[0], qs[1], qs[2] if q.dim() == 4 else 0,
-                        out.data_ptr(), _DT[out.dtype], os_[0], os_[1], os_[2] if q.dim() == 4 else 0,
+        if out.shape != shape or out.device != dev or out.dtype not in _DT or out.stride(-1) != 1:
+            raise ValueError(f"out must be a {tuple(shape)} float tensor on {dev} with a contiguous last dim")
+    elif out_dtype is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out_dtype not in _DT:
+        raise ValueError(f"out dtype {out_dtype} unsupported")
+    else:
+        out = torch.empty(shape, dtype=out_dtype, device=dev)
+    os_ = out.stride()
+    a = N.Fp4DecodeArgs(q.data_ptr(), _DT[q.dtype], strides[0], strides[1], strides[2] if dims == 4 else 0,
+                        out.data_ptr(), _DT[out.dtype], os_[0], os_[1], os_[2] if dims == 4 else 0,
                         B, Hq, Ht, M, pt, pt_sb, pt_sh, W, ln, sm_scale)
     if differential is not None:
         a.differential, a.lam, a.norm_weight, a.eps, a.out_scale = (1, *differential)
