@@ -553,7 +553,7 @@ int iak_prefill(const iak_page_pools* pools, const iak_prefill_args* args, void*
  * as 6, NaN as 0.  With e in [-14, 13] every value a pool can hold is zero or
  * a normal half (2^-15 .. 49152), so the kernels' half operands are exact.
  *
- * head_dim D is 64, 128 or 256; page_size a multiple of 16.  With NB = D / 32,
+ * head_dim D is 64, 128 or 256; page_size a multiple of 16 up to 16384.  With NB = D / 32,
  * 16 rows of K and V lie together in 544 * NB bytes (page p: the page_size / 16
  * such groups from byte p * page_size / 16 * 544 * NB on), ordered as the
  * attention kernel's lanes read them.  Lane 4 g + t (g 0..7, t 0..3) has NB

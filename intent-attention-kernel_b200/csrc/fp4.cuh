@@ -5,6 +5,7 @@
 
 namespace iak {
 
+constexpr int kFp4MaxPage = 16384;
 constexpr int kFp4ScaleMin = 127 - 14, kFp4ScaleMax = 127 + 13;   // scale bytes an append writes
 
 struct Fp4Pool {
@@ -48,14 +49,6 @@ struct Fp4Group {
   static constexpr int kV = 2 * kSet, kKs = 4 * kSet, kVs = kKs + 16 * NB;
   static constexpr int kBytes = 544 * NB;
   static __host__ __device__ constexpr int word(int lane, int w) { return ((w / kPW) * 32 + lane) * kPW + w % kPW; }
-  // K word of row r's channels 32 b + 8 t ..
-  static __device__ __forceinline__ int k_word(int r, int b, int t) {
-    return (r >> 3) * kSet + 4 * word((r & 7) * 4 + t, b);
-  }
-  // the byte of channel c (a multiple of 8, with the next 7) of rows r and r + 1, r even
-  static __device__ __forceinline__ int v_bytes(int r, int c) {
-    return kV + (r >> 3) * kSet + 4 * word(c / (4 * NB) * 4 + ((r & 7) >> 1), (c % (4 * NB)) >> 2);
-  }
   static __device__ __forceinline__ int k_scale(int r, int b) { return kKs + ((r & 7) * 2 + (r >> 3)) * NB + b; }
   static __device__ __forceinline__ int v_scale(int r, int b) {
     return kVs + (b * 4 + ((r & 7) >> 1)) * 4 + (r & 1) + 2 * (r >> 3);

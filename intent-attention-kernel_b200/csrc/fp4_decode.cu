@@ -1,7 +1,7 @@
 // Attention of a sequence's last tokens over an FP4 page pool (iak_fp4_decode), plain and differential.
 //
 // Mathematics.  A table head's queries form NC = G * M * (1 or 2) softmax columns (differential: two per query, the
-// first with q2 = 0 and the second with q1 = 0, so that both halves run as one product).  Per tile of 32 keys (16 for D 256)
+// first with q2 = 0 and the second with q1 = 0, so that both halves run as one product).  Per tile of 32 keys
 //   S' = K Q',  P = exp2(S - m),  O' += V' P'
 // with running maximum m and sum l per column, fp32.  Keys are the rows of the first product and the contraction of
 // the second, columns the narrow side (n = 8 per mma.m16n8k16), so that few queries waste little.
@@ -30,13 +30,15 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
+constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
 constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
 constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small P stay normal halves
 
 struct DecP {
   Fp4Pool pool;
-  int gpp;                           // groups of 16 rows per page
+  int gpp;                           // groups of 16 rows per page, at most 2^10
+  unsigned long long gpp_inv;        // 2^36 / gpp, rounded up
   const void* q; int q_dtype; int64_t q_sb, q_sh, q_sm;
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sm;
   int B, Hq, Ht, G, M;
@@ -52,7 +54,6 @@ struct DecP {
   int direct;                        // one block per unit, nothing to join
   int by_unit;                       // cuts are recorded per unit, not per border
   int min_tiles;                     // tiles a block takes at least
-  int tile_shift;                    // log2 of a tile's keys
   float* ws;
 };
 
@@ -61,44 +62,41 @@ __device__ __forceinline__ int seq_len(const DecP& p, int b) {
   return min(max(p.lengths[b], 0), p.W * p.pool.PS);
 }
 // tiles of one unit; an empty sequence has one, which writes its zeros
-__device__ __forceinline__ int seq_tiles(const DecP& p, int b) {
-  return max(1, (seq_len(p, b) + (1 << p.tile_shift) - 1) >> p.tile_shift);
+__device__ __forceinline__ int tiles_of(const DecP& p, int len) {
+  return max(1, (len + kTileKeys - 1) / kTileKeys);
 }
 
-// all tiles of the call (every lane of every warp has it); the host keeps their number within 31 bits
-__device__ __forceinline__ int total_tiles(const DecP& p) {
-  const int lane = threadIdx.x & 31;
-  int sum = 0;
-  for (int b = lane; b < p.B; b += 32) sum += seq_tiles(p, b);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  return sum * p.HC;
+// Table entry of group g: g / gpp, exact for g < 2^26 and gpp <= 2^10, where g times the inverse's excess stays below 2^36.
+__device__ __forceinline__ int slot_of(const DecP& p, int g) {
+  return static_cast<int>((static_cast<unsigned>(g) * p.gpp_inv) >> 36);
 }
 
-// sequence that holds tile t, and t's offset among that sequence's tiles
-__device__ __forceinline__ void find_sequence(const DecP& p, int t, int& b, int& off) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  b = p.B;
-  off = 0;
-  for (int base = 0; base < p.B; base += 32) {
-    const int i = base + lane;
-    const int n = i < p.B ? seq_tiles(p, i) * p.HC : 0;
-    int inc = n;
+// A warp's view of 32 sequences from `base` on: a lane's length, the tiles of its units, and those with all before it.
+struct Lane32 { int len, n, upto; };
+__device__ __forceinline__ Lane32 scan32(const DecP& p, int base) {
+  const int lane = threadIdx.x & 31, i = base + lane;
+  Lane32 s;
+  s.len = i < p.B ? seq_len(p, i) : 0;
+  s.n = i < p.B ? tiles_of(p, s.len) * p.HC : 0;
+  s.upto = s.n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(~0u, inc, o);
-      if (lane >= o) inc += v;
-    }
-    const unsigned hit = __ballot_sync(~0u, before + inc > t);
-    if (hit) {
-      const int l = __ffs(hit) - 1;
-      b = base + l;
-      off = t - (before + __shfl_sync(~0u, inc - n, l));
-      break;
-    }
-    before += __shfl_sync(~0u, inc, 31);
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(~0u, s.upto, o);
+    if (lane >= o) s.upto += v;
   }
+  return s;
+}
+// all tiles of the call (every lane of every warp has it); the host keeps their number within 31 bits
+__device__ __forceinline__ int total_tiles(const DecP& p, const Lane32& first) {
+  int sum = __shfl_sync(~0u, first.upto, 31);
+  if (p.B > 32) {
+    int rest = 0;
+    for (int b = 32 + (threadIdx.x & 31); b < p.B; b += 32) rest += tiles_of(p, seq_len(p, b));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(~0u, rest, o);
+    sum += rest * p.HC;
+  }
+  return sum;
 }
 
 // The tiles in equal runs: `used` blocks, the first `more` of them with each + 1 tiles.
@@ -191,27 +189,17 @@ __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
 }
 
 // ------------------------------------------------------------- shared layout
-struct Cursor { int left, off, at, b; };   // tiles left to the block; the next one, of sequence b and of all
+struct Cursor { int left, off, at, b, len; };   // tiles left to the block; the next one, of sequence b and of all
 struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, at; };   // at: its first tile, of all
 
 template <int NB>
 struct Lay {
   using Gr = Fp4Group<NB>;
   static constexpr int D = NB * 32;
-  // Groups of a warp's tile: two; one for D 256, whose ring then leaves room for a second block on the SM.
-  static constexpr int TG = NB == 8 ? 1 : 2;
-  static constexpr int kTile = 16 * TG;
   static constexpr int kStages = 3;
-  static constexpr int kStage = TG * Gr::kBytes;
+  static constexpr int kStage = 2 * Gr::kBytes;
   static constexpr int kRing = kWarps * kStages * kStage;
-  // A warp's sums for the join lie in one stage, D / JH channels at a time; in pass dh place i of a lane's NB / JH values
-  // is channel(dh, 32 i + lane).
-  static constexpr int JH = NB == 8 ? 2 : 1;
-  static constexpr int kRun = 4 * NB / JH;                 // a lane's channels that lie side by side
-  static constexpr int kOutStride = D / JH + 4;            // floats of one column in the join buffer
-  static __device__ __forceinline__ int channel(int dh, int pos) {
-    return JH == 1 ? pos : pos / kRun * (4 * NB) + dh * kRun + pos % kRun;
-  }
+  static constexpr int kOutStride = D + 4;                 // floats of one column in the join buffer
   static_assert(8 * kOutStride * 4 <= kStage, "a warp's sums for the join lie in one stage of its ring");
 };
 
@@ -222,14 +210,10 @@ constexpr int smem_bytes() {
          static_cast<int>(sizeof(Runs));
 }
 
-// x: one row's D values; lane i's value of place k is channel i + 32 k, or in the main kernel's order (SPREAD)
-template <int NB, bool SPREAD>
+// x: one row's D values, lane i holding channels i, i + 32, ..
+template <int NB>
 __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m, float (&x)[NB]) {
-  using L = Lay<NB>;
   const int lane = threadIdx.x & 31;
-  auto channel = [&](int k) {
-    return SPREAD ? L::channel(k / (NB / L::JH), k % (NB / L::JH) * 32 + lane) : k * 32 + lane;
-  };
   if (p.diff) {
     float mul = p.out_scale;
     if (p.norm_w) {
@@ -241,11 +225,11 @@ __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m
       mul *= rsqrtf(sq * (1.f / (NB * 32)) + p.eps);
     }
 #pragma unroll
-    for (int i = 0; i < NB; ++i) x[i] *= p.norm_w ? mul * p.norm_w[channel(i)] : mul;
+    for (int i = 0; i < NB; ++i) x[i] *= p.norm_w ? mul * p.norm_w[i * 32 + lane] : mul;
   }
   const int64_t at = b * p.o_sb + head * p.o_sh + m * p.o_sm;
 #pragma unroll
-  for (int i = 0; i < NB; ++i) store_from_float(p.out, p.out_dtype, at + channel(i), x[i]);
+  for (int i = 0; i < NB; ++i) store_from_float(p.out, p.out_dtype, at + i * 32 + lane, x[i]);
 }
 
 __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
@@ -254,7 +238,7 @@ __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f :
 // blocks of an SM: two where shared memory holds two rings and the accumulators leave the registers
 template <int NB, int NT, bool SPLIT>
 constexpr int blocks_per_sm() {
-  return NT <= 2 && NT * NB <= 8 && !(SPLIT && NT * NB > 4) ? 2 : 1;
+  return NB <= 4 && NT <= 2 && !(SPLIT && NT * NB > 4) ? 2 : 1;
 }
 
 template <int NB, int NT, bool SPLIT>
@@ -277,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   // Groups of 16 keys that go through the products together: two, for the independent work, except where the
   // accumulators then leave too few registers.  (32 sequences of 32k, D 128, 16 columns: 328 us with one and two blocks
   // an SM, 354 with two and one block; 32 columns: 152 with two, 168 with one, 8 sequences.)
-  constexpr int TG = L::TG, U = TG == 1 || (NT == 2 && NB >= 4) ? 1 : 2;
+  constexpr int U = NT == 2 && NB == 4 ? 1 : 2;
 
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -294,14 +278,29 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     Cursor cur = {};
     if (p.direct) {
       cur.b = blockIdx.x / p.HC;
-      cur.left = seq_tiles(p, cur.b);
+      cur.len = seq_len(p, cur.b);
+      cur.left = tiles_of(p, cur.len);
       cur.off = (blockIdx.x - cur.b * p.HC) * cur.left;
     } else {
-      const Runs r = make_runs(p, total_tiles(p));
+      Lane32 s = scan32(p, 0);
+      const Runs r = make_runs(p, total_tiles(p, s));
       if (blockIdx.x >= r.used) return;
       cur.at = run_begin(r, blockIdx.x);
       cur.left = run_begin(r, blockIdx.x + 1) - cur.at;
-      find_sequence(p, cur.at, cur.b, cur.off);
+      // the sequence that holds tile cur.at
+      int before = 0;
+      for (int base = 0; base < p.B; base += 32) {
+        if (base) s = scan32(p, base);
+        const unsigned hit = __ballot_sync(~0u, before + s.upto > cur.at);
+        if (hit) {
+          const int l = __ffs(hit) - 1;
+          cur.b = base + l;
+          cur.len = __shfl_sync(~0u, s.len, l);
+          cur.off = cur.at - before - __shfl_sync(~0u, s.upto - s.n, l);
+          break;
+        }
+        before += __shfl_sync(~0u, s.upto, 31);
+      }
       if (threadIdx.x == 0) runs = r;
     }
     if (lane == 0) cursor[warp] = cur;
@@ -313,13 +312,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     if (cur.left <= 0 || cur.b >= p.B) return false;
     Segment sg;
     sg.b = cur.b;
-    sg.len = seq_len(p, cur.b);
-    sg.n_tiles = seq_tiles(p, cur.b);
+    sg.len = cur.len;
+    sg.n_tiles = tiles_of(p, cur.len);
     sg.at = cur.at;
     const int unit = cur.off / sg.n_tiles;                        // of the sequence: table head, column group
     sg.c_begin = cur.off - unit * sg.n_tiles;
     sg.c_end = min(sg.n_tiles, sg.c_begin + cur.left);
-    sg.h = unit / p.CG;
+    sg.h = p.CG == 1 ? unit : unit / p.CG;
     sg.cg = unit - sg.h * p.CG;
     const int n = sg.c_end - sg.c_begin;
     cur.left -= n;
@@ -328,6 +327,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     if (cur.off == sg.n_tiles * p.HC) {
       cur.off = 0;
       ++cur.b;
+      cur.len = cur.left > 0 && cur.b < p.B ? seq_len(p, cur.b) : 0;
     }
     __syncwarp();
     if (lane == 0) {
@@ -341,88 +341,102 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     n_mine = sg.c_end > first && p.pool.num_pages > 0 ? (sg.c_end - first + kWarps - 1) / kWarps : 0;
     return true;
   };
+  // A thread's 8 channels `ch` of column `col` of the segment's queries: where they lie, or null (a column behind the
+  // last, or the half of a differential column that is 0).
+  constexpr int CH = D / 8, Q_BYTES = SPLIT ? 4 : 2;
+  auto query_at = [&](const Segment& sg, int col, int ch) -> const char* {
+    const int j = sg.cg * COLS + col, row = p.diff ? j >> 1 : j;
+    if (j >= p.NC || (p.diff && (ch * 2 >= CH) != (j & 1))) return nullptr;
+    const int gi = p.M == 1 ? row : row / p.M, m = row - gi * p.M;
+    return static_cast<const char*>(p.q) +
+           (sg.b * p.q_sb + (sg.h * p.G + gi) * p.q_sh + m * p.q_sm + ch * 8) * Q_BYTES;
+  };
+  // bring them near, so that the reads below find them there while the page ids are on their way
+  auto touch_queries = [&]() {
+    const Segment& sg = segment[2 * warp];
+    for (int i = threadIdx.x; i < COLS * CH; i += kThreads) {
+      const char* at = query_at(sg, i / CH, i % CH);
+      unsigned short unused;
+      if (at) asm volatile("ld.global.u16 %0, [%1];" : "=h"(unused) : "l"(at));
+    }
+  };
+  // halves after a power of two that puts the row's largest in [1, 2)
   auto stage_queries = [&]() {
     const Segment& sg = segment[2 * warp];
-      // queries: 8 channels per thread, halves after a power of two that puts the row's largest in [1, 2)
-      constexpr int CH = D / 8;
-      for (int i = threadIdx.x; i < COLS * CH; i += kThreads) {
-        const int col = i / CH, ch = i - col * CH;
-        const int j = sg.cg * COLS + col;
-        const int row = p.diff ? j >> 1 : j;
-        float x[8] = {};
-        const bool mine = j < p.NC && (!p.diff || (ch * 2 >= CH) == (j & 1));
-        if (mine) {
-          const int gi = row / p.M, m = row - gi * p.M;
-          const int64_t at = sg.b * p.q_sb + (sg.h * p.G + gi) * p.q_sh + m * p.q_sm + ch * 8;
+    for (int i = threadIdx.x; i < COLS * CH; i += kThreads) {
+      const int col = i / CH, ch = i % CH, j = sg.cg * COLS + col;
+      float x[8] = {};
+      const char* at = query_at(sg, col, ch);
+      if (at) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 8; ++e) {
           if (SPLIT) {
-            x[e] = static_cast<const float*>(p.q)[at + e] * p.sign;
+            x[e] = reinterpret_cast<const float*>(at)[e] * p.sign;
           } else {
-            const uint16_t u = static_cast<const uint16_t*>(p.q)[at + e];
+            const uint16_t u = reinterpret_cast<const uint16_t*>(at)[e];
             x[e] = (p.q_dtype == IAK_DT_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float(u << 16)) * p.sign;
           }
         }
-        }
-        float amax = 0.f;
+      }
+      float amax = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
 #pragma unroll
-        for (int o = 1; o < CH; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-        // exponent of amax, held to normal numbers on both sides
-        const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
-        const float down = __uint_as_float((254 - ex) << 23);
-        unsigned hi[4], lo[4];
+      for (int o = 1; o < CH; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
+      // exponent of amax, held to normal numbers on both sides
+      const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
+      const float down = __uint_as_float((254 - ex) << 23);
+      unsigned hi[4], lo[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float y0 = x[2 * e] * down, y1 = x[2 * e + 1] * down;
-          hi[e] = pack_half2(y0, y1);
-          if (SPLIT) {
-            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-            lo[e] = pack_half2(y0 - back.x, y1 - back.y);
-          }
-        }
-        uint4* dst = reinterpret_cast<uint4*>(q_frag) + ((col >> 3) * NB + (ch >> 2)) * 32 + (col & 7) * 4 + (ch & 3);
-        *dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        if (SPLIT) dst[NT * NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        if (ch == 0) {
-          col_scale[col] = fmaxf(p.scale * __uint_as_float(ex << 23), 1e-37f);
-          col_limit[col] = j < p.NC ? sg.len - (p.M - 1 - row % p.M) : sg.len;
+      for (int e = 0; e < 4; ++e) {
+        const float y0 = x[2 * e] * down, y1 = x[2 * e + 1] * down;
+        hi[e] = pack_half2(y0, y1);
+        if (SPLIT) {
+          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+          lo[e] = pack_half2(y0 - back.x, y1 - back.y);
         }
       }
+      uint4* dst = reinterpret_cast<uint4*>(q_frag) + ((col >> 3) * NB + (ch >> 2)) * 32 + (col & 7) * 4 + (ch & 3);
+      *dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      if (SPLIT) dst[NT * NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (ch == 0) {
+        col_scale[col] = fmaxf(p.scale * __uint_as_float(ex << 23), 1e-37f);
+        col_limit[col] = j < p.NC ? sg.len - (p.M - 1 - (p.diff ? j >> 1 : j) % p.M) : sg.len;
+      }
+    }
   };
-
   // ---------------------------------------------------------------- copies
-  // The warp's tiles are c_begin + warp + kWarps k.  Of every 32 / TG of them lane TG i + u looks up group u of tile i:
-  // it reads the page id a batch ahead and holds the group's number in the pool (0 for a page that does not exist: its
+  // The warp's tiles are c_begin + warp + kWarps k.  Of every 16 of them lane 2 i + u looks up group u of tile i: it
+  // reads the page id a batch ahead and holds the group's number in the pool (0 for a page that does not exist: its
   // rows are masked).
   int next_id = -1, src_group = 0;
-  unsigned history = 0;                           // TG bits per tile issued, the last lowest: its groups' pages exist
-  constexpr int kBatch = 32 / TG;
+  unsigned history = 0;                           // two bits per tile issued, the last in bits 0, 1: its groups' pages exist
+  constexpr int kBatch = 16;
   unsigned batch_ok = 0;
   const uint8_t* const lane_data = p.pool.data + lane * 16;
-  auto group_of = [&](int k) { return (segment[2 * warp].c_begin + warp + kWarps * (k + lane / TG)) * TG + lane % TG; };
+  auto group_of = [&](int k) { return (segment[2 * warp].c_begin + warp + kWarps * (k + (lane >> 1))) * 2 + (lane & 1); };
   auto load_id = [&](int k) {
     const Segment& sg = segment[2 * warp];
     const int gr = group_of(k);
-    return k + lane / TG < n_mine && gr * 16 < sg.len
-               ? __ldg(p.pt + sg.b * p.pt_sb + sg.h * p.pt_sh + static_cast<unsigned>(gr) / p.gpp) : -1;
+    return k + (lane >> 1) < n_mine && gr * 16 < sg.len
+               ? __ldg(p.pt + sg.b * p.pt_sb + sg.h * p.pt_sh + slot_of(p, gr)) : -1;
   };
   auto issue = [&](int k, int to_stage) {
-    history <<= TG;
+    history <<= 2;
     if (k < n_mine) {
       const int i = k % kBatch;
       if (i == 0) {
         const bool ok = next_id >= 0 && next_id < p.pool.num_pages;
-        src_group = ok ? next_id * p.gpp + static_cast<int>(static_cast<unsigned>(group_of(k)) % p.gpp) : 0;
+        const int gr = group_of(k);
+        src_group = ok ? next_id * p.gpp + gr - slot_of(p, gr) * p.gpp : 0;
         batch_ok = __ballot_sync(~0u, ok);
         next_id = load_id(k + kBatch);
       }
-      history |= (batch_ok >> (TG * i)) & ((1 << TG) - 1);
+      history |= (batch_ok >> (2 * i)) & 3;
       const unsigned to = ring + to_stage * L::kStage + lane * 16;
 #pragma unroll
-      for (int u = 0; u < TG; ++u) {
-        const uint8_t* from = lane_data + static_cast<int64_t>(__shfl_sync(~0u, src_group, TG * i + u)) * Gr::kBytes;
+      for (int u = 0; u < 2; ++u) {
+        const uint8_t* from = lane_data + static_cast<int64_t>(__shfl_sync(~0u, src_group, 2 * i + u)) * Gr::kBytes;
 #pragma unroll
         for (int c = 0; c < Gr::kBytes / 512; ++c) copy16(to + u * Gr::kBytes + c * 512, from + c * 512);
         constexpr int rest = Gr::kBytes % 512 / 16;               // lanes of the last copy
@@ -459,7 +473,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   while (true) {
     __syncwarp();
     const bool more = open_segment();
-    if (more) start_copies();
+    if (more) {
+      touch_queries();
+      start_copies();
+    }
 
     if (pending) {
       // ------------------------------------------------------ join the 8 warps
@@ -514,51 +531,46 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
         const bool has_row = warp * per < 8 && cg * COLS + nt * 8 + warp * per < p.NC;
         const int row = (cg * COLS + nt * 8) / per + warp;
         float x[NB];
+        float* dst = reinterpret_cast<float*>(smem + my_join) + 2 * t * L::kOutStride + g * (4 * NB);
 #pragma unroll
-        for (int dh = 0; dh < L::JH; ++dh) {
-          float* dst = reinterpret_cast<float*>(smem + my_join) + 2 * t * L::kOutStride + g * L::kRun;
+        for (int i = 0; i < MT; ++i) {
+            *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[nt][i][0] * f[0], o[nt][i][2] * f[0]);
+          *reinterpret_cast<float2*>(dst + L::kOutStride + 2 * i) = make_float2(o[nt][i][1] * f[1], o[nt][i][3] * f[1]);
+        }
+        __syncthreads();
+        if (has_row) {
+          for (int half = 0; half < per; ++half) {
+            const int lc = warp * per + half, col = nt * 8 + lc;
+            float top = -FLT_MAX, l = 0.f;
 #pragma unroll
-          for (int k = 0; k < MT / L::JH; ++k) {
-            const int i = dh * (MT / L::JH) + k;
-            *reinterpret_cast<float2*>(dst + 2 * k) = make_float2(o[nt][i][0] * f[0], o[nt][i][2] * f[0]);
-            *reinterpret_cast<float2*>(dst + L::kOutStride + 2 * k) = make_float2(o[nt][i][1] * f[1], o[nt][i][3] * f[1]);
-          }
-          __syncthreads();
-          if (has_row) {
-            for (int half = 0; half < per; ++half) {
-              const int lc = warp * per + half, col = nt * 8 + lc;
-              float top = -FLT_MAX, l = 0.f;
+            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + col]);
 #pragma unroll
-              for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + col]);
+            for (int w = 0; w < kWarps; ++w) l += warp_l[w * COLS + col] * tc::ex2(warp_m[w * COLS + col] - top);
+            float acc[NB];
 #pragma unroll
-              for (int w = 0; w < kWarps; ++w) l += warp_l[w * COLS + col] * tc::ex2(warp_m[w * COLS + col] - top);
-              float acc[NB / L::JH];
+            for (int i = 0; i < NB; ++i) {
+              acc[i] = 0.f;
 #pragma unroll
-              for (int i = 0; i < NB / L::JH; ++i) {
-                acc[i] = 0.f;
+              for (int w = 0; w < kWarps; ++w)
+                acc[i] += reinterpret_cast<const float*>(smem + join_at[w])[lc * L::kOutStride + i * 32 + lane];
+            }
+            if (!whole) {
+              float* part = p.ws + ((static_cast<int64_t>(blockIdx.x) * 2 + which) * COLS + col) * (D + 2);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w)
-                  acc[i] += reinterpret_cast<const float*>(smem + join_at[w])[lc * L::kOutStride + i * 32 + lane];
-              }
-              if (!whole) {
-                float* part = p.ws + ((static_cast<int64_t>(blockIdx.x) * 2 + which) * COLS + col) * (D + 2);
+              for (int i = 0; i < NB; ++i) part[i * 32 + lane] = acc[i];
+              if (lane == 0) { part[D] = top; part[D + 1] = l; }
+            } else {
+              const float inv = safe_inverse(l);
+              const float weight = half ? -p.lam[h * p.G + row / p.M] * inv : inv;
 #pragma unroll
-                for (int i = 0; i < NB / L::JH; ++i) part[L::channel(dh, i * 32 + lane)] = acc[i];
-                if (lane == 0 && dh == 0) { part[D] = top; part[D + 1] = l; }
-              } else {
-                const float inv = safe_inverse(l);
-                const float weight = half ? -p.lam[h * p.G + row / p.M] * inv : inv;
-#pragma unroll
-                for (int i = 0; i < NB / L::JH; ++i) {
-                  float& xi = x[dh * (NB / L::JH) + i];
-                  xi = half ? fmaf(acc[i], weight, xi) : acc[i] * weight;
-                }
+              for (int i = 0; i < NB; ++i) {
+                x[i] = half ? fmaf(acc[i], weight, x[i]) : acc[i] * weight;
               }
             }
           }
-          __syncthreads();
         }
-        if (has_row && whole) finish_row<NB, true>(p, done_sg.b, h * p.G + row / p.M, row % p.M, x);
+        __syncthreads();
+        if (has_row && whole) finish_row<NB>(p, done_sg.b, h * p.G + row / p.M, row % p.M, x);
       }
       begins_run = false;
     }
@@ -576,8 +588,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
     }
     const int full_end = segment[2 * warp].len - (p.M - 1);   // every query sees the tokens before it
-    int key0 = (segment[2 * warp].c_begin + warp) * L::kTile;
-    for (int k = 0; k < n_mine; ++k, key0 += kWarps * L::kTile) {
+    int key0 = (segment[2 * warp].c_begin + warp) * kTileKeys;
+    for (int k = 0; k < n_mine; ++k, key0 += kWarps * kTileKeys) {
       // the stage read in the last round is free: every lane is past its reads
       warp_sync();
       issue(k + L::kStages - 1, stage == 0 ? L::kStages - 1 : stage - 1);
@@ -585,11 +597,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
       warp_sync();
       const unsigned at = ring + stage * L::kStage;
       stage = stage + 1 == L::kStages ? 0 : stage + 1;
-      const unsigned ok_here = (history >> (TG * (L::kStages - 1))) & ((1 << TG) - 1);
-      const bool full = ok_here == (1 << TG) - 1 && key0 + L::kTile <= full_end;
+      const unsigned ok_here = (history >> (2 * (L::kStages - 1))) & 3;
+      const bool full = ok_here == 3 && key0 + kTileKeys <= full_end;
 
 #pragma unroll 1
-      for (int v = 0; v < TG; v += U) {
+      for (int v = 0; v < 2; v += U) {
         // ---------------------------------------------------------- S' = K Q'
         float s[U][NT][4];
         {
@@ -773,7 +785,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p)
   const int rows = join_rows(p.NC, COLS, p.diff);
   const int record = blockIdx.x / rows + (p.by_unit ? 0 : 1), r = blockIdx.x % rows;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int used = p.by_unit ? 0 : make_runs(p, total_tiles(p)).used;
+  const int used = p.by_unit ? 0 : make_runs(p, total_tiles(p, scan32(p, 0))).used;
   // every block waits, so that this kernel never ends before the main one
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!p.by_unit && record >= used) return;
@@ -839,7 +851,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p)
       const float scale = half ? -p.lam[d.h * p.G + row / p.M] * inv : inv;
 #pragma unroll
       for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], scale, x[i]) : acc[i] * scale;
-      if (half == per - 1) finish_row<NB, false>(p, d.b, d.h * p.G + row / p.M, row % p.M, x);
+      if (half == per - 1) finish_row<NB>(p, d.b, d.h * p.G + row / p.M, row % p.M, x);
     }
     __syncthreads();
   }
@@ -879,12 +891,11 @@ int make_plan(DecP& p, Plan* plan) {
   if (units * 8 * NT > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: too many rows for one launch");
   p.HC = static_cast<int>(hc);
   p.min_tiles = kWarps;
-  p.tile_shift = Lay<NB>::kTile == 32 ? 5 : 4;
-  const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + Lay<NB>::kTile - 1) / Lay<NB>::kTile;
+  const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + kTileKeys - 1) / kTileKeys;
   // a unit that one tile per warp covers is one block's work: no joining
   plan->direct = most <= kWarps;
   if (most * units > 0x7fffffffLL - 64)
-    return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: tables of more than 2^31 tiles of %d tokens", Lay<NB>::kTile);
+    return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: tables of more than 2^31 tiles of %d tokens", kTileKeys);
   int blocks = 0;
   if (int st = resident_blocks<NB, NT, SPLIT>(&blocks)) return st;
   if (plan->direct) {
@@ -970,6 +981,7 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
   DecP p = {};
   p.pool = {static_cast<uint8_t*>(pool->data), pool->num_pages, pool->page_size, pool->head_dim};
   p.gpp = pool->page_size / 16;
+  p.gpp_inv = ((1ull << 36) + p.gpp - 1) / p.gpp;
   if (pool->num_pages * p.gpp > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "%s: more than 2^31 groups of rows", what);
   p.q = a->q; p.q_dtype = a->q_dtype; p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h; p.q_sm = a->q_stride_m;
   p.out = a->out; p.out_dtype = a->out_dtype;

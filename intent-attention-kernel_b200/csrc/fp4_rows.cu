@@ -1,11 +1,10 @@
 // FP4 page pool: quantise-on-write of new rows (iak_fp4_append) and reading rows back (iak_fp4_read).
 //
 // Both are copies: per row and channel they move 2 * (element size + 17/32) bytes, which bounds them for long
-// prompts; a decode step's few rows are bound by the launch.  One thread owns 8 channels of the two rows 2i and
-// 2i + 1, which share their bytes of V: it moves 16 bytes of each of the four dense rows, independent of one another.
-// A warp has 4 such row pairs by 64 channels, so that it covers 128-byte runs of the dense rows (16-bit types) and
-// 64-byte runs of the group.  A block's largest magnitude spans 4 neighbouring lanes.  A V byte whose other row is not
-// part of the call keeps that row's half.
+// prompts; a decode step's few rows are bound by the launch.  A warp owns 8 aligned rows of K and V, its lanes what the
+// attention kernel's lanes read of them: lane 4 g + t has row g's channels 32 b + 8 t .. + 7 of K (all blocks b) and
+// channels 4 NB g .. of rows 2 t and 2 t + 1 of V.  Codes move as one run of 512 bytes (D 128) per plane, dense rows as
+// 64-byte runs and more.  A V byte whose other row is not part of the call keeps that row's half.
 #include "fp4.cuh"
 
 namespace iak {
@@ -76,36 +75,31 @@ __device__ __forceinline__ void store8(void* base, int dtype, int64_t at, const 
   __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at), make_uint4(u[0], u[1], u[2], u[3]));
 }
 
-// where a thread works: its (b, h), row pair and 8 channels; tokens are 64-bit
+// Where a warp works: 8 rows of one (b, h), tokens 8 k .. 8 k + 7.  Row j is row i0 + j of the call's.
 struct Place {
-  int b, h, l;            // l: which 8 channels
-  int64_t i0;             // the pair's first row among the call's (negative when it starts before them)
-  bool in0, in1;          // rows that the call covers (index in [0, N))
-  bool real0, real1;      // rows below counts[b]
+  int b, h;
+  int64_t i0;             // negative where the rows begin before the call's
+  int n;                  // rows of the call that are real: counts[b], at most N
   uint8_t* group;         // the 16 rows' bytes, or null: no such page
-  int row;                // of the group, even
+  int hi;                 // which 8 of them
+  __device__ __forceinline__ bool in(const RowsParams& p, int j) const { return i0 + j >= 0 && i0 + j < p.N; }
+  __device__ __forceinline__ bool real(int j) const { return i0 + j >= 0 && i0 + j < n; }
 };
 
 template <int NB>
 __device__ __forceinline__ bool find_place(const RowsParams& p, Place& w) {
-  constexpr int LP = NB * 16;                // threads of 8 rows: 4 row pairs, D / 8 channel runs
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * (kRowThreads / LP) + threadIdx.x / LP;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * (kRowThreads / 32) + (threadIdx.x >> 5);
   const int64_t bh = at / p.octets;
-  if (bh >= static_cast<int64_t>(p.B) * p.Ht) return false;   // whole groups of LP threads leave together
-  w.l = (threadIdx.x % LP / 32) * 8 + (threadIdx.x & 7);
+  if (bh >= static_cast<int64_t>(p.B) * p.Ht) return false;
   w.b = static_cast<int>(bh / p.Ht);
   w.h = static_cast<int>(bh - static_cast<int64_t>(w.b) * p.Ht);
   const int64_t pos = p.positions ? p.positions[w.b] : 0;
-  const int n = p.counts ? min(max(p.counts[w.b], 0), p.N) : p.N;
-  const int64_t tok0 = (pos & ~int64_t(7)) + 8 * (at - bh * p.octets) + 2 * ((threadIdx.x >> 3) & 3);
+  w.n = p.counts ? min(max(p.counts[w.b], 0), p.N) : p.N;
+  const int64_t tok0 = (pos & ~int64_t(7)) + 8 * (at - bh * p.octets);
   w.i0 = tok0 - pos;
-  w.in0 = w.i0 >= 0 && w.i0 < p.N;
-  w.in1 = w.i0 + 1 >= 0 && w.i0 + 1 < p.N;
-  w.real0 = w.in0 && w.i0 < n;
-  w.real1 = w.in1 && w.i0 + 1 < n;
+  w.hi = static_cast<int>(tok0 >> 3) & 1;    // page sizes are multiples of 16: so are pages' first tokens
   w.group = nullptr;
-  w.row = static_cast<int>(tok0 & 15);       // page sizes are multiples of 16: so are pages' first tokens
-  if (tok0 >= 0 && (w.real0 || w.real1)) {
+  if (tok0 >= 0 && w.i0 < w.n) {
     const int64_t slot = tok0 / p.pool.PS;
     if (slot < p.W) {
       const int id = p.pt[w.b * p.pt_sb + w.h * p.pt_sh + slot];
@@ -113,151 +107,219 @@ __device__ __forceinline__ bool find_place(const RowsParams& p, Place& w) {
         w.group = p.pool.data + ((static_cast<int64_t>(id) * p.pool.PS + (tok0 - slot * p.pool.PS)) >> 4) * Fp4Group<NB>::kBytes;
     }
   }
-  return w.in0 || w.in1;                     // the 4 lanes of a block agree
+  return w.i0 < p.N;
 }
 
-// 8 values of a block of 4 lanes -> their codes (value i in bits 4i) and the block's scale byte
-__device__ __forceinline__ unsigned quantize8(float (&x)[8], int& byte) {
+__device__ __forceinline__ float largest8(float (&x)[8]) {
   float amax = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     x[i] = x[i] != x[i] ? 0.f : x[i];
     amax = fmaxf(amax, fabsf(x[i]));
   }
-  const unsigned group = 0xfu << (threadIdx.x & 28);      // the block's lanes: all of them are here
-  amax = fmaxf(amax, __shfl_xor_sync(group, amax, 1));
-  amax = fmaxf(amax, __shfl_xor_sync(group, amax, 2));
-  byte = fp4_scale_byte(amax);
-  const float inv = fp4_inv_scale(byte);                  // a power of two: the product is exact
-  unsigned w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w |= fp4_pack2(x[2 * i] * inv, x[2 * i + 1] * inv) << (8 * i);
-  return w;
+  return amax;
 }
 
-// bits 4i of a and b interleaved: byte i = a's code i (low half), b's code i (high half), i = 0..3
-__device__ __forceinline__ unsigned zip_codes(unsigned a, unsigned b) {
-  unsigned r = 0;
+template <int NB>
+__device__ __forceinline__ void put_words(uint8_t* set, int lane, const unsigned (&w)[NB]) {
+  using Gr = Fp4Group<NB>;
+  if constexpr (NB == 2) {
+    *reinterpret_cast<uint2*>(set + 4 * Gr::word(lane, 0)) = make_uint2(w[0], w[1]);
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r |= (((a >> (4 * i)) & 15u) | (((b >> (4 * i)) & 15u) << 4)) << (8 * i);
-  return r;
+    for (int i = 0; i < NB; i += 4)
+      *reinterpret_cast<uint4*>(set + 4 * Gr::word(lane, i)) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  }
+}
+template <int NB>
+__device__ __forceinline__ void get_words(const uint8_t* set, int lane, unsigned (&w)[NB]) {
+  using Gr = Fp4Group<NB>;
+  if constexpr (NB == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(set + 4 * Gr::word(lane, 0));
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < NB; i += 4) {
+      const uint4 v = *reinterpret_cast<const uint4*>(set + 4 * Gr::word(lane, i));
+      w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+    }
+  }
 }
 
 template <int NB, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) fp4_append_kernel(const RowsParams p) {
+  using Gr = Fp4Group<NB>;
   Place w;
   if (!find_place<NB>(p, w)) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if (!w.group) {
-    if (p.dropped && w.l == 0) {
-      const int n = (w.real0 ? 1 : 0) + (w.real1 ? 1 : 0);
-      if (n) atomicAdd(p.dropped, n);
+    if (p.dropped) {
+      const int n = __popc(__ballot_sync(~0u, lane < 8 && w.real(lane)));
+      if (lane == 0 && n) atomicAdd(p.dropped, n);
     }
     return;
   }
-  const int blk = w.l >> 2, t = w.l & 3;      // the thread's block and its word of the block
-  float k0[8] = {}, k1[8] = {}, v0[8] = {}, v1[8] = {};
-  const int64_t kat = w.b * p.k_sb + w.h * p.k_sh + w.i0 * p.k_sn + w.l * 8;
-  const int64_t vat = w.b * p.v_sb + w.h * p.v_sh + w.i0 * p.v_sn + w.l * 8;
-  if (w.real0) {
-    load8<VEC>(p.k, p.dtype, kat, k0);
-    load8<VEC>(p.v, p.dtype, vat, v0);
+  constexpr int VC = NB / 2;                  // runs of 8 channels that a lane has of a V row
+  const bool k_real = w.real(g), v_real0 = w.real(2 * t), v_real1 = w.real(2 * t + 1);
+  float kx[NB][8], vx[2][VC][8];
+  const int64_t kat = w.b * p.k_sb + w.h * p.k_sh + (w.i0 + g) * p.k_sn + t * 8;
+  const int64_t vat = w.b * p.v_sb + w.h * p.v_sh + (w.i0 + 2 * t) * p.v_sn + g * (4 * NB);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) kx[b][i] = 0.f;
+    if (k_real) load8<VEC>(p.k, p.dtype, kat + 32 * b, kx[b]);
   }
-  if (w.real1) {
-    load8<VEC>(p.k, p.dtype, kat + p.k_sn, k1);
-    load8<VEC>(p.v, p.dtype, vat + p.v_sn, v1);
+#pragma unroll
+  for (int c = 0; c < VC; ++c) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) vx[0][c][i] = vx[1][c][i] = 0.f;
+    if (v_real0) load8<VEC>(p.v, p.dtype, vat + 8 * c, vx[0][c]);
+    if (v_real1) load8<VEC>(p.v, p.dtype, vat + p.v_sn + 8 * c, vx[1][c]);
   }
-  int kb0, kb1, vb0, vb1;
-  const unsigned kw0 = quantize8(k0, kb0), kw1 = quantize8(k1, kb1);
-  const unsigned vw0 = quantize8(v0, vb0), vw1 = quantize8(v1, vb1);
-  using Gr = Fp4Group<NB>;
-  if (w.real0) *reinterpret_cast<uint32_t*>(w.group + Gr::k_word(w.row, blk, t)) = kw0;
-  if (w.real1) *reinterpret_cast<uint32_t*>(w.group + Gr::k_word(w.row + 1, blk, t)) = kw1;
-  uint2* vrow = reinterpret_cast<uint2*>(w.group + Gr::v_bytes(w.row, w.l * 8));
-  uint2 vz = make_uint2(zip_codes(vw0, vw1), zip_codes(vw0 >> 16, vw1 >> 16));
-  if (!(w.real0 && w.real1)) {                // the other row's half stays as it is
-    const uint2 old = *vrow;
-    const unsigned mine = w.real0 ? 0x0f0f0f0fu : 0xf0f0f0f0u;
-    vz.x = (vz.x & mine) | (old.x & ~mine);
-    vz.y = (vz.y & mine) | (old.y & ~mine);
+  // K: a block's largest magnitude spans the row's 4 lanes
+  unsigned word[NB];
+  uint8_t scale[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    float amax = largest8(kx[b]);
+    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+    scale[b] = static_cast<uint8_t>(fp4_scale_byte(amax));
+    const float inv = fp4_inv_scale(scale[b]);            // a power of two: the product is exact
+    word[b] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) word[b] |= fp4_pack2(kx[b][2 * i] * inv, kx[b][2 * i + 1] * inv) << (8 * i);
   }
-  *vrow = vz;
-  if (t == 0) {
-    if (w.real0) {
-      w.group[Gr::k_scale(w.row, blk)] = static_cast<uint8_t>(kb0);
-      w.group[Gr::v_scale(w.row, blk)] = static_cast<uint8_t>(vb0);
+  if (k_real) {
+    put_words<NB>(w.group + w.hi * Gr::kSet, lane, word);
+    if (t == 0) {
+      uint8_t* to = w.group + Gr::k_scale(8 * w.hi + g, 0);
+#pragma unroll
+      for (int b = 0; b < NB; b += 2)
+        *reinterpret_cast<uint16_t*>(to + b) = static_cast<uint16_t>(scale[b] | scale[b + 1] << 8);
     }
-    if (w.real1) {
-      w.group[Gr::k_scale(w.row + 1, blk)] = static_cast<uint8_t>(kb1);
-      w.group[Gr::v_scale(w.row + 1, blk)] = static_cast<uint8_t>(vb1);
+  }
+  // V: a block spans 8 / NB neighbouring g
+  int byte[2];
+  float inv[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float amax = 0.f;
+#pragma unroll
+    for (int c = 0; c < VC; ++c) amax = fmaxf(amax, largest8(vx[r][c]));
+    if (NB <= 4) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 4));
+    if (NB <= 2) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 8));
+    byte[r] = fp4_scale_byte(amax);
+    inv[r] = fp4_inv_scale(byte[r]);
+  }
+  if (!v_real0 && !v_real1) return;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {              // byte of a channel: both rows' codes
+    word[j] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = 4 * j + i;
+      word[j] |= fp4_pack2(vx[0][c / 8][c % 8] * inv[0], vx[1][c / 8][c % 8] * inv[1]) << (8 * i);
     }
+  }
+  uint8_t* set = w.group + Gr::kV + w.hi * Gr::kSet;
+  if (!(v_real0 && v_real1)) {                // the other row's half stays as it is
+    unsigned old[NB];
+    get_words<NB>(set, lane, old);
+    const unsigned mine = v_real0 ? 0x0f0f0f0fu : 0xf0f0f0f0u;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) word[j] = (word[j] & mine) | (old[j] & ~mine);
+  }
+  put_words<NB>(set, lane, word);
+  if (g % (8 / NB) == 0) {
+    uint8_t* to = w.group + Gr::v_scale(8 * w.hi + 2 * t, g * NB / 8);
+    if (v_real0) to[0] = static_cast<uint8_t>(byte[0]);
+    if (v_real1) to[1] = static_cast<uint8_t>(byte[1]);
   }
 }
 
-__device__ __forceinline__ void dequant_k(unsigned w, float s, float (&x)[8]) {
-  unsigned h[4];
-  fp4_unpack4(w, h);
+// scale byte (bytes) -> half 2^e in both halves (one in each): the pool's values are halves, so the products are exact
+__device__ __forceinline__ unsigned half_scales(unsigned lo, unsigned hi) {
+  return (lo | hi << 16) * 1024u - 112u * 1024u * 65537u;
+}
+__device__ __forceinline__ unsigned mul2(unsigned a, unsigned b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const unsigned*>(&r);
+}
+// 8 values held as half pairs
+template <bool VEC>
+__device__ __forceinline__ void store_halves(void* base, int dtype, int64_t at, const unsigned* h) {
+  if (VEC && dtype == IAK_DT_F16) {
+    __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at), make_uint4(h[0], h[1], h[2], h[3]));
+    return;
+  }
+  float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-    x[2 * i] = f.x * s;
-    x[2 * i + 1] = f.y * s;
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
   }
-}
-
-__device__ __forceinline__ void dequant_v(uint2 w, float s0, float s1, float (&x0)[8], float (&x1)[8]) {
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    unsigned h[4];
-    fp4_unpack4(j ? w.y : w.x, h);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-      x0[4 * j + i] = f.x * s0;
-      x1[4 * j + i] = f.y * s1;
-    }
-  }
+  store8<VEC>(base, dtype, at, x);
 }
 
 template <int NB, bool VEC>
 __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams p) {
+  using Gr = Fp4Group<NB>;
   Place w;
   if (!find_place<NB>(p, w)) return;
-  float k0[8] = {}, k1[8] = {}, v0[8] = {}, v1[8] = {};
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  unsigned kw[NB] = {}, vw[NB] = {}, ks[NB / 2] = {}, vs = 0;
   if (w.group) {
-    using Gr = Fp4Group<NB>;
-    const int blk = w.l >> 2, t = w.l & 3;
-    const unsigned kw0 = *reinterpret_cast<const uint32_t*>(w.group + Gr::k_word(w.row, blk, t));
-    const unsigned kw1 = *reinterpret_cast<const uint32_t*>(w.group + Gr::k_word(w.row + 1, blk, t));
-    const uint2 vz = *reinterpret_cast<const uint2*>(w.group + Gr::v_bytes(w.row, w.l * 8));
-    const uint16_t vs = *reinterpret_cast<const uint16_t*>(w.group + Gr::v_scale(w.row, blk));
-    dequant_k(kw0, fp4_scale(w.group[Gr::k_scale(w.row, blk)]), k0);
-    dequant_k(kw1, fp4_scale(w.group[Gr::k_scale(w.row + 1, blk)]), k1);
-    dequant_v(vz, fp4_scale(vs & 255), fp4_scale(vs >> 8), v0, v1);
-    // rows from counts[b] on are zeros, whatever the page holds behind the sequence
-    if (!w.real0) {
+    get_words<NB>(w.group + w.hi * Gr::kSet, lane, kw);
+    get_words<NB>(w.group + Gr::kV + w.hi * Gr::kSet, lane, vw);
+    const uint16_t* from = reinterpret_cast<const uint16_t*>(w.group + Gr::k_scale(8 * w.hi + g, 0));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k0[i] = v0[i] = 0.f;
-    }
-    if (!w.real1) {
+    for (int b = 0; b < NB / 2; ++b) ks[b] = from[b];
+    vs = *reinterpret_cast<const uint16_t*>(w.group + Gr::v_scale(8 * w.hi + 2 * t, g * NB / 8));
+  }
+  const int64_t kat = w.b * p.k_sb + w.h * p.k_sh + (w.i0 + g) * p.k_sn + t * 8;
+  const int64_t vat = w.b * p.v_sb + w.h * p.v_sh + (w.i0 + 2 * t) * p.v_sn + g * (4 * NB);
+  // rows from counts[b] on are zeros, whatever the page holds behind the sequence
+  const bool k_real = w.group && w.real(g);
+  if (w.in(p, g)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k1[i] = v1[i] = 0.f;
+    for (int b = 0; b < NB; ++b) {
+      unsigned h[4];
+      fp4_unpack4(kw[b], h);
+      const unsigned byte = b % 2 ? ks[b / 2] >> 8 : ks[b / 2] & 255, s = half_scales(byte, byte);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = k_real ? mul2(h[i], s) : 0;
+      store_halves<VEC>(p.k, p.dtype, kat + 32 * b, h);
     }
   }
-  const int64_t kat = w.b * p.k_sb + w.h * p.k_sh + w.i0 * p.k_sn + w.l * 8;
-  const int64_t vat = w.b * p.v_sb + w.h * p.v_sh + w.i0 * p.v_sn + w.l * 8;
-  if (w.in0) {
-    store8<VEC>(p.k, p.dtype, kat, k0);
-    store8<VEC>(p.v, p.dtype, vat, v0);
-  }
-  if (w.in1) {
-    store8<VEC>(p.k, p.dtype, kat + p.k_sn, k1);
-    store8<VEC>(p.v, p.dtype, vat + p.v_sn, v1);
+  const bool real0 = w.group && w.real(2 * t), real1 = w.group && w.real(2 * t + 1);
+  // (the byte of a row that was never written could borrow from the other half)
+  const unsigned s = half_scales(real0 ? vs & 255 : 112, real1 ? vs >> 8 : 112);
+#pragma unroll
+  for (int c = 0; c < NB / 2; ++c) {          // 8 channels of both rows
+    unsigned r0[4], r1[4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      unsigned h[4];
+      fp4_unpack4(vw[2 * c + j], h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) h[i] = mul2(h[i], s);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        r0[2 * j + i] = real0 ? __byte_perm(h[2 * i], h[2 * i + 1], 0x5410) : 0;
+        r1[2 * j + i] = real1 ? __byte_perm(h[2 * i], h[2 * i + 1], 0x7632) : 0;
+      }
+    }
+    if (w.in(p, 2 * t)) store_halves<VEC>(p.v, p.dtype, vat + 8 * c, r0);
+    if (w.in(p, 2 * t + 1)) store_halves<VEC>(p.v, p.dtype, vat + p.v_sn + 8 * c, r1);
   }
 }
 
 template <int NB>
 int launch_rows(const RowsParams& p, bool append, bool vec, cudaStream_t s) {
-  const int64_t per = kRowThreads / (NB * 16);
+  const int64_t per = kRowThreads / 32;
   const int64_t blocks = (static_cast<int64_t>(p.B) * p.Ht * p.octets + per - 1) / per;
   if (blocks > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4 rows: too many rows for one launch");
   const unsigned g = static_cast<unsigned>(blocks);
@@ -305,8 +367,8 @@ int rows_call(const iak_fp4_pool* pool, const iak_fp4_rows_args* a, bool append,
 int check_fp4_pool(const iak_fp4_pool* pool, const char* what) {
   if (pool->head_dim != 64 && pool->head_dim != 128 && pool->head_dim != 256)
     return fail(IAK_ERR_UNSUPPORTED, "%s: head_dim %d is not 64, 128 or 256", what, pool->head_dim);
-  if (pool->page_size <= 0 || pool->page_size % 16)
-    return fail(IAK_ERR_UNSUPPORTED, "%s: page_size %d is not a multiple of 16", what, pool->page_size);
+  if (pool->page_size <= 0 || pool->page_size % 16 || pool->page_size > kFp4MaxPage)
+    return fail(IAK_ERR_UNSUPPORTED, "%s: page_size %d is not a multiple of 16 up to %d", what, pool->page_size, kFp4MaxPage);
   if (pool->num_pages < 0 || pool->num_pages > 0x7fffffffLL)
     return fail(IAK_ERR_INVALID_ARG, "%s: num_pages out of range", what);
   if (!pool->data && pool->num_pages > 0) return fail(IAK_ERR_INVALID_ARG, "%s: null pool data", what);

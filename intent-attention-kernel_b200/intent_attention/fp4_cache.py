@@ -101,8 +101,8 @@ class Fp4Pool:
         """A pool of ``num_pages`` pages (``zero``: all rows 0; otherwise rows hold nothing until written)."""
         if head_dim not in HEAD_DIMS:
             raise ValueError(f"head_dim must be one of {HEAD_DIMS}, got {head_dim}")
-        if page_size <= 0 or page_size % 16:
-            raise ValueError(f"page_size must be a positive multiple of 16, got {page_size}")
+        if page_size <= 0 or page_size % 16 or page_size > 16384:
+            raise ValueError(f"page_size must be a positive multiple of 16 up to 16384, got {page_size}")
         if num_pages < 0:
             raise ValueError("num_pages must not be negative")
         mk = torch.zeros if zero else torch.empty
