@@ -15,21 +15,24 @@ struct Fp4Pool {
 };
 
 // Scale byte of a block with largest magnitude amax: the smallest e with 6 * 2^e >= amax.  amax = m * 2^k,
-// 1 <= m < 2, and 6 = 1.5 * 4, so e = k - 2 for m <= 1.5 and k - 1 above; subnormals end at the lower bound.
+// 1 <= m < 2, and 6 = 1.5 * 4, so e = k - 2 for m <= 1.5 and k - 1 above, where the addend carries into the exponent;
+// subnormals end at the lower bound, infinity at the upper.
 __device__ __forceinline__ int fp4_scale_byte(float amax) {
-  const unsigned u = __float_as_uint(amax);
-  const int k = static_cast<int>(u >> 23);              // biased; inf gives the upper bound
-  const int b = k - 2 + ((u & 0x7fffffu) > 0x400000u ? 1 : 0);
+  const int b = static_cast<int>((__float_as_uint(amax) + 0x3fffffu) >> 23) - 2;
   return min(max(b, kFp4ScaleMin), kFp4ScaleMax);
 }
 
 __device__ __forceinline__ float fp4_inv_scale(int byte) { return __uint_as_float((254 - byte) << 23); }
 __device__ __forceinline__ float fp4_scale(int byte) { return __uint_as_float(byte << 23); }
 
-// two E2M1 codes in a byte, `lo` in bits 0..3: nearest, ties to the even code, saturating at 6
-__device__ __forceinline__ unsigned fp4_pack2(float lo, float hi) {
-  unsigned short r;
-  asm("{\n.reg .b8 b;\ncvt.rn.satfinite.e2m1x2.f32 b, %1, %2;\nmov.b16 %0, {b, 0};\n}" : "=h"(r) : "f"(hi), "f"(lo));
+// eight E2M1 codes, x[i] in bits 4i..: nearest, ties to the even code, saturating at 6
+__device__ __forceinline__ unsigned fp4_pack8(const float (&x)[8]) {
+  unsigned r;
+  asm("{\n.reg .b8 b0, b1, b2, b3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\ncvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\ncvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n"
+      "mov.b32 %0, {b0, b1, b2, b3};\n}"
+      : "=r"(r) : "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]));
   return r;
 }
 

@@ -22,31 +22,74 @@ struct RowsParams {
 
 constexpr int kRowThreads = 256;
 
-template <bool VEC>
-__device__ __forceinline__ void load8(const void* base, int dtype, int64_t at, float (&x)[8]) {
-  if (!VEC) {
+// How dense rows are read: 16 bytes at a time by type, or an element at a time (any type, any alignment).
+enum { kAny = -1 };
+
+// Eight neighbouring channels of a row as they were read.
+template <int KIND>
+struct Eight {
+  static constexpr int kWords = KIND == IAK_DT_F16 || KIND == IAK_DT_BF16 ? 4 : 8;
+  unsigned w[kWords];
+  __device__ __forceinline__ void load(const void* base, int dtype, int64_t at, bool real) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = load_as_float(base, dtype, at + i);
-    return;
-  }
-  if (dtype == IAK_DT_F32) {
-    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + at);
-    const float4 a = __ldcs(p), b = __ldcs(p + 1);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    return;
-  }
-  const uint4 w = __ldcs(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
-  const unsigned u[4] = {w.x, w.y, w.z, w.w};
+    for (int i = 0; i < kWords; ++i) w[i] = 0;
+    if (!real) return;
+    if constexpr (KIND == kAny) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (dtype == IAK_DT_F16) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-      x[2 * i] = f.x; x[2 * i + 1] = f.y;
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(load_as_float(base, dtype, at + i));
+    } else if constexpr (KIND == IAK_DT_F32) {
+      const uint4* p = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + at);
+      const uint4 a = __ldg(p), b = __ldg(p + 1);
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w; w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
     } else {
-      x[2 * i] = __uint_as_float(u[i] << 16); x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at));
+      w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
     }
   }
-}
+  // the larger magnitude of a and b, of both halves for 16-bit types; the sign is of no use; NaN where there is one
+  static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) {
+    unsigned r;
+    if constexpr (KIND == IAK_DT_F16) asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else if constexpr (KIND == IAK_DT_BF16) asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ unsigned largest() const {
+    unsigned m = larger(w[0], w[1]);
+#pragma unroll
+    for (int i = 2; i < kWords; ++i) m = larger(m, w[i]);
+    return m;
+  }
+  // the magnitude that `largest` (or several of them, joined by `larger`) stands for
+  static __device__ __forceinline__ float magnitude(unsigned m) {
+    if constexpr (kWords == 8) return fabsf(__uint_as_float(m));
+    m = larger(m, m >> 16 | m << 16) & 0x7fffu;
+    if constexpr (KIND == IAK_DT_F16) return __half2float(__ushort_as_half(static_cast<unsigned short>(m)));
+    return __uint_as_float(m << 16);
+  }
+  __device__ __forceinline__ float value(int i) const {
+    if constexpr (kWords == 8) return __uint_as_float(w[i]);
+    const unsigned u = w[i / 2];
+    if constexpr (KIND == IAK_DT_F16) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&u);
+      return i % 2 ? __high2float(h) : __low2float(h);
+    }
+    return __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16);
+  }
+  // NaN -> 0
+  __device__ __forceinline__ void clean() {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if constexpr (kWords == 8) {
+        if ((w[i] & 0x7fffffffu) > 0x7f800000u) w[i] = 0;
+      } else {
+        const unsigned inf = KIND == IAK_DT_F16 ? 0x7c00u : 0x7f80u;
+        if ((w[i] & 0x7fffu) > inf) w[i] &= 0xffff0000u;
+        if ((w[i] >> 16 & 0x7fffu) > inf) w[i] &= 0xffffu;
+      }
+    }
+  }
+};
 
 template <bool VEC>
 __device__ __forceinline__ void store8(void* base, int dtype, int64_t at, const float (&x)[8]) {
@@ -80,8 +123,9 @@ struct Place {
   int b, h;
   int64_t i0;             // negative where the rows begin before the call's
   int n;                  // rows of the call that are real: counts[b], at most N
-  uint8_t* group;         // the 16 rows' bytes, or null: no such page
-  int hi;                 // which 8 of them
+  int id;                 // page, or -1: no such table entry
+  int64_t tok_in_page;
+  int hi;                 // which 8 of the group's 16 rows
   __device__ __forceinline__ bool in(const RowsParams& p, int j) const { return i0 + j >= 0 && i0 + j < p.N; }
   __device__ __forceinline__ bool real(int j) const { return i0 + j >= 0 && i0 + j < n; }
 };
@@ -98,26 +142,21 @@ __device__ __forceinline__ bool find_place(const RowsParams& p, Place& w) {
   const int64_t tok0 = (pos & ~int64_t(7)) + 8 * (at - bh * p.octets);
   w.i0 = tok0 - pos;
   w.hi = static_cast<int>(tok0 >> 3) & 1;    // page sizes are multiples of 16: so are pages' first tokens
-  w.group = nullptr;
+  w.id = -1;
+  w.tok_in_page = 0;
   if (tok0 >= 0 && w.i0 < w.n) {
     const int64_t slot = tok0 / p.pool.PS;
-    if (slot < p.W) {
-      const int id = p.pt[w.b * p.pt_sb + w.h * p.pt_sh + slot];
-      if (id >= 0 && id < p.pool.num_pages)
-        w.group = p.pool.data + ((static_cast<int64_t>(id) * p.pool.PS + (tok0 - slot * p.pool.PS)) >> 4) * Fp4Group<NB>::kBytes;
-    }
+    w.tok_in_page = tok0 - slot * p.pool.PS;
+    if (slot < p.W) w.id = p.pt[w.b * p.pt_sb + w.h * p.pt_sh + slot];
   }
   return w.i0 < p.N;
 }
 
-__device__ __forceinline__ float largest8(float (&x)[8]) {
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    x[i] = x[i] != x[i] ? 0.f : x[i];
-    amax = fmaxf(amax, fabsf(x[i]));
-  }
-  return amax;
+// the 16 rows' bytes, or null: no such page
+template <int NB>
+__device__ __forceinline__ uint8_t* group_of(const RowsParams& p, const Place& w) {
+  if (w.id < 0 || w.id >= p.pool.num_pages) return nullptr;
+  return p.pool.data + ((static_cast<int64_t>(w.id) * p.pool.PS + w.tok_in_page) >> 4) * Fp4Group<NB>::kBytes;
 }
 
 template <int NB>
@@ -146,84 +185,103 @@ __device__ __forceinline__ void get_words(const uint8_t* set, int lane, unsigned
   }
 }
 
-template <int NB, bool VEC>
+template <int NB, int KIND>
 __global__ void __launch_bounds__(kRowThreads) fp4_append_kernel(const RowsParams p) {
   using Gr = Fp4Group<NB>;
+  using E = Eight<KIND>;
   Place w;
   if (!find_place<NB>(p, w)) return;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if (!w.group) {
+  constexpr int VC = NB / 2;                  // runs of 8 channels that a lane has of a V row
+  const bool k_real = w.real(g), v_real0 = w.real(2 * t), v_real1 = w.real(2 * t + 1);
+  // the rows are on their way while the page id is
+  E k[NB], v[2][VC];
+  const int64_t kat = w.b * p.k_sb + w.h * p.k_sh + (w.i0 + g) * p.k_sn + t * 8;
+  const int64_t vat = w.b * p.v_sb + w.h * p.v_sh + (w.i0 + 2 * t) * p.v_sn + g * (4 * NB);
+#pragma unroll
+  for (int b = 0; b < NB; ++b) k[b].load(p.k, p.dtype, kat + 32 * b, k_real);
+#pragma unroll
+  for (int c = 0; c < VC; ++c) {
+    v[0][c].load(p.v, p.dtype, vat + 8 * c, v_real0);
+    v[1][c].load(p.v, p.dtype, vat + p.v_sn + 8 * c, v_real1);
+  }
+  uint8_t* group = group_of<NB>(p, w);
+  if (!group) {
     if (p.dropped) {
       const int n = __popc(__ballot_sync(~0u, lane < 8 && w.real(lane)));
       if (lane == 0 && n) atomicAdd(p.dropped, n);
     }
     return;
   }
-  constexpr int VC = NB / 2;                  // runs of 8 channels that a lane has of a V row
-  const bool k_real = w.real(g), v_real0 = w.real(2 * t), v_real1 = w.real(2 * t + 1);
-  float kx[NB][8], vx[2][VC][8];
-  const int64_t kat = w.b * p.k_sb + w.h * p.k_sh + (w.i0 + g) * p.k_sn + t * 8;
-  const int64_t vat = w.b * p.v_sb + w.h * p.v_sh + (w.i0 + 2 * t) * p.v_sn + g * (4 * NB);
+  // largest magnitudes: of K's blocks over the row's 4 lanes, of V's over 8 / NB neighbouring g
+  float k_max[NB], v_max[2];
+  auto measure = [&]() {
+    bool nan = false;
 #pragma unroll
-  for (int b = 0; b < NB; ++b) {
+    for (int b = 0; b < NB; ++b) {
+      unsigned m = k[b].largest();
+      m = E::larger(m, __shfl_xor_sync(~0u, m, 1));
+      m = E::larger(m, __shfl_xor_sync(~0u, m, 2));
+      k_max[b] = E::magnitude(m);
+      nan = nan || k_max[b] != k_max[b];
+    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) kx[b][i] = 0.f;
-    if (k_real) load8<VEC>(p.k, p.dtype, kat + 32 * b, kx[b]);
+    for (int r = 0; r < 2; ++r) {
+      unsigned m = v[r][0].largest();
+#pragma unroll
+      for (int c = 1; c < VC; ++c) m = E::larger(m, v[r][c].largest());
+      if (NB <= 4) m = E::larger(m, __shfl_xor_sync(~0u, m, 4));
+      if (NB <= 2) m = E::larger(m, __shfl_xor_sync(~0u, m, 8));
+      v_max[r] = E::magnitude(m);
+      nan = nan || v_max[r] != v_max[r];
+    }
+    return __any_sync(~0u, nan);
+  };
+  if (measure()) {                            // a NaN among the rows
+#pragma unroll
+    for (int b = 0; b < NB; ++b) k[b].clean();
+#pragma unroll
+    for (int c = 0; c < VC; ++c) {
+      v[0][c].clean();
+      v[1][c].clean();
+    }
+    measure();
   }
-#pragma unroll
-  for (int c = 0; c < VC; ++c) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) vx[0][c][i] = vx[1][c][i] = 0.f;
-    if (v_real0) load8<VEC>(p.v, p.dtype, vat + 8 * c, vx[0][c]);
-    if (v_real1) load8<VEC>(p.v, p.dtype, vat + p.v_sn + 8 * c, vx[1][c]);
-  }
-  // K: a block's largest magnitude spans the row's 4 lanes
   unsigned word[NB];
-  uint8_t scale[NB];
+  int byte[NB];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
-    float amax = largest8(kx[b]);
-    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-    scale[b] = static_cast<uint8_t>(fp4_scale_byte(amax));
-    const float inv = fp4_inv_scale(scale[b]);            // a power of two: the product is exact
-    word[b] = 0;
+    byte[b] = fp4_scale_byte(k_max[b]);
+    const float inv = fp4_inv_scale(byte[b]);             // a power of two: the products are exact
+    float x[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) word[b] |= fp4_pack2(kx[b][2 * i] * inv, kx[b][2 * i + 1] * inv) << (8 * i);
+    for (int i = 0; i < 8; ++i) x[i] = k[b].value(i) * inv;
+    word[b] = fp4_pack8(x);
   }
   if (k_real) {
-    put_words<NB>(w.group + w.hi * Gr::kSet, lane, word);
+    put_words<NB>(group + w.hi * Gr::kSet, lane, word);
     if (t == 0) {
-      uint8_t* to = w.group + Gr::k_scale(8 * w.hi + g, 0);
+      uint8_t* to = group + Gr::k_scale(8 * w.hi + g, 0);
 #pragma unroll
       for (int b = 0; b < NB; b += 2)
-        *reinterpret_cast<uint16_t*>(to + b) = static_cast<uint16_t>(scale[b] | scale[b + 1] << 8);
+        *reinterpret_cast<uint16_t*>(to + b) = static_cast<uint16_t>(byte[b] | byte[b + 1] << 8);
     }
   }
-  // V: a block spans 8 / NB neighbouring g
-  int byte[2];
-  float inv[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    float amax = 0.f;
-#pragma unroll
-    for (int c = 0; c < VC; ++c) amax = fmaxf(amax, largest8(vx[r][c]));
-    if (NB <= 4) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 4));
-    if (NB <= 2) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 8));
-    byte[r] = fp4_scale_byte(amax);
-    inv[r] = fp4_inv_scale(byte[r]);
-  }
   if (!v_real0 && !v_real1) return;
+  const int b0 = fp4_scale_byte(v_max[0]), b1 = fp4_scale_byte(v_max[1]);
+  const float inv0 = fp4_inv_scale(b0), inv1 = fp4_inv_scale(b1);
 #pragma unroll
   for (int j = 0; j < NB; ++j) {              // byte of a channel: both rows' codes
-    word[j] = 0;
+    float x[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int c = 4 * j + i;
-      word[j] |= fp4_pack2(vx[0][c / 8][c % 8] * inv[0], vx[1][c / 8][c % 8] * inv[1]) << (8 * i);
+      x[2 * i] = v[0][c / 8].value(c % 8) * inv0;
+      x[2 * i + 1] = v[1][c / 8].value(c % 8) * inv1;
     }
+    word[j] = fp4_pack8(x);
   }
-  uint8_t* set = w.group + Gr::kV + w.hi * Gr::kSet;
+  uint8_t* set = group + Gr::kV + w.hi * Gr::kSet;
   if (!(v_real0 && v_real1)) {                // the other row's half stays as it is
     unsigned old[NB];
     get_words<NB>(set, lane, old);
@@ -233,9 +291,9 @@ __global__ void __launch_bounds__(kRowThreads) fp4_append_kernel(const RowsParam
   }
   put_words<NB>(set, lane, word);
   if (g % (8 / NB) == 0) {
-    uint8_t* to = w.group + Gr::v_scale(8 * w.hi + 2 * t, g * NB / 8);
-    if (v_real0) to[0] = static_cast<uint8_t>(byte[0]);
-    if (v_real1) to[1] = static_cast<uint8_t>(byte[1]);
+    uint8_t* to = group + Gr::v_scale(8 * w.hi + 2 * t, g * NB / 8);
+    if (v_real0) to[0] = static_cast<uint8_t>(b0);
+    if (v_real1) to[1] = static_cast<uint8_t>(b1);
   }
 }
 
@@ -270,19 +328,20 @@ __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams 
   Place w;
   if (!find_place<NB>(p, w)) return;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const uint8_t* group = group_of<NB>(p, w);
   unsigned kw[NB] = {}, vw[NB] = {}, ks[NB / 2] = {}, vs = 0;
-  if (w.group) {
-    get_words<NB>(w.group + w.hi * Gr::kSet, lane, kw);
-    get_words<NB>(w.group + Gr::kV + w.hi * Gr::kSet, lane, vw);
-    const uint16_t* from = reinterpret_cast<const uint16_t*>(w.group + Gr::k_scale(8 * w.hi + g, 0));
+  if (group) {
+    get_words<NB>(group + w.hi * Gr::kSet, lane, kw);
+    get_words<NB>(group + Gr::kV + w.hi * Gr::kSet, lane, vw);
+    const uint16_t* from = reinterpret_cast<const uint16_t*>(group + Gr::k_scale(8 * w.hi + g, 0));
 #pragma unroll
     for (int b = 0; b < NB / 2; ++b) ks[b] = from[b];
-    vs = *reinterpret_cast<const uint16_t*>(w.group + Gr::v_scale(8 * w.hi + 2 * t, g * NB / 8));
+    vs = *reinterpret_cast<const uint16_t*>(group + Gr::v_scale(8 * w.hi + 2 * t, g * NB / 8));
   }
   const int64_t kat = w.b * p.k_sb + w.h * p.k_sh + (w.i0 + g) * p.k_sn + t * 8;
   const int64_t vat = w.b * p.v_sb + w.h * p.v_sh + (w.i0 + 2 * t) * p.v_sn + g * (4 * NB);
   // rows from counts[b] on are zeros, whatever the page holds behind the sequence
-  const bool k_real = w.group && w.real(g);
+  const bool k_real = group && w.real(g);
   if (w.in(p, g)) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -294,7 +353,7 @@ __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams 
       store_halves<VEC>(p.k, p.dtype, kat + 32 * b, h);
     }
   }
-  const bool real0 = w.group && w.real(2 * t), real1 = w.group && w.real(2 * t + 1);
+  const bool real0 = group && w.real(2 * t), real1 = group && w.real(2 * t + 1);
   // (the byte of a row that was never written could borrow from the other half)
   const unsigned s = half_scales(real0 ? vs & 255 : 112, real1 ? vs >> 8 : 112);
 #pragma unroll
@@ -324,8 +383,10 @@ int launch_rows(const RowsParams& p, bool append, bool vec, cudaStream_t s) {
   if (blocks > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4 rows: too many rows for one launch");
   const unsigned g = static_cast<unsigned>(blocks);
   if (append) {
-    if (vec) fp4_append_kernel<NB, true><<<g, kRowThreads, 0, s>>>(p);
-    else fp4_append_kernel<NB, false><<<g, kRowThreads, 0, s>>>(p);
+    if (!vec) fp4_append_kernel<NB, kAny><<<g, kRowThreads, 0, s>>>(p);
+    else if (p.dtype == IAK_DT_F32) fp4_append_kernel<NB, IAK_DT_F32><<<g, kRowThreads, 0, s>>>(p);
+    else if (p.dtype == IAK_DT_F16) fp4_append_kernel<NB, IAK_DT_F16><<<g, kRowThreads, 0, s>>>(p);
+    else fp4_append_kernel<NB, IAK_DT_BF16><<<g, kRowThreads, 0, s>>>(p);
   } else {
     if (vec) fp4_read_kernel<NB, true><<<g, kRowThreads, 0, s>>>(p);
     else fp4_read_kernel<NB, false><<<g, kRowThreads, 0, s>>>(p);
