@@ -91,33 +91,6 @@ struct Eight {
   }
 };
 
-template <bool VEC>
-__device__ __forceinline__ void store8(void* base, int dtype, int64_t at, const float (&x)[8]) {
-  if (!VEC) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) store_from_float(base, dtype, at + i, x[i]);
-    return;
-  }
-  if (dtype == IAK_DT_F32) {
-    float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + at);
-    __stcs(p, make_float4(x[0], x[1], x[2], x[3]));
-    __stcs(p + 1, make_float4(x[4], x[5], x[6], x[7]));
-    return;
-  }
-  unsigned u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (dtype == IAK_DT_F16) {
-      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-      u[i] = *reinterpret_cast<const unsigned*>(&h);
-    } else {
-      const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-      u[i] = *reinterpret_cast<const unsigned*>(&h);
-    }
-  }
-  __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at), make_uint4(u[0], u[1], u[2], u[3]));
-}
-
 // Where a warp works: 8 rows of one (b, h), tokens 8 k .. 8 k + 7.  Row j is row i0 + j of the call's.
 struct Place {
   int b, h;
@@ -305,24 +278,41 @@ __device__ __forceinline__ unsigned mul2(unsigned a, unsigned b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const unsigned*>(&r);
 }
-// 8 values held as half pairs
-template <bool VEC>
-__device__ __forceinline__ void store_halves(void* base, int dtype, int64_t at, const unsigned* h) {
-  if (VEC && dtype == IAK_DT_F16) {
-    __stcs(reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at), make_uint4(h[0], h[1], h[2], h[3]));
-    return;
-  }
-  float x[8];
+// 8 values held as half pairs, as 16-bit values of the type
+__device__ __forceinline__ uint4 as_16bit(const unsigned* h, int dtype) {
+  if (dtype == IAK_DT_F16) return make_uint4(h[0], h[1], h[2], h[3]);
+  unsigned u[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+    const __nv_bfloat162 v = __floats2bfloat162_rn(f.x, f.y);
+    u[i] = *reinterpret_cast<const unsigned*>(&v);
   }
-  store8<VEC>(base, dtype, at, x);
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ uint4 as_floats(const unsigned* h) {
+  const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[0]));
+  const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&h[1]));
+  return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+}
+// Two lanes that differ in bit XOR and write the same row have 32 bytes each, a and b; every store of the pair fills a
+// whole 32-byte sector: first the lower lane's, then the upper's.  `to`: this lane's 32 bytes, `gap`: to the other's.
+template <int XOR>
+__device__ __forceinline__ void store_sectors(char* to, int gap, uint4 a, uint4 b, bool write) {
+  const bool upper = threadIdx.x & XOR;
+  const uint4 send = upper ? a : b;
+  uint4 got;
+  got.x = __shfl_xor_sync(~0u, send.x, XOR);
+  got.y = __shfl_xor_sync(~0u, send.y, XOR);
+  got.z = __shfl_xor_sync(~0u, send.z, XOR);
+  got.w = __shfl_xor_sync(~0u, send.w, XOR);
+  if (!write) return;
+  __stcs(reinterpret_cast<uint4*>(upper ? to - gap + 16 : to), upper ? got : a);
+  __stcs(reinterpret_cast<uint4*>(upper ? to + 16 : to + gap), upper ? b : got);
 }
 
-template <int NB, bool VEC>
+// KIND: IAK_DT_F32, IAK_DT_F16 (either 16-bit type) or kAny
+template <int NB, int KIND>
 __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams p) {
   using Gr = Fp4Group<NB>;
   Place w;
@@ -342,37 +332,62 @@ __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams 
   const int64_t vat = w.b * p.v_sb + w.h * p.v_sh + (w.i0 + 2 * t) * p.v_sn + g * (4 * NB);
   // rows from counts[b] on are zeros, whatever the page holds behind the sequence
   const bool k_real = group && w.real(g);
-  if (w.in(p, g)) {
+  const bool k_in = w.in(p, g);
+  constexpr int SIZE = KIND == IAK_DT_F32 ? 4 : 2;
+  auto put = [&](void* base, int64_t at, const unsigned* h, bool write) {      // one element at a time
+    if (!write) return;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      unsigned h[4];
-      fp4_unpack4(kw[b], h);
-      const unsigned byte = b % 2 ? ks[b / 2] >> 8 : ks[b / 2] & 255, s = half_scales(byte, byte);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = k_real ? mul2(h[i], s) : 0;
-      store_halves<VEC>(p.k, p.dtype, kat + 32 * b, h);
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+      store_from_float(base, p.dtype, at + 2 * i, f.x);
+      store_from_float(base, p.dtype, at + 2 * i + 1, f.y);
     }
+  };
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    unsigned h[4];
+    fp4_unpack4(kw[b], h);
+    const unsigned byte = b % 2 ? ks[b / 2] >> 8 : ks[b / 2] & 255, s = half_scales(byte, byte);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = k_real ? mul2(h[i], s) : 0;
+    char* to = static_cast<char*>(p.k) + (kat + 32 * b) * SIZE;
+    if constexpr (KIND == kAny) put(p.k, kat + 32 * b, h, k_in);
+    else if constexpr (KIND == IAK_DT_F32) store_sectors<1>(to, 32, as_floats(h), as_floats(h + 2), k_in);
+    else if (k_in) __stcs(reinterpret_cast<uint4*>(to), as_16bit(h, p.dtype));
   }
   const bool real0 = group && w.real(2 * t), real1 = group && w.real(2 * t + 1);
+  const bool in[2] = {w.in(p, 2 * t), w.in(p, 2 * t + 1)};
   // (the byte of a row that was never written could borrow from the other half)
   const unsigned s = half_scales(real0 ? vs & 255 : 112, real1 ? vs >> 8 : 112);
+  unsigned v[2][2 * NB];                      // the rows' channels as half pairs
 #pragma unroll
-  for (int c = 0; c < NB / 2; ++c) {          // 8 channels of both rows
-    unsigned r0[4], r1[4];
+  for (int j = 0; j < NB; ++j) {
+    unsigned h[4];
+    fp4_unpack4(vw[j], h);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      unsigned h[4];
-      fp4_unpack4(vw[2 * c + j], h);
+    for (int i = 0; i < 4; ++i) h[i] = mul2(h[i], s);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) h[i] = mul2(h[i], s);
+    for (int i = 0; i < 2; ++i) {
+      v[0][2 * j + i] = real0 ? __byte_perm(h[2 * i], h[2 * i + 1], 0x5410) : 0;
+      v[1][2 * j + i] = real1 ? __byte_perm(h[2 * i], h[2 * i + 1], 0x7632) : 0;
+    }
+  }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        r0[2 * j + i] = real0 ? __byte_perm(h[2 * i], h[2 * i + 1], 0x5410) : 0;
-        r1[2 * j + i] = real1 ? __byte_perm(h[2 * i], h[2 * i + 1], 0x7632) : 0;
+  for (int r = 0; r < 2; ++r) {
+    const int64_t at = vat + r * p.v_sn;
+    char* to = static_cast<char*>(p.v) + at * SIZE;
+    constexpr int gap = 4 * NB * SIZE;        // bytes to the next g's channels
+#pragma unroll
+    for (int c = 0; c < NB / 2; ++c) {        // runs of 8 channels
+      const unsigned* h = v[r] + 4 * c;
+      if constexpr (KIND == kAny) put(p.v, at + 8 * c, h, in[r]);
+      else if constexpr (KIND == IAK_DT_F32) store_sectors<4>(to + 32 * c, gap, as_floats(h), as_floats(h + 2), in[r]);
+      else if constexpr (NB == 2) {
+        if (in[r]) __stcs(reinterpret_cast<uint4*>(to), as_16bit(h, p.dtype));
+      } else if (c % 2 == 0) {
+        store_sectors<4>(to + 16 * c, gap, as_16bit(h, p.dtype), as_16bit(h + 4, p.dtype), in[r]);
       }
     }
-    if (w.in(p, 2 * t)) store_halves<VEC>(p.v, p.dtype, vat + 8 * c, r0);
-    if (w.in(p, 2 * t + 1)) store_halves<VEC>(p.v, p.dtype, vat + p.v_sn + 8 * c, r1);
   }
 }
 
@@ -388,8 +403,9 @@ int launch_rows(const RowsParams& p, bool append, bool vec, cudaStream_t s) {
     else if (p.dtype == IAK_DT_F16) fp4_append_kernel<NB, IAK_DT_F16><<<g, kRowThreads, 0, s>>>(p);
     else fp4_append_kernel<NB, IAK_DT_BF16><<<g, kRowThreads, 0, s>>>(p);
   } else {
-    if (vec) fp4_read_kernel<NB, true><<<g, kRowThreads, 0, s>>>(p);
-    else fp4_read_kernel<NB, false><<<g, kRowThreads, 0, s>>>(p);
+    if (!vec) fp4_read_kernel<NB, kAny><<<g, kRowThreads, 0, s>>>(p);
+    else if (p.dtype == IAK_DT_F32) fp4_read_kernel<NB, IAK_DT_F32><<<g, kRowThreads, 0, s>>>(p);
+    else fp4_read_kernel<NB, IAK_DT_F16><<<g, kRowThreads, 0, s>>>(p);
   }
   return check_cuda(cudaGetLastError(), append ? "fp4_append launch" : "fp4_read launch");
 }
