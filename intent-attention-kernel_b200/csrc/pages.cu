@@ -110,21 +110,55 @@ __device__ __forceinline__ void copy_page(const Planes& pl, int64_t from, int64_
   }
 }
 
-// the slice of the pages that block `rank` of the cluster scans, whole runs of a block's threads
+// The pages that block `rank` of the cluster scans, in whole runs of kRun pages: a thread takes 32 at a time.
+constexpr int kRun = 32 * kPlanThreads;
 __device__ __forceinline__ void slice_of(int pages, int rank, int* begin, int* end) {
-  const int64_t per = ((static_cast<int64_t>(pages) + kCluster - 1) / kCluster + kPlanThreads - 1) / kPlanThreads * kPlanThreads;
+  const int64_t per = ((static_cast<int64_t>(pages) + kCluster * 32 - 1) / (kCluster * 32)) * 32;
   *begin = static_cast<int>(min(static_cast<int64_t>(pages), per * rank));
   *end = static_cast<int>(min(static_cast<int64_t>(pages), per * (rank + 1)));
 }
 
-// pages in use in [begin, end)
-__device__ __forceinline__ int count_live(const int32_t* refs, int begin, int end) {
-  int live = 0;
-  for (int p = begin + threadIdx.x; p < end; p += kPlanThreads) live += refs[p] > 0;
-  int all;
-  block_before(live, &all);
-  return all;
+// bit i: page p + i is in use (p + i < end)
+__device__ __forceinline__ unsigned live_mask(const int32_t* refs, int p, int end) {
+  unsigned m = 0;
+  if (p >= end) return 0;
+  if (end - p >= 32 && (reinterpret_cast<uintptr_t>(refs + p) & 15) == 0) {
+    int4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = reinterpret_cast<const int4*>(refs + p)[k];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      m |= ((v[k].x > 0 ? 1u : 0u) | (v[k].y > 0 ? 2u : 0u) | (v[k].z > 0 ? 4u : 0u) | (v[k].w > 0 ? 8u : 0u)) << (4 * k);
+  } else {
+    for (int k = 0; k < min(32, end - p); ++k) m |= (refs[p + k] > 0 ? 1u : 0u) << k;
+  }
+  return m;
 }
+// the low bits of a 32-page run at p that stand for pages below n
+__device__ __forceinline__ unsigned below_mask(int p, int n) {
+  return n <= p ? 0u : (n - p >= 32 ? ~0u : (1u << (n - p)) - 1u);
+}
+
+// A thread's 32 pages of the run at p0; those of the first run (all of them, up to 2^18 pages) stay in a register.
+struct Masks {
+  const int32_t* refs;
+  int begin, end;
+  unsigned first;
+  __device__ __forceinline__ Masks(const int32_t* r, int b, int e) : refs(r), begin(b), end(e) {
+    first = live_mask(refs, begin + 32 * static_cast<int>(threadIdx.x), end);
+  }
+  __device__ __forceinline__ unsigned at(int p0) const {
+    return p0 == begin ? first : live_mask(refs, p0 + 32 * static_cast<int>(threadIdx.x), end);
+  }
+  // the block's pages in use below n
+  __device__ __forceinline__ int count(int n) const {
+    int live = 0, all;
+    for (int p0 = begin; p0 < min(end, n); p0 += kRun)
+      live += __popc(at(p0) & below_mask(p0 + 32 * static_cast<int>(threadIdx.x), n));
+    block_before(live, &all);
+    return all;
+  }
+};
 
 // ------------------------------------------------------------------------ grow
 // Scratch: first[S * Ht] = rank of the (slot, head)'s first new page, < 0 = gets none; shared[S * Ht] (copy the open
@@ -135,39 +169,30 @@ __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPlanThreads)
 grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const GrowScratch w) {
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
-  __shared__ int live_here, wanted;
+  __shared__ int live_here, wanted, cut;               // cut: first slot that the free pages do not reach
   int begin, end;
   slice_of(q.num_pages, rank, &begin, &end);
-  const int live = count_live(q.refs, begin, end);
-  if (threadIdx.x == 0) live_here = live;
-  cluster.sync();
-  int free_before = 0, free_all = 0;                   // free pages below this slice, in all
-  for (int r = 0; r < kCluster; ++r) {
-    int bb, be;
-    slice_of(q.num_pages, r, &bb, &be);
-    const int f = be - bb - *cluster.map_shared_rank(&live_here, r);
-    if (r < rank) free_before += f;
-    free_all += f;
-  }
+  const int64_t n = static_cast<int64_t>(q.S) * q.Ht;
+  int refused = 0;
   if (rank == 0) {
     // ranks of the pages wanted, in order of (slot, head); one thread per (slot, head)
-    __shared__ int cut;                                // first slot that the free pages do not reach
-    if (threadIdx.x == 0) cut = q.S;
+    if (threadIdx.x == 0) {
+      cut = q.S;
+      wanted = 0;
+    }
     int64_t base = 0;
-    const int64_t n = static_cast<int64_t>(q.S) * q.Ht;
-    int refused = 0;
     for (int64_t i0 = 0; i0 < n; i0 += kPlanThreads) {
       const int64_t i = i0 + threadIdx.x;
       int need = 0;
+      bool ok = false;
       if (i < n) {
         const int s = static_cast<int>(i / q.Ht), h = static_cast<int>(i - static_cast<int64_t>(s) * q.Ht);
         const int len = max(q.lengths[s], 0), add = more[s];
         const int64_t total = static_cast<int64_t>(len) + add;
-        bool ok = add > 0 && total <= static_cast<int64_t>(q.W) * q.PS && total <= 0x7fffffff;
+        ok = add > 0 && total <= static_cast<int64_t>(q.W) * q.PS && total <= 0x7fffffff;
         const int old = ok ? pages_of(len, q.PS) : 0;
-        const bool open = ok && len % q.PS != 0;
         bool copy = false;
-        if (open) {
+        if (ok && len % q.PS != 0) {
           // an open page outside the pool refuses the slot, for all of its heads
           for (int k = 0; k < q.Ht; ++k) ok = ok && in_pool(q, q.table[s * q.sb + k * q.sh + old - 1]);
           copy = ok && q.refs[q.table[s * q.sb + h * q.sh + old - 1]] > 1;
@@ -180,24 +205,34 @@ grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const Grow
           w.fresh[s] = fresh;
           if (add != 0 && !ok) ++refused;
         }
-        w.first[i] = ok ? 0 : -1;
       }
       int all;
       const int before = block_before(need, &all);
-      if (i < n) {
-        const int64_t at = base + before;
-        const int s = static_cast<int>(i / q.Ht);
-        if (w.first[i] == 0) {
-          if (at + need > free_all) atomicMin(&cut, s);
-          w.first[i] = static_cast<int32_t>(min(at, static_cast<int64_t>(0x7fffffff)));
-        }
-      }
+      if (i < n) w.first[i] = ok ? static_cast<int32_t>(min(base + before, static_cast<int64_t>(0x7fffffff))) : -1;
       base += all;
     }
-    __syncthreads();
+  }
+  const Masks masks(q.refs, begin, end);
+  const int live = masks.count(end);
+  if (threadIdx.x == 0) live_here = live;
+  cluster.sync();
+  int free_before = 0, free_all = 0;                   // free pages below this slice, in all
+  for (int r = 0; r < kCluster; ++r) {
+    int bb, be;
+    slice_of(q.num_pages, r, &bb, &be);
+    const int f = be - bb - *cluster.map_shared_rank(&live_here, r);
+    if (r < rank) free_before += f;
+    free_all += f;
+  }
+  if (rank == 0) {
     // a slot that does not fit, and every later one that gets tokens, stays as it is
+    for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
+      const int s = static_cast<int>(i / q.Ht);
+      if (w.first[i] >= 0 && static_cast<int64_t>(w.first[i]) + w.fresh[s] + w.shared[i] > free_all) atomicMin(&cut, s);
+    }
+    __syncthreads();
     const int last = cut;
-    int64_t take = 0;
+    int take = 0;
     for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
       const int s = static_cast<int>(i / q.Ht), h = static_cast<int>(i - static_cast<int64_t>(s) * q.Ht);
       if (w.first[i] < 0) continue;
@@ -205,25 +240,23 @@ grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const Grow
         w.first[i] = -1;
         if (h == 0) ++refused;
       } else {
-        take = max(take, static_cast<int64_t>(w.first[i]) + w.fresh[s] + w.shared[i]);
+        take = max(take, w.first[i] + w.fresh[s] + w.shared[i]);
         if (h == 0) q.lengths[s] = max(q.lengths[s], 0) + more[s];
       }
     }
-    if (threadIdx.x == 0) wanted = 0;
-    __syncthreads();
-    atomicMax(&wanted, static_cast<int>(take));
+    if (take) atomicMax(&wanted, take);
     if (rejected && refused) atomicAdd(rejected, refused);
   }
   cluster.sync();
   const int want = *cluster.map_shared_rank(&wanted, 0);
   // the free pages of this slice, in ascending order
   int at = free_before;
-  for (int p0 = begin; p0 < end && at < want; p0 += kPlanThreads) {
-    const int p = p0 + threadIdx.x;
-    const int is_free = p < end && q.refs[p] <= 0;
+  for (int p0 = begin; p0 < end && at < want; p0 += kRun) {
+    const int p = p0 + 32 * static_cast<int>(threadIdx.x);
+    unsigned free_bits = ~masks.at(p0) & below_mask(p, end);
     int all;
-    const int before = block_before(is_free, &all);
-    if (is_free && at + before < want) w.new_ids[at + before] = p;
+    int k = at + block_before(__popc(free_bits), &all);
+    for (; free_bits && k < want; free_bits &= free_bits - 1, ++k) w.new_ids[k] = p + __ffs(free_bits) - 1;
     at += all;
   }
   cluster.sync();                                      // no block leaves while another may read its counts
@@ -323,7 +356,8 @@ compact_plan_kernel(const Seq q, int32_t* num_live, const CompactScratch w) {
   __shared__ int live_here, live_below_n;              // live pages of the slice; of the slice and below n
   int begin, end;
   slice_of(q.num_pages, rank, &begin, &end);
-  const int live = count_live(q.refs, begin, end);
+  const Masks masks(q.refs, begin, end);
+  const int live = masks.count(end);
   if (threadIdx.x == 0) live_here = live;
   cluster.sync();
   int live_before = 0, n = 0;
@@ -332,7 +366,7 @@ compact_plan_kernel(const Seq q, int32_t* num_live, const CompactScratch w) {
     if (r < rank) live_before += x;
     n += x;
   }
-  const int below = count_live(q.refs, begin, min(end, max(n, begin)));
+  const int below = masks.count(n);
   if (threadIdx.x == 0) live_below_n = below;
   cluster.sync();
   int stay = 0;                                        // live pages below n: they keep their place
@@ -342,17 +376,26 @@ compact_plan_kernel(const Seq q, int32_t* num_live, const CompactScratch w) {
     w.head[1] = n - stay;
     if (num_live) *num_live = n;
   }
-  int at = live_before;                                // live pages before p
-  for (int p0 = begin; p0 < end; p0 += kPlanThreads) {
-    const int p = p0 + threadIdx.x;
-    const int is_live = p < end && q.refs[p] > 0;
+  int at = live_before;                                // live pages before the run
+  for (int p0 = begin; p0 < end; p0 += kRun) {
+    const int p = p0 + 32 * static_cast<int>(threadIdx.x);
+    const unsigned live_bits = masks.at(p0), low = below_mask(p, n);
     int all;
-    const int before = at + block_before(is_live, &all);
-    if (p < end) {
-      if (p < n && !is_live) w.to[p - before] = p;
-      if (p >= n && is_live) {
-        w.from[before - stay] = p;
-        w.rank_of[p] = before - stay;
+    const int before = at + block_before(__popc(live_bits), &all);
+    // The k-th free page below n takes the k-th live page from n on.  A lane's 32 pages are written by the warp, a page
+    // per lane, so that neighbours in rank are neighbours in memory.
+    const int lane = threadIdx.x & 31;
+    const unsigned any = __ballot_sync(~0u, ((~live_bits & low) | (live_bits & ~low)) & below_mask(p, end));
+    for (unsigned todo = any; todo; todo &= todo - 1) {
+      const int l = __ffs(todo) - 1, page = __shfl_sync(~0u, p, l) + lane;
+      const unsigned bits = __shfl_sync(~0u, live_bits, l);
+      const int rank = __shfl_sync(~0u, before, l) + __popc(bits & ((1u << lane) - 1u));
+      if (page >= end) continue;
+      const bool is_live = bits >> lane & 1;
+      if (page < n && !is_live) w.to[page - rank] = page;
+      if (page >= n && is_live) {
+        w.from[rank - stay] = page;
+        w.rank_of[page] = rank - stay;
       }
     }
     at += all;
@@ -390,7 +433,7 @@ __global__ void __launch_bounds__(kActThreads) compact_act_kernel(const Seq q, c
 // ------------------------------------------------------------------------ host
 int check_seq(const iak_seq_pages* a, const char* what, Seq* q) {
   if (!a) return fail(IAK_ERR_INVALID_ARG, "%s: null arguments", what);
-  if (a->num_pages < 0 || a->num_pages > 0x7fffffffLL || a->num_slots < 0 || a->num_table_heads < 0 || a->table_width < 0)
+  if (a->num_pages < 0 || a->num_pages > 0x7fff0000LL || a->num_slots < 0 || a->num_table_heads < 0 || a->table_width < 0)
     return fail(IAK_ERR_INVALID_ARG, "%s: bad size", what);
   if (a->page_size <= 0) return fail(IAK_ERR_INVALID_ARG, "%s: page_size must be positive", what);
   const bool entries = a->num_slots > 0 && a->num_table_heads > 0 && a->table_width > 0;
