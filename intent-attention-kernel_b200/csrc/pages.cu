@@ -172,7 +172,7 @@ grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const Grow
   __shared__ int live_here, wanted, cut;               // cut: first slot that the free pages do not reach
   int begin, end;
   slice_of(q.num_pages, rank, &begin, &end);
-  const int64_t n = static_cast<int64_t>(q.S) * q.Ht;
+  const int n = q.S * q.Ht;                            // (the host keeps it within 31 bits)
   int refused = 0;
   if (rank == 0) {
     // ranks of the pages wanted, in order of (slot, head); one thread per (slot, head)
@@ -181,12 +181,12 @@ grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const Grow
       wanted = 0;
     }
     int64_t base = 0;
-    for (int64_t i0 = 0; i0 < n; i0 += kPlanThreads) {
-      const int64_t i = i0 + threadIdx.x;
+    for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+      const int i = i0 + threadIdx.x;
       int need = 0;
       bool ok = false;
       if (i < n) {
-        const int s = static_cast<int>(i / q.Ht), h = static_cast<int>(i - static_cast<int64_t>(s) * q.Ht);
+        const int s = i / q.Ht, h = i - s * q.Ht;
         const int len = max(q.lengths[s], 0), add = more[s];
         const int64_t total = static_cast<int64_t>(len) + add;
         ok = add > 0 && total <= static_cast<int64_t>(q.W) * q.PS && total <= 0x7fffffff;
@@ -194,8 +194,10 @@ grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const Grow
         bool copy = false;
         if (ok && len % q.PS != 0) {
           // an open page outside the pool refuses the slot, for all of its heads
-          for (int k = 0; k < q.Ht; ++k) ok = ok && in_pool(q, q.table[s * q.sb + k * q.sh + old - 1]);
-          copy = ok && q.refs[q.table[s * q.sb + h * q.sh + old - 1]] > 1;
+          const int32_t* open = q.table + s * q.sb + old - 1;
+#pragma unroll 8
+          for (int k = 0; k < q.Ht; ++k) ok = in_pool(q, open[k * q.sh]) & ok;
+          copy = ok && q.refs[open[h * q.sh]] > 1;
         }
         const int fresh = ok ? pages_of(static_cast<int>(total), q.PS) - old : 0;
         need = fresh + (copy ? 1 : 0);
@@ -226,15 +228,15 @@ grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const Grow
   }
   if (rank == 0) {
     // a slot that does not fit, and every later one that gets tokens, stays as it is
-    for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
-      const int s = static_cast<int>(i / q.Ht);
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+      const int s = i / q.Ht;
       if (w.first[i] >= 0 && static_cast<int64_t>(w.first[i]) + w.fresh[s] + w.shared[i] > free_all) atomicMin(&cut, s);
     }
     __syncthreads();
     const int last = cut;
     int take = 0;
-    for (int64_t i = threadIdx.x; i < n; i += kPlanThreads) {
-      const int s = static_cast<int>(i / q.Ht), h = static_cast<int>(i - static_cast<int64_t>(s) * q.Ht);
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+      const int s = i / q.Ht, h = i - s * q.Ht;
       if (w.first[i] < 0) continue;
       if (s >= last) {
         w.first[i] = -1;
@@ -264,11 +266,11 @@ grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const Grow
 
 __global__ void __launch_bounds__(kActThreads) grow_act_kernel(const Seq q, const Planes pl, const GrowScratch w) {
   const int warps = kActThreads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n = static_cast<int64_t>(q.S) * q.Ht;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * warps + warp; i < n; i += static_cast<int64_t>(gridDim.x) * warps) {
+  const int n = q.S * q.Ht;                            // (the host keeps it within 31 bits)
+  for (int i = blockIdx.x * warps + warp; i < n; i += gridDim.x * warps) {
     const int first = w.first[i];
     if (first < 0) continue;
-    const int s = static_cast<int>(i / q.Ht), h = static_cast<int>(i - static_cast<int64_t>(s) * q.Ht);
+    const int s = i / q.Ht, h = i - s * q.Ht;
     int32_t* row = q.table + s * q.sb + h * q.sh;
     const int old = w.old_pages[s], fresh = w.fresh[s], copy = w.shared[i];
     if (copy) {
@@ -416,9 +418,9 @@ __global__ void __launch_bounds__(kActThreads) compact_act_kernel(const Seq q, c
     }
   }
   // table entries of moved pages; rank_of holds anything for other pages, so the move has to agree
-  const int64_t rows = static_cast<int64_t>(q.S) * q.Ht;
-  for (int64_t r = static_cast<int64_t>(blockIdx.x) * warps + warp; r < rows; r += static_cast<int64_t>(gridDim.x) * warps) {
-    const int s = static_cast<int>(r / q.Ht), h = static_cast<int>(r - static_cast<int64_t>(s) * q.Ht);
+  const int rows = q.S * q.Ht;
+  for (int r = blockIdx.x * warps + warp; r < rows; r += gridDim.x * warps) {
+    const int s = r / q.Ht, h = r - s * q.Ht;
     int32_t* row = q.table + s * q.sb + h * q.sh;
     const int held = held_pages(q, s);
     for (int e = lane; e < held; e += 32) {
@@ -435,6 +437,8 @@ int check_seq(const iak_seq_pages* a, const char* what, Seq* q) {
   if (!a) return fail(IAK_ERR_INVALID_ARG, "%s: null arguments", what);
   if (a->num_pages < 0 || a->num_pages > 0x7fff0000LL || a->num_slots < 0 || a->num_table_heads < 0 || a->table_width < 0)
     return fail(IAK_ERR_INVALID_ARG, "%s: bad size", what);
+  if (static_cast<int64_t>(a->num_slots) * a->num_table_heads > 0x7fff0000LL)
+    return fail(IAK_ERR_UNSUPPORTED, "%s: more than 2^31 (slot, head) pairs", what);
   if (a->page_size <= 0) return fail(IAK_ERR_INVALID_ARG, "%s: page_size must be positive", what);
   const bool entries = a->num_slots > 0 && a->num_table_heads > 0 && a->table_width > 0;
   if ((a->num_slots > 0 && !a->lengths) || (a->num_pages > 0 && !a->refs) || (entries && !a->page_table))

@@ -31,33 +31,29 @@ from .paged import _DT, _require_cuda
 
 HEAD_DIMS = (64, 128, 256)
 
-# Per-call host work is most of a small call's time, so the helpers below test the few properties that the kernels rely
-# on and build their messages only when one fails.
-_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+# Per-call host work is most of a small call's time: the helpers below take the device as its index (a CPU tensor's is
+# -1), test the few properties that the kernels rely on and build their messages only when one fails.
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 _NO_SWITCH = contextlib.nullcontext()
 
 
-def _on(device: torch.device):
+def _on(dev: int):
     """The library launches on the current device; switch only when it is another one."""
-    if device.index is None or device.index == _current_device():
-        return _NO_SWITCH
-    return torch.cuda.device(device)
+    return _NO_SWITCH if dev == _current_device() else torch.cuda.device(dev)
 
 
-def _raw_stream(device: torch.device) -> int:
-    if device.index is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _check_device(t, name: str, dev: int) -> None:
+    if not isinstance(t, torch.Tensor) or t.get_device() != dev:
+        _require_cuda(t, name)
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{dev}")
 
 
-def _index_tensor(t: Optional[torch.Tensor], name: str, device: torch.device, numel: Optional[int] = None):
-    """Address of a contiguous int32 tensor on ``device``; None passes."""
+def _index_tensor(t: Optional[torch.Tensor], name: str, dev: int, numel: Optional[int] = None):
+    """Address of a contiguous int32 tensor on device ``dev``; None passes."""
     if t is None:
         return None
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _require_cuda(t, name)
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    _check_device(t, name, dev)
     if t.dtype is not torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor")
     if numel is not None and t.numel() != numel:
@@ -65,12 +61,9 @@ def _index_tensor(t: Optional[torch.Tensor], name: str, device: torch.device, nu
     return t.data_ptr()
 
 
-def _page_table(t: torch.Tensor, device: torch.device, batch: Optional[int] = None, heads: Optional[int] = None):
+def _page_table(t: torch.Tensor, dev: int, batch: Optional[int] = None, heads: Optional[int] = None):
     """(address, stride of b, stride of h, Ht, W) of an int32 [B, Ht, W] table."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _require_cuda(t, "page_table")
-    if t.device != device:
-        raise ValueError(f"page_table is on {t.device}, expected {device}")
+    _check_device(t, "page_table", dev)
     if t.dim() != 3 or t.dtype is not torch.int32:
         raise ValueError("page_table must be int32 [B, Ht, W]")
     B, Ht, W = t.shape
@@ -156,11 +149,9 @@ def append_fp4(pool: Fp4Pool, k_new: torch.Tensor, v_new: torch.Tensor, page_tab
     belong to one (b, h) each, and a sequence is written by one call at a time:
     two rows of V share their bytes.
     """
-    dev = pool.device
-    _require_cuda(k_new, "k_new")
-    _require_cuda(v_new, "v_new")
-    if k_new.device != dev or v_new.device != dev:
-        raise ValueError(f"k_new is on {k_new.device}, v_new on {v_new.device}, the pool on {dev}")
+    s, dev = pool.struct(), pool.data.get_device()
+    _check_device(k_new, "k_new", dev)
+    _check_device(v_new, "v_new", dev)
     shape = k_new.shape
     if len(shape) != 4 or shape != v_new.shape or shape[3] != pool.head_dim:
         raise ValueError(f"k_new / v_new must both be [B, Ht, n, {pool.head_dim}]")
@@ -172,7 +163,6 @@ def append_fp4(pool: Fp4Pool, k_new: torch.Tensor, v_new: torch.Tensor, page_tab
         v_new = v_new.contiguous()
     table = _page_table(page_table, dev, shape[0], shape[1])
     a = _rows_args(dev, k_new, v_new, table, positions, counts, dropped)
-    s = pool.struct()
     with _on(dev):
         N.check(N.lib().iak_fp4_append(ctypes.byref(s), ctypes.byref(a), _raw_stream(dev)), "iak_fp4_append")
 
@@ -184,7 +174,7 @@ def read_fp4(pool: Fp4Pool, page_table: torch.Tensor, positions: Optional[torch.
     [B, Ht, num_rows, D].  Every value a pool holds is exact in all three float
     types.  Rows from ``counts[b]`` on, and rows of slots or pages that do not
     exist, are 0.  ``out``: a (k, v) pair to write into."""
-    dev = pool.device
+    s, dev = pool.struct(), pool.data.get_device()
     table = _page_table(page_table, dev)
     if num_rows < 0:
         raise ValueError("num_rows must not be negative")
@@ -192,18 +182,17 @@ def read_fp4(pool: Fp4Pool, page_table: torch.Tensor, positions: Optional[torch.
     if out is None:
         if dtype not in _DT:
             raise ValueError("dtype must be float32 / float16 / bfloat16")
-        k = torch.empty(shape, dtype=dtype, device=dev)
+        k = torch.empty(shape, dtype=dtype, device=pool.data.device)
         v = torch.empty_like(k)
     else:
         k, v = out
         for name, x in (("out[0]", k), ("out[1]", v)):
-            _require_cuda(x, name)
-            if tuple(x.shape) != shape or x.device != dev or x.dtype not in _DT or x.dtype != k.dtype:
-                raise ValueError(f"{name} must be a {shape} float tensor on {dev}, both of one dtype")
+            _check_device(x, name, dev)
+            if tuple(x.shape) != shape or x.dtype not in _DT or x.dtype != k.dtype:
+                raise ValueError(f"{name} must be a {shape} float tensor, both of one dtype")
             if x.stride(3) != 1:
                 raise ValueError(f"{name} needs a unit stride along head_dim")
     a = _rows_args(dev, k, v, table, positions, counts)
-    s = pool.struct()
     with _on(dev):
         N.check(N.lib().iak_fp4_read(ctypes.byref(s), ctypes.byref(a), _raw_stream(dev)), "iak_fp4_read")
     return k, v
@@ -215,10 +204,8 @@ def read_fp4(pool: Fp4Pool, page_table: torch.Tensor, positions: Optional[torch.
 
 def _decode(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Tensor, lengths: torch.Tensor, sm_scale: float,
             out: Optional[torch.Tensor], out_dtype: Optional[torch.dtype], differential=None) -> torch.Tensor:
-    _require_cuda(q, "q")
-    dev = pool.device
-    if q.device != dev:
-        raise ValueError(f"q is on {q.device}, the pool on {dev}")
+    s, dev = pool.struct(), pool.data.get_device()
+    _check_device(q, "q", dev)
     shape, strides = q.shape, q.stride()
     dims = len(shape)
     if dims not in (3, 4) or shape[-1] != pool.head_dim:
@@ -239,22 +226,21 @@ def _decode(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Tensor, lengths: t
         raise ValueError("lengths [B] is required")
     ln = _index_tensor(lengths, "lengths", dev, B)
     if out is not None:
-        _require_cuda(out, "out")
-        if out.shape != shape or out.device != dev or out.dtype not in _DT or out.stride(-1) != 1:
-            raise ValueError(f"out must be a {tuple(shape)} float tensor on {dev} with a contiguous last dim")
+        _check_device(out, "out", dev)
+        if out.shape != shape or out.dtype not in _DT or out.stride(-1) != 1:
+            raise ValueError(f"out must be a {tuple(shape)} float tensor with a contiguous last dim")
     elif out_dtype is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out_dtype not in _DT:
         raise ValueError(f"out dtype {out_dtype} unsupported")
     else:
-        out = torch.empty(shape, dtype=out_dtype, device=dev)
+        out = torch.empty(shape, dtype=out_dtype, device=q.device)
     os_ = out.stride()
     a = N.Fp4DecodeArgs(q.data_ptr(), _DT[q.dtype], strides[0], strides[1], strides[2] if dims == 4 else 0,
                         out.data_ptr(), _DT[out.dtype], os_[0], os_[1], os_[2] if dims == 4 else 0,
                         B, Hq, Ht, M, pt, pt_sb, pt_sh, W, ln, sm_scale)
     if differential is not None:
         a.differential, a.lam, a.norm_weight, a.eps, a.out_scale = (1, *differential)
-    s = pool.struct()
     L = N.lib()
     nbytes = ctypes.c_size_t(0)
     ps, pa = ctypes.byref(s), ctypes.byref(a)
@@ -262,7 +248,7 @@ def _decode(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Tensor, lengths: t
         N.check(L.iak_fp4_decode_workspace_size(ps, pa, ctypes.byref(nbytes)), "iak_fp4_decode_workspace_size")
         n = nbytes.value
         # of this call alone: calls on other streams, or captured into other graphs, never share it
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
         N.check(L.iak_fp4_decode(ps, pa, ws.data_ptr() if n else None, n, _raw_stream(dev)), "iak_fp4_decode")
     return out
 
@@ -298,9 +284,9 @@ def differential_decode_fp4(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Te
     1 / sqrt(D / 2).  Everything else as in ``paged_decode_fp4``.
     """
     def weight(t, name, n):
-        _require_cuda(t, name)
-        if t.device != pool.device or t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
-            raise ValueError(f"{name} must be {n} contiguous float32 values on {pool.device}")
+        _check_device(t, name, pool.data.get_device())
+        if t.dtype is not torch.float32 or t.numel() != n or not t.is_contiguous():
+            raise ValueError(f"{name} must be {n} contiguous float32 values")
         return t.data_ptr()
 
     if not isinstance(q, torch.Tensor) or q.dim() < 2:

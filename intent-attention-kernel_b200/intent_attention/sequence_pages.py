@@ -22,13 +22,15 @@ from typing import Optional, Sequence, Union
 import torch
 
 from . import _native as N
-from .fp4_cache import Fp4Pool, _index_tensor, _on, _page_table, _raw_stream
+from .fp4_cache import Fp4Pool, _check_device, _index_tensor, _on, _page_table, _raw_stream
 from .paged import PagePool, _require_cuda, _tags_args
 
 _BIT = {f: 1 << getattr(N, f"FMT_{f}") for f in ("F16", "FP8", "INT8", "INT4", "INT4R")}
 _SCALED = _BIT["FP8"] | _BIT["INT8"] | _BIT["INT4"] | _BIT["INT4R"]
-_PLANE_FORMATS = {"f16": _BIT["F16"], "fp8": _BIT["FP8"], "i8": _BIT["INT8"], "i4": _BIT["INT4"] | _BIT["INT4R"],
-                  "i4r": _BIT["INT4R"], "scale": _SCALED, "res_scale": _BIT["INT4R"]}
+# a PagePool's planes and the formats of the pages that use them
+_PLANES = tuple((f"{side}_{name}", bits) for name, bits in (
+    ("f16", _BIT["F16"]), ("fp8", _BIT["FP8"]), ("i8", _BIT["INT8"]), ("i4", _BIT["INT4"] | _BIT["INT4R"]),
+    ("i4r", _BIT["INT4R"]), ("scale", _SCALED), ("res_scale", _BIT["INT4R"])) for side in "kv")
 
 
 @dataclass
@@ -50,9 +52,8 @@ class SequencePages:
                    torch.zeros(num_slots, dtype=torch.int32, device=dev), page_size)
 
     def struct(self) -> N.SeqPages:
-        if not self.refs.is_cuda:
-            _require_cuda(self.refs, "refs")
-        dev = self.refs.device
+        _require_cuda(self.refs, "refs")
+        dev = self.refs.get_device()
         if self.page_size <= 0:
             raise ValueError("page_size must be positive")
         pt, ss, sh, Ht, W = _page_table(self.table, dev)
@@ -65,24 +66,21 @@ def _planes(pool: Union[PagePool, Fp4Pool], pages: SequencePages, page_tags, tag
     if pool.num_pages != pages.refs.numel() or pool.page_size != pages.page_size:
         raise ValueError(f"pages count {pages.refs.numel()} pages of {pages.page_size} rows, the pool has "
                          f"{pool.num_pages} of {pool.page_size}")
-    dev = pages.refs.device
+    dev = pages.refs.get_device()
     if isinstance(pool, Fp4Pool):
-        named = [(t, 0) for t in pool.tensors()]
+        planes = ((pool.data, 0),)
     else:
-        named = [(getattr(pool, f"{side}_{n}"), f) for n, f in _PLANE_FORMATS.items() for side in ("k", "v")]
-        named = [(t, f) for t, f in named if t is not None]
+        planes = [(t, f) for t, f in [(getattr(pool, name), f) for name, f in _PLANES] if t is not None]
     s = N.PagePlanes()
+    base, sizes, formats = s.base, s.bytes, s.formats
     n = 0
-    for t, formats in named:
-        if not t.is_cuda:
-            _require_cuda(t, "page pool")
-        if t.device != dev:
-            raise ValueError(f"the pool is on {t.device}, its pages on {dev}")
+    for t, f in planes:
+        _check_device(t, "page pool", dev)
         if not t.is_contiguous() or t.shape[0] != pool.num_pages:
             raise ValueError("page pools must be contiguous [num_pages, ...] tensors")
-        size = t.numel() * t.element_size()
+        size = t.nbytes
         if size:
-            s.base[n], s.bytes[n], s.formats[n] = t.data_ptr(), size // pool.num_pages, formats
+            base[n], sizes[n], formats[n] = t.data_ptr(), size // pool.num_pages, f
             n += 1
     s.num_planes = n
     if page_tags is not None:
@@ -91,19 +89,20 @@ def _planes(pool: Union[PagePool, Fp4Pool], pages: SequencePages, page_tags, tag
         if tag_map is None:
             raise ValueError("page_tags needs a tag_map")
         s.page_tags, s.tag_bytes = _tags_args(page_tags)
-        if page_tags.numel() < pool.num_pages or page_tags.device != dev:
-            raise ValueError(f"page_tags must hold {pool.num_pages} tags on {dev}")
+        _check_device(page_tags, "page_tags", dev)
+        if page_tags.numel() < pool.num_pages:
+            raise ValueError(f"page_tags must hold {pool.num_pages} tags")
         for i, f in enumerate(tag_map):
             s.tag_map[i] = f
         s.tag_default = tag_default
     return s
 
 
-def _workspace(dev: torch.device, s: N.SeqPages) -> torch.Tensor:
+def _workspace(device: torch.device, s: N.SeqPages) -> torch.Tensor:
     n = ctypes.c_size_t(0)
     N.check(N.lib().iak_pages_workspace_size(ctypes.byref(s), ctypes.byref(n)), "iak_pages_workspace_size")
     # of this call alone, as calls captured into different graphs must not share it
-    return torch.empty(n.value, dtype=torch.uint8, device=dev)
+    return torch.empty(n.value, dtype=torch.uint8, device=device)
 
 
 def grow_sequences(pool: Union[PagePool, Fp4Pool], pages: SequencePages, new_tokens: torch.Tensor,
@@ -121,12 +120,12 @@ def grow_sequences(pool: Union[PagePool, Fp4Pool], pages: SequencePages, new_tok
     every later one that gets tokens.
     """
     s = pages.struct()
-    dev = pages.refs.device
+    dev = pages.refs.get_device()
     more = _index_tensor(new_tokens, "new_tokens", dev, s.num_slots)
     count = _index_tensor(rejected, "rejected", dev, 1)
     pl = _planes(pool, pages, page_tags, tag_map, tag_default)
     with _on(dev):
-        ws = _workspace(dev, s)
+        ws = _workspace(pages.refs.device, s)
         N.check(N.lib().iak_pages_grow(ctypes.byref(s), ctypes.byref(pl), more, count, ws.data_ptr(), ws.numel(),
                                        _raw_stream(dev)), "iak_pages_grow")
 
@@ -139,7 +138,7 @@ def fork_sequences(pages: SequencePages, src: torch.Tensor, dst: torch.Tensor,
     a src that is also a dst of the call.
     """
     s = pages.struct()
-    dev = pages.refs.device
+    dev = pages.refs.get_device()
     a, n = _index_tensor(src, "src", dev), src.numel()
     b = _index_tensor(dst, "dst", dev, n)
     count = _index_tensor(rejected, "rejected", dev, 1)
@@ -151,7 +150,7 @@ def free_sequences(pages: SequencePages, slots: torch.Tensor, rejected: Optional
     """The listed slots (int32 on the device) let go of their pages: table entries -1, length 0.  A slot listed
     twice is freed once; one out of range is refused."""
     s = pages.struct()
-    dev = pages.refs.device
+    dev = pages.refs.get_device()
     a = _index_tensor(slots, "slots", dev)
     count = _index_tensor(rejected, "rejected", dev, 1)
     with _on(dev):
@@ -167,11 +166,11 @@ def compact_pages(pool: Union[PagePool, Fp4Pool], pages: SequencePages, page_tag
     planes of each page's format move, and its tag.
     """
     s = pages.struct()
-    dev = pages.refs.device
+    dev = pages.refs.get_device()
     pl = _planes(pool, pages, page_tags, tag_map, tag_default)
-    live = torch.empty((), dtype=torch.int32, device=dev)
+    live = torch.empty((), dtype=torch.int32, device=pages.refs.device)
     with _on(dev):
-        ws = _workspace(dev, s)
+        ws = _workspace(pages.refs.device, s)
         N.check(N.lib().iak_pages_compact(ctypes.byref(s), ctypes.byref(pl), live.data_ptr(), ws.data_ptr(),
                                           ws.numel(), _raw_stream(dev)), "iak_pages_compact")
     return live
