@@ -16,8 +16,8 @@
 // order of the blocks (no atomics: results do not depend on timing).  Each warp streams its own tiles through a
 // ring of 16-byte asynchronous copies: a group's codes and scales lie together in the order in which lanes read them,
 // so that copies and reads are linear in the lane, free of bank conflicts, and five copies per 16 rows need one address.
-// (Bulk copies, one per 16 rows, were measured and are slower here: each wants its operands in uniform registers, and
-// setting them up cost more issue slots than five plain copies, of which this kernel has none to spare.)
+// (Bulk copies, one per 16 rows and an mbarrier, measured the same at D 128, 141 us for the 32k batch of 32 below, and
+// slower at D 64, 70 us against 66 for 16 sequences of 32k; they would need bounded waits besides.)
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
@@ -28,8 +28,6 @@
 namespace iak {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
 constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
@@ -192,23 +190,29 @@ __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
 struct Cursor { int left, off, at, b, len; };   // tiles left to the block; the next one, of sequence b and of all
 struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, at; };   // at: its first tile, of all
 
-template <int NB>
-struct Lay {
+// What a kernel for D = 32 NB, 8 NT columns a block and (SPLIT) fp32 queries is made of.
+template <int NB, int NT, bool SPLIT>
+struct Shape {
   using Gr = Fp4Group<NB>;
-  static constexpr int D = NB * 32;
+  static constexpr int D = NB * 32, COLS = 8 * NT;
+  // Warps of a block and blocks of an SM: 16 warps with 128 registers each while the accumulators are small, 12 with
+  // 168, 8 with 255.  A tile's two groups of 16 keys go through the products together, for the independent work.
+  // (8 sequences of 32k, D 128, 16 columns: 95 us with 16 warps and one group at a time, 108 with 8, 86 with 12;
+  // 32 columns: 159 with 8, 203 with 12.  D 64, 32 columns: 172 with 8, 166 with 12.)
+  static constexpr bool kTwelve = !SPLIT && NB * NT == 8 && NB < 8;
+  static constexpr int kWarps = kTwelve ? 12 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kBlocks = NB <= 4 && NT * NB * (SPLIT ? 2 : 1) <= 8 && !kTwelve ? 2 : 1;
   static constexpr int kStages = 3;
   static constexpr int kStage = 2 * Gr::kBytes;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kOutStride = D + 4;                 // floats of one column in the join buffer
   static_assert(8 * kOutStride * 4 <= kStage, "a warp's sums for the join lie in one stage of its ring");
+  static constexpr int kSmem = kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + COLS * 8 + kWarps * COLS * 8 +
+                               kWarps * (static_cast<int>(sizeof(Cursor)) + 2 * static_cast<int>(sizeof(Segment)) + 4) +
+                               static_cast<int>(sizeof(Runs));
+  static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
-
-template <int NB, int NT, bool SPLIT>
-constexpr int smem_bytes() {
-  return Lay<NB>::kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + 8 * NT * 8 + kWarps * 8 * NT * 8 +
-         kWarps * (static_cast<int>(sizeof(Cursor)) + 2 * static_cast<int>(sizeof(Segment)) + 4) +
-         static_cast<int>(sizeof(Runs));
-}
 
 // x: one row's D values, lane i holding channels i, i + 32, ..
 template <int NB>
@@ -235,19 +239,13 @@ __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m
 __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
 // ---------------------------------------------------------------- main kernel
-// blocks of an SM: two where shared memory holds two rings and the accumulators leave the registers
 template <int NB, int NT, bool SPLIT>
-constexpr int blocks_per_sm() {
-  return NB <= 4 && NT <= 2 && !(SPLIT && NT * NB > 4) ? 2 : 1;
-}
-
-template <int NB, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_decode_kernel(const DecP p) {
-  using L = Lay<NB>;
-  using Gr = Fp4Group<NB>;
-  constexpr int D = L::D;
-  constexpr int MT = D / 16;
-  constexpr int COLS = 8 * NT;
+__global__ void __launch_bounds__(Shape<NB, NT, SPLIT>::kThreads, Shape<NB, NT, SPLIT>::kBlocks)
+fp4_decode_kernel(const DecP p) {
+  using L = Shape<NB, NT, SPLIT>;
+  using Gr = typename L::Gr;
+  constexpr int D = L::D, MT = D / 16, COLS = L::COLS;
+  constexpr int kWarps = L::kWarps, kThreads = L::kThreads;
   extern __shared__ __align__(128) char smem[];   // (no static shared memory: it would move the ring off its 128 bytes)
   char* q_frag = smem + L::kRing;                                   // [hi, lo][NT][NB][lane] 16 bytes
   float* col_scale = reinterpret_cast<float*>(q_frag + NT * NB * 512 * (SPLIT ? 2 : 1));
@@ -258,11 +256,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
   Segment* segment = reinterpret_cast<Segment*>(cursor + kWarps);                 // [warp][2]
   unsigned* join_at = reinterpret_cast<unsigned*>(segment + 2 * kWarps);          // [warp]: its stage for the join
   Runs& runs = *reinterpret_cast<Runs*>(join_at + kWarps);                        // kept by thread 0
-  // Groups of 16 keys that go through the products together: two, for the independent work, except where the
-  // accumulators then leave too few registers.  (32 sequences of 32k, D 128, 16 columns: 328 us with one and two blocks
-  // an SM, 354 with two and one block; 32 columns: 152 with two, 168 with one, 8 sequences.)
-  constexpr int U = NT == 2 && NB == 4 ? 1 : 2;
-
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
@@ -479,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
     }
 
     if (pending) {
-      // ------------------------------------------------------ join the 8 warps
+      // ------------------------------------------------------ join the warps
       // in the stage of each warp's ring that the next segment's copies leave free
       const unsigned my_join = warp * L::kStages * L::kStage + (stage == 0 ? L::kStages - 1 : stage - 1) * L::kStage;
       if (lane == 0) join_at[warp] = my_join;
@@ -600,165 +593,162 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm<NB, NT, SPLIT>()) fp4_
       const unsigned ok_here = (history >> (2 * (L::kStages - 1))) & 3;
       const bool full = ok_here == 3 && key0 + kTileKeys <= full_end;
 
-#pragma unroll 1
-      for (int v = 0; v < 2; v += U) {
-        // ---------------------------------------------------------- S' = K Q'
-        float s[U][NT][4];
-        {
-          unsigned kw[U][2][NB];
-          float ks[U][2 * NB];
+      // ---------------------------------------------------------- S' = K Q'
+      float s[2][NT][4];
+      {
+        unsigned kw[2][2][NB];
+        float ks[2][2 * NB];
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            read_words(at + (v + u) * Gr::kBytes, kw[u][0]);
-            read_words(at + (v + u) * Gr::kBytes + Gr::kSet, kw[u][1]);
-            unsigned ksw[NB / 2];
-            lds_words<NB / 2>(at + (v + u) * Gr::kBytes + Gr::kKs + g * 2 * NB, ksw);
+        for (int u = 0; u < 2; ++u) {
+          read_words(at + u * Gr::kBytes, kw[u][0]);
+          read_words(at + u * Gr::kBytes + Gr::kSet, kw[u][1]);
+          unsigned ksw[NB / 2];
+          lds_words<NB / 2>(at + u * Gr::kBytes + Gr::kKs + g * 2 * NB, ksw);
 #pragma unroll
-            for (int i = 0; i < NB / 2; ++i) scales4(ksw[i], &ks[u][4 * i]);
+          for (int i = 0; i < NB / 2; ++i) scales4(ksw[i], &ks[u][4 * i]);
+        }
+#pragma unroll
+        for (int bk = 0; bk < NB; ++bk) {
+          uint4 q_hi[NT], q_lo[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            q_hi[nt] = reinterpret_cast<const uint4*>(q_frag)[(nt * NB + bk) * 32 + lane];
+            if (SPLIT) q_lo[nt] = reinterpret_cast<const uint4*>(q_frag)[(NT * NB + nt * NB + bk) * 32 + lane];
           }
 #pragma unroll
-          for (int bk = 0; bk < NB; ++bk) {
-            uint4 q_hi[NT], q_lo[NT];
+          for (int u = 0; u < 2; ++u) {
+            unsigned r0[4], r1[4];
+            fp4_unpack4(kw[u][0][bk], r0);
+            fp4_unpack4(kw[u][1][bk], r1);
+            const float s0 = ks[u][bk], s1 = ks[u][NB + bk];   // of rows g and g + 8
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              q_hi[nt] = reinterpret_cast<const uint4*>(q_frag)[(nt * NB + bk) * 32 + lane];
-              if (SPLIT) q_lo[nt] = reinterpret_cast<const uint4*>(q_frag)[(NT * NB + nt * NB + bk) * 32 + lane];
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-              unsigned r0[4], r1[4];
-              fp4_unpack4(kw[u][0][bk], r0);
-              fp4_unpack4(kw[u][1][bk], r1);
-              const float s0 = ks[u][bk], s1 = ks[u][NB + bk];   // of rows g and g + 8
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                float acc[4];
-                mma16816_new(acc, r0[0], r1[0], r0[1], r1[1], q_hi[nt].x, q_hi[nt].y);
-                mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_hi[nt].z, q_hi[nt].w);
-                if (SPLIT) {
-                  mma16816(acc, r0[0], r1[0], r0[1], r1[1], q_lo[nt].x, q_lo[nt].y);
-                  mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_lo[nt].z, q_lo[nt].w);
-                }
-                if (bk == 0) {
-                  s[u][nt][0] = acc[0] * s0; s[u][nt][1] = acc[1] * s0;
-                  s[u][nt][2] = acc[2] * s1; s[u][nt][3] = acc[3] * s1;
-                } else {
-                  s[u][nt][0] = fmaf(acc[0], s0, s[u][nt][0]); s[u][nt][1] = fmaf(acc[1], s0, s[u][nt][1]);
-                  s[u][nt][2] = fmaf(acc[2], s1, s[u][nt][2]); s[u][nt][3] = fmaf(acc[3], s1, s[u][nt][3]);
-                }
+              float acc[4];
+              mma16816_new(acc, r0[0], r1[0], r0[1], r1[1], q_hi[nt].x, q_hi[nt].y);
+              mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_hi[nt].z, q_hi[nt].w);
+              if (SPLIT) {
+                mma16816(acc, r0[0], r1[0], r0[1], r1[1], q_lo[nt].x, q_lo[nt].y);
+                mma16816(acc, r0[2], r1[2], r0[3], r1[3], q_lo[nt].z, q_lo[nt].w);
+              }
+              if (bk == 0) {
+                s[u][nt][0] = acc[0] * s0; s[u][nt][1] = acc[1] * s0;
+                s[u][nt][2] = acc[2] * s1; s[u][nt][3] = acc[3] * s1;
+              } else {
+                s[u][nt][0] = fmaf(acc[0], s0, s[u][nt][0]); s[u][nt][1] = fmaf(acc[1], s0, s[u][nt][1]);
+                s[u][nt][2] = fmaf(acc[2], s1, s[u][nt][2]); s[u][nt][3] = fmaf(acc[3], s1, s[u][nt][3]);
               }
             }
           }
         }
-        if (!full) {
+      }
+      if (!full) {
 #pragma unroll
-          for (int u = 0; u < U; ++u) {
-            const bool ok = (ok_here >> (v + u)) & 1;
-            const int key = key0 + (v + u) * 16 + g;
+        for (int u = 0; u < 2; ++u) {
+          const bool ok = (ok_here >> u) & 1;
+          const int key = key0 + u * 16 + g;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+          for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const bool seen = ok && key + (i >> 1) * 8 < col_limit[nt * 8 + 2 * t + (i & 1)];
-                if (!seen) s[u][nt][i] = -INFINITY;
-              }
+            for (int i = 0; i < 4; ++i) {
+              const bool seen = ok && key + (i >> 1) * 8 < col_limit[nt * 8 + 2 * t + (i & 1)];
+              if (!seen) s[u][nt][i] = -INFINITY;
             }
           }
         }
+      }
 
-        // ---------------------------------------------------------- softmax
-        float mx[NT][2];
-        bool raise = false;
+      // ---------------------------------------------------------- softmax
+      float mx[NT][2];
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
+          mx[nt][e] = fmaxf(mx[nt][e], fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+          raise = raise || fmaf(mx[nt][e], sc[nt][e], -m_run[nt][e]) > kLazy;
+        }
+      }
+      if (__any_sync(~0u, raise)) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+          float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            mx[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
-            if (U == 2) mx[nt][e] = fmaxf(mx[nt][e], fmaxf(s[U - 1][nt][e], s[U - 1][nt][e + 2]));
-            raise = raise || fmaf(mx[nt][e], sc[nt][e], -m_run[nt][e]) > kLazy;
+            float v = mx[nt][e];
+            v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
+            v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
+            v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
+            const float m_new = fmaxf(m_run[nt][e], fmaf(v, sc[nt][e], -kHead));
+            f[e] = tc::ex2(m_run[nt][e] - m_new);
+            m_run[nt][e] = m_new;
+            l_run[nt][e] *= f[e];
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            o[nt][i][0] *= f[0]; o[nt][i][1] *= f[1];
+            o[nt][i][2] *= f[0]; o[nt][i][3] *= f[1];
           }
         }
-        if (__any_sync(~0u, raise)) {
+      }
+      unsigned pf[2][NT][2], pl[2][NT][2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float f[2];
+      for (int u = 0; u < 2; ++u) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float v = mx[nt][e];
-              v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
-              v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
-              v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
-              const float m_new = fmaxf(m_run[nt][e], fmaf(v, sc[nt][e], -kHead));
-              f[e] = tc::ex2(m_run[nt][e] - m_new);
-              m_run[nt][e] = m_new;
-              l_run[nt][e] *= f[e];
-            }
+        for (int nt = 0; nt < NT; ++nt) {
+          float x[4];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              o[nt][i][0] *= f[0]; o[nt][i][1] *= f[1];
-              o[nt][i][2] *= f[0]; o[nt][i][3] *= f[1];
-            }
+          for (int i = 0; i < 4; ++i) {
+            x[i] = tc::ex2(fmaf(s[u][nt][i], sc[nt][i & 1], -m_run[nt][i & 1]));
+            l_run[nt][i & 1] += x[i];
           }
-        }
-        unsigned pf[U][NT][2], pl[U][NT][2];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              x[i] = tc::ex2(fmaf(s[u][nt][i], sc[nt][i & 1], -m_run[nt][i & 1]));
-              l_run[nt][i & 1] += x[i];
-            }
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const unsigned hi = pack_half2(x[2 * r], x[2 * r + 1]);
-              pf[u][nt][r] = transpose8x8(hi);
-              if (SPLIT) {
-                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                pl[u][nt][r] = transpose8x8(pack_half2(x[2 * r] - back.x, x[2 * r + 1] - back.y));
-              }
+          for (int r = 0; r < 2; ++r) {
+            const unsigned hi = pack_half2(x[2 * r], x[2 * r + 1]);
+            pf[u][nt][r] = transpose8x8(hi);
+            if (SPLIT) {
+              const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+              pl[u][nt][r] = transpose8x8(pack_half2(x[2 * r] - back.x, x[2 * r + 1] - back.y));
             }
           }
         }
+      }
 
-        // ---------------------------------------------------------- O' += V' P'
+      // ---------------------------------------------------------- O' += V' P'
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          unsigned vw[2][NB];
-          read_words(at + (v + u) * Gr::kBytes + Gr::kV, vw[0]);
-          read_words(at + (v + u) * Gr::kBytes + Gr::kV + Gr::kSet, vw[1]);
-          // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the lane's channels' block
-          unsigned vs = lds32(at + (v + u) * Gr::kBytes + Gr::kVs + (g * NB / 8) * 16 + t * 4);
-          if (!full) {          // rows behind the sequence or without a page hold anything: scale 0 keeps NaN away
-            const int key = key0 + (v + u) * 16 + 2 * t;
+      for (int u = 0; u < 2; ++u) {
+        unsigned vw[2][NB];
+        read_words(at + u * Gr::kBytes + Gr::kV, vw[0]);
+        read_words(at + u * Gr::kBytes + Gr::kV + Gr::kSet, vw[1]);
+        // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the lane's channels' block
+        unsigned vs = lds32(at + u * Gr::kBytes + Gr::kVs + (g * NB / 8) * 16 + t * 4);
+        if (!full) {          // rows behind the sequence or without a page hold anything: scale 0 keeps NaN away
+          const int key = key0 + u * 16 + 2 * t;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if (!((ok_here >> (v + u)) & 1) || key + (i & 1) + 8 * (i >> 1) >= full_end + p.M - 1) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
-            }
+          for (int i = 0; i < 4; ++i) {
+            if (!((ok_here >> u) & 1) || key + (i & 1) + 8 * (i >> 1) >= full_end + p.M - 1) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
           }
-          // byte e + 127 -> half 2^e: (byte - 112) << 10 in both halves at once
-          const unsigned v01 = __byte_perm(vs, 0, 0x4140) * 1024u - 112u * 1024u * 65537u;
-          const unsigned v23 = __byte_perm(vs, 0, 0x4342) * 1024u - 112u * 1024u * 65537u;
+        }
+        // byte e + 127 -> half 2^e: (byte - 112) << 10 in both halves at once
+        const unsigned v01 = __byte_perm(vs, 0, 0x4140) * 1024u - 112u * 1024u * 65537u;
+        const unsigned v23 = __byte_perm(vs, 0, 0x4342) * 1024u - 112u * 1024u * 65537u;
 #pragma unroll
-          for (int j = 0; j < NB; ++j) {
-            unsigned r0[4], r1[4];
-            fp4_unpack4(vw[0][j], r0);
-            fp4_unpack4(vw[1][j], r1);
+        for (int j = 0; j < NB; ++j) {
+          unsigned r0[4], r1[4];
+          fp4_unpack4(vw[0][j], r0);
+          fp4_unpack4(vw[1][j], r1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              r0[i] = mul_half2(r0[i], v01);
-              r1[i] = mul_half2(r1[i], v23);
-            }
+          for (int i = 0; i < 4; ++i) {
+            r0[i] = mul_half2(r0[i], v01);
+            r1[i] = mul_half2(r1[i], v23);
+          }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pf[u][nt][0], pf[u][nt][1]);
-              mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pf[u][nt][0], pf[u][nt][1]);
-              if (SPLIT) {
-                mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pl[u][nt][0], pl[u][nt][1]);
-                mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pl[u][nt][0], pl[u][nt][1]);
-              }
+          for (int nt = 0; nt < NT; ++nt) {
+            mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pf[u][nt][0], pf[u][nt][1]);
+            mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pf[u][nt][0], pf[u][nt][1]);
+            if (SPLIT) {
+              mma16816(o[nt][2 * j], r0[0], r0[1], r1[0], r1[1], pl[u][nt][0], pl[u][nt][1]);
+              mma16816(o[nt][2 * j + 1], r0[2], r0[3], r1[2], r1[3], pl[u][nt][0], pl[u][nt][1]);
             }
           }
         }
@@ -870,11 +860,11 @@ int resident_blocks(int* blocks) {
   std::lock_guard<std::mutex> lock(mu);
   if (dev < 0 || dev >= 64 || cache[dev] == 0) {
     auto kern = fp4_decode_kernel<NB, NT, SPLIT>;
-    const int smem = smem_bytes<NB, NT, SPLIT>();
+    const int smem = Shape<NB, NT, SPLIT>::kSmem;
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return check_cuda(e, "fp4_decode shared memory");
     int per_sm = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, kThreads, smem);
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, Shape<NB, NT, SPLIT>::kThreads, smem);
     if (e != cudaSuccess) return check_cuda(e, "fp4_decode occupancy");
     if (per_sm < 1) return fail(IAK_ERR_UNSUPPORTED, "fp4_decode does not fit on an SM");
     if (dev < 0 || dev >= 64) { *blocks = per_sm * device_sm_count(); return IAK_OK; }
@@ -890,6 +880,7 @@ int make_plan(DecP& p, Plan* plan) {
   const int64_t hc = static_cast<int64_t>(p.Ht) * p.CG, units = hc * p.B;
   if (units * 8 * NT > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: too many rows for one launch");
   p.HC = static_cast<int>(hc);
+  constexpr int kWarps = Shape<NB, NT, SPLIT>::kWarps;
   p.min_tiles = kWarps;
   const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + kTileKeys - 1) / kTileKeys;
   // a unit that one tile per warp covers is one block's work: no joining
@@ -921,7 +912,7 @@ int run_shape(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cud
   if (plan.ws > ws_bytes || (plan.ws && !ws))
     return fail(IAK_ERR_WORKSPACE, "iak_fp4_decode needs %zu workspace bytes, got %zu", plan.ws, ws_bytes);
   p.ws = static_cast<float*>(ws);
-  fp4_decode_kernel<NB, NT, SPLIT><<<plan.grid, kThreads, smem_bytes<NB, NT, SPLIT>(), s>>>(p);
+  fp4_decode_kernel<NB, NT, SPLIT><<<plan.grid, Shape<NB, NT, SPLIT>::kThreads, Shape<NB, NT, SPLIT>::kSmem, s>>>(p);
   if (int st = check_cuda(cudaGetLastError(), "fp4_decode launch")) return st;
   if (plan.grid == 1 || plan.direct) return IAK_OK;
   cudaLaunchConfig_t cfg = {};
