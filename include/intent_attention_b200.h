@@ -606,8 +606,10 @@ int iak_fp4_read(const iak_fp4_pool* pool, const iak_fp4_rows_args* args, void* 
  *     x = softmax(sm_scale q1 K1') V - lam[head] softmax(sm_scale q2 K2') V,
  *     out = out_scale * x, and with norm_weight (float [D])
  *     out = out_scale * norm_weight * x / sqrt(mean(x^2) + eps).
- * Scores, softmax statistics and sums are fp32; half / bf16 queries multiply
- * as halves (exact after a power of two per row), fp32 ones as two halves.
+ * Scores, softmax statistics and sums are fp32.  Half / bf16 queries multiply
+ * as halves after a power of two that puts the row's largest in [1, 2) (exact
+ * for elements down to 2^-14 of it), fp32 ones as the sum of two halves;
+ * probabilities round to halves (fp32 queries: to two).
  * The workspace holds partial sums; its content need not survive the call. */
 typedef struct iak_fp4_decode_args {
   const void* q; int32_t q_dtype; int64_t q_stride_b, q_stride_h, q_stride_m;
@@ -660,6 +662,10 @@ int iak_pages_workspace_size(const iak_seq_pages* pages, size_t* bytes);
  * that gets tokens. */
 int iak_pages_grow(const iak_seq_pages* pages, const iak_page_planes* planes, const int32_t* new_tokens,
                    int32_t* rejected, void* workspace, size_t workspace_bytes, void* stream);
+/* takes tokens[s] tokens off the end of every slot (draft tokens that were not
+ * kept); pages that hold none of its tokens any more are let go of.  Refused:
+ * a negative count, more tokens than the slot holds. */
+int iak_pages_shrink(const iak_seq_pages* pages, const int32_t* tokens, int32_t* rejected, void* stream);
 /* dst[i] becomes a sequence that shares all of src[i]'s pages.  Refused: a
  * slot out of range, a dst that holds tokens, a dst listed before, a src that
  * is also a dst of the call. */

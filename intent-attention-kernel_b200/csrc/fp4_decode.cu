@@ -226,7 +226,8 @@ __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m
       for (int i = 0; i < NB; ++i) sq = fmaf(x[i], x[i], sq);
 #pragma unroll
       for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
-      mul *= rsqrtf(sq * (1.f / (NB * 32)) + p.eps);
+      const float ms = sq * (1.f / (NB * 32)) + p.eps;
+      mul = ms > 0.f || ms != ms ? mul * rsqrtf(ms) : 0.f;   // (a row of zeros stays zero with eps 0)
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) x[i] *= p.norm_w ? mul * p.norm_w[i * 32 + lane] : mul;

@@ -1,4 +1,4 @@
-// Page operations of a paged cache: grow (allocate, copy-on-write), fork, free, compact.
+// Page operations of a paged cache: grow (allocate, copy-on-write), shrink, fork, free, compact.
 //
 // A page is free when no table entry holds it (refs 0), so freeing only counts down and needs no order, and the pages
 // to hand out are the lowest free ones: the k-th free page goes to the k-th page wanted, whatever order blocks run in.
@@ -346,6 +346,26 @@ free_kernel(const Seq q, const int32_t* slots, int n, int32_t* rejected) {
   if (rank == 0 && threadIdx.x == 0) q.lengths[s] = 0;
 }
 
+// A block per slot: its threads read the length before one of them writes it.
+__global__ void __launch_bounds__(kActThreads) shrink_kernel(const Seq q, const int32_t* tokens, int32_t* rejected) {
+  const int s = blockIdx.x, off = tokens[s], len = max(q.lengths[s], 0);
+  if (off == 0) return;
+  __syncthreads();
+  if (off < 0 || off > len) {
+    if (rejected && threadIdx.x == 0) atomicAdd(rejected, 1);
+    return;
+  }
+  const int from = min(pages_of(len - off, q.PS), q.W), n = min(pages_of(len, q.PS), q.W) - from;
+  for (int64_t e = threadIdx.x; e < static_cast<int64_t>(q.Ht) * n; e += kActThreads) {
+    const int h = static_cast<int>(e / n), w = from + static_cast<int>(e - static_cast<int64_t>(h) * n);
+    int32_t* at = q.table + s * q.sb + h * q.sh + w;
+    const int id = *at;
+    *at = -1;
+    if (in_pool(q, id)) atomicSub(&q.refs[id], 1);
+  }
+  if (threadIdx.x == 0) q.lengths[s] = len - off;
+}
+
 // --------------------------------------------------------------------- compact
 // Scratch: head[0] = pages in use n, head[1] = pages to move; from[k] and to[k] of move k; rank_of[page] of the pages
 // that move.
@@ -554,6 +574,16 @@ extern "C" int iak_pages_free(const iak_seq_pages* pages, const int32_t* slots, 
   if (!slots) return fail(IAK_ERR_INVALID_ARG, "%s: null slots", what);
   free_kernel<<<count * kCluster, kListThreads, 0, static_cast<cudaStream_t>(stream)>>>(q, slots, count, rejected);
   return check_cuda(cudaGetLastError(), "free launch");
+}
+
+extern "C" int iak_pages_shrink(const iak_seq_pages* pages, const int32_t* tokens, int32_t* rejected, void* stream) {
+  const char* what = "iak_pages_shrink";
+  Seq q;
+  if (int st = check_seq(pages, what, &q)) return st;
+  if (q.S == 0) return IAK_OK;
+  if (!tokens) return fail(IAK_ERR_INVALID_ARG, "%s: null tokens", what);
+  shrink_kernel<<<q.S, kActThreads, 0, static_cast<cudaStream_t>(stream)>>>(q, tokens, rejected);
+  return check_cuda(cudaGetLastError(), "shrink launch");
 }
 
 extern "C" int iak_pages_compact(const iak_seq_pages* pages, const iak_page_planes* planes, int32_t* num_live,

@@ -45,7 +45,14 @@ from .triton_adaptive_format_attention import (
 )
 from .paged import KVStage, PagePool, append_tokens, convert_pages, merge_partials, pack_metadata, paged_decode
 from .fp4_cache import Fp4Pool, append_fp4, differential_decode_fp4, paged_decode_fp4, read_fp4
-from .sequence_pages import SequencePages, compact_pages, fork_sequences, free_sequences, grow_sequences
+from .sequence_pages import (
+    SequencePages,
+    compact_pages,
+    fork_sequences,
+    free_sequences,
+    grow_sequences,
+    shrink_sequences,
+)
 from .device_router import LayoutBatch, RoutedPages, encode_layouts, route_layouts, route_pages
 from .split_kv import (
     SequenceShardedDecoder,
@@ -68,7 +75,7 @@ __all__ = [
     "make_adaptive_page_tables",
     "PagePool", "merge_partials", "pack_metadata", "paged_decode", "KVStage", "append_tokens", "convert_pages",
     "Fp4Pool", "append_fp4", "read_fp4", "paged_decode_fp4", "differential_decode_fp4",
-    "SequencePages", "grow_sequences", "fork_sequences", "free_sequences", "compact_pages",
+    "SequencePages", "grow_sequences", "shrink_sequences", "fork_sequences", "free_sequences", "compact_pages",
     "LayoutBatch", "RoutedPages", "encode_layouts", "route_layouts", "route_pages",
     "SequenceShardedDecoder", "decode_partial_block", "merge_partial_blocks", "shard_bounds", "shard_page_lists",
 ]

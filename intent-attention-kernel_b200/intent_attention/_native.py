@@ -241,6 +241,7 @@ SIGNATURES = {
     "iak_pages_workspace_size": (ctypes.c_int, [ctypes.POINTER(SeqPages), ctypes.POINTER(ctypes.c_size_t)]),
     "iak_pages_grow": (ctypes.c_int, [ctypes.POINTER(SeqPages), ctypes.POINTER(PagePlanes), c_void_p, c_void_p,
                                       c_void_p, ctypes.c_size_t, c_void_p]),
+    "iak_pages_shrink": (ctypes.c_int, [ctypes.POINTER(SeqPages), c_void_p, c_void_p, c_void_p]),
     "iak_pages_fork": (ctypes.c_int, [ctypes.POINTER(SeqPages), c_void_p, c_void_p, c_i32, c_void_p, c_void_p]),
     "iak_pages_free": (ctypes.c_int, [ctypes.POINTER(SeqPages), c_void_p, c_i32, c_void_p, c_void_p]),
     "iak_pages_compact": (ctypes.c_int, [ctypes.POINTER(SeqPages), ctypes.POINTER(PagePlanes), c_void_p, c_void_p,

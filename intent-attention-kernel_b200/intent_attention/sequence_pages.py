@@ -1,4 +1,4 @@
-"""Which sequences hold which pages of a pool: grow, fork, free and compact.
+"""Which sequences hold which pages of a pool: grow, shrink, fork, free and compact.
 
 ``SequencePages`` is the bookkeeping of one layer's pages on the GPU: a count of
 holders per page (0 = free), the page table of every slot and table head, and
@@ -128,6 +128,20 @@ def grow_sequences(pool: Union[PagePool, Fp4Pool], pages: SequencePages, new_tok
         ws = _workspace(pages.refs.device, s)
         N.check(N.lib().iak_pages_grow(ctypes.byref(s), ctypes.byref(pl), more, count, ws.data_ptr(), ws.numel(),
                                        _raw_stream(dev)), "iak_pages_grow")
+
+
+def shrink_sequences(pages: SequencePages, tokens: torch.Tensor, rejected: Optional[torch.Tensor] = None) -> None:
+    """Take ``tokens[s]`` (int32 [slots]) tokens off the end of every slot, as when draft tokens are not kept; pages
+    that are left without a token of the slot are let go of.  Refused: a negative count, more than the slot holds.
+
+    Lengths must not be lowered in any other way: the pages left behind would never be free again.
+    """
+    s = pages.struct()
+    dev = pages.refs.get_device()
+    a = _index_tensor(tokens, "tokens", dev, s.num_slots)
+    count = _index_tensor(rejected, "rejected", dev, 1)
+    with _on(dev):
+        N.check(N.lib().iak_pages_shrink(ctypes.byref(s), a, count, _raw_stream(dev)), "iak_pages_shrink")
 
 
 def fork_sequences(pages: SequencePages, src: torch.Tensor, dst: torch.Tensor,

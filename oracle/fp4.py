@@ -93,6 +93,21 @@ class Pages:
                 self.table[s, h, w] = p
             self.lengths[s] = ln + n
 
+    def shrink(self, tokens):
+        for s, n in enumerate(tokens):
+            n, ln = int(n), max(int(self.lengths[s]), 0)
+            if n == 0:
+                continue
+            if n < 0 or n > ln:
+                self.rejected += 1
+                continue
+            a, b = -(-(ln - n) // self.ps), self.held(s)
+            for p in self.table[s, :, a:b].ravel():
+                if 0 <= p < len(self.refs):
+                    self.refs[p] -= 1
+            self.table[s, :, a:b] = -1
+            self.lengths[s] = ln - n
+
     def fork(self, src, dst):
         S, P = len(self.lengths), len(self.refs)
         lengths = self.lengths.copy()

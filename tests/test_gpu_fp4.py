@@ -351,6 +351,51 @@ def test_nan_query_gives_nan_in_its_rows_only():
     assert torch.equal(got[keep], clean[keep])
 
 
+def test_differential_row_of_zeros_stays_zero():
+    """No token seen, or the maps cancel: 0 for every eps, eps 0 included."""
+    ia = _ia()
+    pool, table, kd, vd = _cache(2, 2, 1, 64, 16, [5, 5])
+    q = torch.zeros(2, 4, 64, device="cuda")
+    lam, w = torch.ones(4, device="cuda"), torch.ones(64, device="cuda")
+    for eps in (0.0, 1e-5):
+        got = ia.differential_decode_fp4(q, pool, table, _i32([0, 5]), lam, norm_weight=w, eps=eps)
+        assert (got[0] == 0).all() and torch.isfinite(got).all()
+
+
+def test_first_call_captured():
+    """The very first call of a process, captured: nothing that a capture forbids happens in a call."""
+    import subprocess
+    import sys
+    code = """
+import sys, torch
+sys.path.insert(0, "intent-attention-kernel_b200")
+import intent_attention as ia
+pool = ia.Fp4Pool.allocate(64, 16, 128, zero=True)
+table = torch.arange(64, dtype=torch.int32, device="cuda").view(1, 1, 64)
+n = torch.tensor([900], dtype=torch.int32, device="cuda")
+k = torch.randn(1, 1, 900, 128, device="cuda").half()
+q = torch.randn(1, 4, 128, device="cuda").half()
+lam = torch.full((4,), 0.5, device="cuda")
+refs = torch.ones(64, dtype=torch.int32, device="cuda")
+pages = ia.SequencePages(refs, table, n, 16)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ia.append_fp4(pool, k, k, table)
+    a = ia.paged_decode_fp4(q, pool, table, n)
+    d = ia.differential_decode_fp4(q, pool, table, n, lam)
+    r = ia.read_fp4(pool, table, None, 900)
+    c = ia.compact_pages(pool, pages)
+g.replay()
+torch.cuda.synchronize()
+assert torch.equal(a, ia.paged_decode_fp4(q, pool, table, n)) and torch.equal(d, ia.differential_decode_fp4(q, pool, table, n, lam))
+assert int(c) == 64 and bool(torch.isfinite(a).all()) and bool((a != 0).any())
+"""
+    root = __file__.rsplit("/tests/", 1)[0]
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
 def test_lengths_beyond_the_table_and_negative():
     ia = _ia()
     pool, table, kd, vd = _cache(2, 3, 1, 64, 16, [64, 64, 64])

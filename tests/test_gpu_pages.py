@@ -135,6 +135,27 @@ def test_fork_of_a_destination_is_refused():
     assert pages.lengths.tolist() == [40, 40, 0, 0]
 
 
+@pytest.mark.parametrize("S,Ht,W", [(5, 1, 3), (40, 8, 30)])
+def test_shrink(S, Ht, W):
+    """Draft tokens given back: pages without a token go, shared ones count down, and growing again copies an open
+    page that others hold."""
+    g = np.random.default_rng(S)
+    lengths = g.integers(0, W * 16 + 1, S).tolist()
+    pool, pages, want = _state(S, 4 * S * Ht * W + 5, 16, S, Ht, W, lengths, share=0.4)
+    off = np.minimum(g.integers(0, W * 16, S), lengths)
+    off[0], off[1], off[2] = lengths[0], lengths[1] + 1, -1
+    r = _counter()
+    _ia().shrink_sequences(pages, _i32(off), rejected=r)
+    want.shrink(off)
+    _same(pool, pages, want)
+    assert int(r) == want.rejected == 2 and int(pages.lengths[0]) == 0
+    more = g.integers(0, 3, S)
+    _ia().grow_sequences(pool, pages, _i32(more), rejected=r)
+    want.grow(more)
+    _same(pool, pages, want)
+    assert int(r) == want.rejected
+
+
 @pytest.mark.parametrize("P,S,Ht,W", [(64, 3, 1, 4), (8192, 16, 4, 20), (70001, 32, 8, 100), (1, 1, 1, 1)])
 def test_compact(P, S, Ht, W):
     g = np.random.default_rng(P)
@@ -246,6 +267,11 @@ def test_serving_run():
     for _ in range(3):
         write([1, 1, 1, 0, 0, 0])
     check()
+    write([4, 4, 4, 0, 0, 0])                     # draft tokens, most of them not kept
+    ia.shrink_sequences(pages, _i32([3, 4, 1, 0, 0, 0]))
+    for s, n in enumerate((3, 4, 1)):
+        held[s] = tuple(x[:, :x.shape[1] - n] for x in held[s])
+    check()
     ia.fork_sequences(pages, _i32([0, 0, 1]), _i32([3, 4, 5]))
     held[3], held[4], held[5] = held[0], held[0], held[1]
     check()
@@ -267,6 +293,7 @@ def test_page_refusals():
     other = ia.SequencePages.allocate(31, 16, 2, 1, 4)
     bad = [
         lambda: ia.grow_sequences(pool, pages, _i32([1])),
+        lambda: ia.shrink_sequences(pages, _i32([1])),
         lambda: ia.grow_sequences(pool, pages, ok.long()),
         lambda: ia.grow_sequences(pool, other, ok),
         lambda: ia.compact_pages(pool, ia.SequencePages.allocate(32, 8, 2, 1, 4)),
