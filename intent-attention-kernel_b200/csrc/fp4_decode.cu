@@ -30,6 +30,9 @@ namespace {
 
 constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
+constexpr int kMinTiles = 2;       // of a run
+constexpr int kDirectTiles = 8;    // units of at most so many tiles are never cut
+constexpr int kManyParts = 12;     // of a unit, from which on a block joins them instead of a warp
 constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
 constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small P stay normal halves
 
@@ -48,10 +51,12 @@ struct DecP {
   int NC;                            // softmax columns of a table head
   int CG;                            // column groups of 8 * NT
   int HC;                            // units of a sequence: Ht * CG
-  int grid;                          // blocks of the main kernel
-  int direct;                        // one block per unit, nothing to join
+  int cols;                          // columns of a unit's partials: min(8 * NT, NC)
+  int q_vec, o_vec;                  // 16-byte accesses to q (out) are aligned
+  int runs;                          // warps of the main kernel
+  int direct;                        // a warp per unit, nothing to join
   int by_unit;                       // cuts are recorded per unit, not per border
-  int min_tiles;                     // tiles a block takes at least
+  int min_tiles;                     // tiles a warp takes at least
   float* ws;
 };
 
@@ -97,27 +102,32 @@ __device__ __forceinline__ int total_tiles(const DecP& p, const Lane32& first) {
   return sum;
 }
 
-// The tiles in equal runs: `used` blocks, the first `more` of them with each + 1 tiles.
+// The tiles in equal runs, one for each of `used` warps, the first `more` of them with each + 1 tiles.
 struct Runs { int used, each, more; };
 __device__ __forceinline__ Runs make_runs(const DecP& p, int total) {
   Runs r;
-  r.used = static_cast<int>(min((static_cast<unsigned>(total) + p.min_tiles - 1) / p.min_tiles, static_cast<unsigned>(p.grid)));
+  r.used = static_cast<int>(min((static_cast<unsigned>(total) + p.min_tiles - 1) / p.min_tiles, static_cast<unsigned>(p.runs)));
   r.each = total / r.used;
   r.more = total - r.each * r.used;
   return r;
 }
 __device__ __forceinline__ int run_begin(const Runs& r, int i) { return i * r.each + min(i, r.more); }
-__device__ __forceinline__ int block_of(const Runs& r, int t) {
+__device__ __forceinline__ int run_of(const Runs& r, int t) {
   const int large = r.more * (r.each + 1);
   return t < large ? t / (r.each + 1) : r.more + (t - large) / r.each;
 }
 
-// What the join kernel reads of a unit cut over several blocks.  Where there are no more units than blocks a record per
-// unit, written by the block that has its first tile; else one per border between two blocks, written by the block
-// that the border begins and empty unless it is a unit's first cut.
-struct Cut { int b, h, j0, first, which, last; };   // first, last: blocks with a part; which: first's; last < 0: none
-__device__ __forceinline__ Cut* cuts(const DecP& p, int cols) {
-  return reinterpret_cast<Cut*>(p.ws + static_cast<size_t>(p.grid) * 2 * cols * (p.pool.D + 2));
+// A run leaves at most two parts of units: [0] of the unit that it begins in, [1] of the one that it ends in.  A part
+// is D sums, the maximum and the sum of the weights for each column.
+__device__ __forceinline__ float* part_at(const DecP& p, int run, int which, int col) {
+  return p.ws + ((static_cast<int64_t>(run) * 2 + which) * p.cols + col) * (p.pool.D + 4);
+}
+// What the join kernel reads of a unit cut over several runs.  Where there are no more units than runs a record per
+// unit, written by the run that has its first tile; else one per border between two runs, written by the run that the
+// border begins and empty unless it is a unit's first cut.
+struct Cut { int b, h, j0, first, which, last; };   // first, last: runs with a part; which: first's; last < 0: none
+__device__ __forceinline__ Cut* cuts(const DecP& p) {
+  return reinterpret_cast<Cut*>(p.ws + static_cast<int64_t>(p.runs) * 2 * p.cols * (p.pool.D + 4));
 }
 
 // ---------------------------------------------------------------------- PTX
@@ -187,32 +197,38 @@ __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
 }
 
 // ------------------------------------------------------------- shared layout
-struct Cursor { int left, off, at, b, len; };   // tiles left to the block; the next one, of sequence b and of all
+struct Cursor { int left, off, at, b, len; };   // tiles left to the run; the next one, of sequence b and of all
 struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, at; };   // at: its first tile, of all
 
-// What a kernel for D = 32 NB, 8 NT columns a block and (SPLIT) fp32 queries is made of.
+// What a kernel for D = 32 NB, 8 NT columns a unit and (SPLIT) fp32 queries is made of.  Warps work alone; a block has
+// four so that an SM's share can be cut finely.
 template <int NB, int NT, bool SPLIT>
 struct Shape {
   using Gr = Fp4Group<NB>;
   static constexpr int D = NB * 32, COLS = 8 * NT;
-  // Warps of a block and blocks of an SM: 16 warps with 128 registers each while the accumulators are small, 12 with
-  // 168, 8 with 255.  A tile's two groups of 16 keys go through the products together, for the independent work.
-  // (8 sequences of 32k, D 128, 16 columns: 95 us with 16 warps and one group at a time, 108 with 8, 86 with 12;
-  // 32 columns: 159 with 8, 203 with 12.  D 64, 32 columns: 172 with 8, 166 with 12.)
-  static constexpr bool kTwelve = !SPLIT && NB * NT == 8 && NB < 8;
-  static constexpr int kWarps = kTwelve ? 12 : 8;
+  static constexpr int kWarps = 4;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kBlocks = NB <= 4 && NT * NB * (SPLIT ? 2 : 1) <= 8 && !kTwelve ? 2 : 1;
-  static constexpr int kStages = 3;
+  // Warps of an SM: 16 with 128 registers each while the accumulators are small, 12 with 168, 8 with 255.  A tile's two
+  // groups of 16 keys go through the products together, for the independent work.
+  static constexpr int kSize = NB * NT * (SPLIT ? 2 : 1);
+  static constexpr int kPerSm = kSize <= 4 && NB == 2 ? 16 : (kSize <= 8 && NB < 8 ? 12 : 8);
+  static constexpr int kBlocks = kPerSm / kWarps;
+  static constexpr int kStages = NB == 8 ? 2 : 3;
   static constexpr int kStage = 2 * Gr::kBytes;
-  static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kOutStride = D + 4;                 // floats of one column in the join buffer
-  static_assert(8 * kOutStride * 4 <= kStage, "a warp's sums for the join lie in one stage of its ring");
-  static constexpr int kSmem = kRing + NT * NB * 512 * (SPLIT ? 2 : 1) + COLS * 8 + kWarps * COLS * 8 +
-                               kWarps * (static_cast<int>(sizeof(Cursor)) + 2 * static_cast<int>(sizeof(Segment)) + 4) +
-                               static_cast<int>(sizeof(Runs));
+  static constexpr int kRing = kStages * kStage;
+  static constexpr int kQuery = NT * NB * 512 * (SPLIT ? 2 : 1);
+  static constexpr int kWarpBytes = kRing + kQuery;        // a multiple of 128
+  static constexpr int kSmem = kWarps * (kWarpBytes + static_cast<int>(sizeof(Cursor)) + static_cast<int>(sizeof(Segment)));
+  static_assert(kWarpBytes % 128 == 0, "copies and reads are linear runs of 128 bytes");
   static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
+
+// 1 / sqrt(mean square + eps) of a row with sum of squares sq (a row of zeros stays zero with eps 0)
+template <int NB>
+__device__ __forceinline__ float norm_factor(const DecP& p, float sq) {
+  const float ms = sq * (1.f / (NB * 32)) + p.eps;
+  return ms > 0.f || ms != ms ? rsqrtf(ms) : 0.f;
+}
 
 // x: one row's D values, lane i holding channels i, i + 32, ..
 template <int NB>
@@ -226,8 +242,7 @@ __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m
       for (int i = 0; i < NB; ++i) sq = fmaf(x[i], x[i], sq);
 #pragma unroll
       for (int o = 16; o; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
-      const float ms = sq * (1.f / (NB * 32)) + p.eps;
-      mul = ms > 0.f || ms != ms ? mul * rsqrtf(ms) : 0.f;   // (a row of zeros stays zero with eps 0)
+      mul *= norm_factor<NB>(p, sq);
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i) x[i] *= p.norm_w ? mul * p.norm_w[i * 32 + lane] : mul;
@@ -239,48 +254,67 @@ __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m
 
 __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
+// x: N neighbouring values of an output row, from element `at` on
+template <int N>
+__device__ __forceinline__ void store_run(const DecP& p, int64_t at, const float (&x)[N]) {
+  if (!p.o_vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) store_from_float(p.out, p.out_dtype, at + i, x[i]);
+  } else if (p.out_dtype == IAK_DT_F32) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+      unsigned u[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (p.out_dtype == IAK_DT_F16) {
+          u[k] = pack_half2(x[i + 2 * k], x[i + 2 * k + 1]);
+        } else {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(x[i + 2 * k], x[i + 2 * k + 1]);
+          u[k] = *reinterpret_cast<const unsigned*>(&v);
+        }
+      }
+      *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + i) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- main kernel
 template <int NB, int NT, bool SPLIT>
 __global__ void __launch_bounds__(Shape<NB, NT, SPLIT>::kThreads, Shape<NB, NT, SPLIT>::kBlocks)
 fp4_decode_kernel(const DecP p) {
   using L = Shape<NB, NT, SPLIT>;
   using Gr = typename L::Gr;
-  constexpr int D = L::D, MT = D / 16, COLS = L::COLS;
-  constexpr int kWarps = L::kWarps, kThreads = L::kThreads;
-  extern __shared__ __align__(128) char smem[];   // (no static shared memory: it would move the ring off its 128 bytes)
-  char* q_frag = smem + L::kRing;                                   // [hi, lo][NT][NB][lane] 16 bytes
-  float* col_scale = reinterpret_cast<float*>(q_frag + NT * NB * 512 * (SPLIT ? 2 : 1));
-  int* col_limit = reinterpret_cast<int*>(col_scale + COLS);
-  float* warp_m = reinterpret_cast<float*>(col_limit + COLS);      // [warp][COLS]
-  float* warp_l = warp_m + kWarps * COLS;
-  Cursor* cursor = reinterpret_cast<Cursor*>(warp_l + kWarps * COLS);              // [warp]
-  Segment* segment = reinterpret_cast<Segment*>(cursor + kWarps);                 // [warp][2]
-  unsigned* join_at = reinterpret_cast<unsigned*>(segment + 2 * kWarps);          // [warp]: its stage for the join
-  Runs& runs = *reinterpret_cast<Runs*>(join_at + kWarps);                        // kept by thread 0
-
+  constexpr int D = L::D, MT = D / 16, COLS = L::COLS, kWarps = L::kWarps;
+  extern __shared__ __align__(128) char smem[];   // (no static shared memory: it would move the rings off their 128 bytes)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const unsigned smem_base = static_cast<unsigned>(__cvta_generic_to_shared(smem));
-  const unsigned ring = smem_base + warp * L::kStages * L::kStage;
+  const int run = blockIdx.x * kWarps + warp;
+  char* const q_frag = smem + warp * L::kWarpBytes + L::kRing;      // [hi, lo][NT][NB][lane] 16 bytes
+  Cursor& cursor = reinterpret_cast<Cursor*>(smem + kWarps * L::kWarpBytes)[warp];
+  Segment& segment = reinterpret_cast<Segment*>(smem + kWarps * (L::kWarpBytes + sizeof(Cursor)))[warp];
+  const unsigned ring = static_cast<unsigned>(__cvta_generic_to_shared(smem)) + warp * L::kWarpBytes;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ------------------------------------------------------------- segments
-  // A segment is the block's run of one unit's tiles.  What only a segment's ends need lies in shared memory, a copy for
-  // each warp: [0] the segment whose copies run, [1] the one before it.
-  int n_mine = 0;                                 // the warp's tiles of the segment
-  int stage = 0;
+  // A segment is the run's share of one unit's tiles.  What only its ends need lies in shared memory.
+  Runs runs = {};
   {
     Cursor cur = {};
     if (p.direct) {
-      cur.b = blockIdx.x / p.HC;
+      cur.b = run / p.HC;
+      if (cur.b >= p.B) return;
       cur.len = seq_len(p, cur.b);
       cur.left = tiles_of(p, cur.len);
-      cur.off = (blockIdx.x - cur.b * p.HC) * cur.left;
+      cur.off = (run - cur.b * p.HC) * cur.left;
     } else {
       Lane32 s = scan32(p, 0);
-      const Runs r = make_runs(p, total_tiles(p, s));
-      if (blockIdx.x >= r.used) return;
-      cur.at = run_begin(r, blockIdx.x);
-      cur.left = run_begin(r, blockIdx.x + 1) - cur.at;
+      runs = make_runs(p, total_tiles(p, s));
+      if (run >= runs.used) return;
+      cur.at = run_begin(runs, run);
+      cur.left = run_begin(runs, run + 1) - cur.at;
       // the sequence that holds tile cur.at
       int before = 0;
       for (int base = 0; base < p.B; base += 32) {
@@ -295,125 +329,26 @@ fp4_decode_kernel(const DecP p) {
         }
         before += __shfl_sync(~0u, s.upto, 31);
       }
-      if (threadIdx.x == 0) runs = r;
     }
-    if (lane == 0) cursor[warp] = cur;
+    if (lane == 0) cursor = cur;
     __syncwarp();
   }
-  // false: no segment is left
-  auto open_segment = [&]() {
-    Cursor cur = cursor[warp];
-    if (cur.left <= 0 || cur.b >= p.B) return false;
-    Segment sg;
-    sg.b = cur.b;
-    sg.len = cur.len;
-    sg.n_tiles = tiles_of(p, cur.len);
-    sg.at = cur.at;
-    const int unit = cur.off / sg.n_tiles;                        // of the sequence: table head, column group
-    sg.c_begin = cur.off - unit * sg.n_tiles;
-    sg.c_end = min(sg.n_tiles, sg.c_begin + cur.left);
-    sg.h = p.CG == 1 ? unit : unit / p.CG;
-    sg.cg = unit - sg.h * p.CG;
-    const int n = sg.c_end - sg.c_begin;
-    cur.left -= n;
-    cur.off += n;
-    cur.at += n;
-    if (cur.off == sg.n_tiles * p.HC) {
-      cur.off = 0;
-      ++cur.b;
-      cur.len = cur.left > 0 && cur.b < p.B ? seq_len(p, cur.b) : 0;
-    }
-    __syncwarp();
-    if (lane == 0) {
-      segment[2 * warp + 1] = segment[2 * warp];
-      segment[2 * warp] = sg;
-      cursor[warp] = cur;
-    }
-    __syncwarp();
-    const int first = sg.c_begin + warp;
-    // (an empty pool has no group that could stand in for the missing ones: its tiles are left out)
-    n_mine = sg.c_end > first && p.pool.num_pages > 0 ? (sg.c_end - first + kWarps - 1) / kWarps : 0;
-    return true;
-  };
-  // A thread's 8 channels `ch` of column `col` of the segment's queries: where they lie, or null (a column behind the
-  // last, or the half of a differential column that is 0).
-  constexpr int CH = D / 8, Q_BYTES = SPLIT ? 4 : 2;
-  auto query_at = [&](const Segment& sg, int col, int ch) -> const char* {
-    const int j = sg.cg * COLS + col, row = p.diff ? j >> 1 : j;
-    if (j >= p.NC || (p.diff && (ch * 2 >= CH) != (j & 1))) return nullptr;
-    const int gi = p.M == 1 ? row : row / p.M, m = row - gi * p.M;
-    return static_cast<const char*>(p.q) +
-           (sg.b * p.q_sb + (sg.h * p.G + gi) * p.q_sh + m * p.q_sm + ch * 8) * Q_BYTES;
-  };
-  // bring them near, so that the reads below find them there while the page ids are on their way
-  auto touch_queries = [&]() {
-    const Segment& sg = segment[2 * warp];
-    for (int i = threadIdx.x; i < COLS * CH; i += kThreads) {
-      const char* at = query_at(sg, i / CH, i % CH);
-      unsigned short unused;
-      if (at) asm volatile("ld.global.u16 %0, [%1];" : "=h"(unused) : "l"(at));
-    }
-  };
-  // halves after a power of two that puts the row's largest in [1, 2)
-  auto stage_queries = [&]() {
-    const Segment& sg = segment[2 * warp];
-    for (int i = threadIdx.x; i < COLS * CH; i += kThreads) {
-      const int col = i / CH, ch = i % CH, j = sg.cg * COLS + col;
-      float x[8] = {};
-      const char* at = query_at(sg, col, ch);
-      if (at) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (SPLIT) {
-            x[e] = reinterpret_cast<const float*>(at)[e] * p.sign;
-          } else {
-            const uint16_t u = reinterpret_cast<const uint16_t*>(at)[e];
-            x[e] = (p.q_dtype == IAK_DT_F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float(u << 16)) * p.sign;
-          }
-        }
-      }
-      float amax = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-#pragma unroll
-      for (int o = 1; o < CH; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, o));
-      // exponent of amax, held to normal numbers on both sides
-      const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
-      const float down = __uint_as_float((254 - ex) << 23);
-      unsigned hi[4], lo[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y0 = x[2 * e] * down, y1 = x[2 * e + 1] * down;
-        hi[e] = pack_half2(y0, y1);
-        if (SPLIT) {
-          const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
-          lo[e] = pack_half2(y0 - back.x, y1 - back.y);
-        }
-      }
-      uint4* dst = reinterpret_cast<uint4*>(q_frag) + ((col >> 3) * NB + (ch >> 2)) * 32 + (col & 7) * 4 + (ch & 3);
-      *dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      if (SPLIT) dst[NT * NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      if (ch == 0) {
-        col_scale[col] = fmaxf(p.scale * __uint_as_float(ex << 23), 1e-37f);
-        col_limit[col] = j < p.NC ? sg.len - (p.M - 1 - (p.diff ? j >> 1 : j) % p.M) : sg.len;
-      }
-    }
-  };
+
   // ---------------------------------------------------------------- copies
-  // The warp's tiles are c_begin + warp + kWarps k.  Of every 16 of them lane 2 i + u looks up group u of tile i: it
-  // reads the page id a batch ahead and holds the group's number in the pool (0 for a page that does not exist: its
-  // rows are masked).
+  // Of every 16 tiles lane 2 i + u looks up group u of tile i: it reads the page id a batch ahead and holds the group's
+  // number in the pool (0 for a page that does not exist: its rows are masked).
+  int n_mine = 0;                                 // tiles of the segment that are copied
+  int stage = 0;                                  // of the ring, next to be read
   int next_id = -1, src_group = 0;
   unsigned history = 0;                           // two bits per tile issued, the last in bits 0, 1: its groups' pages exist
   constexpr int kBatch = 16;
   unsigned batch_ok = 0;
   const uint8_t* const lane_data = p.pool.data + lane * 16;
-  auto group_of = [&](int k) { return (segment[2 * warp].c_begin + warp + kWarps * (k + (lane >> 1))) * 2 + (lane & 1); };
+  auto group_of = [&](int k) { return (segment.c_begin + k + (lane >> 1)) * 2 + (lane & 1); };
   auto load_id = [&](int k) {
-    const Segment& sg = segment[2 * warp];
     const int gr = group_of(k);
-    return k + (lane >> 1) < n_mine && gr * 16 < sg.len
-               ? __ldg(p.pt + sg.b * p.pt_sb + sg.h * p.pt_sh + slot_of(p, gr)) : -1;
+    return k + (lane >> 1) < n_mine && gr * 16 < segment.len
+               ? __ldg(p.pt + segment.b * p.pt_sb + segment.h * p.pt_sh + slot_of(p, gr)) : -1;
   };
   auto issue = [&](int k, int to_stage) {
     history <<= 2;
@@ -439,151 +374,148 @@ fp4_decode_kernel(const DecP p) {
     }
     copy_commit();
   };
-  auto start_copies = [&]() {
-    next_id = load_id(0);
-    int to = stage;
-#pragma unroll 1
-    for (int i = 0; i < L::kStages - 1; ++i) {
-      issue(i, to);
-      to = to + 1 == L::kStages ? 0 : to + 1;
+  auto read_words = [&](unsigned at, unsigned (&w)[NB]) {
+    constexpr int PW = Gr::kPW;
+#pragma unroll
+    for (int i = 0; i < NB / PW; ++i) {
+      unsigned part[PW];
+      lds_words<PW>(at + (i * 32 + lane) * (PW * 4), part);
+#pragma unroll
+      for (int j = 0; j < PW; ++j) w[i * PW + j] = part[j];
     }
   };
-    auto read_words = [&](unsigned at, unsigned (&w)[NB]) {
-      constexpr int PW = Gr::kPW;
-#pragma unroll
-      for (int i = 0; i < NB / PW; ++i) {
-        unsigned part[PW];
-        lds_words<PW>(at + (i * 32 + lane) * (PW * 4), part);
-#pragma unroll
-        for (int j = 0; j < PW; ++j) w[i * PW + j] = part[j];
-      }
-    };
+  // the segment's column `col`: its query row, and the tokens that it sees
+  auto row_of = [&](int col) { return p.diff ? (segment.cg * COLS + col) >> 1 : segment.cg * COLS + col; };
+  auto limit = [&](int col) {
+    return p.M == 1 ? segment.len : segment.len - (p.M - 1 - row_of(col) % p.M);
+  };
 
-  // Each pass opens the next segment and starts its copies, joins the warps' sums of the last one, and runs the tiles.
-  // (One place in the code for each: a cold call fetches its instructions from memory.)
-  float o[NT][MT][4];
-  float m_run[NT][2], l_run[NT][2];
-  bool pending = false, begins_run = true;
+  bool begins_run = true;
   while (true) {
-    __syncwarp();
-    const bool more = open_segment();
-    if (more) {
-      touch_queries();
-      start_copies();
+    {
+      Cursor cur = cursor;
+      if (cur.left <= 0 || cur.b >= p.B) break;
+      Segment sg;
+      sg.b = cur.b;
+      sg.len = cur.len;
+      sg.n_tiles = tiles_of(p, cur.len);
+      sg.at = cur.at;
+      const int unit = cur.off / sg.n_tiles;                      // of the sequence: table head, column group
+      sg.c_begin = cur.off - unit * sg.n_tiles;
+      sg.c_end = min(sg.n_tiles, sg.c_begin + cur.left);
+      sg.h = p.CG == 1 ? unit : unit / p.CG;
+      sg.cg = unit - sg.h * p.CG;
+      const int n = sg.c_end - sg.c_begin;
+      cur.left -= n;
+      cur.off += n;
+      cur.at += n;
+      if (cur.off == sg.n_tiles * p.HC) {
+        cur.off = 0;
+        ++cur.b;
+        cur.len = cur.left > 0 && cur.b < p.B ? seq_len(p, cur.b) : 0;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        segment = sg;
+        cursor = cur;
+      }
+      __syncwarp();
+      // (an empty pool has no group that could stand in for the missing ones: its tiles are left out)
+      n_mine = p.pool.num_pages > 0 ? n : 0;
     }
+    next_id = load_id(0);
 
-    if (pending) {
-      // ------------------------------------------------------ join the warps
-      // in the stage of each warp's ring that the next segment's copies leave free
-      const unsigned my_join = warp * L::kStages * L::kStage + (stage == 0 ? L::kStages - 1 : stage - 1) * L::kStage;
-      if (lane == 0) join_at[warp] = my_join;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float v = l_run[nt][e];
-          v += __shfl_xor_sync(~0u, v, 4);
-          v += __shfl_xor_sync(~0u, v, 8);
-          v += __shfl_xor_sync(~0u, v, 16);
-          if (g == 0) {
-            warp_m[warp * COLS + nt * 8 + 2 * t + e] = m_run[nt][e];
-            warp_l[warp * COLS + nt * 8 + 2 * t + e] = v;
-          }
-        }
-      }
-      __syncthreads();                              // and every warp is past its last read of the queries
-      const Segment& done_sg = segment[2 * warp + (more ? 1 : 0)];
-      const int h = done_sg.h, cg = done_sg.cg;
-      const bool whole = done_sg.c_begin == 0 && done_sg.c_end == done_sg.n_tiles;
-      const int which = begins_run ? 0 : 1;
-      if (!p.direct && threadIdx.x == 0) {
-        const int begin = done_sg.at - done_sg.c_begin;             // the unit's first tile
-        Cut d = {done_sg.b, h, cg * COLS, static_cast<int>(blockIdx.x), which, -1};
-        if (p.by_unit) {
-          if (!whole) d.last = block_of(runs, begin + done_sg.n_tiles - 1);
-          if (done_sg.c_begin == 0) cuts(p, COLS)[done_sg.b * p.HC + h * p.CG + cg] = d;
-        } else if (begins_run) {
-          d.first = blockIdx.x - 1;
-          if (done_sg.c_begin > 0 && run_begin(runs, d.first) <= begin) {
-            d.which = run_begin(runs, d.first) == begin ? 0 : 1;
-            d.last = block_of(runs, begin + done_sg.n_tiles - 1);
-          }
-          cuts(p, COLS)[blockIdx.x] = d;
-        }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float f[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float top = -FLT_MAX;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + nt * 8 + 2 * t + e]);
-          f[e] = tc::ex2(m_run[nt][e] - top);
-        }
-        const int per = p.diff ? 2 : 1;             // columns of an output row; a warp takes a row
-        const bool has_row = warp * per < 8 && cg * COLS + nt * 8 + warp * per < p.NC;
-        const int row = (cg * COLS + nt * 8) / per + warp;
-        float x[NB];
-        float* dst = reinterpret_cast<float*>(smem + my_join) + 2 * t * L::kOutStride + g * (4 * NB);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            *reinterpret_cast<float2*>(dst + 2 * i) = make_float2(o[nt][i][0] * f[0], o[nt][i][2] * f[0]);
-          *reinterpret_cast<float2*>(dst + L::kOutStride + 2 * i) = make_float2(o[nt][i][1] * f[1], o[nt][i][3] * f[1]);
-        }
-        __syncthreads();
-        if (has_row) {
-          for (int half = 0; half < per; ++half) {
-            const int lc = warp * per + half, col = nt * 8 + lc;
-            float top = -FLT_MAX, l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_m[w * COLS + col]);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) l += warp_l[w * COLS + col] * tc::ex2(warp_m[w * COLS + col] - top);
-            float acc[NB];
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
-              acc[i] = 0.f;
-#pragma unroll
-              for (int w = 0; w < kWarps; ++w)
-                acc[i] += reinterpret_cast<const float*>(smem + join_at[w])[lc * L::kOutStride + i * 32 + lane];
-            }
-            if (!whole) {
-              float* part = p.ws + ((static_cast<int64_t>(blockIdx.x) * 2 + which) * COLS + col) * (D + 2);
-#pragma unroll
-              for (int i = 0; i < NB; ++i) part[i * 32 + lane] = acc[i];
-              if (lane == 0) { part[D] = top; part[D + 1] = l; }
-            } else {
-              const float inv = safe_inverse(l);
-              const float weight = half ? -p.lam[h * p.G + row / p.M] * inv : inv;
-#pragma unroll
-              for (int i = 0; i < NB; ++i) {
-                x[i] = half ? fmaf(acc[i], weight, x[i]) : acc[i] * weight;
-              }
-            }
-          }
-        }
-        __syncthreads();
-        if (has_row && whole) finish_row<NB>(p, done_sg.b, h * p.G + row / p.M, row % p.M, x);
-      }
-      begins_run = false;
-    }
-    if (!more) break;
-    stage_queries();
-    __syncthreads();
+    // ------------------------------------------------------------- queries
+    // Lane 4 g + t: channels 32 b + 8 t .. of column 8 nt + g, as halves after a power of two that puts the row's largest
+    // in [1, 2).  A differential column has one half of the channels, the other is 0.
     float sc[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      sc[nt][0] = col_scale[nt * 8 + 2 * t];
-      sc[nt][1] = col_scale[nt * 8 + 2 * t + 1];
+      const int j = segment.cg * COLS + nt * 8 + g, row = row_of(nt * 8 + g);
+      const int gi = p.M == 1 ? row : row / p.M, m = row - gi * p.M;
+      const int64_t at = segment.b * p.q_sb + (segment.h * p.G + gi) * p.q_sh + m * p.q_sm + t * 8;
+      constexpr int WORDS = SPLIT ? 8 : 4;
+      unsigned raw[NB][WORDS];
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int e = 0; e < WORDS; ++e) raw[b][e] = 0;
+        if (j >= p.NC || (p.diff && (2 * b >= NB) != (j & 1))) continue;
+        const int64_t el = at + 32 * b;
+        if (p.q_vec) {
+#pragma unroll
+          for (int e = 0; e < WORDS; e += 4) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const char*>(p.q) + el * (SPLIT ? 4 : 2) + e * 4));
+            raw[b][e] = w.x; raw[b][e + 1] = w.y; raw[b][e + 2] = w.z; raw[b][e + 3] = w.w;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < WORDS; ++e) {
+            if (SPLIT) raw[b][e] = __float_as_uint(static_cast<const float*>(p.q)[el + e]);
+            else raw[b][e] = static_cast<const uint16_t*>(p.q)[el + 2 * e] |
+                             static_cast<unsigned>(static_cast<const uint16_t*>(p.q)[el + 2 * e + 1]) << 16;
+          }
+        }
+      }
+      auto value = [&](int b, int e) {
+        if (SPLIT) return __uint_as_float(raw[b][e]);
+        const unsigned u = e % 2 ? raw[b][e / 2] >> 16 : raw[b][e / 2] & 0xffffu;
+        return p.q_dtype == IAK_DT_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(u)))
+                                       : __uint_as_float(u << 16);
+      };
+      float amax = 0.f;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(value(b, e)));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+      // exponent of amax, held to normal numbers on both sides
+      const int ex = min(max(static_cast<int>(__float_as_uint(amax) >> 23), 2), 252);
+      const float down = __uint_as_float((254 - ex) << 23) * p.sign;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) {
+        unsigned hi[4], lo[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y0 = value(b, 2 * e) * down, y1 = value(b, 2 * e + 1) * down;
+          hi[e] = pack_half2(y0, y1);
+          if (SPLIT) {
+            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
+            lo[e] = pack_half2(y0 - back.x, y1 - back.y);
+          }
+        }
+        uint4* dst = reinterpret_cast<uint4*>(q_frag) + (nt * NB + b) * 32 + lane;
+        *dst = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        if (SPLIT) dst[NT * NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      // of the lane's own columns 8 nt + 2 t and the next
+      const float mine = fmaxf(p.scale * __uint_as_float(ex << 23), 1e-37f);
+      sc[nt][0] = __shfl_sync(~0u, mine, 8 * t);
+      sc[nt][1] = __shfl_sync(~0u, mine, 8 * t + 4);
+    }
+    {
+      int to = stage;
+#pragma unroll 1
+      for (int i = 0; i < L::kStages - 1; ++i) {
+        issue(i, to);
+        to = to + 1 == L::kStages ? 0 : to + 1;
+      }
+    }
+
+    float o[NT][MT][4];
+    float m_run[NT][2], l_run[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
       m_run[nt][0] = m_run[nt][1] = -FLT_MAX;
       l_run[nt][0] = l_run[nt][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
     }
-    const int full_end = segment[2 * warp].len - (p.M - 1);   // every query sees the tokens before it
-    int key0 = (segment[2 * warp].c_begin + warp) * kTileKeys;
-    for (int k = 0; k < n_mine; ++k, key0 += kWarps * kTileKeys) {
+    const int full_end = segment.len - (p.M - 1);         // every query sees the tokens before it
+    int key0 = segment.c_begin * kTileKeys;
+    for (int k = 0; k < n_mine; ++k, key0 += kTileKeys) {
       // the stage read in the last round is free: every lane is past its reads
       warp_sync();
       issue(k + L::kStages - 1, stage == 0 ? L::kStages - 1 : stage - 1);
@@ -651,7 +583,7 @@ fp4_decode_kernel(const DecP p) {
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const bool seen = ok && key + (i >> 1) * 8 < col_limit[nt * 8 + 2 * t + (i & 1)];
+              const bool seen = ok && key + (i >> 1) * 8 < limit(nt * 8 + 2 * t + (i & 1));
               if (!seen) s[u][nt][i] = -INFINITY;
             }
           }
@@ -756,47 +688,134 @@ fp4_decode_kernel(const DecP p) {
       }
     }
 
-    pending = true;
+    // ------------------------------------------------------------- the segment's end
+    float l_all[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = l_run[nt][e];
+        v += __shfl_xor_sync(~0u, v, 4);
+        v += __shfl_xor_sync(~0u, v, 8);
+        v += __shfl_xor_sync(~0u, v, 16);
+        l_all[nt][e] = v;
+      }
+    }
+    const int which = begins_run ? 0 : 1;
+    const bool whole = segment.c_begin == 0 && segment.c_end == segment.n_tiles;
+    if (!p.direct && lane == 0) {
+      const int begin = segment.at - segment.c_begin;              // the unit's first tile
+      Cut d = {segment.b, segment.h, segment.cg * COLS, run, which, -1};
+      if (p.by_unit) {
+        if (!whole) d.last = run_of(runs, begin + segment.n_tiles - 1);
+        if (segment.c_begin == 0) cuts(p)[segment.b * p.HC + segment.h * p.CG + segment.cg] = d;
+      } else if (begins_run) {
+        d.first = run - 1;
+        if (segment.c_begin > 0 && run_begin(runs, run - 1) <= begin) {
+          d.which = run_begin(runs, run - 1) == begin ? 0 : 1;
+          d.last = run_of(runs, begin + segment.n_tiles - 1);
+        }
+        cuts(p)[run] = d;
+      }
+    }
+    // a lane has channels 4 NB g .. of columns 8 nt + 2 t and the next: with differential attention, of a row's two maps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int col = nt * 8 + 2 * t, j = segment.cg * COLS + col;
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (j + e >= p.NC) continue;
+          float* part = part_at(p, run, which, col + e);
+#pragma unroll
+          for (int i = 0; i < MT; i += 2)
+            *reinterpret_cast<float4*>(part + g * (4 * NB) + 2 * i) =
+                make_float4(o[nt][i][e], o[nt][i][e + 2], o[nt][i + 1][e], o[nt][i + 1][e + 2]);
+          if (g == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m_run[nt][e], l_all[nt][e]);
+        }
+        continue;
+      }
+      if (p.diff) {
+        const int row = j >> 1, gi = row / p.M;
+        const bool real = j < p.NC;
+        const float w0 = safe_inverse(l_all[nt][0]);
+        const float w1 = real ? -p.lam[segment.h * p.G + gi] * safe_inverse(l_all[nt][1]) : 0.f;
+        float x[4 * NB], mul = p.out_scale;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          x[2 * i] = fmaf(o[nt][i][1], w1, o[nt][i][0] * w0);
+          x[2 * i + 1] = fmaf(o[nt][i][3], w1, o[nt][i][2] * w0);
+        }
+        if (p.norm_w) {
+          float sq = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4 * NB; ++i) sq = fmaf(x[i], x[i], sq);
+          sq += __shfl_xor_sync(~0u, sq, 4);
+          sq += __shfl_xor_sync(~0u, sq, 8);
+          sq += __shfl_xor_sync(~0u, sq, 16);
+          mul *= norm_factor<NB>(p, sq);
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * NB; ++i) x[i] *= p.norm_w ? mul * p.norm_w[g * (4 * NB) + i] : mul;
+        if (real)
+          store_run(p, segment.b * p.o_sb + (segment.h * p.G + gi) * p.o_sh + (row - gi * p.M) * p.o_sm + g * (4 * NB), x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (j + e >= p.NC) continue;
+          const int row = j + e, gi = p.M == 1 ? row : row / p.M;
+          const float w = safe_inverse(l_all[nt][e]);
+          float x[4 * NB];
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            x[2 * i] = o[nt][i][e] * w;
+            x[2 * i + 1] = o[nt][i][e + 2] * w;
+          }
+          store_run(p, segment.b * p.o_sb + (segment.h * p.G + gi) * p.o_sh + (row - gi * p.M) * p.o_sm + g * (4 * NB), x);
+        }
+      }
+    }
+    begins_run = false;
+    __syncwarp();                                 // before the next segment's record and queries
   }
 }
 
 // ---------------------------------------------------------------- join kernel
-// One block per (record of a cut, output row): the unit's partials are added in order of the blocks that left them.
-constexpr int kJoinWarps = 8;
+// For every (record of a cut, output row) the unit's parts are added in order of the runs that left them: by a block of
+// 16 warps where a unit has many parts (TEAM 16), by a warp where it has few (TEAM 1).
+constexpr int kJoinWarps = 16;
 
-__host__ __device__ inline int join_rows(int NC, int cols, int diff) {
-  return (NC < cols ? NC : cols) / (diff ? 2 : 1);
-}
+__host__ __device__ inline int join_rows(const DecP& p) { return p.cols / (p.diff ? 2 : 1); }
 
-template <int NB, int NT>
-__global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p) {
-  constexpr int D = NB * 32, COLS = 8 * NT;
-  __shared__ float part_sum[kJoinWarps][D + 2];
-  const int per = p.diff ? 2 : 1;
-  const int rows = join_rows(p.NC, COLS, p.diff);
-  const int record = blockIdx.x / rows + (p.by_unit ? 0 : 1), r = blockIdx.x % rows;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+template <int NB, int TEAM>
+__global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p, int records) {
+  constexpr int D = NB * 32;
+  __shared__ float part_sum[TEAM == 1 ? 1 : kJoinWarps][D + 2];
+  const int per = p.diff ? 2 : 1, rows = join_rows(p);
+  const int lane = threadIdx.x & 31, warp = TEAM == 1 ? 0 : threadIdx.x >> 5;
+  const int item = TEAM == 1 ? blockIdx.x * kJoinWarps + (threadIdx.x >> 5) : blockIdx.x;
+  const int record = item / rows + (p.by_unit ? 0 : 1), r = item % rows;
   const int used = p.by_unit ? 0 : make_runs(p, total_tiles(p, scan32(p, 0))).used;
-  // every block waits, so that this kernel never ends before the main one
+  // every warp waits, so that this kernel never ends before the main one
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!p.by_unit && record >= used) return;
-  const Cut d = cuts(p, COLS)[record];
+  if (item / rows >= records || (!p.by_unit && record >= used)) return;
+  const Cut d = cuts(p)[record];
   const int n = d.last - d.first + 1, j0 = d.j0 + r * per;
   if (d.last < 0 || j0 >= p.NC) return;
   float x[NB];
   for (int half = 0; half < per; ++half) {
     const int col = r * per + half;
-    // warp w: parts w, w + 8, .., four at a time, so that their loads run together
+    // a warp takes every TEAM-th part, four at a time, so that their loads run together
     float top = -FLT_MAX, l = 0.f, acc[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) acc[i] = 0.f;
     constexpr int kAt = NB <= 4 ? 4 : 2;
-    for (int c = warp; c < n; c += kAt * kJoinWarps) {
+    for (int c = warp; c < n; c += kAt * TEAM) {
       float m[kAt], pl[kAt], v[kAt][NB];
 #pragma unroll
       for (int k = 0; k < kAt; ++k) {
-        const int part = min(c + k * kJoinWarps, n - 1);
-        const float* at = p.ws + ((static_cast<int64_t>(d.first + part) * 2 + (part == 0 ? d.which : 0)) * COLS + col) * (D + 2);
+        const int part = min(c + k * TEAM, n - 1);
+        const float* at = part_at(p, d.first + part, part == 0 ? d.which : 0, col);
         m[k] = at[D];
         pl[k] = at[D + 1];
 #pragma unroll
@@ -811,8 +830,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p)
       for (int i = 0; i < NB; ++i) acc[i] *= old;
 #pragma unroll
       for (int k = 0; k < kAt; ++k) {
-        const float f = tc::ex2(m[k] - next);
-        if (c + k * kJoinWarps < n) {              // (a part read in place of a missing one may hold NaN)
+        if (c + k * TEAM < n) {                    // (the last part stands in for missing ones)
+          const float f = tc::ex2(m[k] - next);
           l = fmaf(pl[k], f, l);
 #pragma unroll
           for (int i = 0; i < NB; ++i) acc[i] = fmaf(v[k][i], f, acc[i]);
@@ -820,36 +839,41 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p)
       }
       top = next;
     }
+    if constexpr (TEAM > 1) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) part_sum[warp][i * 32 + lane] = acc[i];
-    if (lane == 0) { part_sum[warp][D] = top; part_sum[warp][D + 1] = l; }
-    __syncthreads();
-    if (warp == 0) {
-      float all = -FLT_MAX, sum = 0.f;
+      for (int i = 0; i < NB; ++i) part_sum[warp][i * 32 + lane] = acc[i];
+      if (lane == 0) { part_sum[warp][D] = top; part_sum[warp][D + 1] = l; }
+      __syncthreads();
+      if (warp == 0) {
+        top = -FLT_MAX;
+        l = 0.f;
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) all = fmaxf(all, part_sum[w][D]);
+        for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, part_sum[w][D]);
 #pragma unroll
-      for (int i = 0; i < NB; ++i) acc[i] = 0.f;
+        for (int i = 0; i < NB; ++i) acc[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kJoinWarps; ++w) {
-        const float f = tc::ex2(part_sum[w][D] - all);
-        sum = fmaf(part_sum[w][D + 1], f, sum);
+        for (int w = 0; w < kJoinWarps; ++w) {
+          const float f = tc::ex2(part_sum[w][D] - top);
+          l = fmaf(part_sum[w][D + 1], f, l);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) acc[i] = fmaf(part_sum[w][i * 32 + lane], f, acc[i]);
+          for (int i = 0; i < NB; ++i) acc[i] = fmaf(part_sum[w][i * 32 + lane], f, acc[i]);
+        }
       }
+    }
+    if (warp == 0) {
       const int row = p.diff ? (j0 >> 1) : j0;
-      const float inv = safe_inverse(sum);
+      const float inv = safe_inverse(l);
       const float scale = half ? -p.lam[d.h * p.G + row / p.M] * inv : inv;
 #pragma unroll
       for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], scale, x[i]) : acc[i] * scale;
       if (half == per - 1) finish_row<NB>(p, d.b, d.h * p.G + row / p.M, row % p.M, x);
     }
-    __syncthreads();
+    if (TEAM > 1) __syncthreads();
   }
 }
 
 // -------------------------------------------------------------------- launch
-struct Plan { int grid; bool direct; size_t ws; };
+struct Plan { int grid; size_t ws; };
 
 template <int NB, int NT, bool SPLIT>
 int resident_blocks(int* blocks) {
@@ -877,57 +901,68 @@ int resident_blocks(int* blocks) {
 
 template <int NB, int NT, bool SPLIT>
 int make_plan(DecP& p, Plan* plan) {
-  p.CG = (p.NC + 8 * NT - 1) / (8 * NT);
+  using L = Shape<NB, NT, SPLIT>;
+  p.CG = (p.NC + L::COLS - 1) / L::COLS;
+  p.cols = std::min(p.NC, L::COLS);
   const int64_t hc = static_cast<int64_t>(p.Ht) * p.CG, units = hc * p.B;
-  if (units * 8 * NT > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: too many rows for one launch");
+  if (units * L::COLS > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: too many rows for one launch");
   p.HC = static_cast<int>(hc);
-  constexpr int kWarps = Shape<NB, NT, SPLIT>::kWarps;
-  p.min_tiles = kWarps;
+  p.min_tiles = kMinTiles;
   const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + kTileKeys - 1) / kTileKeys;
-  // a unit that one tile per warp covers is one block's work: no joining
-  plan->direct = most <= kWarps;
   if (most * units > 0x7fffffffLL - 64)
     return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: tables of more than 2^31 tiles of %d tokens", kTileKeys);
+  // units that a warp covers about as fast as two would with their parts joined
+  p.direct = most <= kDirectTiles;
   int blocks = 0;
   if (int st = resident_blocks<NB, NT, SPLIT>(&blocks)) return st;
-  if (plan->direct) {
-    plan->grid = static_cast<int>(units);
+  if (p.direct) {
+    plan->grid = static_cast<int>((units + L::kWarps - 1) / L::kWarps);
+    p.runs = plan->grid * L::kWarps;
+    p.by_unit = 1;
     plan->ws = 0;
-  } else {
-    const int64_t useful = (most * units + kWarps - 1) / kWarps;
-    plan->grid = static_cast<int>(std::min<int64_t>(blocks, useful));
-    plan->ws = static_cast<size_t>(plan->grid) * (2 * 8 * NT * (NB * 32 + 2) * sizeof(float) + sizeof(Cut));
+    return IAK_OK;
   }
-  p.grid = plan->grid;
-  p.direct = plan->direct ? 1 : 0;
-  p.by_unit = units <= plan->grid ? 1 : 0;
+  const int64_t useful = (most * units + kMinTiles - 1) / kMinTiles;
+  plan->grid = static_cast<int>(std::min<int64_t>(blocks, (useful + L::kWarps - 1) / L::kWarps));
+  p.runs = plan->grid * L::kWarps;
+  p.by_unit = units <= p.runs;
+  plan->ws = static_cast<size_t>(p.runs) * (2 * p.cols * (L::D + 4) * sizeof(float) + sizeof(Cut));
   return IAK_OK;
+}
+
+template <int NB, int TEAM>
+int launch_join(const DecP& p, int records, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  const int64_t items = static_cast<int64_t>(records) * join_rows(p);
+  cfg.gridDim = dim3(static_cast<unsigned>(TEAM == 1 ? (items + kJoinWarps - 1) / kJoinWarps : items));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  // starts while the main kernel's last blocks run; it waits for them before it reads a part
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, fp4_join_kernel<NB, TEAM>, p, records), "fp4_join launch");
 }
 
 template <int NB, int NT, bool SPLIT>
 int run_shape(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cudaStream_t s) {
+  using L = Shape<NB, NT, SPLIT>;
   Plan plan;
   if (int st = make_plan<NB, NT, SPLIT>(p, &plan)) return st;
   if (need) *need = plan.ws;
   if (!launch) return IAK_OK;
   if (plan.ws > ws_bytes || (plan.ws && !ws))
     return fail(IAK_ERR_WORKSPACE, "iak_fp4_decode needs %zu workspace bytes, got %zu", plan.ws, ws_bytes);
+  if (reinterpret_cast<uintptr_t>(ws) % 16) return fail(IAK_ERR_INVALID_ARG, "iak_fp4_decode: workspace not 16-byte aligned");
   p.ws = static_cast<float*>(ws);
-  fp4_decode_kernel<NB, NT, SPLIT><<<plan.grid, Shape<NB, NT, SPLIT>::kThreads, Shape<NB, NT, SPLIT>::kSmem, s>>>(p);
+  fp4_decode_kernel<NB, NT, SPLIT><<<plan.grid, L::kThreads, L::kSmem, s>>>(p);
   if (int st = check_cuda(cudaGetLastError(), "fp4_decode launch")) return st;
-  if (plan.grid == 1 || plan.direct) return IAK_OK;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((p.by_unit ? p.B * p.HC : plan.grid - 1) * join_rows(p.NC, 8 * NT, p.diff)));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = s;
-  // starts while the main kernel's last blocks run; it waits for them before it reads a partial
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const DecP cp = p;
-  return check_cuda(cudaLaunchKernelEx(&cfg, fp4_join_kernel<NB, NT>, cp), "fp4_join launch");
+  if (p.direct) return IAK_OK;
+  const int units = p.B * p.HC;
+  const int records = p.by_unit ? units : p.runs - 1;
+  return p.runs / units >= kManyParts ? launch_join<NB, kJoinWarps>(p, records, s) : launch_join<NB, 1>(p, records, s);
 }
 
 // Columns per block: as many n = 8 tiles as the columns need, up to what the accumulators leave registers for; more
@@ -937,7 +972,9 @@ int run_cols(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cuda
   if constexpr (NB < 8 && !SPLIT) {
     if (p.NC > 16) return run_shape<NB, 4, SPLIT>(p, launch, ws, ws_bytes, need, s);
   }
-  if (p.NC > 8) return run_shape<NB, 2, SPLIT>(p, launch, ws, ws_bytes, need, s);
+  if constexpr (NB < 8 || !SPLIT) {
+    if (p.NC > 8) return run_shape<NB, 2, SPLIT>(p, launch, ws, ws_bytes, need, s);
+  }
   return run_shape<NB, 1, SPLIT>(p, launch, ws, ws_bytes, need, s);
 }
 
@@ -989,6 +1026,12 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
   const int64_t nc = static_cast<int64_t>(p.G) * p.M * (1 + p.diff);
   if (nc > (1 << 20)) return fail(IAK_ERR_UNSUPPORTED, "%s: too many query heads", what);
   p.NC = static_cast<int>(nc);
+  auto aligned = [](const void* base, int dtype, int64_t a, int64_t b, int64_t c) {
+    const int64_t per16 = dtype == IAK_DT_F32 ? 4 : 8;
+    return reinterpret_cast<uintptr_t>(base) % 16 == 0 && a % per16 == 0 && b % per16 == 0 && c % per16 == 0 ? 1 : 0;
+  };
+  p.q_vec = aligned(p.q, p.q_dtype, p.q_sb, p.q_sh, p.q_sm);
+  p.o_vec = aligned(p.out, p.out_dtype, p.o_sb, p.o_sh, p.o_sm);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (static_cast<int64_t>(p.W) * p.pool.PS > kMaxTokens)
     return fail(IAK_ERR_UNSUPPORTED, "%s: tables of more than %d tokens", what, kMaxTokens);
