@@ -30,9 +30,7 @@ namespace {
 
 constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
-constexpr int kMinTiles = 2;       // of a run
 constexpr int kDirectTiles = 8;    // units of at most so many tiles are never cut
-constexpr int kManyParts = 12;     // of a unit, from which on a block joins them instead of a warp
 constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
 constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small P stay normal halves
 
@@ -211,6 +209,8 @@ struct Shape {
   // Warps of an SM: 16 with 128 registers each while the accumulators are small, 12 with 168, 8 with 255.  A tile's two
   // groups of 16 keys go through the products together, for the independent work.
   static constexpr int kSize = NB * NT * (SPLIT ? 2 : 1);
+  // tiles of a run, at least: wide heads' parts cost more to join
+  static constexpr int kMinTiles = NB == 8 ? 4 : 1;
   static constexpr int kPerSm = kSize <= 4 && NB == 2 ? 16 : (kSize <= 8 && NB < 8 ? 12 : 8);
   static constexpr int kBlocks = kPerSm / kWarps;
   static constexpr int kStages = NB == 8 ? 2 : 3;
@@ -781,19 +781,19 @@ fp4_decode_kernel(const DecP p) {
 }
 
 // ---------------------------------------------------------------- join kernel
-// For every (record of a cut, output row) the unit's parts are added in order of the runs that left them: by a block of
-// 16 warps where a unit has many parts (TEAM 16), by a warp where it has few (TEAM 1).
-constexpr int kJoinWarps = 16;
+// For every (record of a cut, output row) the unit's parts are added in order of the runs that left them, by a team of
+// warps: a block each, but for TEAM 1, where a block has 16.
+__host__ __device__ constexpr int join_warps(int team) { return team == 1 ? 16 : team; }
 
 __host__ __device__ inline int join_rows(const DecP& p) { return p.cols / (p.diff ? 2 : 1); }
 
 template <int NB, int TEAM>
-__global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p, int records) {
+__global__ void __launch_bounds__(join_warps(TEAM) * 32) fp4_join_kernel(const DecP p, int records) {
   constexpr int D = NB * 32;
-  __shared__ float part_sum[TEAM == 1 ? 1 : kJoinWarps][D + 2];
+  __shared__ float part_sum[TEAM][D + 2];
   const int per = p.diff ? 2 : 1, rows = join_rows(p);
   const int lane = threadIdx.x & 31, warp = TEAM == 1 ? 0 : threadIdx.x >> 5;
-  const int item = TEAM == 1 ? blockIdx.x * kJoinWarps + (threadIdx.x >> 5) : blockIdx.x;
+  const int item = TEAM == 1 ? blockIdx.x * join_warps(1) + (threadIdx.x >> 5) : blockIdx.x;
   const int record = item / rows + (p.by_unit ? 0 : 1), r = item % rows;
   const int used = p.by_unit ? 0 : make_runs(p, total_tiles(p, scan32(p, 0))).used;
   // every warp waits, so that this kernel never ends before the main one
@@ -848,11 +848,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fp4_join_kernel(const DecP p,
         top = -FLT_MAX;
         l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, part_sum[w][D]);
+        for (int w = 0; w < TEAM; ++w) top = fmaxf(top, part_sum[w][D]);
 #pragma unroll
         for (int i = 0; i < NB; ++i) acc[i] = 0.f;
 #pragma unroll
-        for (int w = 0; w < kJoinWarps; ++w) {
+        for (int w = 0; w < TEAM; ++w) {
           const float f = tc::ex2(part_sum[w][D] - top);
           l = fmaf(part_sum[w][D + 1], f, l);
 #pragma unroll
@@ -907,7 +907,7 @@ int make_plan(DecP& p, Plan* plan) {
   const int64_t hc = static_cast<int64_t>(p.Ht) * p.CG, units = hc * p.B;
   if (units * L::COLS > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: too many rows for one launch");
   p.HC = static_cast<int>(hc);
-  p.min_tiles = kMinTiles;
+  p.min_tiles = L::kMinTiles;
   const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + kTileKeys - 1) / kTileKeys;
   if (most * units > 0x7fffffffLL - 64)
     return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: tables of more than 2^31 tiles of %d tokens", kTileKeys);
@@ -922,7 +922,7 @@ int make_plan(DecP& p, Plan* plan) {
     plan->ws = 0;
     return IAK_OK;
   }
-  const int64_t useful = (most * units + kMinTiles - 1) / kMinTiles;
+  const int64_t useful = (most * units + L::kMinTiles - 1) / L::kMinTiles;
   plan->grid = static_cast<int>(std::min<int64_t>(blocks, (useful + L::kWarps - 1) / L::kWarps));
   p.runs = plan->grid * L::kWarps;
   p.by_unit = units <= p.runs;
@@ -934,8 +934,8 @@ template <int NB, int TEAM>
 int launch_join(const DecP& p, int records, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   const int64_t items = static_cast<int64_t>(records) * join_rows(p);
-  cfg.gridDim = dim3(static_cast<unsigned>(TEAM == 1 ? (items + kJoinWarps - 1) / kJoinWarps : items));
-  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.gridDim = dim3(static_cast<unsigned>(TEAM == 1 ? (items + join_warps(1) - 1) / join_warps(1) : items));
+  cfg.blockDim = dim3(join_warps(TEAM) * 32);
   cfg.stream = s;
   // starts while the main kernel's last blocks run; it waits for them before it reads a part
   cudaLaunchAttribute attr[1];
@@ -962,7 +962,13 @@ int run_shape(DecP& p, bool launch, void* ws, size_t ws_bytes, size_t* need, cud
   if (p.direct) return IAK_OK;
   const int units = p.B * p.HC;
   const int records = p.by_unit ? units : p.runs - 1;
-  return p.runs / units >= kManyParts ? launch_join<NB, kJoinWarps>(p, records, s) : launch_join<NB, 1>(p, records, s);
+  // warps per row: as many as share the parts well, while all rows' teams run at once
+  // (8 sequences of 32k, 27 parts a unit, 256 rows: 56 us in all with 16, 63 with 1; 16 of D 64, 18 parts, 2048 rows:
+  // 103 with 16, 92 with 1)
+  const int parts = p.runs / units;
+  const int64_t rows = static_cast<int64_t>(records) * join_rows(p);
+  if (parts >= 12 && rows <= 512) return launch_join<NB, 16>(p, records, s);
+  return parts >= 4 && rows <= 4096 ? launch_join<NB, 4>(p, records, s) : launch_join<NB, 1>(p, records, s);
 }
 
 // Columns per block: as many n = 8 tiles as the columns need, up to what the accumulators leave registers for; more
