@@ -9,15 +9,21 @@
 //      a row's block scale 2^e multiplies the fp32 product of its 32 channels (4 lanes x 8), not its elements.
 //   V: a byte holds one channel of two neighbouring keys, so that its half pair lies along the contraction; it is
 //      multiplied by the two keys' scales (exact: the pool's values are halves).
-//   P: from the accumulator's layout to the operand's by movmatrix.
-// What bounds it: the cache's bytes, 4.25 bits an element.  Work is cut into equal runs of tiles over all
-// (sequence, table head, column group) units, one run per resident block, so that ragged batches and single long
-// sequences fill the GPU alike; a unit cut over several blocks leaves partial (m, l, O) that a second kernel joins in
-// order of the blocks (no atomics: results do not depend on timing).  Each warp streams its own tiles through a
-// ring of 16-byte asynchronous copies: a group's codes and scales lie together in the order in which lanes read them,
-// so that copies and reads are linear in the lane, free of bank conflicts, and five copies per 16 rows need one address.
-// (Bulk copies, one per 16 rows and an mbarrier, measured the same at D 128, 141 us for the 32k batch of 32 below, and
-// slower at D 64, 70 us against 66 for 16 sequences of 32k; they would need bounded waits besides.)
+//   P: rounded to halves (fp32 queries: the sum of two), from the accumulator's layout to the operand's by movmatrix.
+//   m is raised only when a score passes it by 8 or more (P up to 2^15), which leaves the rescaling of O to few tiles.
+// What bounds it: the cache's bytes, 4.25 bits an element, and close behind them the issue slots: per 16 rows a warp
+// spends about 64 conversions, 64 multiplies and 16 products at D 128.
+// Work is cut into equal runs of tiles over all (sequence, table head, column group) units, one for each resident warp,
+// so that ragged batches, many short sequences and one long sequence fill the GPU alike; a unit cut over several runs
+// leaves partial (m, l, O) that a second kernel adds in order of the runs (no atomics: results do not depend on timing).
+// Warps share nothing: with units cut per block of 8 warps, their sums joined in shared memory, 256 sequences of up to
+// 700 tokens took 87 us instead of 42.
+// Each warp streams its tiles through a ring of 16-byte asynchronous copies: a group's codes and scales lie together in
+// the order in which lanes read them, so that copies and reads are linear in the lane, free of bank conflicts, and five
+// copies per 16 rows need one address.  (Bulk copies with an mbarrier measured the same at D 128 and slower at D 64, 70 us
+// against 66 for 16 sequences of 32k; they would need bounded waits besides.)
+// 32 sequences of up to 32k tokens, 32 query and 8 table heads, D 128: 137 us, 5.8 TB/s; 64 of 32k 369 us, 6.2 TB/s; one
+// of 512k 102 us, 5.6 TB/s.
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
@@ -207,11 +213,14 @@ struct Shape {
   static constexpr int kWarps = 4;
   static constexpr int kThreads = kWarps * 32;
   // Warps of an SM: 16 with 128 registers each while the accumulators are small, 12 with 168, 8 with 255.  A tile's two
-  // groups of 16 keys go through the products together, for the independent work.
+  // groups of 16 keys go through the products together, for the independent work.  Measured:
+  //   D 128, 8 columns, 32 sequences of up to 32k: 139 us with 12 warps, 141 with 16 and a stage less
+  //   D 128, 16 columns, 8 sequences of 32k: 80 us with 8, 83 with 12; fp32 queries, 8 columns: 71 with 12, 75 with 8
+  //   D 64, 32 columns, 16 sequences of 32k: 150 us with 8, 153 with 12, 196 with 16
   static constexpr int kSize = NB * NT * (SPLIT ? 2 : 1);
   // tiles of a run, at least: wide heads' parts cost more to join
   static constexpr int kMinTiles = NB == 8 ? 4 : 1;
-  static constexpr int kPerSm = kSize <= 4 && NB == 2 ? 16 : (kSize <= 8 && NB < 8 ? 12 : 8);
+  static constexpr int kPerSm = kSize <= 4 && NB == 2 ? 16 : (kSize <= (SPLIT ? 8 : 4) && NB < 8 ? 12 : 8);
   static constexpr int kBlocks = kPerSm / kWarps;
   static constexpr int kStages = NB == 8 ? 2 : 3;
   static constexpr int kStage = 2 * Gr::kBytes;

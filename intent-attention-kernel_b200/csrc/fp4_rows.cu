@@ -5,6 +5,8 @@
 // attention kernel's lanes read of them: lane 4 g + t has row g's channels 32 b + 8 t .. + 7 of K (all blocks b) and
 // channels 4 NB g .. of rows 2 t and 2 t + 1 of V.  Codes move as one run of 512 bytes (D 128) per plane, dense rows as
 // 64-byte runs and more.  A V byte whose other row is not part of the call keeps that row's half.
+// 8 x 8 x 32768 rows of D 128 read as bf16: 211 us, 6.4 TB/s; 4 ragged prompts of up to 8187 rows, 8 heads, fp16: 27 us to
+// write (5.1 TB/s), 28 to read.
 #include "fp4.cuh"
 
 namespace iak {
