@@ -78,32 +78,58 @@ __device__ __forceinline__ int slot_of(const DecP& p, int g) {
   return static_cast<int>((static_cast<unsigned>(g) * p.gpp_inv) >> 36);
 }
 
-// A warp's view of 32 sequences from `base` on: a lane's length, the tiles of its units, and those with all before it.
-struct Lane32 { int len, n, upto; };
-__device__ __forceinline__ Lane32 scan32(const DecP& p, int base) {
-  const int lane = threadIdx.x & 31, i = base + lane;
-  Lane32 s;
-  s.len = i < p.B ? seq_len(p, i) : 0;
-  s.n = i < p.B ? tiles_of(p, s.len) * p.HC : 0;
-  s.upto = s.n;
+// Inclusive sum over the lanes before and this one.
+__device__ __forceinline__ int lanes_upto(int n) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(~0u, s.upto, o);
-    if (lane >= o) s.upto += v;
+    const int v = __shfl_up_sync(~0u, n, o);
+    if (lane >= o) n += v;
   }
+  return n;
+}
+// A warp's view of the batch: lane l has the sequences from l * chunk on, n of the call's tiles, upto with those before.
+struct Lanes { int chunk, n, upto, len; };     // len: of the lane's last sequence (its only one where chunk is 1)
+__device__ __forceinline__ Lanes scan_batch(const DecP& p) {
+  Lanes s;
+  s.chunk = (p.B + 31) / 32;
+  s.n = s.len = 0;
+  const int first = (threadIdx.x & 31) * s.chunk;
+#pragma unroll 8
+  for (int b = first; b < min(first + s.chunk, p.B); ++b) {
+    s.len = seq_len(p, b);
+    s.n += tiles_of(p, s.len);
+  }
+  s.n *= p.HC;
+  s.upto = lanes_upto(s.n);
   return s;
 }
-// all tiles of the call (every lane of every warp has it); the host keeps their number within 31 bits
-__device__ __forceinline__ int total_tiles(const DecP& p, const Lane32& first) {
-  int sum = __shfl_sync(~0u, first.upto, 31);
-  if (p.B > 32) {
-    int rest = 0;
-    for (int b = 32 + (threadIdx.x & 31); b < p.B; b += 32) rest += tiles_of(p, seq_len(p, b));
-#pragma unroll
-    for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(~0u, rest, o);
-    sum += rest * p.HC;
+// all tiles of the call; the host keeps their number within 31 bits
+__device__ __forceinline__ int total_tiles(const Lanes& s) { return __shfl_sync(~0u, s.upto, 31); }
+// the sequence that holds tile t, its length, and t's offset among its tiles
+__device__ __forceinline__ void find_sequence(const DecP& p, const Lanes& s, int t, int& b, int& len, int& off) {
+  const int lane = threadIdx.x & 31;
+  const int l = __ffs(__ballot_sync(~0u, s.upto > t)) - 1;       // t < total: some lane has it
+  int before = __shfl_sync(~0u, s.upto - s.n, l);
+  b = l * s.chunk;
+  len = __shfl_sync(~0u, s.len, l);
+  if (s.chunk > 1) {
+    const int end = min(b + s.chunk, p.B);
+    for (; b < end; b += 32) {
+      const int own = b + lane < end ? seq_len(p, b + lane) : 0;
+      const int n = b + lane < end ? tiles_of(p, own) * p.HC : 0, upto = lanes_upto(n);
+      const unsigned hit = __ballot_sync(~0u, before + upto > t);
+      if (hit) {
+        const int k = __ffs(hit) - 1;
+        b += k;
+        len = __shfl_sync(~0u, own, k);
+        before += __shfl_sync(~0u, upto - n, k);
+        break;
+      }
+      before += __shfl_sync(~0u, upto, 31);
+    }
   }
-  return sum;
+  off = t - before;
 }
 
 // The tiles in equal runs, one for each of `used` warps, the first `more` of them with each + 1 tiles.
@@ -319,25 +345,12 @@ fp4_decode_kernel(const DecP p) {
       cur.left = tiles_of(p, cur.len);
       cur.off = (run - cur.b * p.HC) * cur.left;
     } else {
-      Lane32 s = scan32(p, 0);
-      runs = make_runs(p, total_tiles(p, s));
+      const Lanes s = scan_batch(p);
+      runs = make_runs(p, total_tiles(s));
       if (run >= runs.used) return;
       cur.at = run_begin(runs, run);
       cur.left = run_begin(runs, run + 1) - cur.at;
-      // the sequence that holds tile cur.at
-      int before = 0;
-      for (int base = 0; base < p.B; base += 32) {
-        if (base) s = scan32(p, base);
-        const unsigned hit = __ballot_sync(~0u, before + s.upto > cur.at);
-        if (hit) {
-          const int l = __ffs(hit) - 1;
-          cur.b = base + l;
-          cur.len = __shfl_sync(~0u, s.len, l);
-          cur.off = cur.at - before - __shfl_sync(~0u, s.upto - s.n, l);
-          break;
-        }
-        before += __shfl_sync(~0u, s.upto, 31);
-      }
+      find_sequence(p, s, cur.at, cur.b, cur.len, cur.off);
     }
     if (lane == 0) cursor = cur;
     __syncwarp();
@@ -466,17 +479,20 @@ fp4_decode_kernel(const DecP p) {
           }
         }
       }
-      auto value = [&](int b, int e) {
-        if (SPLIT) return __uint_as_float(raw[b][e]);
-        const unsigned u = e % 2 ? raw[b][e / 2] >> 16 : raw[b][e / 2] & 0xffffu;
-        return p.q_dtype == IAK_DT_F16 ? __half2float(__ushort_as_half(static_cast<unsigned short>(u)))
-                                       : __uint_as_float(u << 16);
+      // two neighbouring values
+      auto pair = [&](int b, int e) {
+        if constexpr (SPLIT) return make_float2(__uint_as_float(raw[b][2 * e]), __uint_as_float(raw[b][2 * e + 1]));
+        else return p.q_dtype == IAK_DT_F16 ? __half22float2(*reinterpret_cast<const __half2*>(&raw[b][e]))
+                                            : make_float2(__uint_as_float(raw[b][e] << 16), __uint_as_float(raw[b][e] & 0xffff0000u));
       };
       float amax = 0.f;
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(value(b, e)));
+        for (int e = 0; e < 4; ++e) {
+          const float2 v = pair(b, e);
+          amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+        }
       }
       amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
@@ -488,7 +504,8 @@ fp4_decode_kernel(const DecP p) {
         unsigned hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float y0 = value(b, 2 * e) * down, y1 = value(b, 2 * e + 1) * down;
+          const float2 v = pair(b, e);
+          const float y0 = v.x * down, y1 = v.y * down;
           hi[e] = pack_half2(y0, y1);
           if (SPLIT) {
             const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi[e]));
@@ -804,7 +821,7 @@ __global__ void __launch_bounds__(join_warps(TEAM) * 32) fp4_join_kernel(const D
   const int lane = threadIdx.x & 31, warp = TEAM == 1 ? 0 : threadIdx.x >> 5;
   const int item = TEAM == 1 ? blockIdx.x * join_warps(1) + (threadIdx.x >> 5) : blockIdx.x;
   const int record = item / rows + (p.by_unit ? 0 : 1), r = item % rows;
-  const int used = p.by_unit ? 0 : make_runs(p, total_tiles(p, scan32(p, 0))).used;
+  const int used = p.by_unit ? 0 : make_runs(p, total_tiles(scan_batch(p))).used;
   // every warp waits, so that this kernel never ends before the main one
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (item / rows >= records || (!p.by_unit && record >= used)) return;

@@ -256,6 +256,8 @@ SHAPES = [  # B, Ht, G, M, D, PS, lengths, dtype
     (1, 1, 48, 2, 128, 16, [600], "f16"),
     (40, 1, 2, 1, 64, 16, list(range(0, 400, 10)), "bf16"),
     (1, 3, 4, 1, 128, 128, [20011], "bf16"),
+    (1100, 1, 2, 1, 64, 16, [(7 * i) % 301 for i in range(1100)], "f16"),
+    (100, 2, 1, 2, 128, 16, [0] * 60 + [600] + [0] * 38 + [5], "bf16"),
 ]
 
 
