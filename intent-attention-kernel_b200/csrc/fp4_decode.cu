@@ -13,17 +13,19 @@
 //   m is raised only when a score passes it by 8 or more (P up to 2^15), which leaves the rescaling of O to few tiles.
 // What bounds it: the cache's bytes, 4.25 bits an element, and close behind them the issue slots: per 16 rows a warp
 // spends about 64 conversions, 64 multiplies and 16 products at D 128.
-// Work is cut into equal runs of tiles over all (sequence, table head, column group) units, one for each resident warp,
-// so that ragged batches, many short sequences and one long sequence fill the GPU alike; a unit cut over several runs
+// Work is cut into equal runs of steps over all (sequence, table head, column group) units, one for each resident warp,
+// so that ragged batches, many short sequences and one long sequence fill the GPU alike.  A step is a tile; what a unit
+// costs besides its tiles counts as three (256 sequences of up to 512 tokens: 31 us, with equal runs of tiles 44; 16 of up
+// to 8001 with 4 queries and D 256: 43.5 against 48).  A unit cut over several runs
 // leaves partial (m, l, O) that a second kernel adds in order of the runs (no atomics: results do not depend on timing).
 // Warps share nothing: with units cut per block of 8 warps, their sums joined in shared memory, 256 sequences of up to
-// 700 tokens took 87 us instead of 42.
+// 700 tokens took 87 us instead of 39.
 // Each warp streams its tiles through a ring of 16-byte asynchronous copies: a group's codes and scales lie together in
 // the order in which lanes read them, so that copies and reads are linear in the lane, free of bank conflicts, and five
 // copies per 16 rows need one address.  (Bulk copies with an mbarrier measured the same at D 128 and slower at D 64, 70 us
 // against 66 for 16 sequences of 32k; they would need bounded waits besides.)
-// 32 sequences of up to 32k tokens, 32 query and 8 table heads, D 128: 137 us, 5.8 TB/s; 64 of 32k 369 us, 6.2 TB/s; one
-// of 512k 102 us, 5.6 TB/s.
+// 32 sequences of up to 32k tokens, 32 query and 8 table heads, D 128: 134 us, 5.9 TB/s; 64 of 32k 364 us, 6.3 TB/s; one
+// of 512k 101 us, 5.7 TB/s; 4096 of 256 tokens 247 us, 4.6 TB/s.
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
@@ -37,6 +39,7 @@ namespace {
 constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
 constexpr int kDirectTiles = 8;    // units of at most so many tiles are never cut
+constexpr int kOpen = 3;           // a unit's queries, first copies and output take a warp as long as so many tiles
 constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
 constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small P stay normal halves
 
@@ -72,6 +75,8 @@ __device__ __forceinline__ int seq_len(const DecP& p, int b) {
 __device__ __forceinline__ int tiles_of(const DecP& p, int len) {
   return max(1, (len + kTileKeys - 1) / kTileKeys);
 }
+// A unit's steps: kOpen for what a warp does before and after its tiles, then the tiles.
+__device__ __forceinline__ int steps_of(const DecP& p, int len) { return tiles_of(p, len) + kOpen; }
 
 // Table entry of group g: g / gpp, exact for g < 2^26 and gpp <= 2^10, where g times the inverse's excess stays below 2^36.
 __device__ __forceinline__ int slot_of(const DecP& p, int g) {
@@ -88,36 +93,72 @@ __device__ __forceinline__ int lanes_upto(int n) {
   }
   return n;
 }
-// A warp's view of the batch: lane l has the sequences from l * chunk on, n of the call's tiles, upto with those before.
-struct Lanes { int chunk, n, upto, len; };     // len: of the lane's last sequence (its only one where chunk is 1)
-__device__ __forceinline__ Lanes scan_batch(const DecP& p) {
+// Where a run's tiles lie is found in the steps of all units.  A warp's lane holds the steps of one sequence (up to 32
+// of them, chunk 0), or of four threads' sequences: a block's thread i adds up those from i * chunk on, in `sums`; upto
+// counts with all lanes before.  (With sums of its own for each warp, the join's too, 4096 sequences of 256 tokens took
+// 365 us instead of 248.)
+constexpr int kScan = 128;
+struct Lanes { int chunk; int4 n; int upto, len; };
+__device__ __forceinline__ int four(const int4& n) { return n.x + n.y + n.z + n.w; }
+__device__ __forceinline__ Lanes scan_batch(const DecP& p, int* sums) {
   Lanes s;
-  s.chunk = (p.B + 31) / 32;
-  s.n = s.len = 0;
-  const int first = (threadIdx.x & 31) * s.chunk;
+  s.len = 0;
+  if (p.B <= 32) {
+    s.chunk = 0;
+    s.n = make_int4(0, 0, 0, 0);
+    const int b = threadIdx.x & 31;
+    if (b < p.B) {
+      s.len = seq_len(p, b);
+      s.n.x = steps_of(p, s.len) * p.HC;
+    }
+  } else {
+    s.chunk = (p.B + kScan - 1) / kScan;
+    int n = 0;
+    const int first = threadIdx.x * s.chunk;
 #pragma unroll 8
-  for (int b = first; b < min(first + s.chunk, p.B); ++b) {
-    s.len = seq_len(p, b);
-    s.n += tiles_of(p, s.len);
+    for (int b = first; b < min(first + s.chunk, p.B); ++b) n += steps_of(p, seq_len(p, b));
+    sums[threadIdx.x] = n * p.HC;
+    __syncthreads();
+    s.n = reinterpret_cast<const int4*>(sums)[threadIdx.x & 31];
   }
-  s.n *= p.HC;
-  s.upto = lanes_upto(s.n);
+  s.upto = lanes_upto(four(s.n));
   return s;
 }
-// all tiles of the call; the host keeps their number within 31 bits
-__device__ __forceinline__ int total_tiles(const Lanes& s) { return __shfl_sync(~0u, s.upto, 31); }
-// the sequence that holds tile t, its length, and t's offset among its tiles
+// all steps of the call; the host keeps their number within 31 bits
+__device__ __forceinline__ int total_steps(const Lanes& s) { return __shfl_sync(~0u, s.upto, 31); }
+// the sequence that holds step t, its length, and t's offset among its steps
 __device__ __forceinline__ void find_sequence(const DecP& p, const Lanes& s, int t, int& b, int& len, int& off) {
   const int lane = threadIdx.x & 31;
   const int l = __ffs(__ballot_sync(~0u, s.upto > t)) - 1;       // t < total: some lane has it
-  int before = __shfl_sync(~0u, s.upto - s.n, l);
-  b = l * s.chunk;
-  len = __shfl_sync(~0u, s.len, l);
-  if (s.chunk > 1) {
+  int before = __shfl_sync(~0u, s.upto - four(s.n), l);
+  if (s.chunk == 0) {
+    b = l;
+    len = __shfl_sync(~0u, s.len, l);
+    off = t - before;
+    return;
+  }
+  const int n0 = __shfl_sync(~0u, s.n.x, l), n1 = __shfl_sync(~0u, s.n.y, l), n2 = __shfl_sync(~0u, s.n.z, l);
+  b = 4 * l;
+  if (t >= before + n0) {
+    before += n0;
+    ++b;
+    if (t >= before + n1) {
+      before += n1;
+      ++b;
+      if (t >= before + n2) {
+        before += n2;
+        ++b;
+      }
+    }
+  }
+  b *= s.chunk;
+  if (s.chunk == 1) {
+    len = seq_len(p, b);
+  } else {
     const int end = min(b + s.chunk, p.B);
     for (; b < end; b += 32) {
       const int own = b + lane < end ? seq_len(p, b + lane) : 0;
-      const int n = b + lane < end ? tiles_of(p, own) * p.HC : 0, upto = lanes_upto(n);
+      const int n = b + lane < end ? steps_of(p, own) * p.HC : 0, upto = lanes_upto(n);
       const unsigned hit = __ballot_sync(~0u, before + upto > t);
       if (hit) {
         const int k = __ffs(hit) - 1;
@@ -132,7 +173,7 @@ __device__ __forceinline__ void find_sequence(const DecP& p, const Lanes& s, int
   off = t - before;
 }
 
-// The tiles in equal runs, one for each of `used` warps, the first `more` of them with each + 1 tiles.
+// The steps in equal runs, one for each of `used` warps, the first `more` of them with each + 1.
 struct Runs { int used, each, more; };
 __device__ __forceinline__ Runs make_runs(const DecP& p, int total) {
   Runs r;
@@ -154,7 +195,7 @@ __device__ __forceinline__ float* part_at(const DecP& p, int run, int which, int
 }
 // What the join kernel reads of a unit cut over several runs.  Where there are no more units than runs a record per
 // unit, written by the run that has its first tile; else one per border between two runs, written by the run that the
-// border begins and empty unless it is a unit's first cut.
+// border begins (if there is one) and empty unless it is a unit's first cut.
 struct Cut { int b, h, j0, first, which, last; };   // first, last: runs with a part; which: first's; last < 0: none
 __device__ __forceinline__ Cut* cuts(const DecP& p) {
   return reinterpret_cast<Cut*>(p.ws + static_cast<int64_t>(p.runs) * 2 * p.cols * (p.pool.D + 4));
@@ -227,8 +268,8 @@ __device__ __forceinline__ void lds_words(unsigned a, unsigned (&w)[NW]) {
 }
 
 // ------------------------------------------------------------- shared layout
-struct Cursor { int left, off, at, b, len; };   // tiles left to the run; the next one, of sequence b and of all
-struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, at; };   // at: its first tile, of all
+struct Cursor { int left, off, at, b, len; };   // steps left to the run; the next one, of sequence b and of all
+struct Segment { int b, h, cg, len, n_tiles, c_begin, c_end, at; };   // at: the unit's first step, of all
 
 // What a kernel for D = 32 NB, 8 NT columns a unit and (SPLIT) fp32 queries is made of.  Warps work alone; a block has
 // four so that an SM's share can be cut finely.
@@ -253,7 +294,9 @@ struct Shape {
   static constexpr int kRing = kStages * kStage;
   static constexpr int kQuery = NT * NB * 512 * (SPLIT ? 2 : 1);
   static constexpr int kWarpBytes = kRing + kQuery;        // a multiple of 128
-  static constexpr int kSmem = kWarps * (kWarpBytes + static_cast<int>(sizeof(Cursor)) + static_cast<int>(sizeof(Segment)));
+  static constexpr int kOwnBytes = kWarpBytes + static_cast<int>(sizeof(Cursor)) + static_cast<int>(sizeof(Segment));
+  static constexpr int kSmem = kWarps * kOwnBytes + kScan * static_cast<int>(sizeof(int));
+  static_assert(kThreads == kScan && kWarps * kOwnBytes % 16 == 0, "the block's sums of the batch");
   static_assert(kWarpBytes % 128 == 0, "copies and reads are linear runs of 128 bytes");
   static_assert(kBlocks * (kSmem + 1024) <= 228 * 1024, "shared memory of an SM");
 };
@@ -342,12 +385,15 @@ fp4_decode_kernel(const DecP p) {
       cur.b = run / p.HC;
       if (cur.b >= p.B) return;
       cur.len = seq_len(p, cur.b);
-      cur.left = tiles_of(p, cur.len);
+      cur.left = steps_of(p, cur.len);
       cur.off = (run - cur.b * p.HC) * cur.left;
     } else {
-      const Lanes s = scan_batch(p);
-      runs = make_runs(p, total_tiles(s));
-      if (run >= runs.used) return;
+      const Lanes s = scan_batch(p, reinterpret_cast<int*>(smem + kWarps * L::kOwnBytes));
+      runs = make_runs(p, total_steps(s));
+      if (run >= runs.used) {
+        if (lane == 0 && !p.by_unit) cuts(p)[run] = {0, 0, 0, 0, 0, -1};
+        return;
+      }
       cur.at = run_begin(runs, run);
       cur.left = run_begin(runs, run + 1) - cur.at;
       find_sequence(p, s, cur.at, cur.b, cur.len, cur.off);
@@ -421,17 +467,17 @@ fp4_decode_kernel(const DecP p) {
       sg.b = cur.b;
       sg.len = cur.len;
       sg.n_tiles = tiles_of(p, cur.len);
-      sg.at = cur.at;
-      const int unit = cur.off / sg.n_tiles;                      // of the sequence: table head, column group
-      sg.c_begin = cur.off - unit * sg.n_tiles;
-      sg.c_end = min(sg.n_tiles, sg.c_begin + cur.left);
+      const int steps = sg.n_tiles + kOpen, unit = cur.off / steps;   // of the sequence: table head, column group
+      const int from = cur.off - unit * steps, n = min(steps - from, cur.left);
+      sg.at = cur.at - from;
+      sg.c_begin = max(from - kOpen, 0);
+      sg.c_end = max(from + n - kOpen, 0);
       sg.h = p.CG == 1 ? unit : unit / p.CG;
       sg.cg = unit - sg.h * p.CG;
-      const int n = sg.c_end - sg.c_begin;
       cur.left -= n;
       cur.off += n;
       cur.at += n;
-      if (cur.off == sg.n_tiles * p.HC) {
+      if (cur.off == steps * p.HC) {
         cur.off = 0;
         ++cur.b;
         cur.len = cur.left > 0 && cur.b < p.B ? seq_len(p, cur.b) : 0;
@@ -442,8 +488,9 @@ fp4_decode_kernel(const DecP p) {
         cursor = cur;
       }
       __syncwarp();
+      if (sg.c_begin == sg.c_end) continue;                       // the run ends before the unit's first tile
       // (an empty pool has no group that could stand in for the missing ones: its tiles are left out)
-      n_mine = p.pool.num_pages > 0 ? n : 0;
+      n_mine = p.pool.num_pages > 0 ? sg.c_end - sg.c_begin : 0;
     }
     next_id = load_id(0);
 
@@ -730,16 +777,16 @@ fp4_decode_kernel(const DecP p) {
     const int which = begins_run ? 0 : 1;
     const bool whole = segment.c_begin == 0 && segment.c_end == segment.n_tiles;
     if (!p.direct && lane == 0) {
-      const int begin = segment.at - segment.c_begin;              // the unit's first tile
+      const int begin = segment.at + kOpen, end = begin + segment.n_tiles - 1;   // the steps of the first and last tile
       Cut d = {segment.b, segment.h, segment.cg * COLS, run, which, -1};
       if (p.by_unit) {
-        if (!whole) d.last = run_of(runs, begin + segment.n_tiles - 1);
+        if (!whole) d.last = run_of(runs, end);
         if (segment.c_begin == 0) cuts(p)[segment.b * p.HC + segment.h * p.CG + segment.cg] = d;
       } else if (begins_run) {
         d.first = run - 1;
         if (segment.c_begin > 0 && run_begin(runs, run - 1) <= begin) {
-          d.which = run_begin(runs, run - 1) == begin ? 0 : 1;
-          d.last = run_of(runs, begin + segment.n_tiles - 1);
+          d.which = run_begin(runs, run - 1) >= segment.at ? 0 : 1;
+          d.last = run_of(runs, end);
         }
         cuts(p)[run] = d;
       }
@@ -821,10 +868,9 @@ __global__ void __launch_bounds__(join_warps(TEAM) * 32) fp4_join_kernel(const D
   const int lane = threadIdx.x & 31, warp = TEAM == 1 ? 0 : threadIdx.x >> 5;
   const int item = TEAM == 1 ? blockIdx.x * join_warps(1) + (threadIdx.x >> 5) : blockIdx.x;
   const int record = item / rows + (p.by_unit ? 0 : 1), r = item % rows;
-  const int used = p.by_unit ? 0 : make_runs(p, total_tiles(scan_batch(p))).used;
   // every warp waits, so that this kernel never ends before the main one
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (item / rows >= records || (!p.by_unit && record >= used)) return;
+  if (item / rows >= records) return;
   const Cut d = cuts(p)[record];
   const int n = d.last - d.first + 1, j0 = d.j0 + r * per;
   if (d.last < 0 || j0 >= p.NC) return;
@@ -935,7 +981,7 @@ int make_plan(DecP& p, Plan* plan) {
   p.HC = static_cast<int>(hc);
   p.min_tiles = L::kMinTiles;
   const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + kTileKeys - 1) / kTileKeys;
-  if (most * units > 0x7fffffffLL - 64)
+  if ((most + kOpen) * units > 0x7fffffffLL - 64)
     return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: tables of more than 2^31 tiles of %d tokens", kTileKeys);
   // units that a warp covers about as fast as two would with their parts joined
   p.direct = most <= kDirectTiles;
