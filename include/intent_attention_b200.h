@@ -610,7 +610,8 @@ int iak_fp4_read(const iak_fp4_pool* pool, const iak_fp4_rows_args* args, void* 
  * as halves after a power of two that puts the row's largest in [1, 2) (exact
  * for elements down to 2^-14 of it), fp32 ones as the sum of two halves;
  * probabilities round to halves (fp32 queries: to two).
- * The workspace holds partial sums; its content need not survive the call. */
+ * out may be q itself, with the same type and strides.  The workspace, 16-byte
+ * aligned, holds partial sums; its content need not survive the call. */
 typedef struct iak_fp4_decode_args {
   const void* q; int32_t q_dtype; int64_t q_stride_b, q_stride_h, q_stride_m;
   void* out; int32_t out_dtype; int64_t out_stride_b, out_stride_h, out_stride_m;
@@ -659,7 +660,8 @@ int iak_pages_workspace_size(const iak_seq_pages* pages, size_t* bytes);
  * counted once each: a slot with new_tokens < 0, one whose tokens would pass
  * table_width pages, one whose open page lies outside the pool, and, when the
  * free pages run out, the first slot that does not fit and every later one
- * that gets tokens. */
+ * that gets tokens.  1024 (slot, head) pairs may want 2^31 pages at most, by
+ * table_width. */
 int iak_pages_grow(const iak_seq_pages* pages, const iak_page_planes* planes, const int32_t* new_tokens,
                    int32_t* rejected, void* workspace, size_t workspace_bytes, void* stream);
 /* takes tokens[s] tokens off the end of every slot (draft tokens that were not

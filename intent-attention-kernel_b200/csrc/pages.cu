@@ -22,6 +22,8 @@ constexpr int kCluster = 8;
 constexpr int kPlanThreads = 1024;
 constexpr int kActThreads = 256;
 constexpr int kListThreads = 512;
+// Of a page that a warp copies.  (One page of 4.4 MB copied: 18 us, by a single warp 273.)
+constexpr int64_t kPiece = 16384;
 
 struct Seq {
   int32_t* refs; int num_pages;
@@ -31,7 +33,7 @@ struct Seq {
 };
 struct Planes {
   char* base[IAK_MAX_PLANES]; int64_t bytes[IAK_MAX_PLANES]; uint32_t formats[IAK_MAX_PLANES];
-  int num;
+  int num, pieces;    // pieces: of the largest plane's pages
   void* tags; int tag_bytes; uint8_t tag_map[16]; uint8_t tag_default;
 };
 
@@ -69,8 +71,9 @@ __device__ __forceinline__ int block_before(int v, int* all) {
   return inc - v + (warp ? warp_sum[warp - 1] : 0);
 }
 
-// copy page `from` to page `to` by one warp: the planes of the page's format, and its tag
-__device__ __forceinline__ void copy_page(const Planes& pl, int64_t from, int64_t to) {
+// copy piece `piece` of page `from` to page `to` by one warp: kPiece bytes of each plane of the page's format, and with
+// the first the tag
+__device__ __forceinline__ void copy_piece(const Planes& pl, int64_t from, int64_t to, int piece) {
   const int lane = threadIdx.x & 31;
   uint32_t mask = ~0u;
   if (pl.tags) {
@@ -78,16 +81,17 @@ __device__ __forceinline__ void copy_page(const Planes& pl, int64_t from, int64_
                                       : static_cast<const int32_t*>(pl.tags)[from];
     mask = 1u << ((tag >= 0 && tag < 16) ? pl.tag_map[tag] : pl.tag_default);
     __syncwarp();
-    if (lane == 0) {
+    if (lane == 0 && piece == 0) {
       if (pl.tag_bytes == 1) static_cast<uint8_t*>(pl.tags)[to] = static_cast<uint8_t>(tag);
       else static_cast<int32_t*>(pl.tags)[to] = tag;
     }
   }
   for (int i = 0; i < pl.num; ++i) {
     if (pl.tags && !(pl.formats[i] & mask)) continue;
-    const int64_t n = pl.bytes[i];
-    const char* src = pl.base[i] + from * n;
-    char* dst = pl.base[i] + to * n;
+    const int64_t skip = piece * kPiece, n = min(pl.bytes[i] - skip, kPiece);
+    if (n <= 0) continue;
+    const char* src = pl.base[i] + from * pl.bytes[i] + skip;
+    char* dst = pl.base[i] + to * pl.bytes[i] + skip;
     const uintptr_t low = reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(n);
     if ((low & 15) == 0) {
       const uint4* s = reinterpret_cast<const uint4*>(src);
@@ -162,97 +166,100 @@ struct Masks {
 };
 
 // ------------------------------------------------------------------------ grow
-// Scratch: first[S * Ht] = rank of the (slot, head)'s first new page, < 0 = gets none; shared[S * Ht] (copy the open
-// page); old_pages[S], fresh[S]; new_ids[rank].
-struct GrowScratch { int32_t* first; int32_t* shared; int32_t* old_pages; int32_t* fresh; int32_t* new_ids; };
+// Scratch: first[S * Ht] = rank of the (slot, head)'s first new page, < 0 = gets none; open[S * Ht] = the page to copy,
+// < 0 = none; bad[S] (an open page lies outside the pool); old_pages[S], fresh[S]; new_ids[rank].
+struct GrowScratch { int32_t* first; int32_t* open; int32_t* bad; int32_t* old_pages; int32_t* fresh; int32_t* new_ids; };
 
+// Each block of the cluster plans an eighth of the slots, too.  (All in one block, every (slot, head) reading all of the
+// slot's open pages: 466 us for 256 slots of 128 heads, now 57.)
 __global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kPlanThreads)
 grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const GrowScratch w) {
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank());
-  __shared__ int live_here, wanted, cut;               // cut: first slot that the free pages do not reach
+  __shared__ int live_here, cut_here;                  // cut: first slot that the free pages do not reach
+  __shared__ long long wanted_here;                    // pages that the block's slots want
+  const int per_block = (q.S + kCluster - 1) / kCluster;
+  const int s_begin = min(q.S, per_block * rank), s_end = min(q.S, s_begin + per_block);
+  const int i_begin = s_begin * q.Ht, i_end = s_end * q.Ht;        // (the host keeps S * Ht within 31 bits)
+  // the slot's tokens, those to come, and whether they fit its table
+  auto read_slot = [&](int s, int* len, int* add) {
+    *len = max(q.lengths[s], 0);
+    *add = more[s];
+    const int64_t total = static_cast<int64_t>(*len) + *add;
+    return *add > 0 && total <= static_cast<int64_t>(q.W) * q.PS && total <= 0x7fffffff;
+  };
+  if (threadIdx.x == 0) cut_here = q.S;
+  for (int s = s_begin + threadIdx.x; s < s_end; s += kPlanThreads) w.bad[s] = 0;
+  __syncthreads();
+  // open pages; one outside the pool refuses its slot, for all heads
+  for (int i = i_begin + threadIdx.x; i < i_end; i += kPlanThreads) {
+    const int s = i / q.Ht, h = i - s * q.Ht;
+    int len, add, open = -1;
+    if (read_slot(s, &len, &add) && len % q.PS != 0) {
+      const int id = q.table[s * q.sb + h * q.sh + pages_of(len, q.PS) - 1];
+      if (!in_pool(q, id)) w.bad[s] = 1;
+      else if (q.refs[id] > 1) open = id;
+    }
+    w.open[i] = open;
+  }
+  __syncthreads();
+  // ranks of the pages wanted, in order of (slot, head), from the block's first on
+  int refused = 0;
+  int64_t base = 0;
+  for (int i0 = i_begin; i0 < i_end; i0 += kPlanThreads) {
+    const int i = i0 + threadIdx.x;
+    int need = 0;
+    bool ok = false;
+    if (i < i_end) {
+      const int s = i / q.Ht, h = i - s * q.Ht;
+      int len, add;
+      ok = read_slot(s, &len, &add) && !w.bad[s];
+      const int old = ok ? pages_of(len, q.PS) : 0, fresh = ok ? pages_of(len + add, q.PS) - old : 0;
+      need = fresh + (ok && w.open[i] >= 0 ? 1 : 0);
+      if (h == 0) {
+        w.old_pages[s] = old;
+        w.fresh[s] = fresh;
+        if (add != 0 && !ok) ++refused;
+      }
+    }
+    int all;
+    const int before = block_before(need, &all);       // (the host keeps 1024 rows' pages within 31 bits)
+    if (i < i_end) w.first[i] = ok ? static_cast<int32_t>(min(base + before, static_cast<int64_t>(0x7fffffff))) : -1;
+    base += all;
+  }
   int begin, end;
   slice_of(q.num_pages, rank, &begin, &end);
-  const int n = q.S * q.Ht;                            // (the host keeps it within 31 bits)
-  int refused = 0;
-  if (rank == 0) {
-    // ranks of the pages wanted, in order of (slot, head); one thread per (slot, head)
-    if (threadIdx.x == 0) {
-      cut = q.S;
-      wanted = 0;
-    }
-    int64_t base = 0;
-    for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
-      const int i = i0 + threadIdx.x;
-      int need = 0;
-      bool ok = false;
-      if (i < n) {
-        const int s = i / q.Ht, h = i - s * q.Ht;
-        const int len = max(q.lengths[s], 0), add = more[s];
-        const int64_t total = static_cast<int64_t>(len) + add;
-        ok = add > 0 && total <= static_cast<int64_t>(q.W) * q.PS && total <= 0x7fffffff;
-        const int old = ok ? pages_of(len, q.PS) : 0;
-        bool copy = false;
-        if (ok && len % q.PS != 0) {
-          // an open page outside the pool refuses the slot, for all of its heads
-          const int32_t* open = q.table + s * q.sb + old - 1;
-#pragma unroll 8
-          for (int k = 0; k < q.Ht; ++k) ok = in_pool(q, open[k * q.sh]) & ok;
-          copy = ok && q.refs[open[h * q.sh]] > 1;
-        }
-        const int fresh = ok ? pages_of(static_cast<int>(total), q.PS) - old : 0;
-        need = fresh + (copy ? 1 : 0);
-        w.shared[i] = copy;
-        if (h == 0) {
-          w.old_pages[s] = old;
-          w.fresh[s] = fresh;
-          if (add != 0 && !ok) ++refused;
-        }
-      }
-      int all;
-      const int before = block_before(need, &all);
-      if (i < n) w.first[i] = ok ? static_cast<int32_t>(min(base + before, static_cast<int64_t>(0x7fffffff))) : -1;
-      base += all;
-    }
-  }
   const Masks masks(q.refs, begin, end);
   const int live = masks.count(end);
-  if (threadIdx.x == 0) live_here = live;
+  if (threadIdx.x == 0) {
+    live_here = live;
+    wanted_here = base;
+  }
   cluster.sync();
   int free_before = 0, free_all = 0;                   // free pages below this slice, in all
+  int64_t wanted_before = 0, wanted_all = 0;
   for (int r = 0; r < kCluster; ++r) {
     int bb, be;
     slice_of(q.num_pages, r, &bb, &be);
     const int f = be - bb - *cluster.map_shared_rank(&live_here, r);
-    if (r < rank) free_before += f;
+    const int64_t n = *cluster.map_shared_rank(&wanted_here, r);
+    if (r < rank) {
+      free_before += f;
+      wanted_before += n;
+    }
     free_all += f;
+    wanted_all += n;
   }
-  if (rank == 0) {
-    // a slot that does not fit, and every later one that gets tokens, stays as it is
-    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
-      const int s = i / q.Ht;
-      if (w.first[i] >= 0 && static_cast<int64_t>(w.first[i]) + w.fresh[s] + w.shared[i] > free_all) atomicMin(&cut, s);
-    }
-    __syncthreads();
-    const int last = cut;
-    int take = 0;
-    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
-      const int s = i / q.Ht, h = i - s * q.Ht;
-      if (w.first[i] < 0) continue;
-      if (s >= last) {
-        w.first[i] = -1;
-        if (h == 0) ++refused;
-      } else {
-        take = max(take, w.first[i] + w.fresh[s] + w.shared[i]);
-        if (h == 0) q.lengths[s] = max(q.lengths[s], 0) + more[s];
-      }
-    }
-    if (take) atomicMax(&wanted, take);
-    if (rejected && refused) atomicAdd(rejected, refused);
+  // a slot that does not fit, and every later one that gets tokens, stays as it is
+  for (int i = i_begin + threadIdx.x; i < i_end; i += kPlanThreads) {
+    if (w.first[i] < 0) continue;
+    const int s = i / q.Ht;
+    const int64_t first = wanted_before + w.first[i];
+    w.first[i] = static_cast<int32_t>(min(first, static_cast<int64_t>(0x7fffffff)));
+    if (first + w.fresh[s] + (w.open[i] >= 0 ? 1 : 0) > free_all) atomicMin(&cut_here, s);
   }
-  cluster.sync();
-  const int want = *cluster.map_shared_rank(&wanted, 0);
   // the free pages of this slice, in ascending order
+  const int want = static_cast<int>(min(wanted_all, static_cast<int64_t>(free_all)));
   int at = free_before;
   for (int p0 = begin; p0 < end && at < want; p0 += kRun) {
     const int p = p0 + 32 * static_cast<int>(threadIdx.x);
@@ -262,28 +269,44 @@ grow_plan_kernel(const Seq q, const int32_t* more, int32_t* rejected, const Grow
     for (; free_bits && k < want; free_bits &= free_bits - 1, ++k) w.new_ids[k] = p + __ffs(free_bits) - 1;
     at += all;
   }
+  cluster.sync();
+  int last = q.S;
+  for (int r = 0; r < kCluster; ++r) last = min(last, *cluster.map_shared_rank(&cut_here, r));
+  for (int i = i_begin + threadIdx.x; i < i_end; i += kPlanThreads) {
+    if (w.first[i] < 0) continue;
+    const int s = i / q.Ht;
+    const bool slot = i - s * q.Ht == 0;
+    if (s >= last) {
+      w.first[i] = -1;
+      if (slot) ++refused;
+    } else if (slot) {
+      q.lengths[s] = max(q.lengths[s], 0) + more[s];
+    }
+  }
+  if (rejected && refused) atomicAdd(rejected, refused);
   cluster.sync();                                      // no block leaves while another may read its counts
 }
 
 __global__ void __launch_bounds__(kActThreads) grow_act_kernel(const Seq q, const Planes pl, const GrowScratch w) {
   const int warps = kActThreads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n = q.S * q.Ht;                            // (the host keeps it within 31 bits)
-  for (int i = blockIdx.x * warps + warp; i < n; i += gridDim.x * warps) {
+  const int64_t jobs = static_cast<int64_t>(q.S) * q.Ht * pl.pieces;
+  for (int64_t job = blockIdx.x * warps + warp; job < jobs; job += gridDim.x * warps) {
+    const int i = static_cast<int>(job / pl.pieces), piece = static_cast<int>(job - static_cast<int64_t>(i) * pl.pieces);
     const int first = w.first[i];
     if (first < 0) continue;
     const int s = i / q.Ht, h = i - s * q.Ht;
     int32_t* row = q.table + s * q.sb + h * q.sh;
-    const int old = w.old_pages[s], fresh = w.fresh[s], copy = w.shared[i];
+    const int old = w.old_pages[s], fresh = w.fresh[s], from = w.open[i], copy = from >= 0 ? 1 : 0;
     if (copy) {
-      const int from = row[old - 1], to = w.new_ids[first];
-      copy_page(pl, from, to);
-      __syncwarp();
-      if (lane == 0) {
+      const int to = w.new_ids[first];
+      copy_piece(pl, from, to, piece);
+      if (lane == 0 && piece == 0) {
         row[old - 1] = to;
         q.refs[to] = 1;
         atomicSub(&q.refs[from], 1);
       }
     }
+    if (piece) continue;
     for (int k = lane; k < fresh; k += 32) {
       const int id = w.new_ids[first + copy + k];
       row[old + k] = id;
@@ -430,10 +453,12 @@ __global__ void __launch_bounds__(kActThreads) compact_act_kernel(const Seq q, c
   const int n = w.head[0], moves = w.head[1];
   if (moves == 0) return;
   const int warps = kActThreads / 32, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int k = blockIdx.x * warps + warp; k < moves; k += gridDim.x * warps) {
+  const int64_t jobs = static_cast<int64_t>(moves) * pl.pieces;
+  for (int64_t job = blockIdx.x * warps + warp; job < jobs; job += gridDim.x * warps) {
+    const int k = static_cast<int>(job / pl.pieces), piece = static_cast<int>(job - static_cast<int64_t>(k) * pl.pieces);
     const int from = w.from[k], to = w.to[k];
-    copy_page(pl, from, to);
-    if (lane == 0) {
+    copy_piece(pl, from, to, piece);
+    if (lane == 0 && piece == 0) {
       q.refs[to] = q.refs[from];
       q.refs[from] = 0;
     }
@@ -478,8 +503,12 @@ int check_planes(const iak_page_planes* a, const char* what, Planes* p) {
     p->base[i] = static_cast<char*>(a->base[i]);
     p->bytes[i] = a->bytes[i];
     p->formats[i] = a->formats[i];
+    const int64_t pieces = (a->bytes[i] + kPiece - 1) / kPiece;
+    if (pieces > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "%s: pages too large", what);
+    p->pieces = std::max(p->pieces, static_cast<int>(pieces));
   }
   p->num = a->num_planes;
+  p->pieces = std::max(p->pieces, 1);                  // (tables and counts follow without planes too)
   p->tags = a->page_tags;
   if (a->page_tags && a->tag_bytes != 1 && a->tag_bytes != 4)
     return fail(IAK_ERR_INVALID_ARG, "%s: tag_bytes must be 1 or 4", what);
@@ -496,7 +525,7 @@ int check_planes(const iak_page_planes* a, const char* what, Planes* p) {
 // int32 words of scratch: the larger of what grow and compact use
 size_t scratch_words(const iak_seq_pages* a) {
   const size_t rows = static_cast<size_t>(a->num_slots) * a->num_table_heads;
-  const size_t grow = 2 * rows + 2 * static_cast<size_t>(a->num_slots) + static_cast<size_t>(a->num_pages);
+  const size_t grow = 2 * rows + 3 * static_cast<size_t>(a->num_slots) + static_cast<size_t>(a->num_pages);
   const size_t compact = 2 + 3 * static_cast<size_t>(a->num_pages);
   return std::max(grow, compact);
 }
@@ -539,16 +568,19 @@ extern "C" int iak_pages_grow(const iak_seq_pages* pages, const iak_page_planes*
   if (!new_tokens) return fail(IAK_ERR_INVALID_ARG, "%s: null new_tokens", what);
   if (int st = check_ws(pages, workspace, workspace_bytes, what)) return st;
   const int64_t rows = static_cast<int64_t>(q.S) * q.Ht;
+  if (std::min<int64_t>(rows, kPlanThreads) * (static_cast<int64_t>(q.W) + 1) > 0x7fffffffLL)
+    return fail(IAK_ERR_UNSUPPORTED, "%s: tables of %d pages a row", what, q.W);
   GrowScratch w;
   w.first = static_cast<int32_t*>(workspace);
-  w.shared = w.first + rows;
-  w.old_pages = w.shared + rows;
+  w.open = w.first + rows;
+  w.bad = w.open + rows;
+  w.old_pages = w.bad + q.S;
   w.fresh = w.old_pages + q.S;
   w.new_ids = w.fresh + q.S;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   grow_plan_kernel<<<kCluster, kPlanThreads, 0, s>>>(q, new_tokens, rejected, w);
   if (int st = check_cuda(cudaGetLastError(), "grow plan launch")) return st;
-  const int64_t blocks = std::min<int64_t>((rows + kActThreads / 32 - 1) / (kActThreads / 32), 8 * device_sm_count());
+  const int64_t blocks = std::min<int64_t>((rows * pl.pieces + kActThreads / 32 - 1) / (kActThreads / 32), 8 * device_sm_count());
   grow_act_kernel<<<static_cast<unsigned>(blocks), kActThreads, 0, s>>>(q, pl, w);
   return check_cuda(cudaGetLastError(), "grow launch");
 }

@@ -263,7 +263,7 @@ def paged_decode_fp4(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Tensor, l
     tokens before ``lengths[b] - (M - 1 - m)``.  Query head h reads table head
     h // (Hq // Ht).  Lengths beyond the table count as its capacity; pages
     outside the pool are not seen; a query that sees no token gives 0.
-    ``sm_scale`` defaults to 1 / sqrt(D).
+    ``sm_scale`` defaults to 1 / sqrt(D).  ``out`` may be ``q`` itself.
     """
     scale = 1.0 / math.sqrt(pool.head_dim) if sm_scale is None else float(sm_scale)
     return _decode(q, pool, page_table, lengths, scale, out, out_dtype)

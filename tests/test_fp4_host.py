@@ -125,6 +125,22 @@ def test_page_args_rejected_on_the_host():
     assert L.iak_pages_free(r(s), 256, 1, None, None) == N.IAK_ERR_INVALID_ARG
 
 
+def test_shrink_and_wide_tables_rejected_on_the_host():
+    L = N.lib()
+    r = ctypes.byref
+    s, pl = N.SeqPages(), N.PagePlanes()
+    s.page_size = 16
+    assert L.iak_pages_shrink(None, 256, None, None) == N.IAK_ERR_INVALID_ARG
+    assert L.iak_pages_shrink(r(s), None, None, None) == N.IAK_OK                    # no slots
+    s.num_slots, s.num_table_heads, s.table_width, s.num_pages = 1024, 2, 1 << 21, 8
+    s.refs = s.page_table = s.lengths = 256
+    assert L.iak_pages_shrink(r(s), None, None, None) == N.IAK_ERR_INVALID_ARG
+    # 1024 rows' pages are counted in 31 bits
+    assert L.iak_pages_grow(r(s), r(pl), 256, None, 256, 1 << 30, None) == N.IAK_ERR_UNSUPPORTED
+    pl.num_planes, pl.base[0], pl.bytes[0] = 1, 256, 1 << 50
+    assert L.iak_pages_grow(r(s), r(pl), 256, None, 256, 1 << 30, None) == N.IAK_ERR_UNSUPPORTED
+
+
 def test_no_cpu_fallback():
     for args in ((4, 16, 96), (4, 24, 128), (-1, 16, 128)):
         with pytest.raises(ValueError):

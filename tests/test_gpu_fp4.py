@@ -283,6 +283,41 @@ def test_decode_matches_oracle(case, kind):
     _check(q, pool, table, lengths, (kd, vd), got, differential=(lam.astype(float), w, 1e-5, 0.8))
 
 
+@pytest.mark.parametrize("B,Ht,G,M,D,dtype", [(5000, 1, 1, 1, 64, "bf16"), (250, 8, 1, 1, 128, "f16"),
+                                              (33, 40, 9, 1, 128, "bf16"), (310, 4, 2, 3, 256, "f32")])
+def test_many_short_sequences(B, Ht, G, M, D, dtype):
+    """More (sequence, head, column group) units than warps, empty and one-token sequences among them; one is long
+    enough that units are cut."""
+    ia = _ia()
+    lengths = [(13 * i) % 140 if i % 5 else i % 2 for i in range(B)]
+    lengths[B // 3] = 300
+    pool, table, kd, vd = _cache(B, B, Ht, D, 16, lengths, dirty=True)
+    q = _rows(np.random.default_rng(B), (B, Ht * G, M, D), dtype)
+    ln = _i32(lengths)
+    got = ia.paged_decode_fp4(q, pool, table, ln)
+    some = sorted({B // 3, B - 1, *range(0, B, -(-B // 30))})
+    _check(q[some], pool, table[some], [lengths[b] for b in some], (kd[some], vd[some]), got[some])
+    # All of them against calls of 32 sequences, cut in other places: P rounds by 2^-11 at most (twice, as does l), the
+    # output by half a step of its type, both relative to the largest |V|, on either side.
+    again = torch.cat([ia.paged_decode_fp4(q[b:b + 32], pool, table[b:b + 32], ln[b:b + 32]) for b in range(0, B, 32)])
+    tol = float(np.abs(vd).max()) * (torch.finfo(got.dtype).eps + 2.0 ** -8)
+    assert float((got.float() - again.float()).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("D,Ht,G,M,lengths", [(128, 2, 4, 1, [40, 3000]), (64, 1, 40, 2, [5000]),
+                                              (256, 2, 6, 3, [90, 12000, 0])])
+def test_output_over_the_query(D, Ht, G, M, lengths):
+    ia = _ia()
+    B = len(lengths)
+    pool, table, _, _ = _cache(D, B, Ht, D, 16, lengths)
+    q = _rows(np.random.default_rng(D), (B, Ht * G, M, D), "bf16")
+    ln, lam = _i32(lengths), torch.full((Ht * G,), 0.4, device="cuda")
+    for f in (lambda x, **o: ia.paged_decode_fp4(x, pool, table, ln, **o),
+              lambda x, **o: ia.differential_decode_fp4(x, pool, table, ln, lam, **o)):
+        want, x = f(q), q.clone()
+        assert f(x, out=x) is x and torch.equal(x, want)
+
+
 def test_missing_pages_are_not_seen():
     ia = _ia()
     B, Ht, G, D, PS, n = 2, 2, 4, 128, 16, 200

@@ -74,6 +74,39 @@ def test_grow(P, PS, S, Ht, W):
     assert int(r) == want.rejected
 
 
+@pytest.mark.parametrize("S,Ht,P", [(1100, 9, 40000), (260, 17, 9000), (5000, 1, 12000)])
+def test_grow_many_rows(S, Ht, P):
+    """More rows than a block plans at a time, and free pages that end among the slots."""
+    g = np.random.default_rng(S)
+    W, PS = 4, 4
+    lengths = g.integers(0, W * PS // 2 + 1, S).tolist()
+    pool, pages, want = _state(S, P, PS, S, Ht, W, lengths, share=0.3, D=8)
+    r = _counter()
+    for _ in range(2):
+        more = g.integers(0, W * PS // 2, S)
+        more[g.random(S) < 0.4] = 0
+        _ia().grow_sequences(pool, pages, _i32(more), rejected=r)
+        want.grow(more)
+        _same(pool, pages, want)
+        assert int(r) == want.rejected
+    assert want.rejected > 0
+
+
+@pytest.mark.parametrize("PS,D", [(256, 128), (100, 128), (1000, 24), (129, 100)])
+def test_pages_of_several_pieces(PS, D):
+    """Pages that several warps copy, with ends inside a piece, by grow and by compact."""
+    S, W = 6, 3
+    pool, pages, want = _state(PS, 60, PS, S, 2, W, [PS + 3, 2 * PS, 5, 0, PS - 1, 2 * PS + 9], share=0.6, D=D)
+    more = [1, 1, PS, 2, 3, 0]
+    _ia().grow_sequences(pool, pages, _i32(more))
+    want.grow(more)
+    _same(pool, pages, want)
+    _ia().free_sequences(pages, _i32([0, 3]))
+    want.free([0, 3])
+    assert int(_ia().compact_pages(pool, pages)) == want.compact()
+    _same(pool, pages, want)
+
+
 def test_grow_runs_out():
     """Everything up to the first slot that does not fit; later ones stay, those without tokens too."""
     pool, pages, want = _state(3, 40, 16, 6, 2, 8, [17, 5, 0, 40, 16, 3], share=0.5)
