@@ -63,7 +63,7 @@ struct DecP {
   int runs;                          // warps of the main kernel
   int direct;                        // a warp per unit, nothing to join
   int by_unit;                       // cuts are recorded per unit, not per border
-  int min_tiles;                     // tiles a warp takes at least
+  int min_steps;                     // of a run, at least
   float* ws;
 };
 
@@ -177,7 +177,7 @@ __device__ __forceinline__ void find_sequence(const DecP& p, const Lanes& s, int
 struct Runs { int used, each, more; };
 __device__ __forceinline__ Runs make_runs(const DecP& p, int total) {
   Runs r;
-  r.used = static_cast<int>(min((static_cast<unsigned>(total) + p.min_tiles - 1) / p.min_tiles, static_cast<unsigned>(p.runs)));
+  r.used = static_cast<int>(min((static_cast<unsigned>(total) + p.min_steps - 1) / p.min_steps, static_cast<unsigned>(p.runs)));
   r.each = total / r.used;
   r.more = total - r.each * r.used;
   return r;
@@ -195,7 +195,7 @@ __device__ __forceinline__ float* part_at(const DecP& p, int run, int which, int
 }
 // What the join kernel reads of a unit cut over several runs.  Where there are no more units than runs a record per
 // unit, written by the run that has its first tile; else one per border between two runs, written by the run that the
-// border begins (if there is one) and empty unless it is a unit's first cut.
+// border begins (all of them have tiles then) and empty unless it is a unit's first cut.
 struct Cut { int b, h, j0, first, which, last; };   // first, last: runs with a part; which: first's; last < 0: none
 __device__ __forceinline__ Cut* cuts(const DecP& p) {
   return reinterpret_cast<Cut*>(p.ws + static_cast<int64_t>(p.runs) * 2 * p.cols * (p.pool.D + 4));
@@ -285,8 +285,9 @@ struct Shape {
   //   D 128, 16 columns, 8 sequences of 32k: 80 us with 8, 83 with 12; fp32 queries, 8 columns: 71 with 12, 75 with 8
   //   D 64, 32 columns, 16 sequences of 32k: 150 us with 8, 153 with 12, 196 with 16
   static constexpr int kSize = NB * NT * (SPLIT ? 2 : 1);
-  // tiles of a run, at least: wide heads' parts cost more to join
-  static constexpr int kMinTiles = NB == 8 ? 4 : 1;
+  // steps of a run, at least: wide heads' parts cost more to join
+  static constexpr int kMinSteps = NB == 8 ? 4 : 1;
+  static_assert(kMinSteps <= kOpen + 1, "with more units than runs every run has more than kOpen steps, so a tile");
   static constexpr int kPerSm = kSize <= 4 && NB == 2 ? 16 : (kSize <= (SPLIT ? 8 : 4) && NB < 8 ? 12 : 8);
   static constexpr int kBlocks = kPerSm / kWarps;
   static constexpr int kStages = NB == 8 ? 2 : 3;
@@ -979,7 +980,7 @@ int make_plan(DecP& p, Plan* plan) {
   const int64_t hc = static_cast<int64_t>(p.Ht) * p.CG, units = hc * p.B;
   if (units * L::COLS > 0x7fffffffLL) return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: too many rows for one launch");
   p.HC = static_cast<int>(hc);
-  p.min_tiles = L::kMinTiles;
+  p.min_steps = L::kMinSteps;
   const int64_t most = (static_cast<int64_t>(p.W) * p.pool.PS + kTileKeys - 1) / kTileKeys;
   if ((most + kOpen) * units > 0x7fffffffLL - 64)
     return fail(IAK_ERR_UNSUPPORTED, "iak_fp4_decode: tables of more than 2^31 tiles of %d tokens", kTileKeys);
@@ -994,7 +995,7 @@ int make_plan(DecP& p, Plan* plan) {
     plan->ws = 0;
     return IAK_OK;
   }
-  const int64_t useful = (most * units + L::kMinTiles - 1) / L::kMinTiles;
+  const int64_t useful = (most * units + L::kMinSteps - 1) / L::kMinSteps;
   plan->grid = static_cast<int>(std::min<int64_t>(blocks, (useful + L::kWarps - 1) / L::kWarps));
   p.runs = plan->grid * L::kWarps;
   p.by_unit = units <= p.runs;
