@@ -736,9 +736,8 @@ fp4_decode_kernel(const DecP p) {
             if (!((ok_here >> u) & 1) || key + (i & 1) + 8 * (i >> 1) >= full_end + p.M - 1) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
           }
         }
-        // byte e + 127 -> half 2^e: (byte - 112) << 10 in both halves at once
-        const unsigned v01 = __byte_perm(vs, 0, 0x4140) * 1024u - 112u * 1024u * 65537u;
-        const unsigned v23 = __byte_perm(vs, 0, 0x4342) * 1024u - 112u * 1024u * 65537u;
+        const unsigned v01 = fp4_half_scales(__byte_perm(vs, 0, 0x4140));
+        const unsigned v23 = fp4_half_scales(__byte_perm(vs, 0, 0x4342));
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           unsigned r0[4], r1[4];

@@ -272,10 +272,7 @@ __global__ void __launch_bounds__(kRowThreads) fp4_append_kernel(const RowsParam
   }
 }
 
-// scale byte (bytes) -> half 2^e in both halves (one in each): the pool's values are halves, so the products are exact
-__device__ __forceinline__ unsigned half_scales(unsigned lo, unsigned hi) {
-  return (lo | hi << 16) * 1024u - 112u * 1024u * 65537u;
-}
+// the pool's values are halves, so the products are exact
 __device__ __forceinline__ unsigned mul2(unsigned a, unsigned b) {
   const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
   return *reinterpret_cast<const unsigned*>(&r);
@@ -349,7 +346,7 @@ __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams 
   for (int b = 0; b < NB; ++b) {
     unsigned h[4];
     fp4_unpack4(kw[b], h);
-    const unsigned byte = b % 2 ? ks[b / 2] >> 8 : ks[b / 2] & 255, s = half_scales(byte, byte);
+    const unsigned byte = b % 2 ? ks[b / 2] >> 8 : ks[b / 2] & 255, s = fp4_half_scales(byte | byte << 16);
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = k_real ? mul2(h[i], s) : 0;
     char* to = static_cast<char*>(p.k) + (kat + 32 * b) * SIZE;
@@ -359,8 +356,7 @@ __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams 
   }
   const bool real0 = group && w.real(2 * t), real1 = group && w.real(2 * t + 1);
   const bool in[2] = {w.in(p, 2 * t), w.in(p, 2 * t + 1)};
-  // (the byte of a row that was never written could borrow from the other half)
-  const unsigned s = half_scales(real0 ? vs & 255 : 112, real1 ? vs >> 8 : 112);
+  const unsigned s = fp4_half_scales((vs & 255) | vs >> 8 << 16);
   unsigned v[2][2 * NB];                      // the rows' channels as half pairs
 #pragma unroll
   for (int j = 0; j < NB; ++j) {

@@ -186,6 +186,37 @@ def test_strided_rows_and_out():
     np.testing.assert_array_equal(_np(ia.read_fp4(pool, table, None, n)[0]), of.values(_np(k)))
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_rows_beside_rows_never_written(D):
+    """Two rows of V share their bytes: written ones are exact whatever their neighbours hold, and in a zeroed pool rows
+    that were never written are 0 to reads and to attention."""
+    ia = _ia()
+    g = np.random.default_rng(D)
+    PS, T, at = 16, 30, [1, 4, 5, 8, 17, 19, 22]             # odd and even rows alone, and a pair
+    table = _i32([[[2, 0]]])
+    k, v = _rows(g, (1, 1, T, D), "f32"), _rows(g, (1, 1, T, D), "f32")
+    kd, vd = np.zeros((1, 1, T, D)), np.zeros((1, 1, T, D))
+    for t in at:
+        kd[:, :, t], vd[:, :, t] = of.values(_np(k[:, :, t])), of.values(_np(v[:, :, t]))
+    for byte in (0, 111, 143, 255):
+        pool = ia.Fp4Pool.allocate(3, PS, D, zero=True)
+        pool.data.fill_(byte)
+        for t in at:
+            ia.append_fp4(pool, k[:, :, t:t + 1], v[:, :, t:t + 1], table, _i32([t]))
+        for dtype in DT.values():
+            gk, gv = ia.read_fp4(pool, table, None, T, dtype=dtype)
+            np.testing.assert_array_equal(_np(gk)[:, :, at], kd[:, :, at])
+            np.testing.assert_array_equal(_np(gv)[:, :, at], vd[:, :, at])
+            if byte == 0:
+                np.testing.assert_array_equal(_np(gk), kd)
+                np.testing.assert_array_equal(_np(gv), vd)
+        if byte == 0:
+            # one row of V at a time decides the output, its score 12: its scale off by 2^-10 would be above the bounds
+            for t in at:
+                q = torch.from_numpy(12 * D ** -0.5 * kd[:, :, t] / np.square(kd[:, :, t]).mean()).float().cuda()
+                _check(q, pool, table, [T], (kd, vd), ia.paged_decode_fp4(q, pool, table, _i32([T])))
+
+
 # --------------------------------------------------------------------------- #
 #  Attention
 # --------------------------------------------------------------------------- #
