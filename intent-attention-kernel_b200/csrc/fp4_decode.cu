@@ -2,15 +2,16 @@
 //
 // Mathematics.  A table head's queries form NC = G * M * (1 or 2) softmax columns (differential: two per query, the
 // first with q2 = 0 and the second with q1 = 0, so that both halves run as one product).  Per tile of 32 keys
-//   S' = K Q',  P = exp2(S - m),  O' += V' P'
-// with running maximum m and sum l per column, fp32.  Keys are the rows of the first product and the contraction of
+//   S' = K Q',  P = exp2(c (S - m) + 7),  O' += V' P'
+// with running maximum m and sum l per column, fp32, c the softmax scale: the difference is taken before the scale, so
+// that scores of any size keep their distances (a maximum rounded after it lies whole units off from 2^24 on).  Keys are the rows of the first product and the contraction of
 // the second, columns the narrow side (n = 8 per mma.m16n8k16), so that few queries waste little.
 //   K: a lane's 32-bit word holds 8 channels of one row; the byte pairs become half pairs in one conversion each, and
 //      a row's block scale 2^e multiplies the fp32 product of its 32 channels (4 lanes x 8), not its elements.
 //   V: a byte holds one channel of two neighbouring keys, so that its half pair lies along the contraction; it is
 //      multiplied by the two keys' scales (exact: the pool's values are halves).
 //   P: rounded to halves (fp32 queries: the sum of two), from the accumulator's layout to the operand's by movmatrix.
-//   m is raised only when a score passes it by 8 or more (P up to 2^15), which leaves the rescaling of O to few tiles.
+//   m is raised only when c (S - m) passes 8 (P up to 2^15), which leaves the rescaling of O to few tiles.
 // What bounds it: the cache's bytes, 4.25 bits an element, and close behind them the issue slots: per 16 rows a warp
 // spends about 64 conversions, 64 multiplies and 16 products at D 128.
 // Work is cut into equal runs of steps over all (sequence, table head, column group) units, one for each resident warp,
@@ -40,8 +41,11 @@ constexpr int kTileKeys = 32;      // keys of a warp's tile: two groups of 16
 constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
 constexpr int kDirectTiles = 8;    // units of at most so many tiles are never cut
 constexpr int kOpen = 3;           // a unit's queries, first copies and output take a warp as long as so many tiles
-constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
 constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small P stay normal halves
+constexpr float kLazy = 8.f;       // and P may grow by so many powers of two before the maximum is raised
+// Of a column.  With the least, -FLT_MAX as the first maximum still lies more than kLazy below every score; with the
+// largest (products of scale and queries beyond fp32) equal scores keep their equal weights.
+constexpr float kScaleMin = 1e-37f, kScaleMax = FLT_MAX;
 
 struct DecP {
   Fp4Pool pool;
@@ -189,7 +193,7 @@ __device__ __forceinline__ int run_of(const Runs& r, int t) {
 }
 
 // A run leaves at most two parts of units: [0] of the unit that it begins in, [1] of the one that it ends in.  A part
-// is D sums, the maximum and the sum of the weights for each column.
+// is D sums, the maximum, the sum of the weights and the scale for each column.
 __device__ __forceinline__ float* part_at(const DecP& p, int run, int which, int col) {
   return p.ws + ((static_cast<int64_t>(run) * 2 + which) * p.cols + col) * (p.pool.D + 4);
 }
@@ -565,7 +569,7 @@ fp4_decode_kernel(const DecP p) {
         if (SPLIT) dst[NT * NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
       // of the lane's own columns 8 nt + 2 t and the next
-      const float mine = fmaxf(p.scale * __uint_as_float(ex << 23), 1e-37f);
+      const float mine = fminf(fmaxf(p.scale * __uint_as_float(ex << 23), kScaleMin), kScaleMax);
       sc[nt][0] = __shfl_sync(~0u, mine, 8 * t);
       sc[nt][1] = __shfl_sync(~0u, mine, 8 * t + 4);
     }
@@ -673,7 +677,7 @@ fp4_decode_kernel(const DecP p) {
         for (int e = 0; e < 2; ++e) {
           mx[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
           mx[nt][e] = fmaxf(mx[nt][e], fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-          raise = raise || fmaf(mx[nt][e], sc[nt][e], -m_run[nt][e]) > kLazy;
+          raise = raise || (mx[nt][e] - m_run[nt][e]) * sc[nt][e] > kLazy;
         }
       }
       if (__any_sync(~0u, raise)) {
@@ -686,8 +690,8 @@ fp4_decode_kernel(const DecP p) {
             v = fmaxf(v, __shfl_xor_sync(~0u, v, 4));
             v = fmaxf(v, __shfl_xor_sync(~0u, v, 8));
             v = fmaxf(v, __shfl_xor_sync(~0u, v, 16));
-            const float m_new = fmaxf(m_run[nt][e], fmaf(v, sc[nt][e], -kHead));
-            f[e] = tc::ex2(m_run[nt][e] - m_new);
+            const float m_new = fmaxf(m_run[nt][e], v);
+            f[e] = tc::ex2((m_run[nt][e] - m_new) * sc[nt][e]);
             m_run[nt][e] = m_new;
             l_run[nt][e] *= f[e];
           }
@@ -706,7 +710,7 @@ fp4_decode_kernel(const DecP p) {
           float x[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[i] = tc::ex2(fmaf(s[u][nt][i], sc[nt][i & 1], -m_run[nt][i & 1]));
+            x[i] = tc::ex2(fmaf(s[u][nt][i] - m_run[nt][i & 1], sc[nt][i & 1], kHead));
             l_run[nt][i & 1] += x[i];
           }
 #pragma unroll
@@ -804,7 +808,7 @@ fp4_decode_kernel(const DecP p) {
           for (int i = 0; i < MT; i += 2)
             *reinterpret_cast<float4*>(part + g * (4 * NB) + 2 * i) =
                 make_float4(o[nt][i][e], o[nt][i][e + 2], o[nt][i + 1][e], o[nt][i + 1][e + 2]);
-          if (g == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m_run[nt][e], l_all[nt][e]);
+          if (g == 0) *reinterpret_cast<float4*>(part + D) = make_float4(m_run[nt][e], l_all[nt][e], sc[nt][e], 0.f);
         }
         continue;
       }
@@ -878,7 +882,7 @@ __global__ void __launch_bounds__(join_warps(TEAM) * 32) fp4_join_kernel(const D
   for (int half = 0; half < per; ++half) {
     const int col = r * per + half;
     // a warp takes every TEAM-th part, four at a time, so that their loads run together
-    float top = -FLT_MAX, l = 0.f, acc[NB];
+    float top = -FLT_MAX, l = 0.f, sc = 0.f, acc[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) acc[i] = 0.f;
     constexpr int kAt = NB <= 4 ? 4 : 2;
@@ -888,22 +892,24 @@ __global__ void __launch_bounds__(join_warps(TEAM) * 32) fp4_join_kernel(const D
       for (int k = 0; k < kAt; ++k) {
         const int part = min(c + k * TEAM, n - 1);
         const float* at = part_at(p, d.first + part, part == 0 ? d.which : 0, col);
-        m[k] = at[D];
-        pl[k] = at[D + 1];
+        const float4 ends = *reinterpret_cast<const float4*>(at + D);
+        m[k] = ends.x;
+        pl[k] = ends.y;
+        sc = ends.z;                               // the same in every part
 #pragma unroll
         for (int i = 0; i < NB; ++i) v[k][i] = at[i * 32 + lane];
       }
       float next = top;
 #pragma unroll
       for (int k = 0; k < kAt; ++k) next = fmaxf(next, m[k]);
-      const float old = tc::ex2(top - next);
+      const float old = tc::ex2((top - next) * sc);
       l *= old;
 #pragma unroll
       for (int i = 0; i < NB; ++i) acc[i] *= old;
 #pragma unroll
       for (int k = 0; k < kAt; ++k) {
         if (c + k * TEAM < n) {                    // (the last part stands in for missing ones)
-          const float f = tc::ex2(m[k] - next);
+          const float f = tc::ex2((m[k] - next) * sc);
           l = fmaf(pl[k], f, l);
 #pragma unroll
           for (int i = 0; i < NB; ++i) acc[i] = fmaf(v[k][i], f, acc[i]);
@@ -925,7 +931,7 @@ __global__ void __launch_bounds__(join_warps(TEAM) * 32) fp4_join_kernel(const D
         for (int i = 0; i < NB; ++i) acc[i] = 0.f;
 #pragma unroll
         for (int w = 0; w < TEAM; ++w) {
-          const float f = tc::ex2(part_sum[w][D] - top);
+          const float f = tc::ex2((part_sum[w][D] - top) * sc);
           l = fmaf(part_sum[w][D + 1], f, l);
 #pragma unroll
           for (int i = 0; i < NB; ++i) acc[i] = fmaf(part_sum[w][i * 32 + lane], f, acc[i]);

@@ -385,6 +385,53 @@ def test_query_sizes(size):
     _check(q, pool, table, [500], (kd, vd), got, scale=1.0 / size)
 
 
+@pytest.mark.parametrize("T", [45, 9000])
+@pytest.mark.parametrize("q_base,k_base,step,sm_scale,dtype", [
+    (8192.0, 16384.0, 8192.0, 1.0, "f16"), (20480.0, 49152.0, 16384.0, 0.7, "f16"), (8192.0, 16384.0, 8192.0, 1.0, "f32"),
+    (2.0 ** 60, 49152.0, 2.0 ** 60, -3.0, "bf16"), (2.0 ** 100, 24576.0, 2.0 ** 101, 1e30, "f32"),
+    (2.0 ** 100, 24576.0, 2.0 ** 101, 1e30, "bf16"), (8.0, 1024.0, 0.25, 1.0, "f32"), (16.0, 512.0, 0.25, 0.9, "f16")])
+def test_scores_far_from_zero(q_base, k_base, step, sm_scale, dtype, T):
+    """A large score that all keys share and a difference of a few steps.  Every product is a small multiple of one power
+    of two and the sums need 24 bits at most, so the scores are exact: the weights have to be right to the rounding of P
+    and of exp2 (its argument, at most 150 before P leaves the floats, off by 2^-22 of itself with the scale's rounding),
+    however large the scores are."""
+    ia = _ia()
+    g = np.random.default_rng(T)
+    D, B, G = 128, 2, 4
+    k = np.zeros((B, 1, T, D), np.float32)
+    k[..., 0:32] = k[..., 64:96] = k_base
+    more = np.array([0.0, 0.5, 1.0, 2.0, 4.0, 6.0], np.float32)[g.integers(0, 6, (2, B, 1, T))]
+    k[..., 32], k[..., 96] = more
+    v = g.standard_normal((B, 1, T, D)).astype(np.float32)
+    table = _i32(g.permutation(B * (T // 16 + 1)).reshape(B, 1, -1))
+    pool = ia.Fp4Pool.allocate(table.numel(), 16, D, zero=True)
+    ia.append_fp4(pool, torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda(), table)
+    q = np.zeros((B, G, D))
+    q[..., 0:32] = q[..., 64:96] = q_base
+    q[..., 32] = step * np.array([1.0, -1.0, 2.0, 0.0])
+    q[..., 96] = step * np.array([1.0, 1.0, 0.0, -2.0])
+    tq = torch.from_numpy(q).to(DT[dtype]).cuda()
+    lengths, lam = [T, T - 7], [0.5, -0.25, 1.0, 0.0]
+    vd = of.values(v)
+    np.testing.assert_array_equal(of.values(k), k)
+    np.testing.assert_array_equal(_np(tq), q)
+    plain = _np(ia.paged_decode_fp4(tq, pool, table, _i32(lengths), sm_scale=sm_scale, out_dtype=torch.float32))
+    diff = _np(ia.differential_decode_fp4(tq, pool, table, _i32(lengths), torch.tensor(lam, device="cuda"),
+                                          sm_scale=sm_scale, out_dtype=torch.float32))
+    arg = 150 * 2.0 ** -22
+    for b, n in enumerate(lengths):
+        kb, vb, seen = k[b, 0, :n].astype(float), vd[b, 0, :n], np.ones((1, n), bool)
+        for h in range(G):
+            def part(lo, hi):
+                out, A, _ = of.attention(q[b, h, None, lo:hi], kb[:, lo:hi], vb, seen, sm_scale)
+                return out[0], (_tolerance(A, np.zeros(1), vb, D, dtype == "f32") + 2 * arg * A)[0]
+            want, tol = part(0, D)
+            assert (np.abs(plain[b, h] - want) <= tol + 2.0 ** -24 * np.abs(want)).all(), (b, h, plain[b, h][:4], want[:4])
+            (w1, t1), (w2, t2) = part(0, D // 2), part(D // 2, D)
+            want, tol = w1 - lam[h] * w2, t1 + abs(lam[h]) * t2 + 2.0 ** -22 * (np.abs(w1) + np.abs(w2))
+            assert (np.abs(diff[b, h] - want) <= tol).all(), (b, h, diff[b, h][:4], want[:4])
+
+
 def test_large_and_tiny_values():
     """The ends of what a row can hold: values up to 49152 and down to 2^-15, and one strong key."""
     ia = _ia()
