@@ -337,6 +337,10 @@ __device__ __forceinline__ void finish_row(const DecP& p, int b, int head, int m
 
 __device__ __forceinline__ float safe_inverse(float l) { return l == 0.f ? 0.f : 1.f / l; }
 
+// Of two maps' outputs, each rounded before (__fmul_rn keeps the compiler from fusing them in): equal maps of weight 1
+// leave exactly 0, not the rounding of one product, which a norm without eps would make a whole row of.
+__device__ __forceinline__ float difference(float x1, float lam, float x2) { return fmaf(-lam, x2, x1); }
+
 // x: N neighbouring values of an output row, from element `at` on
 template <int N>
 __device__ __forceinline__ void store_run(const DecP& p, int64_t at, const float (&x)[N]) {
@@ -815,13 +819,13 @@ fp4_decode_kernel(const DecP p) {
       if (p.diff) {
         const int row = j >> 1, gi = row / p.M;
         const bool real = j < p.NC;
-        const float w0 = safe_inverse(l_all[nt][0]);
-        const float w1 = real ? -p.lam[segment.h * p.G + gi] * safe_inverse(l_all[nt][1]) : 0.f;
+        const float w0 = safe_inverse(l_all[nt][0]), w1 = safe_inverse(l_all[nt][1]);
+        const float lam = real ? p.lam[segment.h * p.G + gi] : 0.f;
         float x[4 * NB], mul = p.out_scale;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          x[2 * i] = fmaf(o[nt][i][1], w1, o[nt][i][0] * w0);
-          x[2 * i + 1] = fmaf(o[nt][i][3], w1, o[nt][i][2] * w0);
+          x[2 * i] = difference(__fmul_rn(o[nt][i][0], w0), lam, __fmul_rn(o[nt][i][1], w1));
+          x[2 * i + 1] = difference(__fmul_rn(o[nt][i][2], w0), lam, __fmul_rn(o[nt][i][3], w1));
         }
         if (p.norm_w) {
           float sq = 0.f;
@@ -941,9 +945,12 @@ __global__ void __launch_bounds__(join_warps(TEAM) * 32) fp4_join_kernel(const D
     if (warp == 0) {
       const int row = p.diff ? (j0 >> 1) : j0;
       const float inv = safe_inverse(l);
-      const float scale = half ? -p.lam[d.h * p.G + row / p.M] * inv : inv;
+      const float lam = half ? p.lam[d.h * p.G + row / p.M] : 0.f;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) x[i] = half ? fmaf(acc[i], scale, x[i]) : acc[i] * scale;
+      for (int i = 0; i < NB; ++i) {
+        const float part = __fmul_rn(acc[i], inv);
+        x[i] = half ? difference(x[i], lam, part) : part;
+      }
       if (half == per - 1) finish_row<NB>(p, d.b, d.h * p.G + row / p.M, row % p.M, x);
     }
     if (TEAM > 1) __syncthreads();

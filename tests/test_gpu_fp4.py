@@ -477,6 +477,26 @@ def test_differential_row_of_zeros_stays_zero():
         assert (got[0] == 0).all() and torch.isfinite(got).all()
 
 
+@pytest.mark.parametrize("D,M,dtype", [(64, 1, "f32"), (128, 3, "bf16"), (256, 1, "f16")])
+def test_equal_maps_cancel_exactly(D, M, dtype):
+    """Equal halves of queries and keys with weight 1: 0 for every eps, for whole and cut units, not noise of rms 1."""
+    ia = _ia()
+    g = np.random.default_rng(D)
+    lengths = [5, 9000, 300]
+    B, T, W = len(lengths), max(lengths), -(-max(lengths) // 16)
+    half, v = _rows(g, (B, 1, T, D // 2), "f32"), _rows(g, (B, 1, T, D), "f32")
+    pool = ia.Fp4Pool.allocate(B * W, 16, D)
+    table = _i32(g.permutation(B * W).reshape(B, 1, W))
+    ia.append_fp4(pool, torch.cat([half, half], -1), v, table)
+    q = _rows(g, (B, 4, M, D // 2), dtype)
+    q = torch.cat([q, q], -1)
+    lam, w = torch.ones(4, device="cuda"), torch.ones(D, device="cuda")
+    for ln, norm, eps in ((lengths, w, 0.0), (lengths, w, 1e-5), (lengths, None, 0.0), ([5, 40, 90], w, 0.0)):
+        t = table if ln is lengths else table[:, :, :6]                    # (few tiles: a warp a unit, nothing to join)
+        got = ia.differential_decode_fp4(q, pool, t, _i32(ln), lam, norm_weight=norm, eps=eps)
+        assert (got == 0).all()
+
+
 def test_first_call_captured():
     """The very first call of a process, captured: nothing that a capture forbids happens in a call."""
     import subprocess
