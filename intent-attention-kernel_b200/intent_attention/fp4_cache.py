@@ -33,14 +33,16 @@ HEAD_DIMS = (64, 128, 256)
 
 # Per-call host work is most of a small call's time: the helpers below take the device as its index (a CPU tensor's is
 # -1), test the few properties that the kernels rely on and build their messages only when one fails.
-_current_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
 _NO_SWITCH = contextlib.nullcontext()
 
 
 def _on(dev: int):
     """The library launches on the current device; switch only when it is another one."""
-    return _NO_SWITCH if dev == _current_device() else torch.cuda.device(dev)
+    return _NO_SWITCH if dev == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+def _raw_stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)        # (a torch build without CUDA lacks the name: not at import)
 
 
 def _check_device(t, name: str, dev: int) -> None:

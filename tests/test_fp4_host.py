@@ -4,6 +4,7 @@ before any device call."""
 import ctypes
 import os
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -139,6 +140,32 @@ def test_shrink_and_wide_tables_rejected_on_the_host():
     assert L.iak_pages_grow(r(s), r(pl), 256, None, 256, 1 << 30, None) == N.IAK_ERR_UNSUPPORTED
     pl.num_planes, pl.base[0], pl.bytes[0] = 1, 256, 1 << 50
     assert L.iak_pages_grow(r(s), r(pl), 256, None, 256, 1 << 30, None) == N.IAK_ERR_UNSUPPORTED
+
+
+def test_imports_on_a_torch_build_without_cuda():
+    """The package's host side (router, policies, layouts) needs none of torch's CUDA entry points."""
+    code = """
+import torch
+for name in [n for n in vars(torch._C) if n.startswith("_cuda_")]:
+    delattr(torch._C, name)
+import intent_attention as ia
+assert ia.Fp4Pool.allocate(2, 16, 64, device="cpu").nbytes() == 2 * 17 * 64
+assert ia.SequencePages.allocate(2, 16, 1, 1, 2, device="cpu").lengths.tolist() == [0]
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.join(ROOT, "intent-attention-kernel_b200"),
+                       capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_calls_go_to_the_tensors_device(monkeypatch):
+    """Another device than the current one is made current for the call, and its own stream taken."""
+    from intent_attention import fp4_cache as fc
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: 1000 + dev, raising=False)
+    assert fc._on(0) is fc._NO_SWITCH
+    other = fc._on(1)
+    assert isinstance(other, torch.cuda.device) and other.idx == 1
+    assert fc._raw_stream(1) == 1001
 
 
 def test_no_cpu_fallback():
