@@ -661,7 +661,8 @@ int iak_pages_workspace_size(const iak_seq_pages* pages, size_t* bytes);
  * table_width pages, one whose open page lies outside the pool, and, when the
  * free pages run out, the first slot that does not fit and every later one
  * that gets tokens.  1024 (slot, head) pairs may want 2^31 pages at most, by
- * table_width. */
+ * table_width.  A refused slot keeps its length and may still share its open
+ * page: write new rows only where lengths grew. */
 int iak_pages_grow(const iak_seq_pages* pages, const iak_page_planes* planes, const int32_t* new_tokens,
                    int32_t* rejected, void* workspace, size_t workspace_bytes, void* stream);
 /* takes tokens[s] tokens off the end of every slot (draft tokens that were not

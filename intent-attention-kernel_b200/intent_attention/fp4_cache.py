@@ -149,7 +149,8 @@ def append_fp4(pool: Fp4Pool, k_new: torch.Tensor, v_new: torch.Tensor, page_tab
     written.  Rows whose table slot or page does not exist are left out and
     added to ``dropped`` (an int32 CUDA counter).  The pages written in one call
     belong to one (b, h) each, and a sequence is written by one call at a time:
-    two rows of V share their bytes.
+    two rows of V share their bytes.  After ``grow_sequences`` the counts are
+    what the lengths grew by: a slot that was refused may still share its page.
     """
     s, dev = pool.struct(), pool.data.get_device()
     _check_device(k_new, "k_new", dev)

@@ -5,7 +5,23 @@ holders per page (0 = free), the page table of every slot and table head, and
 the tokens of every slot.  Its ``table`` and ``lengths`` are what the attention
 and append calls take.  Sequences share pages after ``fork_sequences``; a shared
 page that is part full is copied by ``grow_sequences`` before its holder writes
-into it.  Pages of ``PagePool`` and ``Fp4Pool`` alike.
+into it.  A step of a serving loop::
+
+    start = pages.lengths.clone()
+    grow_sequences(pool, pages, new_tokens)
+    got = pages.lengths - start
+    append_fp4(pool, k_new, v_new, pages.table, start, got)
+
+``got`` is 0 for the slots that were refused (no free page, a full table):
+rows written for them all the same would land in an open page that other
+sequences may still share.  Their outputs of the step are over the old tokens.
+
+The operations copy and move pages of ``PagePool`` and ``Fp4Pool`` alike, but
+only ``Fp4Pool``'s calls follow a table and lengths.  ``append_tokens`` and
+``route_pages`` name a ``PagePool``'s pages by ``bases`` (those of a sequence
+lie together, the open one staged in ``KVStage``) and do not apply to pages
+that these operations hand out: write such pages with ``PagePool.quantize_``
+and attend to whole pages by table and page counts (``paged_decode``).
 
 All operations run on the device without reading anything back, are exact and
 do not depend on the order in which blocks run; ``rejected`` (an int32 CUDA
@@ -114,7 +130,8 @@ def grow_sequences(pool: Union[PagePool, Fp4Pool], pages: SequencePages, new_tok
     table entry).  A slot that gets tokens while its last page is part full and
     held by others too first gets a copy of that page (all planes of the
     pool; with ``page_tags`` and ``tag_map`` those of the page's format, and its
-    tag).  The tokens themselves are the caller's to write.  Refused: a
+    tag).  The tokens themselves are the caller's to write, for slots whose
+    length has grown.  Refused: a
     negative count; tokens beyond the table's width; an open page outside the
     pool; and, once the free pages run out, the first slot that does not fit and
     every later one that gets tokens.

@@ -319,6 +319,41 @@ def test_serving_run():
     check()
 
 
+def test_refused_growth_leaves_shared_pages_alone():
+    """The documented step, with no page free for a copy: slot 2 shares slot 1's open page and was shrunk into it, so its
+    new rows would be slot 1's tokens.  Slot 0 grows inside a page of its own."""
+    ia = _ia()
+    from intent_attention import sequence_pages
+    PS, D, Ht, W = 16, 64, 2, 3
+    P = 2 * Ht + Ht
+    pool, pages = ia.Fp4Pool.allocate(P, PS, D), ia.SequencePages.allocate(P, PS, 3, Ht, W)
+    gen = torch.Generator("cuda").manual_seed(3)
+
+    def rows(n):
+        return [torch.randn(3, Ht, n, D, device="cuda", generator=gen) for _ in range(2)]
+
+    lines = sequence_pages.__doc__.split("loop::\n\n")[1].split("\n\n")[0]
+    step = compile("\n".join(x.strip() for x in lines.splitlines()), "step", "exec")
+
+    def run(n, new_tokens):
+        k, v = rows(n)
+        exec(step, dict(vars(ia), pool=pool, pages=pages, k_new=k, v_new=v, new_tokens=_i32(new_tokens)))
+        return k, v
+
+    k, v = run(20, [5, 20, 0])
+    ia.fork_sequences(pages, _i32([1]), _i32([2]))
+    ia.shrink_sequences(pages, _i32([0, 0, 2]))
+    assert int((pages.refs == 0).sum()) == 0
+    k2, v2 = run(1, [1, 0, 1])
+    assert pages.lengths.tolist() == [6, 20, 18]
+    for x, new, got in zip((k, v), (k2, v2), ia.read_fp4(pool, pages.table, None, 20, pages.lengths, dtype=torch.float32)):
+        want = torch.zeros_like(got)
+        held = torch.from_numpy(of.values(x.double().cpu().numpy())).float().cuda()
+        want[0, :, :5], want[1], want[2, :, :18] = held[0, :, :5], held[1], held[1, :, :18]
+        want[0, :, 5] = torch.from_numpy(of.values(new[0, :, 0].double().cpu().numpy())).float().cuda()
+        assert torch.equal(got, want)
+
+
 def test_page_refusals():
     ia = _ia()
     pool, pages, _ = _state(1, 32, 16, 2, 1, 4, [10, 0])
