@@ -51,7 +51,8 @@ _PLANES = tuple((f"{side}_{name}", bits) for name, bits in (
 
 @dataclass
 class SequencePages:
-    """``refs`` int32 [num_pages], ``table`` int32 [slots, Ht, W], ``lengths`` int32 [slots], all on one device."""
+    """``refs`` int32 [num_pages], ``table`` int32 [slots, Ht, W], ``lengths`` int32 [slots], all on one device.
+    The table may be a view with strides; its rows are contiguous and do not overlap."""
 
     refs: torch.Tensor
     table: torch.Tensor
@@ -74,6 +75,11 @@ class SequencePages:
             raise ValueError("page_size must be positive")
         pt, ss, sh, Ht, W = _page_table(self.table, dev)
         slots = self.table.shape[0]
+        # every entry is written on its own: rows one after another, slots or heads outermost
+        inner, outer = ((sh, Ht), (ss, slots)) if ss >= sh else ((ss, slots), (sh, Ht))
+        row = W if inner[1] <= 1 else W + (inner[1] - 1) * inner[0]
+        if (inner[1] > 1 and inner[0] < W) or (outer[1] > 1 and outer[0] < row):
+            raise ValueError("table rows must not overlap (an expanded view?)")
         return N.SeqPages(_index_tensor(self.refs, "refs", dev), self.refs.numel(), pt, ss, sh, W,
                           _index_tensor(self.lengths, "lengths", dev, slots), slots, Ht, self.page_size)
 

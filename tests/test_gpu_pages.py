@@ -354,6 +354,54 @@ def test_refused_growth_leaves_shared_pages_alone():
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("view", ["heads_outside", "slices"])
+def test_tables_with_strides(view):
+    """The table as a view: heads outermost, or every other row of a wider one; what lies between stays."""
+    ia = _ia()
+    S, Ht, W = 7, 3, 6
+    pool, pages, want = _state(11, 300, 16, S, Ht, W, [40, 17, 90, 0, 0, 5, 64], share=0.3)
+    if view == "heads_outside":
+        wide = pages.table.transpose(0, 1).contiguous()
+        pages.table = wide.transpose(0, 1)
+    else:
+        wide = torch.full((2 * S, Ht + 1, W + 3), 77, dtype=torch.int32, device="cuda")
+        wide[::2, 1:, 2:2 + W] = pages.table
+        pages.table = wide[::2, 1:, 2:2 + W]
+    r = _counter()
+    more = [1, 15, 6, 3, 0, 40, 1]
+    ia.grow_sequences(pool, pages, _i32(more), rejected=r)
+    want.grow(more)
+    ia.fork_sequences(pages, _i32([2]), _i32([4]), rejected=r)
+    want.fork([2], [4])
+    ia.shrink_sequences(pages, _i32([2, 0, 33, 1, 0, 0, 0]), rejected=r)
+    want.shrink([2, 0, 33, 1, 0, 0, 0])
+    ia.free_sequences(pages, _i32([0, 6]), rejected=r)
+    want.free([0, 6])
+    assert int(ia.compact_pages(pool, pages)) == want.compact()
+    _same(pool, pages, want)
+    assert int(r) == want.rejected
+    if view == "slices":
+        wide[::2, 1:, 2:2 + W] = 77
+        assert (wide == 77).all()
+
+
+def test_tables_that_overlap_are_refused():
+    """An expanded table would give one entry to several slots or heads, each writing its own page into it."""
+    ia = _ia()
+    refs, ln = torch.zeros(8, dtype=torch.int32, device="cuda"), _i32([0, 0])
+    one = torch.full((2, 1, 4), -1, dtype=torch.int32, device="cuda")
+    for table in (one.expand(2, 3, 4), one[:1].expand(2, 1, 4), one.as_strided((2, 1, 4), (3, 4, 1)),
+                  one.as_strided((2, 2, 2), (1, 2, 1)), one.as_strided((2, 2, 2), (2, 2, 1))):
+        pages = ia.SequencePages(refs, table, ln, 16)
+        pool = ia.Fp4Pool.allocate(8, 16, 64)
+        for f in (lambda: ia.grow_sequences(pool, pages, ln), lambda: ia.free_sequences(pages, ln),
+                  lambda: ia.compact_pages(pool, pages)):
+            with pytest.raises(ValueError, match="overlap"):
+                f()
+    for table in (one.expand(2, 1, 4), one[:1], one[:, :, :1], one[:, :, :0], one[:0]):
+        ia.SequencePages(refs, table, ln[:table.shape[0]], 16).struct()
+
+
 def test_page_refusals():
     ia = _ia()
     pool, pages, _ = _state(1, 32, 16, 2, 1, 4, [10, 0])
