@@ -621,7 +621,7 @@ typedef struct iak_fp4_decode_args {
   float sm_scale;
   int32_t differential;
   const float* lam;                                  /* [Hq], differential only                     */
-  const float* norm_weight; float eps, out_scale;    /* differential only                           */
+  const float* norm_weight; float eps, out_scale;    /* differential only; finite, eps >= 0         */
 } iak_fp4_decode_args;
 int iak_fp4_decode_workspace_size(const iak_fp4_pool* pool, const iak_fp4_decode_args* args, size_t* bytes);
 int iak_fp4_decode(const iak_fp4_pool* pool, const iak_fp4_decode_args* args, void* workspace,

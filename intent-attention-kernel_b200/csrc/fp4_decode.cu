@@ -1088,6 +1088,8 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
     return fail(IAK_ERR_INVALID_ARG, "%s: bad dtype", what);
   if (a->num_queries > IAK_FP4_MAX_QUERIES)
     return fail(IAK_ERR_UNSUPPORTED, "%s: %d queries, at most %d", what, a->num_queries, IAK_FP4_MAX_QUERIES);
+  if (a->differential && !(a->eps >= 0.f && a->eps - a->eps == 0.f && a->out_scale - a->out_scale == 0.f))
+    return fail(IAK_ERR_INVALID_ARG, "%s: eps must be finite and not negative, out_scale finite", what);
   if (a->batch == 0 || a->num_q_heads == 0 || a->num_queries == 0) return IAK_OK;
   if (a->num_table_heads == 0 || a->num_q_heads % a->num_table_heads)
     return fail(IAK_ERR_INVALID_ARG, "%s: query heads (%d) must be a multiple of table heads (%d)", what,

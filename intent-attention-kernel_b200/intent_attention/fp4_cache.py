@@ -296,7 +296,5 @@ def differential_decode_fp4(q: torch.Tensor, pool: Fp4Pool, page_table: torch.Te
         raise ValueError("q must be [B, Hq, D] or [B, Hq, M, D]")
     lam_ptr = weight(lam, "lam", q.shape[1])
     norm_ptr = None if norm_weight is None else weight(norm_weight, "norm_weight", pool.head_dim)
-    if not (eps >= 0.0 and math.isfinite(eps) and math.isfinite(out_scale)):
-        raise ValueError("eps must be finite and not negative, out_scale finite")
     scale = 1.0 / math.sqrt(pool.head_dim // 2) if sm_scale is None else float(sm_scale)
     return _decode(q, pool, page_table, lengths, scale, out, out_dtype, (lam_ptr, norm_ptr, float(eps), float(out_scale)))

@@ -98,6 +98,22 @@ def test_fp4_args_rejected_on_the_host():
     assert L.iak_fp4_decode_workspace_size(r(p), r(d), None) == N.IAK_ERR_INVALID_ARG
 
 
+@pytest.mark.parametrize("field,value", [("eps", -1e-6), ("eps", float("nan")), ("eps", 1e39), ("out_scale", 1e39),
+                                         ("out_scale", float("nan"))])
+def test_differential_numbers_rejected_on_the_host(field, value):
+    """What is not finite as a float (1e39 is as a double), and an eps that could make a mean square negative."""
+    L = N.lib()
+    r = ctypes.byref
+    d, p = N.Fp4DecodeArgs(), _pool()
+    d.batch, d.num_q_heads, d.num_table_heads, d.num_queries, d.table_width = 1, 4, 2, 1, 2
+    d.q = d.out = d.lengths = d.page_table = d.lam = 256
+    d.sm_scale, d.out_scale, d.differential = 1.0, 1.0, 1
+    setattr(d, field, value)
+    n = ctypes.c_size_t(0)
+    assert L.iak_fp4_decode_workspace_size(r(p), r(d), r(n)) == N.IAK_ERR_INVALID_ARG and b"eps" in L.iak_last_error()
+    assert L.iak_fp4_decode(r(p), r(d), None, 0, None) == N.IAK_ERR_INVALID_ARG
+
+
 def test_page_args_rejected_on_the_host():
     L = N.lib()
     r = ctypes.byref
