@@ -233,6 +233,106 @@ def test_tagged_pages_copy_their_format():
             getattr(pool, n).copy_(t)
 
 
+PLANES = {0: [], 1: ["f16"], 2: ["fp8", "scale"], 3: ["i8", "scale"], 4: ["i4", "scale"],
+          5: ["i4", "i4r", "scale", "res_scale"], 6: []}
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int32])
+@pytest.mark.parametrize("op", ["grow", "compact"])
+def test_tagged_pages_copy_nothing_else(op, dtype):
+    """A page of every format (SKIP, SPARSE and a tag beyond the map included), by copy-on-write and by packing: the
+    planes of its format and its tag arrive, every other byte of the pool stays."""
+    ia = _ia()
+    from intent_attention.paged import make_tag_map
+    g = np.random.default_rng(3)
+    P, PS, D = 48, 16, 64
+    pool = ia.PagePool.allocate(P, PS, D, scale_mode="group32", zero=True)
+    planes = {n: t for n, t in vars(pool).items() if torch.is_tensor(t)}
+    assert len(planes) == 14
+    for t in planes.values():
+        t.view(torch.uint8).copy_(torch.from_numpy(g.integers(0, 255, (*t.shape[:-1], t.shape[-1] * t.element_size()),
+                                                              dtype=np.uint8)))
+    before = {n: t.view(torch.uint8).clone() for n, t in planes.items()}
+    # tag 10 + format, 9 SPARSE; 200 is beyond the map: the default, INT8 as tag 3
+    formats = [0, 1, 2, 3, 4, 5, 6, 3, 3]
+    tag_of = [10, 11, 12, 13, 14, 15, 9, 3, 200]
+    tag_map = make_tag_map({**{10 + c: c for c in range(6)}, 9: 6, 3: 3})
+    tags = torch.full((P,), 11, dtype=dtype, device="cuda")
+    S = len(formats)
+    ids = 20 + g.permutation(P - 20)[:S]
+    tags[torch.from_numpy(ids).cuda()] = torch.tensor(tag_of, dtype=dtype, device="cuda")
+    tags0 = tags.clone()
+    refs = np.zeros(P, np.int32)
+    refs[ids] = 1
+    table = np.full((2 * S, 1, 2), -1, np.int32)
+    table[:S, 0, 0] = ids
+    pages = ia.SequencePages(_i32(refs), _i32(table), _i32([5] * S + [0] * S), PS)
+    if op == "grow":
+        ia.fork_sequences(pages, _i32(range(S)), _i32(range(S, 2 * S)))
+        ia.grow_sequences(pool, pages, _i32([0] * S + [1] * S), page_tags=tags, tag_map=tag_map, tag_default=3)
+        at = slice(S, 2 * S)
+        assert pages.table[:S, 0, 0].tolist() == ids.tolist() and int(pages.refs.max()) == 1
+    else:
+        assert int(ia.compact_pages(pool, pages, page_tags=tags, tag_map=tag_map, tag_default=3)) == S
+        at = slice(0, S)
+    new = pages.table[at, 0, 0].tolist()
+    assert sorted(new) == list(range(S))
+    want_tags = tags0.clone()
+    for i, p in enumerate(new):
+        want_tags[p] = tags0[int(ids[i])]
+    assert torch.equal(tags, want_tags)
+    for n, t in planes.items():
+        want = before[n].clone()
+        for i, p in enumerate(new):
+            if n[2:] in PLANES[formats[i]]:
+                want[p] = before[n][int(ids[i])]
+        assert torch.equal(t.view(torch.uint8), want), n
+
+
+@pytest.mark.parametrize("P", [(1 << 18) + 1, 300000, 800011])
+def test_pools_of_several_runs_a_block(P):
+    """More pages than a block of the plan holds in registers: free pages far apart, in every run, are found in order."""
+    g = np.random.default_rng(P)
+    PS, S, Ht, W = 1, 96, 8, 260
+    pool, pages, want = _state(P, P, PS, S, Ht, W, g.integers(0, 200, S).tolist(), share=0.1, D=4)
+    ia = _ia()
+    # nearly all other pages in use by somebody else: the free ones are few and anywhere
+    busy = (want.refs == 0) & (g.random(P) > 0.06)
+    want.refs[busy] = 1
+    pages.refs.copy_(_i32(want.refs))
+    r = _counter()
+    for _ in range(2):
+        more = g.integers(0, 60, S)
+        ia.grow_sequences(pool, pages, _i32(more), rejected=r)
+        want.grow(more)
+        _same(pool, pages, want)
+        assert int(r) == want.rejected
+    ia.free_sequences(pages, _i32(range(0, S, 3)))
+    want.free(list(range(0, S, 3)))
+    # (the others let go of theirs)
+    want.refs[busy] = 0
+    pages.refs[_i32(np.flatnonzero(busy)).long()] = 0
+    assert int(ia.compact_pages(pool, pages)) == want.compact()
+    _same(pool, pages, want)
+
+
+def test_wants_beyond_31_bits():
+    """Slots that together want more than 2^31 pages: those that the free pages reach grow, the sums do not wrap."""
+    ia = _ia()
+    S, W, P = 4096, 1 << 20, 3000
+    table = torch.empty((S, 1, W), dtype=torch.int32, device="cuda")       # 17 GB; only entries of accepted slots are written
+    pages = ia.SequencePages(torch.zeros(P, dtype=torch.int32, device="cuda"), table, _i32([0] * S), 1)
+    pool = ia.PagePool(P, 1, 4, k_f16=torch.zeros(P, 1, 4, dtype=torch.float16, device="cuda"))
+    more = np.full(S, W)
+    more[:3] = [1000, 0, 1500]
+    more[7] = -1
+    r = _counter()
+    ia.grow_sequences(pool, pages, _i32(more), rejected=r)
+    assert pages.lengths.tolist() == [1000, 0, 1500] + [0] * (S - 3)
+    assert int(r) == S - 3 and int(pages.refs.sum()) == 2500 and int(pages.refs[:2500].min()) == 1
+    assert table[0, 0, :1000].tolist() == list(range(1000)) and table[2, 0, :1500].tolist() == list(range(1000, 2500))
+
+
 def test_page_ops_captured():
     ia = _ia()
     pool, pages, want = _state(9, 4000, 16, 12, 4, 10, [100, 33, 64, 0, 0, 0, 0, 0, 0, 0, 0, 0], share=0.0)
