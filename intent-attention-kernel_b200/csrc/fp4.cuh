@@ -44,11 +44,14 @@ __device__ __forceinline__ void fp4_unpack4(unsigned w, unsigned (&h)[4]) {
       : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
 }
 
-// Two scale bytes e + 127 (bits 0..7 and 16..23) -> the halves 2^e.  A half's exponent, e + 15, is the byte - 112 in five
-// bits: the byte's low five with bit 4 turned.  Nothing carries from one to the other: the byte of a row that was never
-// written may be anything (0 in a zeroed pool), its neighbour keeps its scale.
-__device__ __forceinline__ unsigned fp4_half_scales(unsigned bytes) {
-  return ((bytes ^ 0x00100010u) & 0x001f001fu) << 10;
+// Four scale bytes e + 127 -> the upper bytes of the halves 2^e (the lower ones are 0).  A half's exponent, e + 15, is the
+// byte - 112 in five bits: the byte's low five with bit 4 turned.  Nothing carries from one to the next: the byte of a row
+// that was never written may be anything (0 in a zeroed pool), its neighbour keeps its scale.
+__device__ __forceinline__ unsigned fp4_half_tops(unsigned bytes) { return (bytes * 4u ^ 0x40404040u) & 0x7c7c7c7cu; }
+// the half pair 2^e of bytes I (low) and J
+template <int I, int J>
+__device__ __forceinline__ unsigned fp4_scale_pair(unsigned tops) {
+  return __byte_perm(tops, 0, J << 12 | 4 << 8 | I << 4 | 4);
 }
 
 // A group of 16 rows: byte offsets (the public header has the layout in words).

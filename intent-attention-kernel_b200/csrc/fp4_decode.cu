@@ -42,8 +42,8 @@ constexpr int kMaxTokens = 1 << 30; // of a table row: token numbers stay 32-bit
 constexpr int kDirectTiles = 8;    // units of at most so many tiles are never cut
 constexpr int kOpen = 3;           // a unit's queries, first copies and output take a warp as long as so many tiles
 constexpr float kHead = 7.f;       // the maximum's own P is 2^7, so that small P stay normal halves
-constexpr float kLazy = 8.f;       // and P may grow by so many powers of two before the maximum is raised
-// Of a column.  With the least, -FLT_MAX as the first maximum still lies more than kLazy below every score; with the
+constexpr float kLazy = 15.f;      // P may grow to 2^15 before the maximum is raised
+// Of a column.  With the least, -FLT_MAX as the first maximum still is raised by every score; with the
 // largest (products of scale and queries beyond fp32) equal scores keep their equal weights.
 constexpr float kScaleMin = 1e-37f, kScaleMax = FLT_MAX;
 
@@ -255,6 +255,18 @@ __device__ __forceinline__ void copy16(unsigned dst, const void* src) {
 // a volatile statement, as the reads of the copied bytes are: they keep their order
 __device__ __forceinline__ void warp_sync() { asm volatile("bar.warp.sync 0xffffffff;" ::: "memory"); }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Pairs of floats, one instruction for both: c (s - m) + 7 (the difference before the scale is what an fma alone would
+// leave out, at no more instructions than it), and sums.
+__device__ __forceinline__ void exponents(const float* s, const float* m, const float* c, float* e) {
+  asm("{\n.reg .b64 s, m, c, h;\nmov.b64 s, {%2, %3};\nmov.b64 m, {%4, %5};\nmov.b64 c, {%6, %7};\nmov.b64 h, {%8, %8};\n"
+      "sub.rn.f32x2 s, s, m;\nfma.rn.f32x2 s, s, c, h;\nmov.b64 {%0, %1}, s;\n}"
+      : "=f"(e[0]), "=f"(e[1])
+      : "f"(s[0]), "f"(s[1]), "f"(m[0]), "f"(m[1]), "f"(c[0]), "f"(c[1]), "f"(kHead));
+}
+__device__ __forceinline__ void add_pair(float* a, const float* b) {
+  asm("{\n.reg .b64 a, b;\nmov.b64 a, {%0, %1};\nmov.b64 b, {%2, %3};\nadd.rn.f32x2 a, a, b;\nmov.b64 {%0, %1}, a;\n}"
+      : "+f"(a[0]), "+f"(a[1]) : "f"(b[0]), "f"(b[1]));
+}
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -681,8 +693,10 @@ fp4_decode_kernel(const DecP p) {
         for (int e = 0; e < 2; ++e) {
           mx[nt][e] = fmaxf(s[0][nt][e], s[0][nt][e + 2]);
           mx[nt][e] = fmaxf(mx[nt][e], fmaxf(s[1][nt][e], s[1][nt][e + 2]));
-          raise = raise || (mx[nt][e] - m_run[nt][e]) * sc[nt][e] > kLazy;
         }
+        float top[2];
+        exponents(mx[nt], m_run[nt], sc[nt], top);
+        raise = raise || top[0] > kLazy || top[1] > kLazy;
       }
       if (__any_sync(~0u, raise)) {
 #pragma unroll
@@ -713,9 +727,11 @@ fp4_decode_kernel(const DecP p) {
         for (int nt = 0; nt < NT; ++nt) {
           float x[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[i] = tc::ex2(fmaf(s[u][nt][i] - m_run[nt][i & 1], sc[nt][i & 1], kHead));
-            l_run[nt][i & 1] += x[i];
+          for (int i = 0; i < 4; i += 2) {
+            exponents(&s[u][nt][i], m_run[nt], sc[nt], &x[i]);
+            x[i] = tc::ex2(x[i]);
+            x[i + 1] = tc::ex2(x[i + 1]);
+            add_pair(l_run[nt], &x[i]);
           }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
@@ -744,8 +760,7 @@ fp4_decode_kernel(const DecP p) {
             if (!((ok_here >> u) & 1) || key + (i & 1) + 8 * (i >> 1) >= full_end + p.M - 1) vs = (vs & ~(255u << (8 * i))) | (112u << (8 * i));
           }
         }
-        const unsigned v01 = fp4_half_scales(__byte_perm(vs, 0, 0x4140));
-        const unsigned v23 = fp4_half_scales(__byte_perm(vs, 0, 0x4342));
+        const unsigned tops = fp4_half_tops(vs), v01 = fp4_scale_pair<0, 1>(tops), v23 = fp4_scale_pair<2, 3>(tops);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           unsigned r0[4], r1[4];

@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams 
   for (int b = 0; b < NB; ++b) {
     unsigned h[4];
     fp4_unpack4(kw[b], h);
-    const unsigned byte = b % 2 ? ks[b / 2] >> 8 : ks[b / 2] & 255, s = fp4_half_scales(byte | byte << 16);
+    const unsigned tops = fp4_half_tops(ks[b / 2]), s = b % 2 ? fp4_scale_pair<1, 1>(tops) : fp4_scale_pair<0, 0>(tops);
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = k_real ? mul2(h[i], s) : 0;
     char* to = static_cast<char*>(p.k) + (kat + 32 * b) * SIZE;
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(kRowThreads) fp4_read_kernel(const RowsParams 
   }
   const bool real0 = group && w.real(2 * t), real1 = group && w.real(2 * t + 1);
   const bool in[2] = {w.in(p, 2 * t), w.in(p, 2 * t + 1)};
-  const unsigned s = fp4_half_scales((vs & 255) | vs >> 8 << 16);
+  const unsigned s = fp4_scale_pair<0, 1>(fp4_half_tops(vs));
   unsigned v[2][2 * NB];                      // the rows' channels as half pairs
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
