@@ -23,7 +23,6 @@ __device__ __forceinline__ int fp4_scale_byte(float amax) {
 }
 
 __device__ __forceinline__ float fp4_inv_scale(int byte) { return __uint_as_float((254 - byte) << 23); }
-__device__ __forceinline__ float fp4_scale(int byte) { return __uint_as_float(byte << 23); }
 
 // eight E2M1 codes, x[i] in bits 4i..: nearest, ties to the even code, saturating at 6
 __device__ __forceinline__ unsigned fp4_pack8(const float (&x)[8]) {

@@ -12,8 +12,8 @@
 //      multiplied by the two keys' scales (exact: the pool's values are halves).
 //   P: rounded to halves (fp32 queries: the sum of two), from the accumulator's layout to the operand's by movmatrix.
 //   m is raised only when c (S - m) passes 8 (P up to 2^15), which leaves the rescaling of O to few tiles.
-// What bounds it: the cache's bytes, 4.25 bits an element, and close behind them the issue slots: per 16 rows a warp
-// spends about 64 conversions, 64 multiplies and 16 products at D 128.
+// What bounds it: the cache's bytes, 4.25 bits an element, and close behind them the issue slots: of 233 per 16
+// rows at D 128 and 8 columns a warp spends 64 on conversions, 32 on V's scales, 16 on K's and 16 on products.
 // Work is cut into equal runs of steps over all (sequence, table head, column group) units, one for each resident warp,
 // so that ragged batches, many short sequences and one long sequence fill the GPU alike.  A step is a tile; what a unit
 // costs besides its tiles counts as three (256 sequences of up to 512 tokens: 31 us, with equal runs of tiles 44; 16 of up
@@ -53,7 +53,7 @@ struct DecP {
   unsigned long long gpp_inv;        // 2^36 / gpp, rounded up
   const void* q; int q_dtype; int64_t q_sb, q_sh, q_sm;
   void* out; int out_dtype; int64_t o_sb, o_sh, o_sm;
-  int B, Hq, Ht, G, M;
+  int B, Ht, G, M;
   const int32_t* pt; int64_t pt_sb, pt_sh; int W;
   const int32_t* lengths;
   float scale;                       // |sm_scale| * log2(e)
@@ -296,7 +296,7 @@ struct Shape {
   static constexpr int kWarps = 4;
   static constexpr int kThreads = kWarps * 32;
   // Warps of an SM: 16 with 128 registers each while the accumulators are small, 12 with 168, 8 with 255.  A tile's two
-  // groups of 16 keys go through the products together, for the independent work.  Measured:
+  // groups of 16 keys go through the products together, for the independent work.  Measured when chosen:
   //   D 128, 8 columns, 32 sequences of up to 32k: 139 us with 12 warps, 141 with 16 and a stage less
   //   D 128, 16 columns, 8 sequences of 32k: 80 us with 8, 83 with 12; fp32 queries, 8 columns: 71 with 12, 75 with 8
   //   D 64, 32 columns, 16 sequences of 32k: 150 us with 8, 153 with 12, 196 with 16
@@ -1123,7 +1123,7 @@ int decode_call(const iak_fp4_pool* pool, const iak_fp4_decode_args* a, bool lau
   p.q = a->q; p.q_dtype = a->q_dtype; p.q_sb = a->q_stride_b; p.q_sh = a->q_stride_h; p.q_sm = a->q_stride_m;
   p.out = a->out; p.out_dtype = a->out_dtype;
   p.o_sb = a->out_stride_b; p.o_sh = a->out_stride_h; p.o_sm = a->out_stride_m;
-  p.B = a->batch; p.Hq = a->num_q_heads; p.Ht = a->num_table_heads; p.G = p.Hq / p.Ht; p.M = a->num_queries;
+  p.B = a->batch; p.Ht = a->num_table_heads; p.G = a->num_q_heads / p.Ht; p.M = a->num_queries;
   p.pt = a->page_table; p.pt_sb = a->pt_stride_b; p.pt_sh = a->pt_stride_h;
   p.W = pool->num_pages > 0 ? a->table_width : 0;      // an empty pool holds no token
   p.lengths = a->lengths;

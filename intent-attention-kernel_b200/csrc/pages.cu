@@ -115,7 +115,8 @@ __device__ __forceinline__ void copy_piece(const Planes& pl, int64_t from, int64
   }
 }
 
-// The pages that block `rank` of the cluster scans, in whole runs of kRun pages: a thread takes 32 at a time.
+// The pages that block `rank` of the cluster scans: an eighth of them in whole runs of 32.  A thread takes 32 at a time,
+// the block kRun.
 constexpr int kRun = 32 * kPlanThreads;
 __device__ __forceinline__ void slice_of(int pages, int rank, int* begin, int* end) {
   const int64_t per = ((static_cast<int64_t>(pages) + kCluster * 32 - 1) / (kCluster * 32)) * 32;
