@@ -566,8 +566,9 @@ int iak_prefill(const iak_page_pools* pools, const iak_prefill_args* args, void*
  *                      channel 4 NB g + k of row 2 t (low half) and 2 t + 1 (high half)
  *   bytes 512 NB ..    K scales [g 8][hi 2][NB], of row g + 8 hi
  *   bytes 528 NB ..    V scales [NB][t 4][j 4], of row 2 t + (j & 1) + 8 (j >> 1)
- * Rows never written may hold anything: no call reads them.  The data is
- * 16-byte aligned.
+ * Rows never written may hold anything, and a call whose counts or lengths
+ * reach over them gets anything for them (0 in zeroed memory); written rows
+ * beside them keep their values.  The data is 16-byte aligned.
  * ------------------------------------------------------------------------ */
 #define IAK_FP4_MAX_QUERIES 16
 typedef struct iak_fp4_pool {

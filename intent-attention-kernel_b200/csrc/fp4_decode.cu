@@ -17,7 +17,7 @@
 // Work is cut into equal runs of steps over all (sequence, table head, column group) units, one for each resident warp,
 // so that ragged batches, many short sequences and one long sequence fill the GPU alike.  A step is a tile; what a unit
 // costs besides its tiles counts as three (256 sequences of up to 512 tokens: 31 us, with equal runs of tiles 44; 16 of up
-// to 8001 with 4 queries and D 256: 43.5 against 48).  A unit cut over several runs
+// to 8001 with 4 queries and D 256: 43 against 48).  A unit cut over several runs
 // leaves partial (m, l, O) that a second kernel adds in order of the runs (no atomics: results do not depend on timing).
 // Warps share nothing: with units cut per block of 8 warps, their sums joined in shared memory, 256 sequences of up to
 // 700 tokens took 87 us instead of 39.
@@ -25,8 +25,8 @@
 // the order in which lanes read them, so that copies and reads are linear in the lane, free of bank conflicts, and five
 // copies per 16 rows need one address.  (Bulk copies with an mbarrier measured the same at D 128 and slower at D 64, 70 us
 // against 66 for 16 sequences of 32k; they would need bounded waits besides.)
-// 32 sequences of up to 32k tokens, 32 query and 8 table heads, D 128: 134 us, 5.9 TB/s; 64 of 32k 364 us, 6.3 TB/s; one
-// of 512k 101 us, 5.7 TB/s; 4096 of 256 tokens 247 us, 4.6 TB/s.
+// 32 sequences of up to 32k tokens, 32 query and 8 table heads, D 128, launched one after another: 135 us, 5.9 TB/s; 64 of
+// 32k 366 us, 6.2 TB/s; one of 512k 102 us, 5.6 TB/s; 4096 of 256 tokens 245 us, 4.7 TB/s.
 #include <algorithm>
 #include <cfloat>
 #include <mutex>
